@@ -210,7 +210,7 @@ def _workspace(nbytes):
 
 def _own_tree(s):
     c, case = _context(), s["case"]
-    need = c.tree_attention_workspace(s["q"].shape, s["k"].shape, max_len=case["len"], weights=case["weights"])
+    need = c.tree_attention_workspace(s["q"].shape, s["k"].shape, max_len=case["len"], account=case["weights"])
     c.tree_attention(s["q"], s["k"], s["v"], s["kscale"], s["vscale"], s["lens"], s["out"], mask=s["mask"], counts=s["counts"], lse=s["lse"],
                      account=s["account"] if case["weights"] else None, decay=s["decay"] if case["weights"] else 1.0, max_len=case["len"],
                      workspace=_workspace(need), stream=torch.cuda.current_stream().cuda_stream, wait=False)
