@@ -311,6 +311,144 @@ int qxg_kv_read_position(qxg_ctx *ctx, uint32_t position, uint32_t layers, int8_
  * fails, like it, on a non-finite value or a bad length. */
 int qxg_q8k_quantize(qxg_ctx *ctx, const float *x, uint32_t n, void *blocks_out, char *err, uint64_t err_len);
 
+/* ---- operators on device memory (no reference counterpart) ----
+ *
+ * For programs that keep their activations and caches on the GPU: a drafted tree of tokens
+ * attends over an INT8 cache of the context's format, the cache is kept within a budget, and
+ * logits are adjusted and picked from.  Every pointer in the argument structs is device memory
+ * of the context's GPU, owned by the caller and allocated by the HIP runtime that this library
+ * uses; other pointers are refused.  A call queues its kernels on `stream` (a hipStream_t of
+ * that GPU as void *; NULL: HIP's default stream) and returns; with wait != 0 it returns when
+ * they have finished.  Work of other streams on the same memory is the caller's to order.  A
+ * call allocates nothing and copies nothing, so it can be captured into a graph.  Its workspace
+ * is the caller's: calls that may run at the same time (other streams, graphs) need one each.
+ * The qxg_*_workspace functions return the bytes that a call with these arguments needs (0 if
+ * it would be refused).  Indexes, lengths and counts in device memory are 32-bit unsigned and
+ * clamped to the arrays' sizes by the kernels.  Calls do not touch the context's own buffers
+ * and stream, and may be made from several threads on one context.
+ *
+ * Value types are GGML types: 0 F32, 1 F16, 30 BF16. */
+#define QXG_TYPE_F32 0u
+#define QXG_TYPE_F16 1u
+#define QXG_TYPE_BF16 30u
+
+/* Attention of a tree of drafted tokens (nodes) over an INT8 cache.  Sequence b has
+ * lens[b] cached positions; its count = counts[b] nodes' K and V rows stand behind them at
+ * positions lens[b] .. lens[b] + count - 1.  Node i sees every cached position and the nodes
+ * that its mask row names (bit j % 32 of word j / 32: node j; a node that is to see itself has
+ * its own bit set).  For q head h, kv head g = h / (heads / kv_heads):
+ *     s[p] = scale * kscale[p] * sum_d q[i][h][d] k[p][g][d]        over the visible positions
+ *     out[i][h] = sum_p softmax(s)[p] vscale[p] v[p][g]             (f32 sums, rounded once)
+ *     lse[i][h] = log sum_p exp(s[p])
+ * A row that sees nothing has out 0 and lse -inf.  What stands in positions that a row does not see
+ * (scales that are infinite or NaN among them) does not reach it.  Rows of nodes at and behind
+ * count are left as they were.  With account, each position's weight is added to it:
+ *     account[p] = decay * account[p] + sum over nodes and heads of softmax(s)[p]
+ * for p < lens[b] + count, in a fixed order (equal calls give equal bits).
+ * An F32 q is multiplied as two halves of 11 bits each, and its weights too (errors as of f32
+ * products); for F16 and BF16 the weights are rounded to 11 bits.  nodes = 1 without a mask is
+ * ordinary decoding. */
+typedef struct qxg_tree_attention_args {
+    const void *q;            /* [batch][nodes][heads][dim] of `type`, 16-byte aligned */
+    const int8_t *k, *v;      /* [batch][positions][kv_heads][dim], 16-byte aligned */
+    const float *kscale, *vscale;   /* [batch][positions] */
+    const uint32_t *lens;     /* [batch] cached positions; count + lens[b] is clamped to positions */
+    const uint32_t *counts;   /* [batch] nodes in use, or NULL: all */
+    const uint32_t *mask;     /* [batch][nodes][(nodes + 31) / 32], or NULL: node i sees nodes 0 .. i */
+    void *out;                /* as q, 16-byte aligned; not overlapping q */
+    float *lse;               /* [batch][nodes][heads], or NULL */
+    float *account;           /* [batch][positions], or NULL */
+    void *workspace;          /* 16-byte aligned */
+    uint64_t workspace_bytes;
+    uint64_t q_batch, q_node;         /* strides in elements; 16 bytes divide the strides' sizes */
+    uint64_t out_batch, out_node;
+    uint64_t kv_batch, kv_row;        /* of k and v, in bytes, multiples of 16 */
+    uint64_t scale_batch;             /* of kscale and vscale, in floats */
+    uint64_t account_batch;
+    uint32_t type;
+    uint32_t batch, nodes, heads, kv_heads;   /* batch <= 65535, nodes <= 1024, heads a multiple of kv_heads */
+    uint32_t dim;             /* 64 or 128 */
+    uint32_t positions;       /* of the cache arrays */
+    uint32_t max_len;         /* about the longest of lens (shapes the launch; results hold for any) */
+    float scale, decay;
+} qxg_tree_attention_args;
+int qxg_tree_attention(qxg_ctx *ctx, const qxg_tree_attention_args *args, void *stream, int wait, char *err, uint64_t err_len);
+uint64_t qxg_tree_attention_workspace(const qxg_tree_attention_args *args);
+
+/* Which positions of each group (a layer, a sequence) to keep within `budget`: the first `sinks`,
+ * the last `recent`, and of those between the ones with the largest account (the lower position
+ * where equal; NaN as -inf).  keep[g][0 .. kept[g]) receives them in ascending order, kept[g] =
+ * min(lens[g], budget); the rest of keep is left as it was. */
+typedef struct qxg_kv_select_args {
+    const float *account;     /* [groups][positions] */
+    const uint32_t *lens;     /* [groups] */
+    uint32_t *keep;           /* [groups][budget] */
+    uint32_t *kept;           /* [groups] */
+    uint64_t account_group, keep_group;   /* strides in elements */
+    uint32_t groups, positions, budget, sinks, recent;   /* sinks + recent <= budget */
+    uint32_t max_len;         /* as in qxg_tree_attention */
+} qxg_kv_select_args;
+int qxg_kv_select(qxg_ctx *ctx, const qxg_kv_select_args *args, void *stream, int wait, char *err, uint64_t err_len);
+
+/* Moves the rows of each group's cache in place: row first + i becomes what row keep[g][i] was,
+ * for i < min(kept[g], slots).  keep[g] ascends strictly and keep[g][i] >= first + i, as
+ * qxg_kv_select writes it, or as a program lists the accepted nodes of a tree behind its cached
+ * positions (first = lens[b]); of a list that does not, the moved rows are undefined (never
+ * anything else).  Rows at and behind first + kept[g] are left as they were.  account_out[first +
+ * i] = account[keep[i]] in another array.  Entries outside the cache are skipped. */
+typedef struct qxg_kv_compact_args {
+    int8_t *k, *v;            /* [groups][positions][row_bytes], 16-byte aligned */
+    float *kscale, *vscale;   /* [groups][positions] */
+    const uint32_t *keep;     /* [groups][slots] */
+    const uint32_t *kept;     /* [groups] */
+    const float *account;     /* [groups][positions], or NULL with account_out */
+    float *account_out;
+    void *workspace;          /* 16-byte aligned */
+    uint64_t workspace_bytes;
+    uint64_t kv_group, kv_row;        /* in bytes, multiples of 16 */
+    uint64_t scale_group;             /* in floats */
+    uint64_t keep_group, kept_group;  /* in elements; 0: one list for all groups */
+    uint64_t account_group, account_out_group;
+    uint32_t groups, positions, slots, first, row_bytes;   /* row_bytes a multiple of 16, at most 4096 */
+} qxg_kv_compact_args;
+int qxg_kv_compact(qxg_ctx *ctx, const qxg_kv_compact_args *args, void *stream, int wait, char *err, uint64_t err_len);
+uint64_t qxg_kv_compact_workspace(const qxg_kv_compact_args *args);
+
+/* Penalties, biases, temperature and grammar mask on rows of logits, and the best tokens.  Per
+ * row, for token v with logit x (f32 arithmetic, one rounding an operation, in this order):
+ *     v anywhere in the history:                x = x > 0 ? x / repetition : x * repetition
+ *     v occurs c > 0 times behind the prompt:   x = x - frequency * c;  x = x - presence
+ *     v in the bias list:                       x = x + (its biases, added in list order)
+ *                                               x = x / temperature
+ *     the token's mask bit is 0:                x = -inf
+ * out = x rounded once to the type; lse = log sum exp(x) (NaN if an x is); top_ids / top_logits = the
+ * top_n tokens by (x desc, id asc), as qxg_final_head ranks them; NaN and -inf are never picked: where no
+ * others are left the id is QXG_NO_TOKEN and the logit -inf.  History and bias entries that are no token (>= vocab)
+ * are skipped, so unused entries can be filled with QXG_NO_TOKEN. */
+#define QXG_NO_TOKEN 0xffffffffu
+typedef struct qxg_adjust_logits_args {
+    const void *logits;       /* [rows][vocab] of `type`; any alignment of the type */
+    void *out;                /* as logits; may be logits itself with the same stride */
+    const uint32_t *history;  /* [rows][history_slots], or NULL */
+    const uint32_t *history_lens;   /* [rows] entries in use, or NULL: all */
+    const uint32_t *prompt_lens;    /* [rows] entries that are prompt, or NULL: none */
+    const float *penalties;   /* [rows][3] repetition, frequency, presence; NULL: 1, 0, 0 */
+    const float *temperature; /* [rows], or NULL: 1 */
+    const uint32_t *bias_ids; /* [rows][biases], or NULL */
+    const float *bias_values;
+    const uint32_t *mask;     /* [masks][(vocab + 31) / 32] bits, bit v % 32 of word v / 32, or NULL */
+    const uint32_t *mask_rows;      /* [rows] the row's mask; no mask where >= masks; NULL: row r takes mask r */
+    uint32_t *top_ids;        /* [rows][top_n], or NULL with top_n 0 */
+    float *top_logits;        /* [rows][top_n], or NULL */
+    float *lse;               /* [rows], or NULL */
+    void *workspace;          /* 16-byte aligned */
+    uint64_t workspace_bytes;
+    uint64_t logits_row, out_row, history_row;   /* strides in elements */
+    uint32_t type, rows, vocab, history_slots, biases, masks, top_n;   /* rows <= 65535, biases <= 1024, top_n <= 32 */
+} qxg_adjust_logits_args;
+int qxg_adjust_logits(qxg_ctx *ctx, const qxg_adjust_logits_args *args, void *stream, int wait, char *err, uint64_t err_len);
+uint64_t qxg_adjust_logits_workspace(const qxg_adjust_logits_args *args);
+
 /* ---- measurement (no reference counterpart: the reference times with clock(),
  *      src/qx_format.c:6245, 6642-6653) ---- */
 

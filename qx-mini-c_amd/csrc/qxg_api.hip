@@ -2,6 +2,7 @@
 // model binding, INT8 KV cache, and the launch sequence of one decode step.
 #include "qxg.h"
 #include "qxg_internal.h"
+#include "qxg_ops.h"
 #include "qx_grids.h"
 
 #include <cmath>
@@ -1039,6 +1040,8 @@ bool scratch_address(int device, uint8_t **addr, char *err, uint64_t n) {
     return true;
 }
 }  // namespace
+
+int qxg_ctx_device(const qxg_ctx *c) { return c->device; }
 
 extern "C" {
 

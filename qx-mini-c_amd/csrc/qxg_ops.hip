@@ -1,0 +1,225 @@
+// Host side of the operators on device memory (include/qxg.h): argument checks, workspaces, launches.
+// The checks of sizes come first and use no GPU.
+#include "qxg_ops.h"
+
+#include <algorithm>
+#include <cstdarg>
+#include <cstdio>
+#include <cmath>
+
+namespace {
+struct Err {
+    char *err;
+    uint64_t n;
+    __attribute__((format(printf, 2, 3))) bool operator()(const char *fmt, ...) const {
+        if (err && n) {
+            va_list ap;
+            va_start(ap, fmt);
+            vsnprintf(err, (size_t)n, fmt, ap);
+            va_end(ap);
+        }
+        return false;
+    }
+};
+
+// bytes of a value; 0 for another type
+uint32_t type_size(uint32_t t) { return t == QXG_TYPE_F32 ? 4 : t == QXG_TYPE_F16 || t == QXG_TYPE_BF16 ? 2 : 0; }
+
+struct Arg {
+    const void *p;
+    const char *name;
+    bool need;         // may not be NULL
+    uint32_t align;
+};
+
+// Runs `go` with the context's GPU current (and the caller's GPU again after it), once every pointer is
+// known to be memory of that GPU.
+template <size_t N, typename F>
+bool on_device(const qxg_ctx *c, const Arg (&args)[N], hipStream_t s, int wait, const Err &fail, F go) {
+    if (!c) return fail("invalid context");
+    const int dev = qxg_ctx_device(c);
+    for (const Arg &a : args) {
+        if (!a.p) continue;
+        hipPointerAttribute_t at{};
+        if (hipPointerGetAttributes(&at, a.p) != hipSuccess) {
+            (void)hipGetLastError();
+            return fail("%s is not device memory of this library's HIP runtime", a.name);
+        }
+        if (at.type != hipMemoryTypeDevice || at.device != dev) return fail("%s is not memory of the context's device %d", a.name, dev);
+    }
+    int before = dev;
+    if (hipGetDevice(&before) != hipSuccess || (before != dev && hipSetDevice(dev) != hipSuccess)) return fail("hipSetDevice failed");
+    (void)hipGetLastError();
+    go();
+    hipError_t e = hipGetLastError();
+    if (e == hipSuccess && wait) e = hipStreamSynchronize(s);
+    if (before != dev) (void)hipSetDevice(before);
+    return e == hipSuccess || fail("%s", hipGetErrorString(e));
+}
+template <size_t N> bool pointers_ok(const Arg (&args)[N], const Err &fail) {
+    for (const Arg &a : args) {
+        if (!a.p && a.need) return fail("%s is NULL", a.name);
+        if ((uintptr_t)a.p % a.align) return fail("%s is not aligned to %u bytes", a.name, a.align);
+    }
+    return true;
+}
+uint64_t up16(uint64_t v) { return (v + 15) & ~15ull; }
+
+// ---- tree attention
+// Splits of the positions: about 1024 workgroups (two fit a CU, twice over) of at least four 32-position
+// chunks, one a wave.
+uint32_t tree_splits(const qxg_tree_attention_args &a, uint32_t tiles) {
+    const uint64_t wgs = (uint64_t)a.kv_heads * tiles * a.batch, most = std::max<uint64_t>(1, ((uint64_t)a.max_len + a.nodes) / 128);
+    return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(1024 / wgs, most));
+}
+bool tree_plan(const qxg_tree_attention_args *p, QxaArgs &A, uint64_t &bytes, const Err &fail) {
+    if (!p) return fail("invalid argument");
+    const qxg_tree_attention_args &a = A.a = *p;
+    const uint32_t size = type_size(a.type);
+    if (!size) return fail("unsupported value type %u", a.type);
+    if (!a.batch || a.batch > 65535) return fail("batch must be between 1 and 65535");
+    if (!a.nodes || a.nodes > 1024) return fail("nodes must be between 1 and 1024");
+    if (a.dim != 64 && a.dim != 128) return fail("dim must be 64 or 128");
+    if (!a.kv_heads || !a.heads || a.heads % a.kv_heads || a.heads > 1024) return fail("heads must be a multiple of kv_heads, at most 1024");
+    if (!a.positions || a.positions > 0x7fffffffu || a.max_len > 0x7fffffffu) return fail("positions and max_len must be below 2^31");
+    if (a.q_batch * size % 16 || a.q_node * size % 16 || a.out_batch * size % 16 || a.out_node * size % 16)
+        return fail("the strides of q and out must be multiples of 16 bytes");
+    if (a.kv_batch % 16 || a.kv_row % 16) return fail("the strides of k and v must be multiples of 16 bytes");
+    if (!std::isfinite(a.scale) || !(a.scale > 0.0f)) return fail("scale must be positive and finite");
+    if (!std::isfinite(a.decay)) return fail("decay must be finite");
+    A.group = a.heads / a.kv_heads;
+    A.columns = a.nodes * A.group;
+    A.tiles = (A.columns + 31) / 32;
+    A.splits = tree_splits(a, A.tiles);
+    A.words = (a.nodes + 31) / 32;
+    A.scale2 = (float)((double)a.scale * 1.4426950408889634);
+    const uint64_t rows = (uint64_t)a.batch * a.nodes * a.heads;
+    const uint64_t part = A.splits > 1 ? up16(A.splits * rows * a.dim * 4) : 0, md = A.splits > 1 ? up16(A.splits * rows * 8) : 0;
+    const uint64_t lse = a.account && !a.lse ? up16(rows * 4) : 0;
+    uint8_t *w = (uint8_t *)a.workspace;
+    A.part = (float *)w;
+    A.md = (float2 *)(w + part);
+    A.lse = a.lse ? a.lse : a.account ? (float *)(w + part + md) : nullptr;
+    bytes = part + md + lse;
+    return true;
+}
+
+// ---- eviction
+bool select_ok(const qxg_kv_select_args *p, const Err &fail) {
+    if (!p) return fail("invalid argument");
+    if (!p->groups) return fail("groups must be positive");
+    if (!p->positions || p->positions > 0x7fffffffu || p->max_len > 0x7fffffffu) return fail("positions and max_len must be below 2^31");
+    if (!p->budget) return fail("budget must be positive");
+    if ((uint64_t)p->sinks + p->recent > p->budget) return fail("sinks + recent exceed the budget");
+    return true;
+}
+bool compact_plan(const qxg_kv_compact_args *p, uint64_t &bytes, const Err &fail) {
+    if (!p) return fail("invalid argument");
+    if (!p->groups || p->groups > 65535) return fail("groups must be between 1 and 65535");
+    if (!p->positions || p->positions > 0x7fffffffu) return fail("positions must be below 2^31");
+    if (!p->slots) return fail("slots must be positive");
+    if (p->first >= p->positions) return fail("first is outside the cache");
+    if (!p->row_bytes || p->row_bytes % 16 || p->row_bytes > 4096) return fail("row_bytes must be a multiple of 16 up to 4096");
+    if (p->kv_group % 16 || p->kv_row % 16) return fail("the strides of k and v must be multiples of 16 bytes");
+    if (p->kv_row < p->row_bytes) return fail("the rows of k and v overlap");
+    if (!p->account != !p->account_out) return fail("account and account_out go together");
+    if (p->account && p->account == p->account_out) return fail("account_out must be another array than account");
+    bytes = 0;
+    return true;
+}
+
+// ---- logits
+bool adjust_plan(const qxg_adjust_logits_args *p, QxsArgs &A, uint64_t &bytes, const Err &fail) {
+    if (!p) return fail("invalid argument");
+    const qxg_adjust_logits_args &a = A.a = *p;
+    if (!type_size(a.type)) return fail("unsupported value type %u", a.type);
+    if (!a.rows || a.rows > 65535) return fail("rows must be between 1 and 65535");
+    if (!a.vocab || a.vocab > 0x7fffffffu) return fail("vocab must be between 1 and 2^31 - 1");
+    if (a.top_n > QXG_MAX_TOPN) return fail("top_n must be at most %u", QXG_MAX_TOPN);
+    if (a.biases > 1024) return fail("biases must be at most 1024");
+    if (a.rows > 1 && (a.logits_row < a.vocab || a.out_row < a.vocab)) return fail("rows of logits or out overlap");
+    if (a.logits == a.out && a.rows > 1 && a.logits_row != a.out_row) return fail("in place, the row strides must be equal");
+    if (a.history && !a.history_slots) return fail("history without slots");
+    if (!a.history && (a.history_lens || a.prompt_lens)) return fail("history_lens or prompt_lens without history");
+    if (!a.bias_ids != !a.bias_values || !a.bias_ids != !a.biases) return fail("bias_ids, bias_values and biases go together");
+    if (!a.mask != !a.masks || (!a.mask && a.mask_rows)) return fail("mask, masks and mask_rows go together");
+    if (a.mask && !a.mask_rows && a.masks < a.rows) return fail("fewer masks than rows without mask_rows");
+    if (!a.top_n != !a.top_ids || (!a.top_n && a.top_logits)) return fail("top_n, top_ids and top_logits go together");
+    A.slices = (a.vocab + QXS_SLICE - 1) / QXS_SLICE;
+    A.words = (a.vocab + 31) / 32;
+    const uint64_t keys = up16((uint64_t)a.rows * A.slices * a.top_n * 8), ms = up16((uint64_t)a.rows * A.slices * 8);
+    A.keys = (uint64_t *)a.workspace;
+    A.ms = (float2 *)((uint8_t *)a.workspace + keys);
+    bytes = keys + ms;
+    return true;
+}
+bool workspace_ok(const void *p, uint64_t have, uint64_t need, const Err &fail) {
+    return !need || (p && have >= need) || fail("the workspace holds %llu bytes; this call needs %llu", (unsigned long long)(p ? have : 0), (unsigned long long)need);
+}
+}  // namespace
+
+extern "C" {
+
+int qxg_tree_attention(qxg_ctx *c, const qxg_tree_attention_args *p, void *stream, int wait, char *err, uint64_t err_len) {
+    const Err fail{err, err_len};
+    QxaArgs A{};
+    uint64_t need = 0;
+    if (!tree_plan(p, A, need, fail)) return 0;
+    const Arg args[] = {{p->q, "q", true, 16}, {p->k, "k", true, 16}, {p->v, "v", true, 16}, {p->kscale, "kscale", true, 4},
+                        {p->vscale, "vscale", true, 4}, {p->lens, "lens", true, 4}, {p->counts, "counts", false, 4}, {p->mask, "mask", false, 4},
+                        {p->out, "out", true, 16}, {p->lse, "lse", false, 4}, {p->account, "account", false, 4},
+                        {p->workspace, "workspace", false, 16}};
+    if (!pointers_ok(args, fail) || !workspace_ok(p->workspace, p->workspace_bytes, need, fail)) return 0;
+    return on_device(c, args, (hipStream_t)stream, wait, fail, [&] { qxa_launch(A, (hipStream_t)stream); });
+}
+uint64_t qxg_tree_attention_workspace(const qxg_tree_attention_args *p) {
+    QxaArgs A{};
+    uint64_t need = 0;
+    return tree_plan(p, A, need, Err{}) ? need : 0;
+}
+
+int qxg_kv_select(qxg_ctx *c, const qxg_kv_select_args *p, void *stream, int wait, char *err, uint64_t err_len) {
+    const Err fail{err, err_len};
+    if (!select_ok(p, fail)) return 0;
+    const Arg args[] = {{p->account, "account", true, 4}, {p->lens, "lens", true, 4}, {p->keep, "keep", true, 4}, {p->kept, "kept", true, 4}};
+    if (!pointers_ok(args, fail)) return 0;
+    return on_device(c, args, (hipStream_t)stream, wait, fail, [&] { qxe_launch_select(*p, (hipStream_t)stream); });
+}
+
+int qxg_kv_compact(qxg_ctx *c, const qxg_kv_compact_args *p, void *stream, int wait, char *err, uint64_t err_len) {
+    const Err fail{err, err_len};
+    uint64_t need = 0;
+    if (!compact_plan(p, need, fail)) return 0;
+    const Arg args[] = {{p->k, "k", true, 16}, {p->v, "v", true, 16}, {p->kscale, "kscale", true, 4}, {p->vscale, "vscale", true, 4},
+                        {p->keep, "keep", true, 4}, {p->kept, "kept", true, 4}, {p->account, "account", false, 4},
+                        {p->account_out, "account_out", false, 4}, {p->workspace, "workspace", false, 16}};
+    if (!pointers_ok(args, fail) || !workspace_ok(p->workspace, p->workspace_bytes, need, fail)) return 0;
+    return on_device(c, args, (hipStream_t)stream, wait, fail, [&] { qxe_launch_compact(*p, (hipStream_t)stream); });
+}
+uint64_t qxg_kv_compact_workspace(const qxg_kv_compact_args *p) {
+    uint64_t need = 0;
+    return compact_plan(p, need, Err{}) ? need : 0;
+}
+
+int qxg_adjust_logits(qxg_ctx *c, const qxg_adjust_logits_args *p, void *stream, int wait, char *err, uint64_t err_len) {
+    const Err fail{err, err_len};
+    QxsArgs A{};
+    uint64_t need = 0;
+    if (!adjust_plan(p, A, need, fail)) return 0;
+    const uint32_t size = type_size(p->type);
+    const Arg args[] = {{p->logits, "logits", true, size}, {p->out, "out", true, size}, {p->history, "history", false, 4},
+                        {p->history_lens, "history_lens", false, 4}, {p->prompt_lens, "prompt_lens", false, 4},
+                        {p->penalties, "penalties", false, 4}, {p->temperature, "temperature", false, 4}, {p->bias_ids, "bias_ids", false, 4},
+                        {p->bias_values, "bias_values", false, 4}, {p->mask, "mask", false, 4}, {p->mask_rows, "mask_rows", false, 4},
+                        {p->top_ids, "top_ids", false, 4}, {p->top_logits, "top_logits", false, 4}, {p->lse, "lse", false, 4},
+                        {p->workspace, "workspace", false, 16}};
+    if (!pointers_ok(args, fail) || !workspace_ok(p->workspace, p->workspace_bytes, need, fail)) return 0;
+    return on_device(c, args, (hipStream_t)stream, wait, fail, [&] { qxs_launch(A, (hipStream_t)stream); });
+}
+uint64_t qxg_adjust_logits_workspace(const qxg_adjust_logits_args *p) {
+    QxsArgs A{};
+    uint64_t need = 0;
+    return adjust_plan(p, A, need, Err{}) ? need : 0;
+}
+
+}  // extern "C"

@@ -86,4 +86,32 @@ DEV void a_read(uint4 (&ah)[MT], uint4 (&al)[MT], const uint4 *buf, const ALane 
         if (R > 16) al[mt] = *reinterpret_cast<const uint4 *>(p + mt * 4096 + a.at[2 * (s & 1) + 1]);
     }
 }
+
+DEV float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+DEV uint4 i8x8_to_f16(uint32_t vx, uint32_t vy) {   // 8 int8 -> 8 exact fp16 (bias 0x64 trick: 1024 + (b ^ 0x80) - 1152)
+    const h2v bias = {(_Float16)1152.0f, (_Float16)1152.0f};
+    const uint32_t x = vx ^ 0x80808080u, y = vy ^ 0x80808080u;
+    const uint32_t c = 0x64646464u;
+    auto cv = [&](uint32_t w) { return __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2v, w) - bias); };
+    return make_uint4(cv(perm(c, x, 0x04010400u)), cv(perm(c, x, 0x04030402u)), cv(perm(c, y, 0x04010400u)),
+                      cv(perm(c, y, 0x04030402u)));
+}
+DEV void split8(const float *v, float sc, uint4 &hi, uint4 &lo) {   // v * sc = hi + lo (+ 2^-22 rel)
+    h8v h, l;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float a = v[i] * sc;
+        const _Float16 t = (_Float16)a;
+        h[i] = t;
+        l[i] = (_Float16)(a - (float)t);
+    }
+    hi = __builtin_bit_cast(uint4, h);
+    lo = __builtin_bit_cast(uint4, l);
+}
+// 2^(k - e) with |v| = f * 2^e, f in [0.5, 1); 1 for zero, subnormal and non-finite v
+DEV float pow2_scale(float v, int k) {
+    const int e = (int)((__float_as_uint(v) >> 23) & 255u);
+    const int s = 127 + k + 126 - e;   // exponent field of the result
+    return e == 0 || e == 255 ? 1.0f : __uint_as_float((uint32_t)(s < 1 ? 1 : s > 254 ? 254 : s) << 23);
+}
 }  // namespace

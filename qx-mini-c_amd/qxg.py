@@ -3,7 +3,9 @@
 Loads lib/libqxg.so and lib/libqxhost.so built in-tree by the Makefile next to
 this file; raises if they are missing (there is no fallback path)."""
 import ctypes
+import functools
 import os
+import struct
 
 import numpy as np
 
@@ -100,6 +102,10 @@ _sig(_g, "qxg_decode_head_sums", [vp, u32, vp, *ERR])
 _sig(_g, "qxg_decode_final_norm", [vp, vp, *ERR])
 _sig(_g, "qxg_kv_read_position", [vp, u32, u32, vp, vp, vp, vp, *ERR])
 _sig(_g, "qxg_device_bytes", [vp], u64)
+for _name in ("qxg_tree_attention", "qxg_kv_select", "qxg_kv_compact", "qxg_adjust_logits"):
+    _sig(_g, _name, [vp, cp, vp, c_int, *ERR])
+for _name in ("qxg_tree_attention_workspace", "qxg_kv_compact_workspace", "qxg_adjust_logits_workspace"):
+    _sig(_g, _name, [cp], u64)
 _sig(_g, "qxg_profile_kernel", [vp, c_int])
 _sig(_g, "qxg_profile_result", [vp, ctypes.POINTER(u32), ctypes.POINTER(c_double)])
 _sig(_h, "qxgen_write", [cp, ctypes.POINTER(GenSpec), ctypes.POINTER(u64), *ERR])
@@ -156,6 +162,89 @@ def kvsnap_read(path, layers, ctx, seed):
                               ctypes.byref(nt), err, 512):
         raise QxgError(err.value.decode())
     return k, v, ks, vs, pos.value, nt.value
+
+
+# ---- operators on device memory: device arrays and the argument structs of include/qxg.h
+#
+# A device array is a torch tensor on the GPU, or any object with its data_ptr(), shape, stride() (in
+# elements) and dtype.  torch brings a HIP runtime of its own: import it before this module, so that both
+# use that one (memory of another runtime is refused).
+NO_TOKEN = 0xffffffff
+_TREE = struct.Struct("=12Q9Q8I2f")
+_SELECT = struct.Struct("=4Q2Q6I")
+_COMPACT = struct.Struct("=9Q8Q5I4x")
+_ADJUST = struct.Struct("=15Q4Q7I4x")
+_KINDS = {}   # dtype -> "f32", ...
+_NAMES = {"float32": "f32", "float16": "f16", "bfloat16": "bf16", "int32": "i32", "uint32": "i32", "int8": "i8", "uint8": "u8"}
+_VALUE_TYPES = {"f32": 0, "f16": 1, "bf16": 30}   # GGML's numbers
+_SIZES = {"f32": 4, "f16": 2, "bf16": 2}
+
+
+def _kind(t):
+    k = _KINDS.get(t.dtype)
+    if k is None:
+        k = _KINDS[t.dtype] = _NAMES.get(str(t.dtype).rpartition(".")[2], str(t.dtype))
+    return k
+
+
+def _dense(shape):
+    """The strides of a contiguous array."""
+    out, n = [], 1
+    for d in reversed(shape):
+        out.append(n)
+        n *= d
+    return tuple(reversed(out))
+
+
+def _arr(t, name, kind, shape, inner=None):
+    """Address of a device array of that kind and shape, its last `inner` dimensions (all of them if
+    None) contiguous; 0 for None."""
+    if t is None:
+        return 0
+    if _kind(t) != kind:
+        raise ValueError(f"{name} has dtype {t.dtype}, not {kind}")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, not {shape}")
+    rest = shape if inner is None else shape[len(shape) - inner:]
+    if rest and tuple(t.stride())[len(shape) - len(rest):] != _dense(rest):
+        if any(d != 1 and s != e for d, s, e in zip(rest, tuple(t.stride())[len(shape) - len(rest):], _dense(rest))):
+            raise ValueError(f"{name} is not contiguous in its last {len(rest)} dimensions")
+    return t.data_ptr()
+
+
+def _sized(t, name):
+    """(address, bytes) of a workspace: a contiguous uint8 array."""
+    if t is None:
+        return 0, 0
+    return _arr(t, name, "u8", tuple(t.shape)), t.shape[0]
+
+
+def _tree_pack(ptrs, strides, kind, q_shape, k_shape, max_len, scale, decay, account_stride=0):
+    if len(q_shape) != 4 or len(k_shape) != 4:
+        raise ValueError("q has the dimensions [batch, nodes, heads, dim], k and v [batch, positions, kv_heads, dim]")
+    batch, nodes, heads, dim = q_shape
+    positions, kv_heads = k_shape[1:3]
+    if max_len is None:
+        max_len = positions
+    if scale is None:
+        scale = dim ** -0.5
+    return _TREE.pack(*ptrs, *strides, account_stride, _VALUE_TYPES[kind], batch, nodes, heads, kv_heads, dim, positions, max_len, scale, decay)
+
+
+@functools.lru_cache(maxsize=256)
+def _tree_workspace(q_shape, k_shape, max_len, account):
+    return _g.qxg_tree_attention_workspace(_tree_pack([0] * 10 + [16 * account] + [0], [0] * 8, "f32", q_shape, k_shape, max_len, 1.0, 1.0))
+
+
+@functools.lru_cache(maxsize=256)
+def _compact_workspace(k_shape, keep_shape):
+    return _g.qxg_kv_compact_workspace(_COMPACT.pack(*[0] * 9, *[0, 0, k_shape[2]], *[0] * 5, k_shape[0], k_shape[1], keep_shape[1], 0, k_shape[2]))
+
+
+@functools.lru_cache(maxsize=256)
+def _adjust_workspace(shape, top_n):
+    rows, vocab = shape
+    return _g.qxg_adjust_logits_workspace(_ADJUST.pack(*[0] * 11, 16 if top_n else 0, 0, 16, 0, 0, vocab, vocab, 0, 0, rows, vocab, 0, 0, 0, top_n))
 
 
 class MemModel:
@@ -420,6 +509,105 @@ class Context:
         out = np.zeros(292 * (len(x) // 256), np.uint8)
         self._check(_g.qxg_q8k_quantize(self._c, x.ctypes.data_as(vp), len(x), out.ctypes.data_as(vp), self._err, 1024))
         return out
+
+    # ---- operators on device memory (device arrays, see above).  stream: the handle of the HIP
+    # stream to queue on (torch.cuda.current_stream().cuda_stream; 0: the default stream); wait=False
+    # returns once the work is queued.
+
+    def tree_attention_workspace(self, q_shape, k_shape, max_len=None, account=False):
+        """Bytes of workspace that tree_attention with these shapes needs."""
+        return _tree_workspace(tuple(q_shape), tuple(k_shape), max_len, bool(account))
+
+    def tree_attention(self, q, k, v, kscale, vscale, lens, out, mask=None, counts=None, lse=None, account=None, decay=1.0,
+                       max_len=None, scale=None, workspace=None, stream=0, wait=True):
+        """qxg_tree_attention: q, out [batch, nodes, heads, dim] f32, f16 or bf16; k, v [batch, positions,
+        kv_heads, dim] int8 with scales [batch, positions] f32; lens, counts [batch] int32; mask [batch,
+        nodes, words] int32 bits (None: node i sees nodes 0 .. i); lse [batch, nodes, heads] f32; account
+        [batch, positions] f32.  scale: 1 / sqrt(dim) unless given."""
+        kind, qs, ks = _kind(q), tuple(q.shape), tuple(k.shape)
+        if kind not in _VALUE_TYPES:
+            raise ValueError(f"q has dtype {q.dtype}, not f32, f16 or bf16")
+        if len(qs) != 4 or len(ks) != 4 or ks[0] != qs[0] or ks[3] != qs[3]:
+            raise ValueError("q has the dimensions [batch, nodes, heads, dim], k and v [batch, positions, kv_heads, dim]")
+        batch, nodes, heads, _ = qs
+        bp, q_st, o_st, k_st = ks[:2], q.stride(), out.stride(), k.stride()
+        if tuple(v.stride()) != tuple(k_st):
+            raise ValueError("k and v have different strides")
+        ws, wn = _sized(workspace, "workspace")
+        sc_st = kscale.stride()[0]
+        if vscale.stride()[0] != sc_st:
+            raise ValueError("kscale and vscale have different strides")
+        args = _tree_pack(
+            (_arr(q, "q", kind, qs, 2), _arr(k, "k", "i8", ks, 2), _arr(v, "v", "i8", ks, 2), _arr(kscale, "kscale", "f32", bp, 1),
+             _arr(vscale, "vscale", "f32", bp, 1), _arr(lens, "lens", "i32", (batch,)), _arr(counts, "counts", "i32", (batch,)),
+             _arr(mask, "mask", "i32", (batch, nodes, (nodes + 31) // 32)), _arr(out, "out", kind, qs, 2),
+             _arr(lse, "lse", "f32", (batch, nodes, heads)), _arr(account, "account", "f32", bp, 1), ws),
+            (wn, q_st[0], q_st[1], o_st[0], o_st[1], k_st[0], k_st[1], sc_st),
+            kind, qs, ks, max_len, scale, decay, account.stride()[0] if account is not None else 0)
+        self._check(_g.qxg_tree_attention(self._c, args, stream, wait, self._err, 1024))
+
+    def kv_select(self, account, lens, keep, kept, sinks=0, recent=0, max_len=None, stream=0, wait=True):
+        """qxg_kv_select: account [groups, positions] f32, lens [groups] int32; writes keep [groups, budget]
+        and kept [groups] int32."""
+        groups, positions = account.shape
+        args = _SELECT.pack(_arr(account, "account", "f32", (groups, positions), 1), _arr(lens, "lens", "i32", (groups,)),
+                            _arr(keep, "keep", "i32", (groups, keep.shape[1]), 1), _arr(kept, "kept", "i32", (groups,)),
+                            account.stride()[0], keep.stride()[0], groups, positions, keep.shape[1], sinks, recent,
+                            positions if max_len is None else max_len)
+        self._check(_g.qxg_kv_select(self._c, args, stream, wait, self._err, 1024))
+
+    def kv_compact_workspace(self, k_shape, keep_shape):
+        """Bytes of workspace that kv_compact with these shapes needs."""
+        return _compact_workspace(tuple(k_shape), tuple(keep_shape))
+
+    def kv_compact(self, k, v, kscale, vscale, keep, kept, account=None, account_out=None, first=0, workspace=None, stream=0, wait=True):
+        """qxg_kv_compact: k, v [groups, positions, row bytes] int8, kscale, vscale and the accounts [groups,
+        positions] f32, keep [groups, slots] and kept [groups] int32 (stride 0 over groups: one list for all)."""
+        groups, positions, row = k.shape
+        gp, st = (groups, positions), k.stride()
+        if tuple(v.stride()) != tuple(st):
+            raise ValueError("k and v have different strides")
+        if vscale.stride()[0] != kscale.stride()[0]:
+            raise ValueError("kscale and vscale have different strides")
+        ws, wn = _sized(workspace, "workspace")
+        args = _COMPACT.pack(_arr(k, "k", "i8", (*gp, row), 1), _arr(v, "v", "i8", (*gp, row), 1), _arr(kscale, "kscale", "f32", gp, 1),
+                             _arr(vscale, "vscale", "f32", gp, 1), _arr(keep, "keep", "i32", (groups, keep.shape[1]), 1),
+                             _arr(kept, "kept", "i32", (groups,), 0), _arr(account, "account", "f32", gp, 1),
+                             _arr(account_out, "account_out", "f32", gp, 1), ws, wn, st[0], st[1], kscale.stride()[0], keep.stride()[0],
+                             kept.stride()[0], account.stride()[0] if account is not None else 0,
+                             account_out.stride()[0] if account_out is not None else 0, groups, positions, keep.shape[1], first, row)
+        self._check(_g.qxg_kv_compact(self._c, args, stream, wait, self._err, 1024))
+
+    def adjust_logits_workspace(self, shape, top_n=0):
+        """Bytes of workspace that adjust_logits on [rows, vocab] logits needs."""
+        return _adjust_workspace(tuple(shape), top_n)
+
+    def adjust_logits(self, logits, out, history=None, history_lens=None, prompt_lens=None, penalties=None, temperature=None,
+                      bias_ids=None, bias_values=None, mask=None, mask_rows=None, top_ids=None, top_logits=None, lse=None,
+                      workspace=None, stream=0, wait=True):
+        """qxg_adjust_logits: logits, out [rows, vocab] f32, f16 or bf16; history [rows, slots] int32 with
+        history_lens, prompt_lens [rows] int32; penalties [rows, 3] (repetition, frequency, presence) and
+        temperature [rows] f32; bias_ids int32, bias_values f32 [rows, biases]; mask [masks, words] int32
+        bits with mask_rows [rows] int32; top_ids int32, top_logits f32 [rows, top_n]; lse [rows] f32."""
+        kind = _kind(logits)
+        if kind not in _VALUE_TYPES:
+            raise ValueError(f"logits has dtype {logits.dtype}, not f32, f16 or bf16")
+        shape = rows, vocab = tuple(logits.shape)
+        slots = history.shape[1] if history is not None else 0
+        biases = bias_ids.shape[1] if bias_ids is not None else 0
+        masks = mask.shape[0] if mask is not None else 0
+        top_n = top_ids.shape[1] if top_ids is not None else 0
+        ws, wn = _sized(workspace, "workspace")
+        args = _ADJUST.pack(
+            _arr(logits, "logits", kind, shape, 1), _arr(out, "out", kind, shape, 1), _arr(history, "history", "i32", (rows, slots), 1),
+            _arr(history_lens, "history_lens", "i32", (rows,)), _arr(prompt_lens, "prompt_lens", "i32", (rows,)),
+            _arr(penalties, "penalties", "f32", (rows, 3)), _arr(temperature, "temperature", "f32", (rows,)),
+            _arr(bias_ids, "bias_ids", "i32", (rows, biases)), _arr(bias_values, "bias_values", "f32", (rows, biases)),
+            _arr(mask, "mask", "i32", (masks, (vocab + 31) // 32)), _arr(mask_rows, "mask_rows", "i32", (rows,)),
+            _arr(top_ids, "top_ids", "i32", (rows, top_n)), _arr(top_logits, "top_logits", "f32", (rows, top_n)),
+            _arr(lse, "lse", "f32", (rows,)), ws, wn, logits.stride()[0], out.stride()[0], history.stride()[0] if slots else 0,
+            _VALUE_TYPES[kind], rows, vocab, slots, biases, masks, top_n)
+        self._check(_g.qxg_adjust_logits(self._c, args, stream, wait, self._err, 1024))
 
     def time_kernel(self, which, layer=0, iters=20):
         ms = c_float()
