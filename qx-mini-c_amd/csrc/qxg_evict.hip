@@ -3,135 +3,326 @@
 #include "qxg_ops.h"
 
 namespace {
-// Weights as unsigned keys in their order; NaN as -inf, -0 as +0
-DEV uint32_t weight_key(float w) {
+// Weights as unsigned numbers in their order, 1 or more; NaN as -inf, -0 as +0
+DEV uint32_t weight_rank(float w) {
     const uint32_t u = __float_as_uint(w == w ? w + 0.0f : -INFINITY);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
-// exclusive prefix of a flag count over the block's 1024 threads (16 waves), and the total
-DEV uint32_t block_rank(bool f, uint32_t *s_w, uint32_t &total) {
-    const uint64_t m = __ballot(f);
+// sum of a over the block's 16 waves' lanes before this thread, and over all of them
+DEV uint2 block_before(uint2 a, uint2 *s_w, uint2 &all) {
     const int wave = wave_id(), lane = threadIdx.x & 63;
-    __syncthreads();
-    if (lane == 0) s_w[wave] = __popcll(m);
-    __syncthreads();
-    uint32_t before = 0, all = 0;
-    for (int w = 0; w < 16; ++w) {
-        before += w < wave ? s_w[w] : 0u;
-        all += s_w[w];
+    uint2 v = a;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t x = (uint32_t)__shfl_up((int)v.x, o), y = (uint32_t)__shfl_up((int)v.y, o);
+        if (lane >= o) { v.x += x; v.y += y; }
     }
-    total = all;
-    return before + __popcll(m & ((1ull << lane) - 1ull));
+    if (lane == 63) s_w[wave] = v;
+    __syncthreads();
+    uint2 before = make_uint2(0, 0);
+    all = make_uint2(0, 0);
+#pragma unroll
+    for (int w = 0; w < 16; ++w) {
+        const uint2 x = s_w[w];
+        if (w < wave) { before.x += x.x; before.y += x.y; }
+        all.x += x.x;
+        all.y += x.y;
+    }
+    return make_uint2(before.x + v.x - a.x, before.y + v.y - a.y);
+}
+struct Group { uint32_t len, kept; };
+DEV Group group_of(const qxg_kv_select_args &A, uint32_t g) {
+    Group x;
+    x.len = min(A.lens[g], A.positions);
+    x.kept = min(x.len, A.budget);
+    return x;
+}
+// rank of position p: the largest number for those kept in any case, 0 behind the end
+DEV uint32_t rank_at(const qxg_kv_select_args &A, float w, uint32_t p, uint32_t len) {
+    return p >= len ? 0u : p < A.sinks || p >= len - A.recent ? ~0u : weight_rank(w);
 }
 }  // namespace
 
-// A workgroup a group.  The smallest key that is kept is found a byte at a time from the top (a
-// histogram of the keys that share the bytes found so far), then the positions are listed in order.
-extern "C" __global__ __launch_bounds__(1024) void qxe_select(qxg_kv_select_args A) {
-    __shared__ uint32_t s_hist[16][256], s_w[16], s_key, s_need;
-    const int tid = threadIdx.x;
-    const uint32_t g = blockIdx.x, len = min(A.lens[g], A.positions), kept = min(len, A.budget);
+namespace {
+// The smallest rank among the block's k[] (E a thread, 0: none) that `want` of them reach, found a bit at a time
+// from bit `top` down below the bits of `least`; `above`: how many are larger.  The count of ranks that
+// reach it is one ballot a wave and register.
+template <int E>
+DEV uint32_t block_nth(const uint32_t (&k)[E], uint32_t want, uint32_t least, int top, uint32_t (&s_n)[2][16], uint32_t &above) {
+    const int lane = threadIdx.x & 63, wave = wave_id();
+    above = 0;
+#pragma unroll 1
+    for (int b = top; b >= 0; --b) {
+        const uint32_t at = least | 1u << b;
+        uint32_t n = 0;
+#pragma unroll
+        for (int i = 0; i < E; ++i) n += (uint32_t)__popcll(__ballot(k[i] >= at));
+        if (lane == 0) s_n[b & 1][wave] = n;
+        __syncthreads();   // (the other half is written next, so one barrier a bit is enough)
+        n = s_n[b & 1][lane & 15];
+        n += (uint32_t)dppi<DPP_XOR1>((int)n); n += (uint32_t)dppi<DPP_XOR2>((int)n);
+        n += (uint32_t)dppi<DPP_ROR4>((int)n); n += (uint32_t)dppi<DPP_ROR8>((int)n);
+        if (n >= want) least = at;
+        else above = n;
+    }
+    return least;
+}
+// Lists the kept ones of positions p0 .. p0 + E - 1 of every thread: ranks above `least`, and the lowest `need`
+// equal ones.  done: how many of either lie before the block's first position.
+template <int E>
+DEV void list_kept(const uint32_t (&k)[E], uint32_t p0, uint32_t least, uint32_t need, uint2 &done, uint2 *s_w, uint32_t *keep) {
+    uint2 own = make_uint2(0, 0), all;
+#pragma unroll
+    for (int i = 0; i < E; ++i) { own.x += k[i] > least; own.y += k[i] == least; }
+    uint2 at = block_before(own, s_w, all);
+    at.x += done.x;
+    at.y += done.y;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        const bool gt = k[i] > least, eq = k[i] == least;
+        if (gt || (eq && at.y < need)) keep[at.x + min(at.y, need)] = p0 + i;
+        at.x += gt;
+        at.y += eq;
+    }
+    done.x += all.x;
+    done.y += all.y;
+}
+template <int E>
+DEV void load_ranks(const qxg_kv_select_args &A, const float *acc, uint32_t p0, uint32_t len, uint32_t (&k)[E]) {
+    float w[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) w[i] = p0 + i < len ? acc[p0 + i] : 0.0f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) k[i] = rank_at(A, w[i], p0 + i, len);
+}
+}  // namespace
+
+// Up to 1024 E positions, a workgroup a group: a thread holds E neighbouring positions' ranks in registers.  The
+// counts of its 32 steps bound it.  (Byte-wise histograms in LDS, their bins searched by one thread: 26 us
+// for 700 positions.)
+template <int E>
+__global__ __launch_bounds__(1024) void qxe_select(qxg_kv_select_args A) {
+    __shared__ uint32_t s_n[2][16];
+    __shared__ uint2 s_w[16];
+    const uint32_t g = blockIdx.x;
+    const Group G = group_of(A, g);
     uint32_t *keep = A.keep + g * A.keep_group;
-    const float *acc = A.account + g * A.account_group;
-    if (tid == 0) A.kept[g] = kept;
-    if (len <= A.budget) {
-        for (uint32_t p = tid; p < len; p += 1024) keep[p] = p;
+    if (threadIdx.x == 0) A.kept[g] = G.kept;
+    if (G.len <= A.budget) {
+        for (uint32_t p = threadIdx.x; p < G.len; p += 1024) keep[p] = p;
         return;
     }
-    const uint32_t lo = A.sinks, hi = len - A.recent;
-    uint32_t need = A.budget - A.sinks - A.recent, key = 0;
-    if (need) {
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            for (int i = tid; i < 16 * 256; i += 1024) (&s_hist[0][0])[i] = 0;
-            __syncthreads();
-            for (uint32_t p = lo + tid; p < hi; p += 1024) {
-                const uint32_t k = weight_key(acc[p]);
-                if (shift == 24 || (k >> (shift + 8)) == (key >> (shift + 8))) atomicAdd(&s_hist[tid >> 6][(k >> shift) & 255], 1u);
-            }
-            __syncthreads();
-            if (tid < 256) {
-                uint32_t n = 0;
-                for (int w = 0; w < 16; ++w) n += s_hist[w][tid];
-                s_hist[0][tid] = n;
-            }
-            __syncthreads();
-            if (tid == 0) {
-                int d = 255;
-                while (s_hist[0][d] < need) need -= s_hist[0][d--];
-                s_key = key | (uint32_t)d << shift;
-                s_need = need;
-            }
-            __syncthreads();
-            key = s_key;
-            need = s_need;
-            __syncthreads();
-        }
-    } else {
-        key = ~0u;   // none of the middle
+    uint32_t k[E], above;
+    load_ranks<E>(A, A.account + g * A.account_group, threadIdx.x * E, G.len, k);
+    const uint32_t least = block_nth<E>(k, A.budget, 0, 31, s_n, above);
+    uint2 done = make_uint2(0, 0);
+    list_kept<E>(k, threadIdx.x * E, least, A.budget - above, done, s_w, keep);
+}
+
+// More positions than registers hold: a histogram of the ranks' top 11 bits (each bin 16 times, by lane, as
+// equal bins of a wave's lanes would be added one after the other), then the ranks of the bin that holds
+// the smallest kept one go to LDS, where its other bits are found as above; a bin of more than ROOM ranks
+// is halved further by another histogram.  The account is read three times, from the caches after the
+// first: one workgroup's loads bound it.
+__global__ __launch_bounds__(1024) void qxe_select_long(qxg_kv_select_args A) {
+    constexpr int E = 16, BINS = 2048, COPIES = 16, ROOM = 16384;
+    __shared__ uint32_t s_hist[BINS * COPIES], s_n[2][16], s_digit, s_above, s_count;
+    __shared__ uint2 s_w[16];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const uint32_t g = blockIdx.x;
+    const Group G = group_of(A, g);
+    uint32_t *keep = A.keep + g * A.keep_group;
+    const float *acc = A.account + g * A.account_group;
+    if (tid == 0) A.kept[g] = G.kept;
+    if (G.len <= A.budget) {
+        for (uint32_t p = tid; p < G.len; p += 1024) keep[p] = p;
+        return;
     }
-    uint32_t at = 0, equal = 0;
-    for (uint32_t p0 = 0; p0 < len; p0 += 1024) {
-        const uint32_t p = p0 + tid;
-        const bool mid = p >= lo && p < hi;
-        const uint32_t k = mid ? weight_key(acc[p]) : 0u;
-        uint32_t eqs, ns;
-        const uint32_t er = block_rank(mid && k == key, s_w, eqs);
-        const bool f = p < len && (!mid || k > key || (k == key && equal + er < need));
-        const uint32_t r = block_rank(f, s_w, ns);
-        if (f) keep[at + r] = p;
-        at += ns;
-        equal += eqs;
+    uint32_t least = 0, above = 0;   // bits found, and ranks above them
+    int shift = 32;                  // bits still to find
+    while (shift > 0) {
+        const int bits = min(shift, 11);
+        for (int i = tid; i < BINS * COPIES / 4; i += 1024) reinterpret_cast<uint4 *>(s_hist)[i] = make_uint4(0, 0, 0, 0);
+        __syncthreads();
+        for (uint32_t p0 = 0; p0 < G.len; p0 += 1024 * E) {
+            float w[E];
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                const uint32_t p = p0 + 1024 * i + tid;
+                w[i] = p < G.len ? acc[p] : 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                const uint32_t p = p0 + 1024 * i + tid, k = rank_at(A, w[i], p, G.len);
+                if (p < G.len && (shift == 32 || k >> shift == least >> shift))
+                    atomicAdd(&s_hist[((k >> (shift - bits)) & ((1u << bits) - 1u)) * COPIES + (lane & 15)], 1u);
+            }
+        }
+        __syncthreads();
+        // the bins from the top: thread t has bins 2047 - 2 t and 2046 - 2 t
+        uint32_t n[2] = {0, 0};
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int c = 0; c < COPIES; ++c) n[i] += s_hist[(BINS - 1 - 2 * tid - i) * COPIES + ((c + tid) & 15)];
+        uint2 all;
+        const uint32_t before = above + block_before(make_uint2(n[0] + n[1], 0), s_w, all).x;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t b = before + (i ? n[0] : 0u);
+            if (b < A.budget && b + n[i] >= A.budget) {
+                s_digit = BINS - 1 - 2 * tid - i;
+                s_above = b;
+                s_count = n[i];
+            }
+        }
+        __syncthreads();
+        shift -= bits;
+        least |= s_digit << shift;
+        above = s_above;
+        const uint32_t count = s_count;
+        __syncthreads();
+        if (shift && count <= ROOM) {
+            if (tid == 0) s_count = 0;
+            __syncthreads();
+            for (uint32_t p0 = 0; p0 < G.len; p0 += 1024 * E) {
+                float w[E];
+#pragma unroll
+                for (int i = 0; i < E; ++i) {
+                    const uint32_t p = p0 + 1024 * i + tid;
+                    w[i] = p < G.len ? acc[p] : 0.0f;
+                }
+#pragma unroll
+                for (int i = 0; i < E; ++i) {
+                    const uint32_t p = p0 + 1024 * i + tid, k = rank_at(A, w[i], p, G.len);
+                    if (p < G.len && k >> shift == least >> shift) s_hist[atomicAdd(&s_count, 1u)] = k;   // (< count, in any order)
+                }
+            }
+            __syncthreads();
+            uint32_t k[E], more;
+#pragma unroll
+            for (int i = 0; i < E; ++i) k[i] = (uint32_t)(1024 * i + tid) < count ? s_hist[1024 * i + tid] : 0u;
+            least = block_nth<E>(k, A.budget - above, least, shift - 1, s_n, more);
+            above += more;
+            shift = 0;
+        }
+    }
+    uint2 done = make_uint2(0, 0);
+    uint32_t k[E];
+    load_ranks<E>(A, acc, tid * E, G.len, k);
+    for (uint32_t p0 = tid * E; p0 < (G.len + 1024 * E - 1) / (1024 * E) * (1024 * E); p0 += 1024 * E) {
+        uint32_t next[E];
+        load_ranks<E>(A, acc, p0 + 1024 * E, G.len, next);
+        list_kept<E>(k, p0, least, A.budget - above, done, s_w, keep);
+        __syncthreads();   // s_w is read
+#pragma unroll
+        for (int i = 0; i < E; ++i) k[i] = next[i];
     }
 }
 
-// Rows moved in place.  A workgroup takes a strip of 128 bytes of a group's K or V rows (or its scales
-// and account) and goes through the list in order, 256 rows at a time: all are read before any is
-// written, and no later row's source lies below what an earlier step writes.
-extern "C" __global__ __launch_bounds__(256) void qxe_compact(qxg_kv_compact_args A) {
+// Rows moved in place.  Tiles of R rows (32 KB of K, or one row) are claimed in order: a workgroup reads its tile's
+// sources, says so, waits until the earlier tiles of its group whose sources lie where it is about to
+// write have been read, and writes.  A claimed tile reads without waiting, and waits only for tiles
+// claimed before it, so every wait ends (a bound on the polls ends it also where two calls share a workspace,
+// which is not allowed).  Each row is read and written once.  (Strips of columns, each walked in order by
+// one workgroup, left most of the GPU idle: 989 us for 3 groups of 32768 rows.)  state: the ticket, then
+// a word a tile.
+extern "C" __global__ __launch_bounds__(256) void qxe_clear(uint32_t *state, uint32_t n) {
+    for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < n; i += gridDim.x * 256) state[i] = 0;
+}
+extern "C" __global__ __launch_bounds__(256) void qxe_compact(QxeCompact C) {
+    const qxg_kv_compact_args &A = C.a;
+    constexpr int U = QXE_UNITS / 256;
+    __shared__ uint32_t s_ticket, s_keep[QXE_UNITS];
     const int tid = threadIdx.x;
-    const uint32_t g = blockIdx.y, strips = (A.row_bytes + 127) / 128;
+    if (tid == 0) s_ticket = __hip_atomic_fetch_add(C.state, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    const uint32_t ticket = s_ticket;
+    if (ticket >= A.groups * C.tiles) return;
+    const uint32_t g = ticket / C.tiles, tile = ticket % C.tiles, i0 = tile * C.rows;
     const uint32_t n = min(A.kept[g * A.kept_group], min(A.slots, A.positions - A.first));
-    const uint32_t *keep = A.keep + g * A.keep_group;
-    constexpr int U = 8;
-    if (blockIdx.x < 2 * strips) {
-        const uint32_t strip = blockIdx.x >> 1, byte = strip * 128 + (tid & 7) * 16;
-        uint8_t *base = (uint8_t *)(blockIdx.x & 1 ? A.v : A.k) + g * A.kv_group + byte;
-        const bool in = byte < A.row_bytes;
-        for (uint32_t i0 = 0; i0 < n; i0 += 32 * U) {
-            uint4 x[U];
-            bool ok[U];
+    if (i0 >= n) return;
+    const uint32_t *keep = A.keep + g * A.keep_group, here = min(C.rows, n - i0), to = A.first + i0;
+    uint32_t *read = C.state + 1 + g * C.tiles;   // [tile] 1: its sources are in registers
+    bool moves = false;
+    for (uint32_t i = tid; i < here; i += 256) {
+        const uint32_t p = keep[i0 + i];
+        s_keep[i] = p;
+        moves = moves || (p != to + i && p < A.positions);
+    }
+    const bool any = __syncthreads_or(moves);
+    // the scales and accounts of rows tid, tid + 256, ..., and 16-byte units of the rows
+    const float *acc = A.account ? A.account + g * A.account_group : nullptr;
+    float *ks = A.kscale + g * A.scale_group, *vs = A.vscale + g * A.scale_group;
+    if (acc) {
+        float *out = A.account_out + g * A.account_out_group + to;
+        for (uint32_t i = tid; i < here; i += 256)
+            if (s_keep[i] < A.positions) out[i] = acc[s_keep[i]];
+    }
+    nt4 k[U], v[U];
+    float sk[U], sv[U];
+    uint64_t dst[U];
+    if (any) {
+        const uint8_t *kb = (const uint8_t *)A.k + g * A.kv_group, *vb = (const uint8_t *)A.v + g * A.kv_group;
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const uint32_t i = i0 + 32 * u + (tid >> 3), p = i < n ? keep[i] : ~0u;
-                ok[u] = in && p < A.positions && p != A.first + i;
-                if (ok[u]) x[u] = *reinterpret_cast<const uint4 *>(base + p * A.kv_row);
+        for (int j = 0; j < U; ++j) {
+            const uint32_t x = tid + 256 * j, row = (x * C.inverse) >> 20, unit = x - row * C.units;
+            const uint32_t p = row < here ? s_keep[row] : ~0u;
+            dst[j] = ~0ull;
+            if (p < A.positions && p != to + row) {
+                const uint64_t off = p * A.kv_row + 16 * unit;
+                k[j] = *reinterpret_cast<const nt4 *>(kb + off);
+                v[j] = *reinterpret_cast<const nt4 *>(vb + off);
+                dst[j] = (to + row) * A.kv_row + 16 * unit;
             }
-            __syncthreads();
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (ok[u]) *reinterpret_cast<uint4 *>(base + (A.first + i0 + 32 * u + (tid >> 3)) * A.kv_row) = x[u];
-            __syncthreads();
+            if (256 * j < C.rows) {   // (uniform)
+                const uint32_t q = x < here ? s_keep[x] : ~0u;
+                if (q < A.positions) { sk[j] = ks[q]; sv[j] = vs[q]; }
+            }
         }
-    } else {
-        float *ks = A.kscale + g * A.scale_group, *vs = A.vscale + g * A.scale_group;
-        for (uint32_t i0 = 0; i0 < n; i0 += 256) {
-            const uint32_t i = i0 + tid, p = i < n ? keep[i] : ~0u;
-            const bool ok = p < A.positions;
-            const float a = ok ? ks[p] : 0.0f, b = ok ? vs[p] : 0.0f;
-            if (ok && A.account) A.account_out[g * A.account_out_group + A.first + i] = A.account[g * A.account_group + p];
-            __syncthreads();
-            if (ok) {
-                ks[A.first + i] = a;
-                vs[A.first + i] = b;
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the wave's loads have returned (a barrier alone does not wait for them)
+    __syncthreads();
+    if (tid == 0) __hip_atomic_store(&read[tile], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (!any) return;
+    for (uint32_t c = tile; c-- > 0;) {   // earlier tiles, the nearest first, 256 at a time
+        const bool mine = c >= (uint32_t)tid;
+        const uint32_t t = c - tid;
+        bool wait = false;
+        if (mine) {
+            wait = keep[t * C.rows + C.rows - 1] >= to;   // its last source lies at or behind the first written row
+            for (uint32_t polls = 0; wait && polls < 1u << 20; ++polls) {
+                if (__hip_atomic_load(&read[t], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) break;
+                __builtin_amdgcn_s_sleep(1);
             }
-            __syncthreads();
+        }
+        // farther tiles' sources lie lower: none of them is awaited once one of these is not
+        if (!__syncthreads_and(mine && wait)) break;
+        c -= 255;
+    }
+    uint8_t *kb = (uint8_t *)A.k + g * A.kv_group, *vb = (uint8_t *)A.v + g * A.kv_group;
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+        if (dst[j] != ~0ull) {
+            *reinterpret_cast<nt4 *>(kb + dst[j]) = k[j];
+            *reinterpret_cast<nt4 *>(vb + dst[j]) = v[j];
+        }
+        const uint32_t x = tid + 256 * j;
+        if (256 * j < C.rows && x < here && s_keep[x] < A.positions) {
+            ks[to + x] = sk[j];
+            vs[to + x] = sv[j];
         }
     }
 }
 
 void qxe_launch_select(const qxg_kv_select_args &a, hipStream_t s) {
-    hipLaunchKernelGGL(qxe_select, dim3(a.groups), dim3(1024), 0, s, a);
+    if (a.positions <= 1024) hipLaunchKernelGGL(qxe_select<1>, dim3(a.groups), dim3(1024), 0, s, a);
+    else if (a.positions <= 4096) hipLaunchKernelGGL(qxe_select<4>, dim3(a.groups), dim3(1024), 0, s, a);
+    else if (a.positions <= 16384) hipLaunchKernelGGL(qxe_select<16>, dim3(a.groups), dim3(1024), 0, s, a);
+    else hipLaunchKernelGGL(qxe_select_long, dim3(a.groups), dim3(1024), 0, s, a);
 }
-void qxe_launch_compact(const qxg_kv_compact_args &a, hipStream_t s) {
-    hipLaunchKernelGGL(qxe_compact, dim3(2 * ((a.row_bytes + 127) / 128) + 1, a.groups), dim3(256), 0, s, a);
+void qxe_launch_compact(const QxeCompact &C, hipStream_t s) {
+    const uint32_t words = 1 + C.a.groups * C.tiles;
+    hipLaunchKernelGGL(qxe_clear, dim3(std::min<uint32_t>(64, (words + 255) / 256)), dim3(256), 0, s, C.state, words);
+    hipLaunchKernelGGL(qxe_compact, dim3(C.a.groups * C.tiles), dim3(256), 0, s, C);
 }

@@ -17,16 +17,24 @@ struct QxaArgs {
 };
 void qxa_launch(const QxaArgs &A, hipStream_t s);
 
-// Eviction
+// Eviction.  A tile of the compaction is `rows` rows, QXE_UNITS 16-byte units of K (and of V) at most.
+constexpr uint32_t QXE_UNITS = 2048;
+struct QxeCompact {
+    qxg_kv_compact_args a;
+    uint32_t units, inverse;   // of a row; ceil(2^20 / units): x / units = x * inverse >> 20 for x < QXE_UNITS
+    uint32_t rows, tiles;      // of a tile; of a group
+    uint32_t *state;           // 1 + groups * tiles words
+};
 void qxe_launch_select(const qxg_kv_select_args &a, hipStream_t s);
-void qxe_launch_compact(const qxg_kv_compact_args &a, hipStream_t s);
+void qxe_launch_compact(const QxeCompact &C, hipStream_t s);
 
-// Logits.  A slice of a row leaves its top_n keys and (maximum, sum of exponentials) to the merge.
+// Logits.  Each of the 4 waves of a slice of a row leaves its top_n keys, largest first, and (maximum, sum
+// of exponentials) to the join.
 struct QxsArgs {
     qxg_adjust_logits_args a;
     uint32_t slices, words;
-    uint64_t *keys;    // [rows][slices][top_n]
-    float2 *ms;        // [rows][slices]
+    uint64_t *keys;    // [rows][slices * 4][top_n]
+    float2 *ms;        // [rows][slices * 4]
 };
 constexpr uint32_t QXS_SLICE = 4096;
 void qxs_launch(const QxsArgs &A, hipStream_t s);

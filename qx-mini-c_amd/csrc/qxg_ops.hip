@@ -113,7 +113,7 @@ bool select_ok(const qxg_kv_select_args *p, const Err &fail) {
     if ((uint64_t)p->sinks + p->recent > p->budget) return fail("sinks + recent exceed the budget");
     return true;
 }
-bool compact_plan(const qxg_kv_compact_args *p, uint64_t &bytes, const Err &fail) {
+bool compact_plan(const qxg_kv_compact_args *p, QxeCompact &C, uint64_t &bytes, const Err &fail) {
     if (!p) return fail("invalid argument");
     if (!p->groups || p->groups > 65535) return fail("groups must be between 1 and 65535");
     if (!p->positions || p->positions > 0x7fffffffu) return fail("positions must be below 2^31");
@@ -124,7 +124,14 @@ bool compact_plan(const qxg_kv_compact_args *p, uint64_t &bytes, const Err &fail
     if (p->kv_row < p->row_bytes) return fail("the rows of k and v overlap");
     if (!p->account != !p->account_out) return fail("account and account_out go together");
     if (p->account && p->account == p->account_out) return fail("account_out must be another array than account");
-    bytes = 0;
+    C.a = *p;
+    C.units = p->row_bytes / 16;
+    C.inverse = ((1u << 20) + C.units - 1) / C.units;
+    C.rows = QXE_UNITS / C.units;
+    C.tiles = (std::min(p->slots, p->positions - p->first) + C.rows - 1) / C.rows;
+    if ((uint64_t)p->groups * C.tiles >= 1u << 31) return fail("too many rows for one call");
+    C.state = (uint32_t *)p->workspace;
+    bytes = up16(4 + 4ull * p->groups * C.tiles);
     return true;
 }
 
@@ -140,6 +147,7 @@ bool adjust_plan(const qxg_adjust_logits_args *p, QxsArgs &A, uint64_t &bytes, c
     if (a.rows > 1 && (a.logits_row < a.vocab || a.out_row < a.vocab)) return fail("rows of logits or out overlap");
     if (a.logits == a.out && a.rows > 1 && a.logits_row != a.out_row) return fail("in place, the row strides must be equal");
     if (a.history && !a.history_slots) return fail("history without slots");
+    if (a.history_slots > 1u << 29) return fail("history_slots must be at most 2^29");   // (a count has 30 bits)
     if (!a.history && (a.history_lens || a.prompt_lens)) return fail("history_lens or prompt_lens without history");
     if (!a.bias_ids != !a.bias_values || !a.bias_ids != !a.biases) return fail("bias_ids, bias_values and biases go together");
     if (!a.mask != !a.masks || (!a.mask && a.mask_rows)) return fail("mask, masks and mask_rows go together");
@@ -147,7 +155,7 @@ bool adjust_plan(const qxg_adjust_logits_args *p, QxsArgs &A, uint64_t &bytes, c
     if (!a.top_n != !a.top_ids || (!a.top_n && a.top_logits)) return fail("top_n, top_ids and top_logits go together");
     A.slices = (a.vocab + QXS_SLICE - 1) / QXS_SLICE;
     A.words = (a.vocab + 31) / 32;
-    const uint64_t keys = up16((uint64_t)a.rows * A.slices * a.top_n * 8), ms = up16((uint64_t)a.rows * A.slices * 8);
+    const uint64_t keys = up16((uint64_t)a.rows * A.slices * 4 * a.top_n * 8), ms = up16((uint64_t)a.rows * A.slices * 4 * 8);
     A.keys = (uint64_t *)a.workspace;
     A.ms = (float2 *)((uint8_t *)a.workspace + keys);
     bytes = keys + ms;
@@ -188,17 +196,19 @@ int qxg_kv_select(qxg_ctx *c, const qxg_kv_select_args *p, void *stream, int wai
 
 int qxg_kv_compact(qxg_ctx *c, const qxg_kv_compact_args *p, void *stream, int wait, char *err, uint64_t err_len) {
     const Err fail{err, err_len};
+    QxeCompact C{};
     uint64_t need = 0;
-    if (!compact_plan(p, need, fail)) return 0;
+    if (!compact_plan(p, C, need, fail)) return 0;
     const Arg args[] = {{p->k, "k", true, 16}, {p->v, "v", true, 16}, {p->kscale, "kscale", true, 4}, {p->vscale, "vscale", true, 4},
                         {p->keep, "keep", true, 4}, {p->kept, "kept", true, 4}, {p->account, "account", false, 4},
                         {p->account_out, "account_out", false, 4}, {p->workspace, "workspace", false, 16}};
     if (!pointers_ok(args, fail) || !workspace_ok(p->workspace, p->workspace_bytes, need, fail)) return 0;
-    return on_device(c, args, (hipStream_t)stream, wait, fail, [&] { qxe_launch_compact(*p, (hipStream_t)stream); });
+    return on_device(c, args, (hipStream_t)stream, wait, fail, [&] { qxe_launch_compact(C, (hipStream_t)stream); });
 }
 uint64_t qxg_kv_compact_workspace(const qxg_kv_compact_args *p) {
+    QxeCompact C{};
     uint64_t need = 0;
-    return compact_plan(p, need, Err{}) ? need : 0;
+    return compact_plan(p, C, need, Err{}) ? need : 0;
 }
 
 int qxg_adjust_logits(qxg_ctx *c, const qxg_adjust_logits_args *p, void *stream, int wait, char *err, uint64_t err_len) {

@@ -187,6 +187,7 @@ def _kind(t):
     return k
 
 
+@functools.lru_cache(maxsize=4096)
 def _dense(shape):
     """The strides of a contiguous array."""
     out, n = [], 1
@@ -203,12 +204,13 @@ def _arr(t, name, kind, shape, inner=None):
         return 0
     if _kind(t) != kind:
         raise ValueError(f"{name} has dtype {t.dtype}, not {kind}")
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{name} has shape {tuple(t.shape)}, not {shape}")
-    rest = shape if inner is None else shape[len(shape) - inner:]
-    if rest and tuple(t.stride())[len(shape) - len(rest):] != _dense(rest):
-        if any(d != 1 and s != e for d, s, e in zip(rest, tuple(t.stride())[len(shape) - len(rest):], _dense(rest))):
-            raise ValueError(f"{name} is not contiguous in its last {len(rest)} dimensions")
+    strides, dense = t.stride(), _dense(shape)
+    if strides != dense:
+        last = len(shape) - (len(shape) if inner is None else inner)
+        if any(d != 1 and s != e for d, s, e in zip(shape[last:], strides[last:], dense[last:])):
+            raise ValueError(f"{name} is not contiguous in its last {len(shape) - last} dimensions")
     return t.data_ptr()
 
 
@@ -216,7 +218,7 @@ def _sized(t, name):
     """(address, bytes) of a workspace: a contiguous uint8 array."""
     if t is None:
         return 0, 0
-    return _arr(t, name, "u8", tuple(t.shape)), t.shape[0]
+    return _arr(t, name, "u8", t.shape), t.shape[0]
 
 
 def _tree_pack(ptrs, strides, kind, q_shape, k_shape, max_len, scale, decay, account_stride=0):
