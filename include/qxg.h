@@ -444,7 +444,7 @@ typedef struct qxg_adjust_logits_args {
     void *workspace;          /* 16-byte aligned */
     uint64_t workspace_bytes;
     uint64_t logits_row, out_row, history_row;   /* strides in elements */
-    uint32_t type, rows, vocab, history_slots, biases, masks, top_n;   /* rows <= 65535, biases <= 1024, top_n <= 32 */
+    uint32_t type, rows, vocab, history_slots, biases, masks, top_n;   /* rows <= 65535, history_slots < 2^20, biases <= 1024, top_n <= 32 */
 } qxg_adjust_logits_args;
 int qxg_adjust_logits(qxg_ctx *ctx, const qxg_adjust_logits_args *args, void *stream, int wait, char *err, uint64_t err_len);
 uint64_t qxg_adjust_logits_workspace(const qxg_adjust_logits_args *args);

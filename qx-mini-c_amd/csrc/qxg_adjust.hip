@@ -3,8 +3,10 @@
 #include "qxg_ops.h"
 
 namespace {
-constexpr int PER = QXS_SLICE / 256;    // tokens a thread
-constexpr uint32_t HAS_BIAS = 0x40000000u, SEEN = 0x80000000u;
+// of a token in LDS: occurrences behind the prompt, the index of its first bias entry, whether it has one, and
+// whether it is anywhere in the history
+constexpr uint32_t COUNT = (1u << 20) - 1, BIAS_SHIFT = 20, HAS_BIAS = 0x40000000u, SEEN = 0x80000000u;
+static_assert(QXS_HISTORY <= COUNT && QXS_BIASES <= 1u << (30 - BIAS_SHIFT), "the fields of a token's word");
 
 // Order of a logit as an unsigned number, 0 (never picked) for -inf and NaN; -0 as +0.  A key is that
 // over ~token: larger first, then the lower token; no two are alike.
@@ -58,32 +60,49 @@ DEV float lse_of(float2 v) { return v.y != v.y ? NAN : fabsf(v.x) == INFINITY ? 
 template <typename T> struct Pack { T v[16 / sizeof(T)]; };
 }  // namespace
 
-// A workgroup takes QXS_SLICE tokens of a row, 16 bytes of it a thread and step.  It reads the row's
-// whole history and bias list and keeps those of its tokens in LDS (counts by integer atomics, biases
-// summed in list order by the first entry of each token), so the dense pass reads and writes each
-// logit once.  The best tokens are taken wave by wave: the n-th largest of the 64 lanes' largest bounds the
-// wave's n-th largest from below and at most n lanes reach it, so at most 16 n keys are
-// left, which are ranked by counting.
-template <typename T>
+// A workgroup takes a slice of a row, 16 bytes of it a thread and step.  It reads the row's whole history
+// and bias list and keeps those of its tokens in LDS (counts by integer atomics, biases summed in list
+// order by the first entry of each token), so the dense pass reads and writes each logit once.  The best
+// tokens: the n-th largest of a wave's 64 lanes' largest bounds the wave's n-th largest from below, and
+// so the slice's; at most n lanes of a wave reach it, so at most PER n of its keys do, about n / 2 of most
+// rows.  Only of more than n are the n largest taken, by counting.
+template <typename T, int STEPS>
 __global__ __launch_bounds__(256) void qxs_slice(QxsArgs A) {
-    constexpr int N = 16 / sizeof(T), STEPS = PER / N;
+    constexpr int N = 16 / sizeof(T), PER = N * STEPS, EARLY = 16;
+    constexpr uint32_t SLICE = 256 * PER;
     __shared__ union {
-        struct { uint32_t count[QXS_SLICE]; float bias[QXS_SLICE]; } s;   // count: SEEN, HAS_BIAS, occurrences behind the prompt
-        uint64_t keys[4][16 * QXG_MAX_TOPN];
+        uint32_t token[SLICE];
+        uint64_t keys[4][PER * QXG_MAX_TOPN];
     } u;
-    __shared__ uint32_t s_ids[1024];
+    __shared__ uint32_t s_ids[QXS_BIASES];
+    __shared__ float s_sum[QXS_BIASES];
+    __shared__ uint64_t s_least[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
-    const uint32_t r = blockIdx.y, v0 = blockIdx.x * QXS_SLICE, V = A.a.vocab;
+    const uint32_t r = blockIdx.y, v0 = blockIdx.x * SLICE, V = A.a.vocab;
     const T *in = (const T *)A.a.logits + r * A.a.logits_row + v0;
     T *out = (T *)A.a.out + r * A.a.out_row + v0;
-    const uint32_t here = min(QXS_SLICE, V - v0);   // tokens of the slice
+    const uint32_t here = min(SLICE, V - v0);   // tokens of the slice
     const bool wide_in = (uintptr_t)in % 16 == 0, wide_out = (uintptr_t)out % 16 == 0;
+    // Everything that needs nothing else is loaded at once, whether it turns out to be used or not (absent
+    // arrays: the workspace's first words): one after the other, the loads' latencies were half of the time.
+    const float *none = reinterpret_cast<const float *>(A.ms);
+    const float *pen = A.a.penalties ? A.a.penalties + 3 * r : none, *tem = A.a.temperature ? A.a.temperature + r : none;
+    const uint32_t *lens = A.a.history_lens ? A.a.history_lens + r : (const uint32_t *)none,
+                   *made = A.a.prompt_lens ? A.a.prompt_lens + r : (const uint32_t *)none,
+                   *rows = A.a.mask_rows ? A.a.mask_rows + r : (const uint32_t *)none;
+    float rep = pen[0], freq = pen[1], pres = pen[2], temp = tem[0];
+    uint32_t entries = lens[0], prompt = made[0], mrow = rows[0];
+    const uint32_t slots = A.a.history ? A.a.history_slots : 0u;
+    const uint32_t *hist = A.a.history + r * A.a.history_row;
+    uint32_t early[EARLY];   // the history's first entries
+#pragma unroll
+    for (int k = 0; k < EARLY; ++k) early[k] = tid + 256 * k < slots ? hist[tid + 256 * k] : QXG_NO_TOKEN;
     float x[PER];
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
         const uint32_t t = (s * 256 + tid) * N;
         if (wide_in && t + N <= here) {
-            const Pack<T> p = __builtin_bit_cast(Pack<T>, *reinterpret_cast<const uint4 *>(in + t));
+            const Pack<T> p = __builtin_bit_cast(Pack<T>, *reinterpret_cast<const nt4 *>(in + t));
 #pragma unroll
             for (int j = 0; j < N; ++j) x[s * N + j] = (float)p.v[j];
         } else {
@@ -91,95 +110,98 @@ __global__ __launch_bounds__(256) void qxs_slice(QxsArgs A) {
             for (int j = 0; j < N; ++j) x[s * N + j] = t + j < here ? (float)in[t + j] : -INFINITY;
         }
     }
-    const float rep = A.a.penalties ? A.a.penalties[3 * r] : 1.0f, freq = A.a.penalties ? A.a.penalties[3 * r + 1] : 0.0f,
-                pres = A.a.penalties ? A.a.penalties[3 * r + 2] : 0.0f, temp = A.a.temperature ? A.a.temperature[r] : 1.0f;
-    const uint32_t mrow = A.a.mask_rows ? A.a.mask_rows[r] : r;
-    const uint32_t *mask = A.a.mask && mrow < A.a.masks ? A.a.mask + (uint64_t)mrow * A.words : nullptr;
-    uint32_t open[STEPS];   // the mask bits of the thread's tokens, from bit 0
-#pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
-        const uint32_t t = (s * 256 + tid) * N;
-        open[s] = mask && t < here ? mask[(v0 + t) >> 5] >> (t & 31) : ~0u;
-    }
-    const bool sparse = A.a.history || A.a.bias_ids;
+    const bool sparse = slots || A.a.biases;
     if (sparse) {
 #pragma unroll
-        for (int i = 0; i < PER / 4; ++i) reinterpret_cast<uint4 *>(u.s.count)[i * 256 + tid] = make_uint4(0, 0, 0, 0);
-        for (uint32_t i = tid; i < A.a.biases; i += 256) s_ids[i] = A.a.bias_ids[(uint64_t)r * A.a.biases + i];
-        __syncthreads();
-        if (A.a.history) {
-            const uint32_t n = A.a.history_lens ? min(A.a.history_lens[r], A.a.history_slots) : A.a.history_slots;
-            const uint32_t prompt = A.a.prompt_lens ? A.a.prompt_lens[r] : 0u;
-            const uint32_t *hist = A.a.history + r * A.a.history_row;
-            for (uint32_t i0 = tid; i0 < n; i0 += 8 * 256) {
-                uint32_t t[8];
-#pragma unroll
-                for (int k = 0; k < 8; ++k) t[k] = i0 + 256 * k < n ? hist[i0 + 256 * k] - v0 : ~0u;
-#pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    if (t[k] < here) {
-                        atomicOr(&u.s.count[t[k]], SEEN);
-                        if (i0 + 256 * k >= prompt) atomicAdd(&u.s.count[t[k]], 1u);
-                    }
-            }
-        }
+        for (int i = 0; i < PER / 4; ++i) reinterpret_cast<nt4 *>(u.token)[i * 256 + tid] = nt4{0, 0, 0, 0};
         for (uint32_t i = tid; i < A.a.biases; i += 256) {
-            const uint32_t v = s_ids[i];
-            if (v - v0 >= here) continue;
-            bool first = true;
-            for (uint32_t j = 0; j < i; ++j) first = first && s_ids[j] != v;
-            if (!first) continue;
-            const float *val = A.a.bias_values + (uint64_t)r * A.a.biases;
-            float sum = val[i];
-            for (uint32_t j = i + 1; j < A.a.biases; ++j)
-                if (s_ids[j] == v) sum += val[j];
-            u.s.bias[v - v0] = sum;
-            atomicOr(&u.s.count[v - v0], HAS_BIAS);
+            s_ids[i] = A.a.bias_ids[(uint64_t)r * A.a.biases + i];
+            s_sum[i] = A.a.bias_values[(uint64_t)r * A.a.biases + i];
+        }
+    }
+    mrow = A.a.mask_rows ? mrow : r;
+    const uint32_t *mask = A.a.mask && mrow < A.a.masks ? A.a.mask + (uint64_t)mrow * A.words : nullptr;
+    uint32_t open[STEPS];   // the mask bits of the thread's tokens, from bit 0; 0 behind the vocabulary
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+        const uint32_t t = (s * 256 + tid) * N, left = here > t ? here - t : 0u;
+        open[s] = (mask && left ? mask[(v0 + t) >> 5] >> (t & 31) : ~0u) & (left < N ? (1u << left) - 1u : ~0u);
+    }
+    if (!A.a.penalties) { rep = 1.0f; freq = pres = 0.0f; }
+    if (!A.a.temperature) temp = 1.0f;
+    entries = A.a.history_lens ? min(entries, slots) : slots;
+    prompt = A.a.prompt_lens ? prompt : 0u;
+    if (sparse) {
+        __syncthreads();
+        auto note = [&](uint32_t i, uint32_t v) {
+            if (v - v0 >= here || i >= entries) return;
+            atomicOr(&u.token[v - v0], SEEN);
+            if (i >= prompt) atomicAdd(&u.token[v - v0], 1u);
+        };
+#pragma unroll
+        for (int k = 0; k < EARLY; ++k) note(tid + 256 * k, early[k]);
+        for (uint32_t i = tid + 256 * EARLY; i < entries; i += 256) note(i, hist[i]);
+        if (A.a.biases) {
+            float sum[QXS_BIASES / 256];
+            bool first[QXS_BIASES / 256];   // entry tid + 256 k is its token's first
+#pragma unroll
+            for (int k = 0; k < (int)QXS_BIASES / 256; ++k) {
+                const uint32_t i = tid + 256 * k, v = i < A.a.biases ? s_ids[i] : QXG_NO_TOKEN;
+                first[k] = v - v0 < here;
+                if (!first[k]) continue;
+                for (uint32_t j = 0; j < i; ++j) first[k] = first[k] && s_ids[j] != v;
+                if (!first[k]) continue;
+                sum[k] = s_sum[i];
+                for (uint32_t j = i + 1; j < A.a.biases; ++j)
+                    if (s_ids[j] == v) sum[k] += s_sum[j];
+                atomicOr(&u.token[v - v0], HAS_BIAS | i << BIAS_SHIFT);
+            }
+            __syncthreads();   // every entry's own value is read
+#pragma unroll
+            for (int k = 0; k < (int)QXS_BIASES / 256; ++k)
+                if (first[k]) s_sum[tid + 256 * k] = sum[k];
         }
         __syncthreads();
     }
-    float m = -INFINITY;
+    float m = -INFINITY;   // the thread's largest and its place (the first of equal ones is the lower token)
+    uint32_t at = 0;
     bool nan = false;
-    uint32_t best = 0, at = 0;   // the thread's largest, by rank (the first of equal ones is the lower token)
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
         const uint32_t t = (s * 256 + tid) * N;
         Pack<T> p;
 #pragma unroll
         for (int j4 = 0; j4 < N; j4 += 4) {
-            uint4 c4 = make_uint4(0, 0, 0, 0);
-            if (sparse) c4 = *reinterpret_cast<const uint4 *>(&u.s.count[t + j4]);
-            const uint32_t c[4] = {c4.x, c4.y, c4.z, c4.w};
+            nt4 c4 = {0, 0, 0, 0};
+            if (sparse) c4 = *reinterpret_cast<const nt4 *>(&u.token[t + j4]);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const int j = j4 + k;
+                const uint32_t c = c4[k];
                 float y = x[s * N + j];
-                if (c[k]) {
-                    if (c[k] & SEEN) y = y > 0.0f ? y / rep : y * rep;
-                    const uint32_t made = c[k] & 0x3fffffffu;
-                    if (made) {
-                        y -= freq * (float)made;
+                if (c) {
+                    if (c & SEEN) y = y > 0.0f ? y / rep : y * rep;
+                    if (c & COUNT) {
+                        y -= freq * (float)(c & COUNT);
                         y -= pres;
                     }
-                    if (c[k] & HAS_BIAS) y += u.s.bias[t + j];
+                    if (c & HAS_BIAS) y += s_sum[(c >> BIAS_SHIFT) & (QXS_BIASES - 1)];
                 }
                 y /= temp;
-                if (!((open[s] >> j) & 1) || t + j >= here) y = -INFINITY;
+                if (!((open[s] >> j) & 1)) y = -INFINITY;
                 x[s * N + j] = y;
                 p.v[j] = (T)y;
-                m = fmaxf(m, y);
                 nan = nan || y != y;
-                const uint32_t k32 = rank_of(y);
-                if (k32 > best) { best = k32; at = t + j; }
+                if (y > m) { m = y; at = t + j; }
             }
         }
-        if (wide_out && t + N <= here) *reinterpret_cast<uint4 *>(out + t) = __builtin_bit_cast(uint4, p);
+        if (wide_out && t + N <= here) *reinterpret_cast<nt4 *>(out + t) = __builtin_bit_cast(nt4, p);
         else
 #pragma unroll
             for (int j = 0; j < N; ++j)
                 if (t + j < here) out[t + j] = p.v[j];
     }
-    const uint32_t list = blockIdx.x * 4 + wave;   // one of the row's lists of n keys
+    const uint64_t list = (uint64_t)r * A.slices * 4 + blockIdx.x * 4 + wave;
     if (A.a.lse) {
         float sum = 0.0f;
         if (m > -INFINITY) {
@@ -187,16 +209,20 @@ __global__ __launch_bounds__(256) void qxs_slice(QxsArgs A) {
             for (int i = 0; i < PER; ++i) sum += x[i] == m ? 1.0f : __builtin_amdgcn_exp2f((x[i] - m) * 1.4426950408889634f);
         }
         const float2 ms = wave_join(make_float2(m, nan ? NAN : sum));
-        if (lane == 0) A.ms[((uint64_t)r * A.slices) * 4 + list] = ms;
+        if (lane == 0) A.ms[list] = ms;
     }
     const uint32_t n = A.a.top_n;
     if (!n) return;
-    const uint64_t least = wave_nth(key_of(best, v0 + at), n);
-    __syncthreads();   // the counts are read: their space takes the keys
+    uint64_t least = wave_nth(key_of(rank_of(m), v0 + at), n);
+    if (lane == 0) s_least[wave] = least;
+    __syncthreads();   // (also: the tokens' words are read, their space takes the keys)
+    least = umax64(umax64(s_least[0], s_least[1]), umax64(s_least[2], s_least[3]));
+    const float low = least ? key_value(least) : -INFINITY;
     uint64_t *keys = u.keys[wave];
     uint32_t have = 0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
+        if (__ballot(x[i] >= low) == 0) continue;
         const uint64_t k = key_of(rank_of(x[i]), v0 + ((i / N) * 256 + tid) * N + i % N);
         const bool f = k && k >= least;
         const uint64_t b = __ballot(f);
@@ -204,7 +230,11 @@ __global__ __launch_bounds__(256) void qxs_slice(QxsArgs A) {
         have += (uint32_t)__popcll(b);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    uint64_t *to = A.keys + ((uint64_t)r * A.slices * 4 + list) * n;
+    uint64_t *to = A.keys + list * n;
+    if (have <= n) {
+        if (lane < n) to[lane] = lane < have ? keys[lane] : 0;
+        return;
+    }
     for (uint32_t i = lane; i < have; i += 64) {
         const uint64_t k = keys[i];
         uint32_t above = 0;
@@ -212,43 +242,52 @@ __global__ __launch_bounds__(256) void qxs_slice(QxsArgs A) {
         for (uint32_t j = 0; j < have; ++j) above += keys[j] > k;
         if (above < n) to[above] = k;
     }
-    if (have < n && lane >= have && lane < n) to[lane] = 0;
 }
 
-// The lists of a row joined: a workgroup a row.  The n-th largest of 64 strips' largest keys bounds the n-th of
-// all from below; the keys that reach it are ranked by counting.
+// The lists of a row joined: a workgroup a row.  The n-th largest of 64 strips' largest keys (strip: every
+// 64th key) bounds the n-th of all from below; the keys that reach it are ranked by counting.
 template <typename T>
-__global__ __launch_bounds__(256) void qxs_join(QxsArgs A) {
+__global__ __launch_bounds__(1024) void qxs_join(QxsArgs A) {
     constexpr uint32_t ROOM = 4096;
-    __shared__ uint64_t s_key[ROOM], s_best[4][64];
-    __shared__ float2 s_ms[4];
+    constexpr int HELD = 8;   // keys a thread holds; those behind are read twice
+    __shared__ uint64_t s_key[ROOM], s_best[16][64];
+    __shared__ float2 s_ms[16];
     __shared__ uint32_t s_have;
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
-    const uint32_t r = blockIdx.x, lists = A.slices * 4, n = A.a.top_n;
-    const uint64_t *keys = A.keys + (uint64_t)r * lists * n;
+    const uint32_t r = blockIdx.x, lists = A.slices * 4, n = A.a.top_n, total = lists * n;
+    const uint64_t *keys = A.keys + (uint64_t)r * total;
+    uint64_t k[HELD], best = 0;   // of strip tid % 64
+#pragma unroll
+    for (int j = 0; j < HELD; ++j) k[j] = tid + 1024u * j < total ? keys[tid + 1024 * j] : 0;
     if (tid == 0) s_have = 0;
     if (A.a.lse) {
         float2 ms = make_float2(-INFINITY, 0.0f);
-        for (uint32_t i = tid; i < lists; i += 256) ms = join(ms, A.ms[(uint64_t)r * lists + i]);
+        for (uint32_t i = tid; i < lists; i += 1024) ms = join(ms, A.ms[(uint64_t)r * lists + i]);
         ms = wave_join(ms);
         if (lane == 0) s_ms[wave] = ms;
     }
-    uint64_t best = 0;   // of the lists of strip tid % 64: each list's first key is its largest
-    if (n)
-        for (uint32_t i = tid; i < lists; i += 256) best = umax64(best, keys[(uint64_t)i * n]);
+#pragma unroll
+    for (int j = 0; j < HELD; ++j) best = umax64(best, k[j]);
+    for (uint32_t i = tid + 1024 * HELD; i < total; i += 1024) best = umax64(best, keys[i]);
     s_best[wave][lane] = best;
     __syncthreads();
-    if (A.a.lse && tid == 0) A.a.lse[r] = lse_of(join(join(s_ms[0], s_ms[1]), join(s_ms[2], s_ms[3])));
-    if (!n) return;
-    best = umax64(umax64(s_best[0][lane], s_best[1][lane]), umax64(s_best[2][lane], s_best[3][lane]));
-    const uint64_t least = wave_nth(best, n);
-    for (uint32_t i = tid; i < lists * n; i += 256) {
-        const uint64_t k = keys[i];
-        if (k && k >= least) {
-            const uint32_t at = atomicAdd(&s_have, 1u);
-            if (at < ROOM) s_key[at] = k;
-        }
+    if (A.a.lse && wave == 0) {
+        const float2 ms = wave_join(lane < 16 ? s_ms[lane] : make_float2(-INFINITY, 0.0f));
+        if (lane == 0) A.a.lse[r] = lse_of(ms);
     }
+    if (!n) return;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) best = umax64(best, s_best[w][lane]);
+    const uint64_t least = wave_nth(best, n);
+    auto offer = [&](uint64_t key) {
+        if (key && key >= least) {
+            const uint32_t at = atomicAdd(&s_have, 1u);
+            if (at < ROOM) s_key[at] = key;
+        }
+    };
+#pragma unroll
+    for (int j = 0; j < HELD; ++j) offer(k[j]);
+    for (uint32_t i = tid + 1024 * HELD; i < total; i += 1024) offer(keys[i]);
     __syncthreads();
     const uint32_t have = s_have;
     auto put = [&](uint32_t at, uint64_t k) {
@@ -259,7 +298,7 @@ __global__ __launch_bounds__(256) void qxs_join(QxsArgs A) {
         if (A.a.top_logits) A.a.top_logits[(uint64_t)r * n + at] = x;
     };
     if (have <= ROOM) {
-        for (uint32_t i = tid; i < have; i += 256) {
+        for (uint32_t i = tid; i < have; i += 1024) {
             const uint64_t k = s_key[i];
             uint32_t above = 0;
 #pragma unroll 4
@@ -273,7 +312,7 @@ __global__ __launch_bounds__(256) void qxs_join(QxsArgs A) {
     uint64_t last = ~0ull;
     for (uint32_t k = 0; k < n; ++k) {
         uint64_t b = 0;
-        for (uint32_t i = tid; i < lists * n; i += 256) {
+        for (uint32_t i = tid; i < total; i += 1024) {
             const uint64_t y = keys[i];
             b = y < last ? umax64(b, y) : b;
         }
@@ -281,15 +320,17 @@ __global__ __launch_bounds__(256) void qxs_join(QxsArgs A) {
         __syncthreads();
         if (lane == 0) s_best[0][wave] = b;
         __syncthreads();
-        last = umax64(umax64(s_best[0][0], s_best[0][1]), umax64(s_best[0][2], s_best[0][3]));
+        last = wave_max_u64(s_best[0][lane & 15]);
         if (tid == 0) put(k, last);
     }
 }
 
 namespace {
 template <typename T> void launch(const QxsArgs &A, hipStream_t s) {
-    hipLaunchKernelGGL(qxs_slice<T>, dim3(A.slices, A.a.rows), dim3(256), 0, s, A);
-    if (A.a.lse || A.a.top_n) hipLaunchKernelGGL(qxs_join<T>, dim3(A.a.rows), dim3(256), 0, s, A);
+    constexpr int STEPS = QXS_SLICE * sizeof(T) / 4096;
+    if (A.small) hipLaunchKernelGGL((qxs_slice<T, 1>), dim3(A.slices, A.a.rows), dim3(256), 0, s, A);
+    else hipLaunchKernelGGL((qxs_slice<T, STEPS>), dim3(A.slices, A.a.rows), dim3(256), 0, s, A);
+    if (A.a.lse || A.a.top_n) hipLaunchKernelGGL(qxs_join<T>, dim3(A.a.rows), dim3(1024), 0, s, A);
 }
 }  // namespace
 

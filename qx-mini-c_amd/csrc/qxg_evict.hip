@@ -5,19 +5,13 @@
 namespace {
 // Weights as unsigned numbers in their order, 1 or more; NaN as -inf, -0 as +0
 DEV uint32_t weight_rank(float w) {
-    const uint32_t u = __float_as_uint(w == w ? w + 0.0f : -INFINITY);
-    return u & 0x80000000u ? ~u : u | 0x80000000u;
+    const uint32_t u = __float_as_uint(fmaxf(w, -INFINITY) + 0.0f);   // (the larger of NaN and a number is the number)
+    return u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
 }
-// sum of a over the block's 16 waves' lanes before this thread, and over all of them
-DEV uint2 block_before(uint2 a, uint2 *s_w, uint2 &all) {
-    const int wave = wave_id(), lane = threadIdx.x & 63;
-    uint2 v = a;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t x = (uint32_t)__shfl_up((int)v.x, o), y = (uint32_t)__shfl_up((int)v.y, o);
-        if (lane >= o) { v.x += x; v.y += y; }
-    }
-    if (lane == 63) s_w[wave] = v;
+// sums of a wave's two counts (the same in all its lanes) over the waves before it, and over all 16
+DEV uint2 waves_before(uint2 a, uint2 *s_w, uint2 &all) {
+    const int wave = wave_id();
+    if ((threadIdx.x & 63) == 0) s_w[wave] = a;
     __syncthreads();
     uint2 before = make_uint2(0, 0);
     all = make_uint2(0, 0);
@@ -28,7 +22,7 @@ DEV uint2 block_before(uint2 a, uint2 *s_w, uint2 &all) {
         all.x += x.x;
         all.y += x.y;
     }
-    return make_uint2(before.x + v.x - a.x, before.y + v.y - a.y);
+    return before;
 }
 struct Group { uint32_t len, kept; };
 DEV Group group_of(const qxg_kv_select_args &A, uint32_t g) {
@@ -67,37 +61,61 @@ DEV uint32_t block_nth(const uint32_t (&k)[E], uint32_t want, uint32_t least, in
     }
     return least;
 }
-// Lists the kept ones of positions p0 .. p0 + E - 1 of every thread: ranks above `least`, and the lowest `need`
-// equal ones.  done: how many of either lie before the block's first position.
+// Positions p0 + 64 E wave + 64 i + lane of a thread: a wave's 64 E are neighbours, read 64 at a time
+template <int E> DEV uint32_t place_of(uint32_t p0, int i) { return p0 + 64 * (E * wave_id() + i) + (threadIdx.x & 63); }
+// Lists the kept ones of the block's 1024 E positions from p0 on: ranks above `least`, and the lowest `need`
+// equal ones.  done: how many of either lie before p0.
 template <int E>
 DEV void list_kept(const uint32_t (&k)[E], uint32_t p0, uint32_t least, uint32_t need, uint2 &done, uint2 *s_w, uint32_t *keep) {
     uint2 own = make_uint2(0, 0), all;
 #pragma unroll
-    for (int i = 0; i < E; ++i) { own.x += k[i] > least; own.y += k[i] == least; }
-    uint2 at = block_before(own, s_w, all);
+    for (int i = 0; i < E; ++i) {
+        own.x += (uint32_t)__popcll(__ballot(k[i] > least));
+        own.y += (uint32_t)__popcll(__ballot(k[i] == least));
+    }
+    uint2 at = waves_before(own, s_w, all);
     at.x += done.x;
     at.y += done.y;
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-        const bool gt = k[i] > least, eq = k[i] == least;
-        if (gt || (eq && at.y < need)) keep[at.x + min(at.y, need)] = p0 + i;
-        at.x += gt;
-        at.y += eq;
+        const uint64_t gt = __ballot(k[i] > least), eq = __ballot(k[i] == least);
+        const uint32_t place = at.x + __builtin_amdgcn_mbcnt_hi((uint32_t)(gt >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)gt, 0));
+        if (eq == 0 || at.y >= need) {   // (uniform)
+            if (k[i] > least) keep[place + min(at.y, need)] = place_of<E>(p0, i);
+        } else {
+            const uint32_t y = at.y + __builtin_amdgcn_mbcnt_hi((uint32_t)(eq >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)eq, 0));
+            if (k[i] > least || (k[i] == least && y < need)) keep[place + min(y, need)] = place_of<E>(p0, i);
+        }
+        at.x += (uint32_t)__popcll(gt);
+        at.y += (uint32_t)__popcll(eq);
     }
     done.x += all.x;
     done.y += all.y;
 }
 template <int E>
-DEV void load_ranks(const qxg_kv_select_args &A, const float *acc, uint32_t p0, uint32_t len, uint32_t (&k)[E]) {
-    float w[E];
+DEV void load_weights(const float *acc, uint32_t p0, uint32_t len, float (&w)[E]) {
+    if (p0 + 1024 * E <= len) {   // (uniform)
+        const float *p = acc + place_of<E>(p0, 0);
 #pragma unroll
-    for (int i = 0; i < E; ++i) w[i] = p0 + i < len ? acc[p0 + i] : 0.0f;
+        for (int i = 0; i < E; ++i) w[i] = p[64 * i];
+    } else {
 #pragma unroll
-    for (int i = 0; i < E; ++i) k[i] = rank_at(A, w[i], p0 + i, len);
+        for (int i = 0; i < E; ++i) w[i] = place_of<E>(p0, i) < len ? acc[place_of<E>(p0, i)] : 0.0f;
+    }
+}
+template <int E>
+DEV void ranks_of(const qxg_kv_select_args &A, const float (&w)[E], uint32_t p0, uint32_t len, uint32_t (&k)[E]) {
+    if (p0 >= A.sinks && p0 + 1024 * E <= len - A.recent) {   // (uniform; nothing kept in any case, nothing behind the end)
+#pragma unroll
+        for (int i = 0; i < E; ++i) k[i] = weight_rank(w[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i) k[i] = rank_at(A, w[i], place_of<E>(p0, i), len);
+    }
 }
 }  // namespace
 
-// Up to 1024 E positions, a workgroup a group: a thread holds E neighbouring positions' ranks in registers.  The
+// Up to 1024 E positions, a workgroup a group: a thread holds E positions' ranks in registers.  The
 // counts of its 32 steps bound it.  (Byte-wise histograms in LDS, their bins searched by one thread: 26 us
 // for 700 positions.)
 template <int E>
@@ -113,10 +131,12 @@ __global__ __launch_bounds__(1024) void qxe_select(qxg_kv_select_args A) {
         return;
     }
     uint32_t k[E], above;
-    load_ranks<E>(A, A.account + g * A.account_group, threadIdx.x * E, G.len, k);
+    float w[E];
+    load_weights<E>(A.account + g * A.account_group, 0, G.len, w);
+    ranks_of<E>(A, w, 0, G.len, k);
     const uint32_t least = block_nth<E>(k, A.budget, 0, 31, s_n, above);
     uint2 done = make_uint2(0, 0);
-    list_kept<E>(k, threadIdx.x * E, least, A.budget - above, done, s_w, keep);
+    list_kept<E>(k, 0, least, A.budget - above, done, s_w, keep);
 }
 
 // More positions than registers hold: a histogram of the ranks' top 11 bits (each bin 16 times, by lane, as
@@ -144,19 +164,16 @@ __global__ __launch_bounds__(1024) void qxe_select_long(qxg_kv_select_args A) {
         const int bits = min(shift, 11);
         for (int i = tid; i < BINS * COPIES / 4; i += 1024) reinterpret_cast<uint4 *>(s_hist)[i] = make_uint4(0, 0, 0, 0);
         __syncthreads();
+        uint32_t k[E];
+        float next[E];   // the next round's weights, on their way
+        load_weights<E>(acc, 0, G.len, next);
         for (uint32_t p0 = 0; p0 < G.len; p0 += 1024 * E) {
-            float w[E];
+            ranks_of<E>(A, next, p0, G.len, k);
+            load_weights<E>(acc, p0 + 1024 * E, G.len, next);
 #pragma unroll
-            for (int i = 0; i < E; ++i) {
-                const uint32_t p = p0 + 1024 * i + tid;
-                w[i] = p < G.len ? acc[p] : 0.0f;
-            }
-#pragma unroll
-            for (int i = 0; i < E; ++i) {
-                const uint32_t p = p0 + 1024 * i + tid, k = rank_at(A, w[i], p, G.len);
-                if (p < G.len && (shift == 32 || k >> shift == least >> shift))
-                    atomicAdd(&s_hist[((k >> (shift - bits)) & ((1u << bits) - 1u)) * COPIES + (lane & 15)], 1u);
-            }
+            for (int i = 0; i < E; ++i)   // (positions behind the end have rank 0, no other has)
+                if (k[i] && (shift == 32 || k[i] >> shift == least >> shift))
+                    atomicAdd(&s_hist[((k[i] >> (shift - bits)) & ((1u << bits) - 1u)) * COPIES + (lane & 15)], 1u);
         }
         __syncthreads();
         // the bins from the top: thread t has bins 2047 - 2 t and 2046 - 2 t
@@ -166,7 +183,13 @@ __global__ __launch_bounds__(1024) void qxe_select_long(qxg_kv_select_args A) {
 #pragma unroll
             for (int c = 0; c < COPIES; ++c) n[i] += s_hist[(BINS - 1 - 2 * tid - i) * COPIES + ((c + tid) & 15)];
         uint2 all;
-        const uint32_t before = above + block_before(make_uint2(n[0] + n[1], 0), s_w, all).x;
+        uint32_t run = n[0] + n[1];   // running count over the wave's lanes
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t y = (uint32_t)__shfl_up((int)run, o);
+            if (lane >= o) run += y;
+        }
+        const uint32_t before = above + run - n[0] - n[1] + waves_before(make_uint2((uint32_t)__shfl((int)run, 63), 0), s_w, all).x;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const uint32_t b = before + (i ? n[0] : 0u);
@@ -185,21 +208,23 @@ __global__ __launch_bounds__(1024) void qxe_select_long(qxg_kv_select_args A) {
         if (shift && count <= ROOM) {
             if (tid == 0) s_count = 0;
             __syncthreads();
+            load_weights<E>(acc, 0, G.len, next);
             for (uint32_t p0 = 0; p0 < G.len; p0 += 1024 * E) {
-                float w[E];
+                ranks_of<E>(A, next, p0, G.len, k);
+                load_weights<E>(acc, p0 + 1024 * E, G.len, next);
 #pragma unroll
                 for (int i = 0; i < E; ++i) {
-                    const uint32_t p = p0 + 1024 * i + tid;
-                    w[i] = p < G.len ? acc[p] : 0.0f;
-                }
-#pragma unroll
-                for (int i = 0; i < E; ++i) {
-                    const uint32_t p = p0 + 1024 * i + tid, k = rank_at(A, w[i], p, G.len);
-                    if (p < G.len && k >> shift == least >> shift) s_hist[atomicAdd(&s_count, 1u)] = k;   // (< count, in any order)
+                    const bool f = k[i] && k[i] >> shift == least >> shift;
+                    const uint64_t b = __ballot(f);
+                    if (!b) continue;
+                    uint32_t first = 0;
+                    if (lane == 0) first = atomicAdd(&s_count, (uint32_t)__popcll(b));
+                    first = (uint32_t)__builtin_amdgcn_readfirstlane((int)first);
+                    if (f) s_hist[first + (uint32_t)__popcll(b & ((1ull << lane) - 1ull))] = k[i];   // (< count, in any order)
                 }
             }
             __syncthreads();
-            uint32_t k[E], more;
+            uint32_t more;
 #pragma unroll
             for (int i = 0; i < E; ++i) k[i] = (uint32_t)(1024 * i + tid) < count ? s_hist[1024 * i + tid] : 0u;
             least = block_nth<E>(k, A.budget - above, least, shift - 1, s_n, more);
@@ -209,14 +234,13 @@ __global__ __launch_bounds__(1024) void qxe_select_long(qxg_kv_select_args A) {
     }
     uint2 done = make_uint2(0, 0);
     uint32_t k[E];
-    load_ranks<E>(A, acc, tid * E, G.len, k);
-    for (uint32_t p0 = tid * E; p0 < (G.len + 1024 * E - 1) / (1024 * E) * (1024 * E); p0 += 1024 * E) {
-        uint32_t next[E];
-        load_ranks<E>(A, acc, p0 + 1024 * E, G.len, next);
+    float next[E];
+    load_weights<E>(acc, 0, G.len, next);
+    for (uint32_t p0 = 0; p0 < G.len; p0 += 1024 * E) {
+        ranks_of<E>(A, next, p0, G.len, k);
+        load_weights<E>(acc, p0 + 1024 * E, G.len, next);
         list_kept<E>(k, p0, least, A.budget - above, done, s_w, keep);
         __syncthreads();   // s_w is read
-#pragma unroll
-        for (int i = 0; i < E; ++i) k[i] = next[i];
     }
 }
 

@@ -28,15 +28,16 @@ struct QxeCompact {
 void qxe_launch_select(const qxg_kv_select_args &a, hipStream_t s);
 void qxe_launch_compact(const QxeCompact &C, hipStream_t s);
 
-// Logits.  Each of the 4 waves of a slice of a row leaves its top_n keys, largest first, and (maximum, sum
-// of exponentials) to the join.
+// Logits.  Each of the 4 waves of a slice of a row leaves up to top_n keys, its largest among them, the
+// others 0, and (maximum, sum of exponentials) to the join.
 struct QxsArgs {
     qxg_adjust_logits_args a;
     uint32_t slices, words;
+    uint32_t small;    // slices of one 16-byte step a thread instead of QXS_SLICE tokens
     uint64_t *keys;    // [rows][slices * 4][top_n]
     float2 *ms;        // [rows][slices * 4]
 };
-constexpr uint32_t QXS_SLICE = 4096;
+constexpr uint32_t QXS_SLICE = 4096, QXS_BIASES = 1024, QXS_HISTORY = (1u << 20) - 1;
 void qxs_launch(const QxsArgs &A, hipStream_t s);
 
 // the context's device (qxg_api.hip)

@@ -143,17 +143,20 @@ bool adjust_plan(const qxg_adjust_logits_args *p, QxsArgs &A, uint64_t &bytes, c
     if (!a.rows || a.rows > 65535) return fail("rows must be between 1 and 65535");
     if (!a.vocab || a.vocab > 0x7fffffffu) return fail("vocab must be between 1 and 2^31 - 1");
     if (a.top_n > QXG_MAX_TOPN) return fail("top_n must be at most %u", QXG_MAX_TOPN);
-    if (a.biases > 1024) return fail("biases must be at most 1024");
+    if (a.biases > QXS_BIASES) return fail("biases must be at most %u", QXS_BIASES);
     if (a.rows > 1 && (a.logits_row < a.vocab || a.out_row < a.vocab)) return fail("rows of logits or out overlap");
     if (a.logits == a.out && a.rows > 1 && a.logits_row != a.out_row) return fail("in place, the row strides must be equal");
     if (a.history && !a.history_slots) return fail("history without slots");
-    if (a.history_slots > 1u << 29) return fail("history_slots must be at most 2^29");   // (a count has 30 bits)
+    if (a.history_slots > QXS_HISTORY) return fail("history_slots must be at most %u", QXS_HISTORY);
     if (!a.history && (a.history_lens || a.prompt_lens)) return fail("history_lens or prompt_lens without history");
     if (!a.bias_ids != !a.bias_values || !a.bias_ids != !a.biases) return fail("bias_ids, bias_values and biases go together");
     if (!a.mask != !a.masks || (!a.mask && a.mask_rows)) return fail("mask, masks and mask_rows go together");
     if (a.mask && !a.mask_rows && a.masks < a.rows) return fail("fewer masks than rows without mask_rows");
     if (!a.top_n != !a.top_ids || (!a.top_n && a.top_logits)) return fail("top_n, top_ids and top_logits go together");
-    A.slices = (a.vocab + QXS_SLICE - 1) / QXS_SLICE;
+    // few rows: small slices, so that the launch is not a few workgroups' chain of latencies
+    const uint32_t tokens = 4096 / type_size(a.type);   // of a small slice
+    A.small = (uint64_t)a.rows * ((a.vocab + QXS_SLICE - 1) / QXS_SLICE) < 256;
+    A.slices = (a.vocab + (A.small ? tokens : QXS_SLICE) - 1) / (A.small ? tokens : QXS_SLICE);
     A.words = (a.vocab + 31) / 32;
     const uint64_t keys = up16((uint64_t)a.rows * A.slices * 4 * a.top_n * 8), ms = up16((uint64_t)a.rows * A.slices * 4 * 8);
     A.keys = (uint64_t *)a.workspace;
