@@ -20,27 +20,22 @@ DEV float key_value(uint64_t k) {
     const uint32_t u = (uint32_t)(k >> 32);
     return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
 }
-// The n-th largest of the wave's 64 keys (unlike ones but for 0), found a bit at a time: 0 when fewer are
-// not 0.  The token bits are searched only where several keys share the n-th's rank.
+// A bound that exactly n of the wave's 64 keys reach (unlike ones but for 0), found a bit at a time until it
+// is one; 0 when fewer than n are not 0.  The token bits are searched only where several keys share the
+// n-th's rank.
 DEV uint64_t wave_nth(uint64_t k, uint32_t n) {
     const uint32_t hi = (uint32_t)(k >> 32), lo = (uint32_t)k;
-    uint32_t th = 0;
-#pragma unroll
-    for (int b = 31; b >= 0; --b)
-        if ((uint32_t)__popcll(__ballot(hi >= (th | 1u << b))) >= n) th |= 1u << b;
+    uint32_t th = 0, tl = 0;
+    for (int b = 31; b >= 0; --b) {
+        const uint32_t c = (uint32_t)__popcll(__ballot(hi >= (th | 1u << b)));
+        if (c >= n) th |= 1u << b;
+        if (c == n) return (uint64_t)th << 32;
+    }
     if (th == 0) return 0;
     const uint32_t above = (uint32_t)__popcll(__ballot(hi > th));
     const bool at = hi == th;
-    uint32_t tl = 0;
-    if (above + (uint32_t)__popcll(__ballot(at)) == n) {
-        uint32_t low = at ? lo : ~0u;   // the smallest of those
-#pragma unroll
-        for (int o = 32; o; o >>= 1) low = min(low, (uint32_t)__shfl_xor((int)low, o));
-        tl = low;
-    } else {
-        for (int b = 31; b >= 0; --b)
-            if (above + (uint32_t)__popcll(__ballot(at && lo >= (tl | 1u << b))) >= n) tl |= 1u << b;
-    }
+    for (int b = 31; b >= 0; --b)
+        if (above + (uint32_t)__popcll(__ballot(at && lo >= (tl | 1u << b))) >= n) tl |= 1u << b;
     return (uint64_t)th << 32 | tl;
 }
 // (maximum, sum of exp(x - maximum)) of two sets; NaN in the sum stays
@@ -63,8 +58,8 @@ template <typename T> struct Pack { T v[16 / sizeof(T)]; };
 // A workgroup takes a slice of a row, 16 bytes of it a thread and step.  It reads the row's whole history
 // and bias list and keeps those of its tokens in LDS (counts by integer atomics, biases summed in list
 // order by the first entry of each token), so the dense pass reads and writes each logit once.  The best
-// tokens: the n-th largest of a wave's 64 lanes' largest bounds the wave's n-th largest from below, and
-// so the slice's; at most n lanes of a wave reach it, so at most PER n of its keys do, about n / 2 of most
+// tokens: a bound that n of a wave's 64 lanes' largest reach bounds the wave's n-th largest from below, and
+// so the slice's; at most n lanes of a wave reach the slice's, so at most PER n of its keys do, about n / 2 of most
 // rows.  Only of more than n are the n largest taken, by counting.
 template <typename T, int STEPS>
 __global__ __launch_bounds__(256) void qxs_slice(QxsArgs A) {
@@ -77,6 +72,7 @@ __global__ __launch_bounds__(256) void qxs_slice(QxsArgs A) {
     __shared__ uint32_t s_ids[QXS_BIASES];
     __shared__ float s_sum[QXS_BIASES];
     __shared__ uint64_t s_least[4];
+    __shared__ uint32_t s_twice;
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
     const uint32_t r = blockIdx.y, v0 = blockIdx.x * SLICE, V = A.a.vocab;
     const T *in = (const T *)A.a.logits + r * A.a.logits_row + v0;
@@ -112,6 +108,7 @@ __global__ __launch_bounds__(256) void qxs_slice(QxsArgs A) {
     }
     const bool sparse = slots || A.a.biases;
     if (sparse) {
+        if (tid == 0) s_twice = 0;
 #pragma unroll
         for (int i = 0; i < PER / 4; ++i) reinterpret_cast<nt4 *>(u.token)[i * 256 + tid] = nt4{0, 0, 0, 0};
         for (uint32_t i = tid; i < A.a.biases; i += 256) {
@@ -141,11 +138,18 @@ __global__ __launch_bounds__(256) void qxs_slice(QxsArgs A) {
 #pragma unroll
         for (int k = 0; k < EARLY; ++k) note(tid + 256 * k, early[k]);
         for (uint32_t i = tid + 256 * EARLY; i < entries; i += 256) note(i, hist[i]);
-        if (A.a.biases) {
-            float sum[QXS_BIASES / 256];
-            bool first[QXS_BIASES / 256];   // entry tid + 256 k is its token's first
+        constexpr int EACH = QXS_BIASES / 256;
 #pragma unroll
-            for (int k = 0; k < (int)QXS_BIASES / 256; ++k) {
+        for (int k = 0; k < EACH; ++k) {
+            const uint32_t i = tid + 256 * k, v = i < A.a.biases ? s_ids[i] : QXG_NO_TOKEN;
+            if (v - v0 < here && (atomicOr(&u.token[v - v0], HAS_BIAS | i << BIAS_SHIFT) & HAS_BIAS)) s_twice = 1;
+        }
+        if (A.a.biases) __syncthreads();
+        if (A.a.biases && s_twice) {   // (uniform) a token of several entries: its first one takes the sum, in order
+            float sum[EACH];
+            bool first[EACH];
+#pragma unroll
+            for (int k = 0; k < EACH; ++k) {
                 const uint32_t i = tid + 256 * k, v = i < A.a.biases ? s_ids[i] : QXG_NO_TOKEN;
                 first[k] = v - v0 < here;
                 if (!first[k]) continue;
@@ -154,11 +158,11 @@ __global__ __launch_bounds__(256) void qxs_slice(QxsArgs A) {
                 sum[k] = s_sum[i];
                 for (uint32_t j = i + 1; j < A.a.biases; ++j)
                     if (s_ids[j] == v) sum[k] += s_sum[j];
-                atomicOr(&u.token[v - v0], HAS_BIAS | i << BIAS_SHIFT);
+                u.token[v - v0] = (u.token[v - v0] & ~((QXS_BIASES - 1) << BIAS_SHIFT)) | i << BIAS_SHIFT;
             }
             __syncthreads();   // every entry's own value is read
 #pragma unroll
-            for (int k = 0; k < (int)QXS_BIASES / 256; ++k)
+            for (int k = 0; k < EACH; ++k)
                 if (first[k]) s_sum[tid + 256 * k] = sum[k];
         }
         __syncthreads();

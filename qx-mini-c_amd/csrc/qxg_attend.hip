@@ -3,8 +3,10 @@
 // Mathematics.  s = dot * ks[pos] * scale with dot = q . code.  The codes are exact in fp16; q is
 // scaled by a power of two into [2^13, 2^14) and taken as fp16 (16-bit q: exact) or hi + lo (f32 q:
 // 22 bits), so the matrix cores' f32 sums are those of f32 products.  The softmax runs in base 2 in
-// one pass with a running maximum and denominator a column; weights times vs[pos] go into the second
-// product as fp16 (hi + lo for f32) under a power-of-two scale of the column in the chunk.
+// one pass: a column keeps a reference M, the sum of e = 2^(s - M) and the context, the sum of e vs[pos] v.
+// M follows the running maximum to within 2^8 and is shifted by a power of two that keeps e vs, which enters
+// the second product as fp16 (hi + lo for f32 and f16 values, whose own rounding is not coarser than
+// that of 11 bits), in fp16's range; it cancels in the end.
 //
 // Tiles.  v_mfma_f32_32x32x16_f16, rows positions, columns (node, q head of the kv head).  Lane half h
 // of A and B holds dims (D / 2) h + 8 s + j of k-step s, so a lane's K codes are D / 2 consecutive
@@ -84,14 +86,147 @@ template <int D> DEV uint4 k_step(const KRow<D> &x, int s) {
 }
 }  // namespace
 
-// A workgroup takes a tile of columns of one kv head and a run of 32-position chunks; its 4 waves take
-// every fourth chunk, each with its own running maximum, denominator and context, merged at the end.
+namespace {
+// A column's softmax state.  Both halves of a wave hold their columns' m, M and limit; den is each lane's own
+// sum.  m (the maximum, rounded, as of the last time that it grew by 8) and M are whole numbers, so that
+// moving M and scaling what has been summed by the power of two that belongs to it agree exactly.
+template <int D> struct State {
+    float m = -INFINITY, M = -INFINITY, den = 0.0f, limit = 0.0f;   // limit: the largest e vs before M has to move
+    f16x acc[D / 32];
+    DEV State() {
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) acc[d] = zero16();
+    }
+    DEV void rescale(float f) {
+        den *= f;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[d][r] *= f;
+    }
+};
+DEV float max_of_halves(float v) {   // of lanes l and l ^ 32
+    const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+}
+template <typename T> constexpr bool two_halves_q = sizeof(T) == 4;
+template <typename T> constexpr bool two_halves_p = !__is_same(T, __bf16);
+
+// The chunk's scores (dots, not yet scaled) into weights: phi, plo the second product's operands.  ks, vs: the
+// scales of the chunk's 32 positions; bits: those that the column sees (edge: some do not).
+template <typename T, int D>
+DEV void weigh(State<D> &S, f16x dot, float sf, const float *ks, const float *vs, bool edge, uint32_t bits, int h, uint4 (&phi)[2],
+               uint4 (&plo)[2]) {
+    float s[16], cmax = -INFINITY, pmx = 0.0f;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const f4x k4 = *reinterpret_cast<const f4x *>(ks + 8 * q + 4 * h);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[4 * q + r] = dot[4 * q + r] * k4[r];
+    }
+    if (edge) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = seen(bits, r, h) ? s[r] : -INFINITY;
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) cmax = fmaxf(cmax, s[r]);
+    cmax = max_of_halves(cmax) * sf;   // (sf > 0, or NaN)
+    if (__ballot(cmax > S.m + 8.0f) != 0) {   // (whole wave)
+        const bool grow = cmax > S.m + 8.0f;
+        const float mn = rintf(cmax);
+        S.rescale(!grow || S.m == -INFINITY ? 1.0f : exp2_fast(S.m - mn));
+        if (grow) {
+            S.M = S.m == -INFINITY ? mn : mn - (S.m - S.M);
+            S.m = mn;
+        }
+    }
+    const float M = S.M == -INFINITY ? 0.0f : S.M;
+    float p[16], den = 0.0f;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const f4x v4 = *reinterpret_cast<const f4x *>(vs + 8 * q + 4 * h);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float e = exp2_fast(fmaf(s[4 * q + r], sf, -M));
+            den += e;
+            p[4 * q + r] = e * v4[r];
+        }
+    }
+    if (edge) {   // (a masked position's scales do not count, whatever they are; fma(-inf, NaN) is NaN)
+        if (sf != sf && bits == 0) den = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) p[r] = seen(bits, r, h) ? p[r] : 0.0f;
+    }
+    S.den += den;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) pmx = fmaxf(pmx, fabsf(p[r]));
+    pmx = max_of_halves(pmx);
+    if (__ballot(pmx > S.limit) != 0) {   // the first weights of a column, or one beyond fp16
+        const bool move = pmx > S.limit && pmx < INFINITY;
+        // to [2^6, 2^7), but e itself (up to 2^8 times the shift) stays far inside f32
+        int k = (int)(__float_as_uint(pow2_scale(pmx, 7)) >> 23) - 127;
+        k = move ? min(k, 96 - (int)(S.m - M)) : 0;
+        const float f = __uint_as_float((uint32_t)(127 + max(k, -126)) << 23);
+        if (move) {
+            S.M = M - (float)max(k, -126);
+            S.limit = 32768.0f;
+        }
+        S.rescale(f);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) p[r] *= f;
+    }
+    if constexpr (two_halves_p<T>) {
+        split8(p, 1.0f, phi[0], plo[0]);
+        split8(p + 8, 1.0f, phi[1], plo[1]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            h8v x;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = (_Float16)p[8 * i + j];
+            phi[i] = __builtin_bit_cast(uint4, x);
+        }
+    }
+}
+// a column's result: out and lse, or with several splits its state
+template <typename T, int D>
+DEV void finish_column(const QxaArgs &A, const State<D> &S, float den, uint32_t b, uint32_t node, uint32_t head, int h) {
+    const uint64_t row = ((uint64_t)b * A.a.nodes + node) * A.a.heads + head;
+    if (A.splits == 1) {
+        const float inv = den == 0.0f ? 0.0f : 1.0f / den;
+        T *out = (T *)A.a.out + b * A.a.out_batch + node * A.a.out_node + head * D;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                store4(out + 32 * d + 8 * k + 4 * h, make_float4(S.acc[d][4 * k] * inv, S.acc[d][4 * k + 1] * inv,
+                                                                 S.acc[d][4 * k + 2] * inv, S.acc[d][4 * k + 3] * inv));
+        if (h == 0 && A.lse) A.lse[row] = den == 0.0f ? -INFINITY : (S.M + __log2f(den)) * 0.69314718055994531f;
+    } else {
+        const uint64_t at = (uint64_t)blockIdx.y * A.a.batch * A.a.nodes * A.a.heads + row;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                store4(A.part + at * D + 32 * d + 8 * k + 4 * h,
+                       make_float4(S.acc[d][4 * k], S.acc[d][4 * k + 1], S.acc[d][4 * k + 2], S.acc[d][4 * k + 3]));
+        if (h == 0) A.md[at] = make_float2(S.M, den);
+    }
+}
+}  // namespace
+
+// Few columns (a tile or two a kv head).  A workgroup takes a tile of columns of one kv head and a run of
+// 32-position chunks; its 4 waves take every fourth chunk, each with a state of its own, merged at the end.  The
+// next chunk's rows are on their way while one is worked on.  The cache's bytes, or with few of them the
+// chain of latencies, bound it.
 template <typename T, int D>
 __global__ __launch_bounds__(256, 2) void qxa_tree(QxaArgs A) {
-    constexpr bool SPLIT = sizeof(T) == 4;
+    constexpr bool SPLIT = two_halves_q<T>;
     constexpr int KS = D / 16, DT = D / 32, NP = SPLIT ? 2 : 1;
     __shared__ uint4 s_q[KS * NP * 64];
-    __shared__ float s_sf[32], s_ks[4][32], s_vs[4][32], s_m[2][32], s_den[2][32];
+    __shared__ float s_sf[32];
+    __shared__ __align__(16) float s_ks[4][32], s_vs[4][32];
+    __shared__ float s_m[2][32], s_den[2][32];
     __shared__ union { uint32_t vt[4][D * 9]; float acc[2][32][D + 1]; } u;
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), col = lane & 31, h = lane >> 5;
     const uint32_t g = blockIdx.x / A.tiles, tile = blockIdx.x % A.tiles, b = blockIdx.z;
@@ -101,6 +236,22 @@ __global__ __launch_bounds__(256, 2) void qxa_tree(QxaArgs A) {
     if (tile * 32 / A.group >= q.count) return;   // the whole tile is behind count
     const uint32_t total = q.len + q.count, nchunk = (total + 31) / 32;
     const uint32_t c_lo = (uint64_t)nchunk * blockIdx.y / A.splits, c_hi = (uint64_t)nchunk * (blockIdx.y + 1) / A.splits;
+    struct { KRow<D> k; uint32_t v[4 * DT]; float ks, vs; } nx;
+    auto load = [&](uint32_t ci) {   // (rows past the last read it again)
+        const uint32_t pb = ci * 32, pk = min(pb + col, total - 1);
+        nx.k = load_k<D>(A, b, g, pk, h);
+        nx.ks = A.a.kscale[b * A.a.scale_batch + pk];
+        nx.vs = A.a.vscale[b * A.a.scale_batch + pk];
+#pragma unroll
+        for (int i = 0; i < DT; ++i) {   // 4 positions x 4 dims of bytes a lane and step
+            const int bq = lane + 64 * i, dq = bq % (D / 4), pq = bq / (D / 4);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                nx.v[4 * i + r] = *reinterpret_cast<const uint32_t *>(A.a.v + b * A.a.kv_batch + min(pb + 4 * pq + r, total - 1) * A.a.kv_row +
+                                                                      g * D + 4 * dq);
+        }
+    };
+    if (c_lo + wave < c_hi) load(c_lo + wave);
     {   // q fragments: a thread takes D / 8 dims of a column
         const int qc = tid >> 3, seg = tid & 7;
         const uint32_t cc = tile * 32 + qc, n = cc / A.group;
@@ -133,27 +284,20 @@ __global__ __launch_bounds__(256, 2) void qxa_tree(QxaArgs A) {
     }
     __syncthreads();
     const float sf = s_sf[col];
-    float m = -INFINITY, den = 0.0f;
-    f16x acc[DT];
-#pragma unroll
-    for (int d = 0; d < DT; ++d) acc[d] = zero16();
+    State<D> S;
     uint32_t *vt = u.vt[wave];
 #pragma unroll 1
     for (uint32_t ci = c_lo + wave; ci < c_hi; ci += 4) {
-        const uint32_t pb = ci * 32, pk = min(pb + col, total - 1);   // (rows past the last read it again)
-        const KRow<D> kr = load_k<D>(A, b, g, pk, h);
+        const uint32_t pb = ci * 32;
+        const KRow<D> kr = nx.k;
         if (lane < 32) {
-            s_ks[wave][lane] = A.a.kscale[b * A.a.scale_batch + pk];
-            s_vs[wave][lane] = A.a.vscale[b * A.a.scale_batch + pk];
+            s_ks[wave][lane] = nx.ks;
+            s_vs[wave][lane] = nx.vs;
         }
-        // V transposed: 4 positions x 4 dims of bytes a lane and step
 #pragma unroll
         for (int i = 0; i < DT; ++i) {
-            const int bq = lane + 64 * i, pq = bq & 7, dq = bq >> 3;
-            uint32_t w[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                w[r] = *reinterpret_cast<const uint32_t *>(A.a.v + b * A.a.kv_batch + min(pb + 4 * pq + r, total - 1) * A.a.kv_row + g * D + 4 * dq);
+            const int bq = lane + 64 * i, dq = bq % (D / 4), pq = bq / (D / 4);
+            const uint32_t *w = nx.v + 4 * i;
             const uint32_t a0 = perm(w[1], w[0], 0x05010400u), a1 = perm(w[3], w[2], 0x05010400u);
             const uint32_t a2 = perm(w[1], w[0], 0x07030602u), a3 = perm(w[3], w[2], 0x07030602u);
             vt[(4 * dq + 0) * 9 + pq] = perm(a1, a0, 0x05040100u);
@@ -162,63 +306,31 @@ __global__ __launch_bounds__(256, 2) void qxa_tree(QxaArgs A) {
             vt[(4 * dq + 3) * 9 + pq] = perm(a3, a2, 0x07060302u);
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        f16x sh = zero16(), sl = zero16();
+        if (ci + 4 < c_hi) load(ci + 4);
+        f16x dot = zero16();
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             const uint4 kf = k_step<D>(kr, s);
-            sh = mfma(kf, s_q[(s * NP) * 64 + lane], sh);
-            if (SPLIT) sl = mfma(kf, s_q[(s * NP + 1) * 64 + lane], sl);
+            if (SPLIT) dot = mfma(kf, s_q[(s * NP + 1) * 64 + lane], dot);
+            dot = mfma(kf, s_q[(s * NP) * 64 + lane], dot);
         }
         const bool edge = pb + 32 > q.len;   // the chunk holds nodes
         const uint32_t bits = edge ? visible(A, q, b, node, pb) : ~0u;
-        float sc[16], e[16], pv[16], cmax = -INFINITY, pmx = 0.0f;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const float k = s_ks[wave][8 * (r >> 2) + 4 * h + (r & 3)];
-            sc[r] = (SPLIT ? sh[r] + sl[r] : sh[r]) * k * sf;
-            if (edge) sc[r] = seen(bits, r, h) ? sc[r] : -INFINITY;
-            cmax = fmaxf(cmax, sc[r]);
-        }
-        cmax = fmaxf(cmax, __shfl_xor(cmax, 32));
-        if (__ballot(cmax > m + 8.0f) != 0) {
-            const float mn = fmaxf(m, cmax), alpha = m == mn ? 1.0f : exp2_fast(m - mn);
-            m = mn;
-            den *= alpha;
-#pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) acc[d][r] *= alpha;
-        }
-        const float mm = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            e[r] = exp2_fast(sc[r] - mm);
-            pv[r] = e[r] * s_vs[wave][8 * (r >> 2) + 4 * h + (r & 3)];
-            if (edge) pv[r] = seen(bits, r, h) ? pv[r] : 0.0f;
-            den += e[r];
-            pmx = fmaxf(pmx, fabsf(pv[r]));
-        }
-        pmx = fmaxf(pmx, __shfl_xor(pmx, 32));
-        const float psc = pow2_scale(pmx, 15), pinv = 1.0f / psc;
         uint4 phi[2], plo[2];
-        split8(pv, psc, phi[0], plo[0]);
-        split8(pv + 8, psc, phi[1], plo[1]);
+        weigh<T, D>(S, dot, sf, s_ks[wave], s_vs[wave], edge, bits, h, phi, plo);
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
-            f16x x = zero16();
             const uint32_t *row = vt + (32 * d + col) * 9;
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
                 const uint4 vf = i8x8_to_f16(row[4 * s + h], row[4 * s + 2 + h]);
-                x = mfma(vf, phi[s], x);
-                if (SPLIT) x = mfma(vf, plo[s], x);
+                if constexpr (two_halves_p<T>) S.acc[d] = mfma(vf, plo[s], S.acc[d]);
+                S.acc[d] = mfma(vf, phi[s], S.acc[d]);
             }
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[d][r] = fmaf(x[r], pinv, acc[d][r]);
         }
     }
     // merge the 4 waves: 2 + 3 into 0 + 1, then 1 into 0
-    den += __shfl_xor(den, 32);
+    float den = S.den + __shfl_xor(S.den, 32);
     __syncthreads();
 #pragma unroll 1
     for (int nw = 2; nw; nw >>= 1) {
@@ -227,71 +339,185 @@ __global__ __launch_bounds__(256, 2) void qxa_tree(QxaArgs A) {
 #pragma unroll
             for (int d = 0; d < DT; ++d)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) u.acc[slot][col][32 * d + 8 * (r >> 2) + 4 * h + (r & 3)] = acc[d][r];
-            if (h == 0) { s_m[slot][col] = m; s_den[slot][col] = den; }
+                for (int r = 0; r < 16; ++r) u.acc[slot][col][32 * d + 8 * (r >> 2) + 4 * h + (r & 3)] = S.acc[d][r];
+            if (h == 0) { s_m[slot][col] = S.M; s_den[slot][col] = den; }
         }
         __syncthreads();
         if (wave < nw) {
-            const float mo = s_m[wave][col], mn = fmaxf(m, mo);
-            const float fa = m == mn ? 1.0f : exp2_fast(m - mn), fb = mo == mn ? 1.0f : exp2_fast(mo - mn);
+            const float mo = s_m[wave][col], mn = fmaxf(S.M, mo);
+            const float fa = S.M == mn ? 1.0f : exp2_fast(S.M - mn), fb = mo == mn ? 1.0f : exp2_fast(mo - mn);
 #pragma unroll
             for (int d = 0; d < DT; ++d)
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    acc[d][r] = acc[d][r] * fa + u.acc[wave][col][32 * d + 8 * (r >> 2) + 4 * h + (r & 3)] * fb;
+                    S.acc[d][r] = S.acc[d][r] * fa + u.acc[wave][col][32 * d + 8 * (r >> 2) + 4 * h + (r & 3)] * fb;
             den = den * fa + s_den[wave][col] * fb;
-            m = mn;
+            S.M = mn;
         }
         __syncthreads();
     }
-    if (wave == 0 && used) {
-        const uint64_t row = ((uint64_t)b * A.a.nodes + node) * A.a.heads + head;
-        if (A.splits == 1) {
-            const float inv = den == 0.0f ? 0.0f : 1.0f / den;
-            T *out = (T *)A.a.out + b * A.a.out_batch + node * A.a.out_node + head * D;
-#pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    store4(out + 32 * d + 8 * k + 4 * h,
-                           make_float4(acc[d][4 * k] * inv, acc[d][4 * k + 1] * inv, acc[d][4 * k + 2] * inv, acc[d][4 * k + 3] * inv));
-            if (h == 0 && A.lse) A.lse[row] = den == 0.0f ? -INFINITY : (m + __log2f(den)) * 0.69314718055994531f;
-        } else {
-            const uint64_t at = (uint64_t)blockIdx.y * A.a.batch * A.a.nodes * A.a.heads + row;
-#pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    store4(A.part + at * D + 32 * d + 8 * k + 4 * h,
-                           make_float4(acc[d][4 * k], acc[d][4 * k + 1], acc[d][4 * k + 2], acc[d][4 * k + 3]));
-            if (h == 0) A.md[at] = make_float2(m, den);
-        }
-    }
+    if (wave == 0 && used) finish_column<T, D>(A, S, den, b, node, head, h);
 }
 
-// The splits of a row joined: a wave a row, splits in order.
+// Many columns.  The 4 waves of a workgroup take a tile of 32 columns of one kv head each and go through the
+// same chunks of 4096 / D positions, whose codes the workgroup stages in LDS as fp16 (K by rows; V
+// transposed, a dim's 32 positions in the order of the second product's k): one conversion of a code
+// for 128 columns.  Two buffers, so one barrier a chunk; the next chunk's codes are on their way.
+// The softmax's vector work and the matrix products bound it, each about 1000 cycles a tile and chunk.
+template <typename T, int D>
+__global__ __launch_bounds__(256, 2) void qxa_wide(QxaArgs A) {
+    constexpr bool SPLIT = two_halves_q<T>;
+    constexpr int KS = D / 16, DT = D / 32, SUB = 128 / D, CP = 32 * SUB;
+    constexpr int KP = D + 8, VP = 40;   // fp16 from one row to the next: 16 rows' 16-byte pieces lie in 16 bank groups
+    __shared__ __align__(16) _Float16 s_k[2][CP * KP], s_v[2][SUB * D * VP];
+    __shared__ __align__(16) float s_ks[2][CP], s_vs[2][CP];
+    const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), col = lane & 31, h = lane >> 5;
+    const uint32_t wgs = (A.tiles + 3) / 4, g = blockIdx.x / wgs, tile = blockIdx.x % wgs * 4 + wave, b = blockIdx.z;
+    const Seq q = sequence(A, b);
+    if (blockIdx.x % wgs * 128 / A.group >= q.count) return;   // all tiles are behind count
+    const uint32_t c = tile * 32 + col, node = min(c / A.group, A.a.nodes - 1), head = g * A.group + c % A.group;
+    const bool busy = tile < A.tiles && tile * 32 / A.group < q.count, used = c < A.columns && node < q.count;   // busy: of the wave
+    const uint32_t total = q.len + q.count, nchunk = (total + CP - 1) / CP;
+    const uint32_t c_lo = (uint64_t)nchunk * blockIdx.y / A.splits, c_hi = (uint64_t)nchunk * (blockIdx.y + 1) / A.splits;
+    // staging: K, a row's 16 bytes a thread; V, 4 positions x 4 dims
+    const int kpos = tid / (D / 16), kpiece = tid % (D / 16), dq = tid % (D / 4), pq = tid / (D / 4);
+    const int8_t *kbase = A.a.k + b * A.a.kv_batch + g * D + 16 * kpiece, *vbase = A.a.v + b * A.a.kv_batch + g * D + 4 * dq;
+    const float *ksb = A.a.kscale + b * A.a.scale_batch, *vsb = A.a.vscale + b * A.a.scale_batch;
+    nt4 nk;
+    uint32_t nv[4];
+    float ns = 0.0f;
+    auto load = [&](uint32_t ci) {
+        const uint32_t pb = ci * CP;
+        nk = *reinterpret_cast<const nt4 *>(kbase + min(pb + kpos, total - 1) * A.a.kv_row);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) nv[r] = *reinterpret_cast<const uint32_t *>(vbase + min(pb + 4 * pq + r, total - 1) * A.a.kv_row);
+        if (tid < 2 * CP) ns = (tid < CP ? ksb : vsb)[min(pb + tid % CP, total - 1)];
+    };
+    if (c_lo < c_hi) load(c_lo);
+    uint4 qh[KS], ql[SPLIT ? KS : 1];
+    float sf = 0.0f;
+    if (busy) {   // q fragments: a lane holds its column's D / 2 dims of its half
+        const T *row = (const T *)A.a.q + b * A.a.q_batch + (used ? node : 0) * A.a.q_node + (used ? head : g * A.group) * D + (D / 2) * h;
+        float mx = 0.0f;
+        bool fin = true;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            float v[8];
+            load8(row + 8 * s, v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) { fin = fin && isfinite(v[j]); mx = fmaxf(mx, fabsf(v[j])); }
+        }
+        mx = max_of_halves(fin ? mx : INFINITY);
+        const bool bad = !(mx < INFINITY);
+        const float sc = pow2_scale(bad ? 0.0f : mx, 14);
+        sf = bad ? NAN : A.scale2 / sc;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {   // (read again, from the caches: all of it at once would not fit the registers)
+            float v[8];
+            load8(row + 8 * s, v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = bad ? 0.0f : v[j];
+            uint4 lo;
+            split8(v, sc, qh[s], lo);
+            if constexpr (SPLIT) ql[s] = lo;
+        }
+    }
+    State<D> S;
+    int buf = 0;
+#pragma unroll 1
+    for (uint32_t ci = c_lo; ci < c_hi; ++ci, buf ^= 1) {
+        {
+            uint4 *to = reinterpret_cast<uint4 *>(&s_k[buf][kpos * KP + 16 * kpiece]);
+            to[0] = i8x8_to_f16(nk.x, nk.y);
+            to[1] = i8x8_to_f16(nk.z, nk.w);
+            const uint32_t a0 = perm(nv[1], nv[0], 0x05010400u), a1 = perm(nv[3], nv[2], 0x05010400u);
+            const uint32_t a2 = perm(nv[1], nv[0], 0x07030602u), a3 = perm(nv[3], nv[2], 0x07030602u);
+            const uint4 v01 = i8x8_to_f16(perm(a1, a0, 0x05040100u), perm(a1, a0, 0x07060302u));
+            const uint4 v23 = i8x8_to_f16(perm(a3, a2, 0x05040100u), perm(a3, a2, 0x07060302u));
+            // positions 4 w .. 4 w + 3 (w = pq % 8) are half w / 2 % 2 of the 16 bytes that lane half w % 2 reads in step
+            // w / 4; the place of the 16 bytes turns with dim / 16, so that the lanes' writes spread over the banks
+            const int w = pq & 7, slot = ((w >> 2) * 2 + (w & 1)) ^ ((dq >> 2) & 3);
+            uint2 *vd = reinterpret_cast<uint2 *>(&s_v[buf][((pq >> 3) * D + 4 * dq) * VP + 8 * slot + 4 * ((w >> 1) & 1)]);
+            vd[0] = make_uint2(v01.x, v01.y);
+            vd[VP / 4] = make_uint2(v01.z, v01.w);
+            vd[2 * (VP / 4)] = make_uint2(v23.x, v23.y);
+            vd[3 * (VP / 4)] = make_uint2(v23.z, v23.w);
+            if (tid < 2 * CP) (tid < CP ? s_ks : s_vs)[buf][tid % CP] = ns;
+        }
+        if (ci + 1 < c_hi) load(ci + 1);
+        __syncthreads();
+        if (!busy) continue;
+#pragma unroll
+        for (int sub = 0; sub < SUB; ++sub) {
+            const uint32_t pb = ci * CP + 32 * sub;
+            if (SUB > 1 && pb >= total) break;
+            f16x dot = zero16();
+            const _Float16 *kr = &s_k[buf][(32 * sub + col) * KP + (D / 2) * h];
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                const uint4 kf = *reinterpret_cast<const uint4 *>(kr + 8 * s);
+                if constexpr (SPLIT) dot = mfma(kf, ql[s], dot);
+                dot = mfma(kf, qh[s], dot);
+            }
+            const bool edge = pb + 32 > q.len;
+            const uint32_t bits = edge ? visible(A, q, b, node, pb) : ~0u;
+            uint4 phi[2], plo[2];
+            weigh<T, D>(S, dot, sf, &s_ks[buf][32 * sub], &s_vs[buf][32 * sub], edge, bits, h, phi, plo);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                const _Float16 *vr = &s_v[buf][(sub * D + 32 * d + col) * VP];
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    const uint4 vf = *reinterpret_cast<const uint4 *>(vr + 8 * ((2 * s + h) ^ ((2 * d + (col >> 4)) & 3)));
+                    if constexpr (two_halves_p<T>) S.acc[d] = mfma(vf, plo[s], S.acc[d]);
+                    S.acc[d] = mfma(vf, phi[s], S.acc[d]);
+                }
+            }
+        }
+    }
+    const float den = S.den + __shfl_xor(S.den, 32);
+    if (busy && used) finish_column<T, D>(A, S, den, b, node, head, h);
+}
+
+// The splits of a row joined: a workgroup a row, its 256 / (D / 4) strips of threads every so many splits, the
+// strips in order.  (A wave a row, a split's state after the other: 12 us for 32 splits of 128 rows.)
 template <typename T, int D>
 __global__ __launch_bounds__(256) void qxa_join(QxaArgs A) {
-    const uint64_t rows = (uint64_t)A.a.batch * A.a.nodes * A.a.heads, row = blockIdx.x * 4ull + wave_id();
-    if (row >= rows) return;
-    const int lane = threadIdx.x & 63;
+    constexpr int W = D / 4, STRIPS = 256 / W;
+    __shared__ float s_m[STRIPS], s_den[STRIPS];
+    __shared__ __align__(16) float s_v[STRIPS][D];
+    const uint64_t rows = (uint64_t)A.a.batch * A.a.nodes * A.a.heads, row = blockIdx.x;
+    const int at = threadIdx.x % W, strip = threadIdx.x / W;
     const uint32_t head = row % A.a.heads, node = row / A.a.heads % A.a.nodes, b = row / A.a.heads / A.a.nodes;
     if (node >= sequence(A, b).count) return;
-    float m = -INFINITY, den = 0.0f, v[D / 64] = {};
-    for (uint32_t z = 0; z < A.splits; ++z) m = fmaxf(m, A.md[z * rows + row].x);
-    for (uint32_t z = 0; z < A.splits; ++z) {
-        const uint64_t at = z * rows + row;
-        const float2 s = A.md[at];
-        const float f = s.x == m ? 1.0f : exp2_fast(s.x - m);
-        den = fmaf(f, s.y, den);
+    float m = -INFINITY, den = 0.0f;
+    f4x v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (uint32_t z = strip; z < A.splits; z += STRIPS) {
+        const float2 s = A.md[z * rows + row];
+        const f4x x = *reinterpret_cast<const f4x *>(A.part + (z * rows + row) * D + 4 * at);
+        const float mn = fmaxf(m, s.x), f = m == mn ? 1.0f : exp2_fast(m - mn), fz = s.x == mn ? 1.0f : exp2_fast(s.x - mn);
+        den = fmaf(den, f, s.y * fz);
 #pragma unroll
-        for (int i = 0; i < D / 64; ++i) v[i] = fmaf(f, A.part[at * D + 64 * i + lane], v[i]);
+        for (int i = 0; i < 4; ++i) v[i] = fmaf(v[i], f, x[i] * fz);
+        m = mn;
+    }
+    if (at == 0) { s_m[strip] = m; s_den[strip] = den; }
+    *reinterpret_cast<f4x *>(&s_v[strip][4 * at]) = v;
+    __syncthreads();
+    if (threadIdx.x >= W) return;
+#pragma unroll
+    for (int k = 1; k < STRIPS; ++k) {
+        const float mn = fmaxf(m, s_m[k]), f = m == mn ? 1.0f : exp2_fast(m - mn), fz = s_m[k] == mn ? 1.0f : exp2_fast(s_m[k] - mn);
+        const f4x x = *reinterpret_cast<const f4x *>(&s_v[k][4 * at]);
+        den = fmaf(den, f, s_den[k] * fz);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = fmaf(v[i], f, x[i] * fz);
+        m = mn;
     }
     const float inv = den == 0.0f ? 0.0f : 1.0f / den;
-    T *out = (T *)A.a.out + b * A.a.out_batch + node * A.a.out_node + head * D;
-#pragma unroll
-    for (int i = 0; i < D / 64; ++i) out[64 * i + lane] = (T)(v[i] * inv);
-    if (lane == 0 && A.lse) A.lse[row] = den == 0.0f ? -INFINITY : (m + __log2f(den)) * 0.69314718055994531f;
+    store4((T *)A.a.out + b * A.a.out_batch + node * A.a.out_node + head * D + 4 * at, make_float4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv));
+    if (at == 0 && A.lse) A.lse[row] = den == 0.0f ? -INFINITY : (m + __log2f(den)) * 0.69314718055994531f;
 }
 
 // account[p] = decay * account[p] + sum over nodes and heads of 2^(s - lse).  A workgroup takes 32
@@ -373,8 +599,9 @@ __global__ __launch_bounds__(256) void qxa_account(QxaArgs A) {
 namespace {
 template <typename T, int D> void launch(const QxaArgs &A, hipStream_t s) {
     const uint64_t rows = (uint64_t)A.a.batch * A.a.nodes * A.a.heads;
-    hipLaunchKernelGGL((qxa_tree<T, D>), dim3(A.a.kv_heads * A.tiles, A.splits, A.a.batch), dim3(256), 0, s, A);
-    if (A.splits > 1) hipLaunchKernelGGL((qxa_join<T, D>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, A);
+    if (A.wide) hipLaunchKernelGGL((qxa_wide<T, D>), dim3(A.a.kv_heads * ((A.tiles + 3) / 4), A.splits, A.a.batch), dim3(256), 0, s, A);
+    else hipLaunchKernelGGL((qxa_tree<T, D>), dim3(A.a.kv_heads * A.tiles, A.splits, A.a.batch), dim3(256), 0, s, A);
+    if (A.splits > 1) hipLaunchKernelGGL((qxa_join<T, D>), dim3((unsigned)rows), dim3(256), 0, s, A);
     if (A.a.account) {
         const uint32_t chunks = (uint32_t)std::min<uint64_t>(65535, ((uint64_t)A.a.max_len + A.a.nodes + 31) / 32);
         hipLaunchKernelGGL((qxa_account<T, D>), dim3(chunks, A.a.batch), dim3(256), 0, s, A);

@@ -6,10 +6,11 @@
 
 // Tree attention.  A column is a (node, q head of the kv head) pair, node * group + head; a tile is
 // 32 columns.  With several splits of the positions, a split's unnormalised context goes to part
-// and its (maximum, denominator) in base 2 to md, at [split][batch][node][head].
+// and its (reference, denominator) in base 2 to md, at [split][batch][node][head].
 struct QxaArgs {
     qxg_tree_attention_args a;
     uint32_t group, columns, tiles, splits, words;
+    uint32_t wide;     // tiles four at a time, chunks staged for all of them
     float scale2;      // scale * log2(e)
     float *part;
     float2 *md;

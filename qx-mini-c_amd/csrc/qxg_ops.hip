@@ -66,11 +66,10 @@ template <size_t N> bool pointers_ok(const Arg (&args)[N], const Err &fail) {
 uint64_t up16(uint64_t v) { return (v + 15) & ~15ull; }
 
 // ---- tree attention
-// Splits of the positions: about 1024 workgroups (two fit a CU, twice over) of at least four 32-position
-// chunks, one a wave.
-uint32_t tree_splits(const qxg_tree_attention_args &a, uint32_t tiles) {
-    const uint64_t wgs = (uint64_t)a.kv_heads * tiles * a.batch, most = std::max<uint64_t>(1, ((uint64_t)a.max_len + a.nodes) / 128);
-    return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(1024 / wgs, most));
+// Splits of the positions: about 512 workgroups (two fit a CU) of at least four 32-position chunks.
+uint32_t tree_splits(const qxg_tree_attention_args &a, uint64_t wgs) {
+    const uint64_t most = std::max<uint64_t>(1, ((uint64_t)a.max_len + a.nodes) / 128);
+    return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(512 / wgs, most));
 }
 bool tree_plan(const qxg_tree_attention_args *p, QxaArgs &A, uint64_t &bytes, const Err &fail) {
     if (!p) return fail("invalid argument");
@@ -90,7 +89,8 @@ bool tree_plan(const qxg_tree_attention_args *p, QxaArgs &A, uint64_t &bytes, co
     A.group = a.heads / a.kv_heads;
     A.columns = a.nodes * A.group;
     A.tiles = (A.columns + 31) / 32;
-    A.splits = tree_splits(a, A.tiles);
+    A.wide = A.tiles > 2;
+    A.splits = tree_splits(a, (uint64_t)a.kv_heads * a.batch * (A.wide ? (A.tiles + 3) / 4 : A.tiles));
     A.words = (a.nodes + 31) / 32;
     A.scale2 = (float)((double)a.scale * 1.4426950408889634);
     const uint64_t rows = (uint64_t)a.batch * a.nodes * a.heads;
