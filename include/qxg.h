@@ -362,7 +362,7 @@ typedef struct qxg_tree_attention_args {
     uint64_t workspace_bytes;
     uint64_t q_batch, q_node;         /* strides in elements; 16 bytes divide the strides' sizes */
     uint64_t out_batch, out_node;
-    uint64_t kv_batch, kv_row;        /* of k and v, in bytes, multiples of 16 */
+    uint64_t kv_batch, kv_row;        /* of k and v, in bytes, multiples of 16; kv_row below 2^26 */
     uint64_t scale_batch;             /* of kscale and vscale, in floats */
     uint64_t account_batch;
     uint32_t type;

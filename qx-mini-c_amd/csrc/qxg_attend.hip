@@ -49,6 +49,37 @@ DEV Seq sequence(const QxaArgs &A, uint32_t b) {
     s.len = min(A.a.lens[b], A.a.positions - s.count);
     return s;
 }
+// The splits of sequence b: their number and where they start among all sequences' (the states in part and md
+// lie in that order).  About A.splits for the whole batch, shared out by the sequences' chunks of 32
+// positions, so that a split is about as long in each; beyond 64 sequences as many for each.
+struct Splits { uint32_t count, first; };
+DEV Splits splits_of(const QxaArgs &A, uint32_t b) {
+    Splits s;
+    if (A.a.batch > 64 || A.splits == 1) {
+        s.count = A.splits;
+        s.first = b * A.splits;
+        return s;
+    }
+    const uint32_t lane = threadIdx.x & 63;
+    uint32_t chunks = 0;
+    if (lane < A.a.batch) {
+        const Seq q = sequence(A, lane);
+        chunks = max(1u, (q.len + q.count + 31) / 32);
+    }
+    uint32_t all = chunks;
+#pragma unroll
+    for (int o = 32; o; o >>= 1) all += (uint32_t)__shfl_xor((int)all, o);
+    const uint32_t n = lane < A.a.batch ? min(min(chunks, A.grid_splits), max(1u, (uint32_t)((uint64_t)chunks * A.splits / all))) : 0u;
+    uint32_t run = n;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t x = (uint32_t)__shfl_up((int)run, o);
+        run += lane >= (uint32_t)o ? x : 0u;
+    }
+    s.count = (uint32_t)__builtin_amdgcn_readlane((int)n, (int)b);
+    s.first = (uint32_t)__builtin_amdgcn_readlane((int)(run - n), (int)b);
+    return s;
+}
 // The positions from p0 on that the node sees, as bits: the cached ones, then the mask's nodes
 DEV uint32_t visible(const QxaArgs &A, const Seq &q, uint32_t b, uint32_t node, uint32_t p0) {
     uint32_t bits, end = q.len + q.count;
@@ -112,8 +143,30 @@ DEV float max_of_halves(float v) {   // of lanes l and l ^ 32
 template <typename T> constexpr bool two_halves_q = sizeof(T) == 4;
 template <typename T> constexpr bool two_halves_p = !__is_same(T, __bf16);
 
+// v = hi + lo (+ 2^-22 of it), a conversion for two values and one mixed-precision fma a remainder (its factor is
+// hidden, or it becomes a conversion back and a subtraction)
+typedef float f2v __attribute__((ext_vector_type(2)));
+template <bool LO> DEV void split_pairs(const float *v, uint4 &hi, uint4 &lo) {
+    float minus = -1.0f;
+    asm("" : "+s"(minus));
+    uint32_t a[4], b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const f2v x = {v[2 * i], v[2 * i + 1]};
+        const h2v h = __builtin_convertvector(x, h2v);
+        a[i] = __builtin_bit_cast(uint32_t, h);
+        if constexpr (LO) {
+            const h2v l = {(_Float16)fmaf((float)h[0], minus, x[0]), (_Float16)fmaf((float)h[1], minus, x[1])};
+            b[i] = __builtin_bit_cast(uint32_t, l);
+        }
+    }
+    hi = make_uint4(a[0], a[1], a[2], a[3]);
+    if constexpr (LO) lo = make_uint4(b[0], b[1], b[2], b[3]);
+}
+
 // The chunk's scores (dots, not yet scaled) into weights: phi, plo the second product's operands.  ks, vs: the
-// scales of the chunk's 32 positions; bits: those that the column sees (edge: some do not).
+// scales of the chunk's 32 positions; bits: those that the column sees (edge: not all of them, for
+// some column; each of the two uses opens the word anew, or the tests of its bits move into every chunk).
 template <typename T, int D>
 DEV void weigh(State<D> &S, f16x dot, float sf, const float *ks, const float *vs, bool edge, uint32_t bits, int h, uint4 (&phi)[2],
                uint4 (&plo)[2]) {
@@ -125,8 +178,10 @@ DEV void weigh(State<D> &S, f16x dot, float sf, const float *ks, const float *vs
         for (int r = 0; r < 4; ++r) s[4 * q + r] = dot[4 * q + r] * k4[r];
     }
     if (edge) {
+        uint32_t w = bits;
+        asm volatile("" : "+v"(w));
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = seen(bits, r, h) ? s[r] : -INFINITY;
+        for (int r = 0; r < 16; ++r) s[r] = seen(w, r, h) ? s[r] : -INFINITY;
     }
 #pragma unroll
     for (int r = 0; r < 16; ++r) cmax = fmaxf(cmax, s[r]);
@@ -153,9 +208,11 @@ DEV void weigh(State<D> &S, f16x dot, float sf, const float *ks, const float *vs
         }
     }
     if (edge) {   // (a masked position's scales do not count, whatever they are; fma(-inf, NaN) is NaN)
-        if (sf != sf && bits == 0) den = 0.0f;
+        uint32_t w = bits;
+        asm volatile("" : "+v"(w));
+        if (sf != sf && w == 0) den = 0.0f;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) p[r] = seen(bits, r, h) ? p[r] : 0.0f;
+        for (int r = 0; r < 16; ++r) p[r] = seen(w, r, h) ? p[r] : 0.0f;
     }
     S.den += den;
 #pragma unroll
@@ -175,22 +232,12 @@ DEV void weigh(State<D> &S, f16x dot, float sf, const float *ks, const float *vs
 #pragma unroll
         for (int r = 0; r < 16; ++r) p[r] *= f;
     }
-    if constexpr (two_halves_p<T>) {
-        split8(p, 1.0f, phi[0], plo[0]);
-        split8(p + 8, 1.0f, phi[1], plo[1]);
-    } else {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            h8v x;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = (_Float16)p[8 * i + j];
-            phi[i] = __builtin_bit_cast(uint4, x);
-        }
-    }
+    for (int i = 0; i < 2; ++i) split_pairs<two_halves_p<T>>(p + 8 * i, phi[i], plo[i]);
 }
 // a column's result: out and lse, or with several splits its state
 template <typename T, int D>
-DEV void finish_column(const QxaArgs &A, const State<D> &S, float den, uint32_t b, uint32_t node, uint32_t head, int h) {
+DEV void finish_column(const QxaArgs &A, const State<D> &S, float den, uint32_t b, uint32_t node, uint32_t head, Splits sp, int h) {
     const uint64_t row = ((uint64_t)b * A.a.nodes + node) * A.a.heads + head;
     if (A.splits == 1) {
         const float inv = den == 0.0f ? 0.0f : 1.0f / den;
@@ -203,7 +250,7 @@ DEV void finish_column(const QxaArgs &A, const State<D> &S, float den, uint32_t 
                                                                  S.acc[d][4 * k + 2] * inv, S.acc[d][4 * k + 3] * inv));
         if (h == 0 && A.lse) A.lse[row] = den == 0.0f ? -INFINITY : (S.M + __log2f(den)) * 0.69314718055994531f;
     } else {
-        const uint64_t at = (uint64_t)blockIdx.y * A.a.batch * A.a.nodes * A.a.heads + row;
+        const uint64_t at = (uint64_t)(sp.first + blockIdx.y) * A.a.nodes * A.a.heads + node * A.a.heads + head;
 #pragma unroll
         for (int d = 0; d < D / 32; ++d)
 #pragma unroll
@@ -233,9 +280,10 @@ __global__ __launch_bounds__(256, 2) void qxa_tree(QxaArgs A) {
     const Seq q = sequence(A, b);
     const uint32_t c = tile * 32 + col, node = min(c / A.group, A.a.nodes - 1), head = g * A.group + c % A.group;
     const bool used = c < A.columns && node < q.count;
-    if (tile * 32 / A.group >= q.count) return;   // the whole tile is behind count
+    const Splits sp = splits_of(A, b);
+    if (tile * 32 / A.group >= q.count || blockIdx.y >= sp.count) return;   // the whole tile is behind count
     const uint32_t total = q.len + q.count, nchunk = (total + 31) / 32;
-    const uint32_t c_lo = (uint64_t)nchunk * blockIdx.y / A.splits, c_hi = (uint64_t)nchunk * (blockIdx.y + 1) / A.splits;
+    const uint32_t c_lo = (uint64_t)nchunk * blockIdx.y / sp.count, c_hi = (uint64_t)nchunk * (blockIdx.y + 1) / sp.count;
     struct { KRow<D> k; uint32_t v[4 * DT]; float ks, vs; } nx;
     auto load = [&](uint32_t ci) {   // (rows past the last read it again)
         const uint32_t pb = ci * 32, pk = min(pb + col, total - 1);
@@ -284,6 +332,11 @@ __global__ __launch_bounds__(256, 2) void qxa_tree(QxaArgs A) {
     }
     __syncthreads();
     const float sf = s_sf[col];
+    if (A.pack && blockIdx.y == 0) {   // the account's q
+        const uint64_t at = ((uint64_t)b * A.a.kv_heads + g) * A.tiles + tile;
+        for (int i = tid; i < KS * NP * 64; i += 256) A.pack[at * (KS * NP * 64) + i] = s_q[i];
+        if (tid < 32) A.pack_sf[at * 32 + tid] = s_sf[tid];
+    }
     State<D> S;
     uint32_t *vt = u.vt[wave];
 #pragma unroll 1
@@ -356,7 +409,7 @@ __global__ __launch_bounds__(256, 2) void qxa_tree(QxaArgs A) {
         }
         __syncthreads();
     }
-    if (wave == 0 && used) finish_column<T, D>(A, S, den, b, node, head, h);
+    if (wave == 0 && used) finish_column<T, D>(A, S, den, b, node, head, sp, h);
 }
 
 // Many columns.  The 4 waves of a workgroup take a tile of 32 columns of one kv head each and go through the
@@ -374,24 +427,34 @@ __global__ __launch_bounds__(256, 2) void qxa_wide(QxaArgs A) {
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), col = lane & 31, h = lane >> 5;
     const uint32_t wgs = (A.tiles + 3) / 4, g = blockIdx.x / wgs, tile = blockIdx.x % wgs * 4 + wave, b = blockIdx.z;
     const Seq q = sequence(A, b);
-    if (blockIdx.x % wgs * 128 / A.group >= q.count) return;   // all tiles are behind count
+    const Splits sp = splits_of(A, b);
+    if (blockIdx.x % wgs * 128 / A.group >= q.count || blockIdx.y >= sp.count) return;   // all tiles are behind count
     const uint32_t c = tile * 32 + col, node = min(c / A.group, A.a.nodes - 1), head = g * A.group + c % A.group;
     const bool busy = tile < A.tiles && tile * 32 / A.group < q.count, used = c < A.columns && node < q.count;   // busy: of the wave
     const uint32_t total = q.len + q.count, nchunk = (total + CP - 1) / CP;
-    const uint32_t c_lo = (uint64_t)nchunk * blockIdx.y / A.splits, c_hi = (uint64_t)nchunk * (blockIdx.y + 1) / A.splits;
-    // staging: K, a row's 16 bytes a thread; V, 4 positions x 4 dims
-    const int kpos = tid / (D / 16), kpiece = tid % (D / 16), dq = tid % (D / 4), pq = tid / (D / 4);
-    const int8_t *kbase = A.a.k + b * A.a.kv_batch + g * D + 16 * kpiece, *vbase = A.a.v + b * A.a.kv_batch + g * D + 4 * dq;
+    const uint32_t c_lo = (uint64_t)nchunk * blockIdx.y / sp.count, c_hi = (uint64_t)nchunk * (blockIdx.y + 1) / sp.count;
+    // staging: K, a row's 16 bytes a thread; V, 4 positions x 4 dims.  Offsets inside a chunk fit 32 bits (the
+    // row stride is below 2^26), the chunk's base is the same in all lanes.
+    const uint32_t kpos = tid / (D / 16), kpiece = tid % (D / 16), dq = tid % (D / 4), pq = tid / (D / 4), row_bytes = (uint32_t)A.a.kv_row;
+    const int8_t *kbase = A.a.k + b * A.a.kv_batch + g * D, *vbase = A.a.v + b * A.a.kv_batch + g * D;
     const float *ksb = A.a.kscale + b * A.a.scale_batch, *vsb = A.a.vscale + b * A.a.scale_batch;
+    const uint32_t koff = kpos * row_bytes + 16 * kpiece, voff = 4 * pq * row_bytes + 4 * dq;
     nt4 nk;
     uint32_t nv[4];
     float ns = 0.0f;
     auto load = [&](uint32_t ci) {
-        const uint32_t pb = ci * CP;
-        nk = *reinterpret_cast<const nt4 *>(kbase + min(pb + kpos, total - 1) * A.a.kv_row);
+        const uint32_t pb = ci * CP, last = total - 1 - pb;   // (rows past the last read it again)
+        const int8_t *kc = kbase + pb * A.a.kv_row, *vc = vbase + pb * A.a.kv_row;
+        if (pb + CP <= total) {
+            nk = *reinterpret_cast<const nt4 *>(kc + koff);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) nv[r] = *reinterpret_cast<const uint32_t *>(vbase + min(pb + 4 * pq + r, total - 1) * A.a.kv_row);
-        if (tid < 2 * CP) ns = (tid < CP ? ksb : vsb)[min(pb + tid % CP, total - 1)];
+            for (int r = 0; r < 4; ++r) nv[r] = *reinterpret_cast<const uint32_t *>(vc + r * A.a.kv_row + voff);
+        } else {
+            nk = *reinterpret_cast<const nt4 *>(kc + (min(kpos, last) * row_bytes + 16 * kpiece));
+#pragma unroll
+            for (int r = 0; r < 4; ++r) nv[r] = *reinterpret_cast<const uint32_t *>(vc + (min(4 * pq + r, last) * row_bytes + 4 * dq));
+        }
+        if (tid < 2 * CP) ns = (tid < CP ? ksb : vsb)[pb + min((uint32_t)tid % CP, last)];
     };
     if (c_lo < c_hi) load(c_lo);
     uint4 qh[KS], ql[SPLIT ? KS : 1];
@@ -420,6 +483,16 @@ __global__ __launch_bounds__(256, 2) void qxa_wide(QxaArgs A) {
             uint4 lo;
             split8(v, sc, qh[s], lo);
             if constexpr (SPLIT) ql[s] = lo;
+        }
+        if (A.pack && blockIdx.y == 0) {   // the account's q
+            const uint64_t at = ((uint64_t)b * A.a.kv_heads + g) * A.tiles + tile;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                uint4 *to = A.pack + (at * KS + s) * (SPLIT ? 128 : 64) + lane;
+                to[0] = qh[s];
+                if constexpr (SPLIT) to[64] = ql[s];
+            }
+            if (h == 0) A.pack_sf[at * 32 + col] = sf;
         }
     }
     State<D> S;
@@ -459,7 +532,7 @@ __global__ __launch_bounds__(256, 2) void qxa_wide(QxaArgs A) {
                 if constexpr (SPLIT) dot = mfma(kf, ql[s], dot);
                 dot = mfma(kf, qh[s], dot);
             }
-            const bool edge = pb + 32 > q.len;
+            const bool edge = pb + 32 > q.len;   // the chunk holds nodes
             const uint32_t bits = edge ? visible(A, q, b, node, pb) : ~0u;
             uint4 phi[2], plo[2];
             weigh<T, D>(S, dot, sf, &s_ks[buf][32 * sub], &s_vs[buf][32 * sub], edge, bits, h, phi, plo);
@@ -476,7 +549,7 @@ __global__ __launch_bounds__(256, 2) void qxa_wide(QxaArgs A) {
         }
     }
     const float den = S.den + __shfl_xor(S.den, 32);
-    if (busy && used) finish_column<T, D>(A, S, den, b, node, head, h);
+    if (busy && used) finish_column<T, D>(A, S, den, b, node, head, sp, h);
 }
 
 // The splits of a row joined: a workgroup a row, its 256 / (D / 4) strips of threads every so many splits, the
@@ -486,16 +559,18 @@ __global__ __launch_bounds__(256) void qxa_join(QxaArgs A) {
     constexpr int W = D / 4, STRIPS = 256 / W;
     __shared__ float s_m[STRIPS], s_den[STRIPS];
     __shared__ __align__(16) float s_v[STRIPS][D];
-    const uint64_t rows = (uint64_t)A.a.batch * A.a.nodes * A.a.heads, row = blockIdx.x;
+    const uint64_t rows = (uint64_t)A.a.nodes * A.a.heads, row = blockIdx.x;
     const int at = threadIdx.x % W, strip = threadIdx.x / W;
     const uint32_t head = row % A.a.heads, node = row / A.a.heads % A.a.nodes, b = row / A.a.heads / A.a.nodes;
     if (node >= sequence(A, b).count) return;
+    const Splits sp = splits_of(A, b);
+    const uint64_t first = sp.first * rows + node * A.a.heads + head;   // the row's first state; the next lie `rows` apart
     float m = -INFINITY, den = 0.0f;
     f4x v = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
-    for (uint32_t z = strip; z < A.splits; z += STRIPS) {
-        const float2 s = A.md[z * rows + row];
-        const f4x x = *reinterpret_cast<const f4x *>(A.part + (z * rows + row) * D + 4 * at);
+    for (uint32_t z = strip; z < sp.count; z += STRIPS) {
+        const float2 s = A.md[first + z * rows];
+        const f4x x = *reinterpret_cast<const f4x *>(A.part + (first + z * rows) * D + 4 * at);
         const float mn = fmaxf(m, s.x), f = m == mn ? 1.0f : exp2_fast(m - mn), fz = s.x == mn ? 1.0f : exp2_fast(s.x - mn);
         den = fmaf(den, f, s.y * fz);
 #pragma unroll
@@ -520,91 +595,116 @@ __global__ __launch_bounds__(256) void qxa_join(QxaArgs A) {
     if (at == 0 && A.lse) A.lse[row] = den == 0.0f ? -INFINITY : (m + __log2f(den)) * 0.69314718055994531f;
 }
 
-// account[p] = decay * account[p] + sum over nodes and heads of 2^(s - lse).  A workgroup takes 32
-// positions; its waves take every fourth (kv head, tile), compute the scores again and keep, per lane,
-// its column's sums of the 16 positions that its registers hold; lanes and waves are added up in a
-// fixed order, so no two workgroups add to one position.
-template <typename T, int D>
-__global__ __launch_bounds__(256) void qxa_account(QxaArgs A) {
-    constexpr bool SPLIT = sizeof(T) == 4;
-    constexpr int KS = D / 16;
-    __shared__ float s_sum[4][32];
+// account[p] = decay * account[p] + sum over nodes and heads of 2^(s - lse), the scores computed again from the q
+// that the attention has left as matrix operands.  A wave keeps, per lane, its column's sums of the 16
+// positions that its registers hold; columns and waves are added up in a fixed order, and no two
+// workgroups add to one position.  SHARE waves take the same 32 positions and every SHARE-th (kv head, tile): 8
+// where there are few positions, whose chain of pairs would be the time; else 1 and four chunks a
+// workgroup, which then read each q from the first-level cache.
+template <typename T, int D, int SHARE>
+__global__ __launch_bounds__(SHARE == 1 ? 256 : 64 * SHARE, 1) void qxa_account(QxaArgs A) {
+    constexpr bool SPLIT = two_halves_q<T>;
+    constexpr int KS = D / 16, NP = SPLIT ? 2 : 1, CHUNKS = SHARE == 1 ? 4 : 1;
+    __shared__ float s_sum[SHARE == 1 ? 1 : SHARE][32];
     const int lane = threadIdx.x & 63, wave = wave_id(), col = lane & 31, h = lane >> 5;
     const uint32_t b = blockIdx.y;
     const Seq q = sequence(A, b);
     const uint32_t total = q.len + q.count, nchunk = (total + 31) / 32;
-    for (uint32_t ci = blockIdx.x; ci < nchunk; ci += gridDim.x) {
-        const uint32_t pb = ci * 32, pk = min(pb + col, total - 1);
-        const bool edge = pb + 32 > q.len;
-        float ks[16], sum[16];
+    const uint32_t tiles = min(A.tiles, (q.count * A.group + 31) / 32), pairs = A.a.kv_heads * tiles;   // those with nodes in use
+    for (uint32_t c0 = blockIdx.x * CHUNKS; c0 < nchunk; c0 += gridDim.x * CHUNKS) {
+        const uint32_t ci = c0 + (SHARE == 1 ? wave : 0), pb = ci * 32;
+        float sum[16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sum[r] = 0.0f;
+        if (ci < nchunk) {
+            const uint32_t pk = min(pb + col, total - 1);
+            const bool edge = pb + 32 > q.len;
+            float ks[16];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) ks[r] = A.a.kscale[b * A.a.scale_batch + min(pb + 8 * (r >> 2) + 4 * h + (r & 3), total - 1)];
+            uint4 kf[KS];
+            uint32_t held = ~0u;   // the kv head whose codes kf holds
+#pragma unroll 1
+            for (uint32_t pair = SHARE == 1 ? 0 : wave; pair < pairs; pair += SHARE) {
+                const uint32_t g = pair / tiles, tile = pair % tiles, c = tile * 32 + col;
+                const uint32_t node = min(c / A.group, A.a.nodes - 1), head = g * A.group + c % A.group;
+                const bool used = c < A.columns && node < q.count;
+                const uint64_t at = ((uint64_t)b * A.a.kv_heads + g) * A.tiles + tile;
+                const uint4 *qp = A.pack + at * (KS * NP * 64) + lane;
+                uint4 qf[KS * NP];
+#pragma unroll
+                for (int s = 0; s < KS * NP; ++s) qf[s] = qp[64 * s];
+                const float sf = A.pack_sf[at * 32 + col];
+                const float l = used ? A.lse[((uint64_t)b * A.a.nodes + node) * A.a.heads + head] : -INFINITY;
+                if (g != held) {
+                    const KRow<D> kr = load_k<D>(A, b, g, pk, h);
+#pragma unroll
+                    for (int s = 0; s < KS; ++s) kf[s] = k_step<D>(kr, s);
+                    held = g;
+                }
+                f16x dot = zero16();
+#pragma unroll
+                for (int s = 0; s < KS; ++s) {
+                    if constexpr (SPLIT) dot = mfma(kf[s], qf[s * NP + 1], dot);
+                    dot = mfma(kf[s], qf[s * NP], dot);
+                }
+                // a column that is not used or sees nothing adds 0: its exponent becomes -inf
+                const bool none = l == -INFINITY;
+                const float f = none ? 0.0f : sf, l2 = none ? INFINITY : l * 1.4426950408889634f;
+                if (edge) {
+                    const uint32_t bits = visible(A, q, b, node, pb);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const float e = exp2_fast(fmaf(dot[r] * ks[r], f, -l2));
+                        sum[r] += seen(bits, r, h) && !none ? e : 0.0f;
+                    }
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) sum[r] += exp2_fast(fmaf(dot[r] * ks[r], f, -l2));
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {   // over the 32 columns
+                float v = sum[r];
+                v += dppf<DPP_XOR1>(v); v += dppf<DPP_XOR2>(v); v += dppf<DPP_ROR4>(v); v += dppf<DPP_ROR8>(v);
+                const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+                sum[r] = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+            }
+        }
+        float mine = 0.0f;   // position pb + lane % 32's
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            ks[r] = A.a.kscale[b * A.a.scale_batch + min(pb + 8 * (r >> 2) + 4 * h + (r & 3), total - 1)];
-            sum[r] = 0.0f;
+            const int p = 8 * (r >> 2) + (r & 3);   // + 4 h
+            const float lo = rdlanef(sum[r], 0), hi = rdlanef(sum[r], 32);
+            mine = col == p ? lo : col == p + 4 ? hi : mine;
         }
-        for (uint32_t pair = wave; pair < A.a.kv_heads * A.tiles; pair += 4) {
-            const uint32_t g = pair / A.tiles, c = pair % A.tiles * 32 + col, node = min(c / A.group, A.a.nodes - 1);
-            if (pair % A.tiles * 32 / A.group >= q.count) continue;
-            const bool used = c < A.columns && node < q.count;
-            const uint32_t head = g * A.group + (used ? c % A.group : 0);
-            const KRow<D> kr = load_k<D>(A, b, g, pk, h);
-            const T *row = (const T *)A.a.q + b * A.a.q_batch + (used ? node : 0) * A.a.q_node + head * D + (D / 2) * h;
-            float v[KS][8], mx = 0.0f;
-            bool fin = true;
+        if constexpr (SHARE > 1) {
+            if (h == 0) s_sum[wave][col] = mine;
+            __syncthreads();
+            mine = 0.0f;
 #pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                load8(row + 8 * s, v[s]);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) { fin = fin && isfinite(v[s][j]); mx = fmaxf(mx, fabsf(v[s][j])); }
-            }
-            mx = fin ? mx : INFINITY;
-            mx = fmaxf(mx, __shfl_xor(mx, 32));
-            const bool bad = !(mx < INFINITY);
-            const float psc = pow2_scale(bad ? 0.0f : mx, 14), sf = bad ? NAN : A.scale2 / psc;
-            f16x sh = zero16(), sl = zero16();
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                const uint4 kf = k_step<D>(kr, s);
-                uint4 hi, lo;
-                split8(v[s], bad ? 0.0f : psc, hi, lo);
-                sh = mfma(kf, hi, sh);
-                if (SPLIT) sl = mfma(kf, lo, sl);
-            }
-            const float l = used ? A.lse[((uint64_t)b * A.a.nodes + node) * A.a.heads + head] : -INFINITY;
-            const float l2 = l * 1.4426950408889634f;
-            const uint32_t bits = l == -INFINITY ? 0u : edge ? visible(A, q, b, node, pb) : ~0u;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const float sc = (SPLIT ? sh[r] + sl[r] : sh[r]) * ks[r] * sf;
-                sum[r] += seen(bits, r, h) ? exp2_fast(sc - l2) : 0.0f;
-            }
+            for (int w = 0; w < SHARE; ++w) mine += s_sum[w][col];
+            __syncthreads();
         }
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-#pragma unroll
-            for (int o = 16; o; o >>= 1) sum[r] += __shfl_xor(sum[r], o);
-            if (col == 0) s_sum[wave][8 * (r >> 2) + 4 * h + (r & 3)] = sum[r];
+        if (h == 0 && (SHARE == 1 || wave == 0) && pb + col < total) {
+            float *to = A.a.account + b * A.a.account_batch + pb + col;
+            *to = *to * A.a.decay + mine;
         }
-        __syncthreads();
-        const uint32_t p = pb + threadIdx.x;
-        if (threadIdx.x < 32 && p < total) {
-            float *at = A.a.account + b * A.a.account_batch + p;
-            const int t = threadIdx.x;
-            *at = *at * A.a.decay + ((s_sum[0][t] + s_sum[1][t]) + (s_sum[2][t] + s_sum[3][t]));
-        }
-        __syncthreads();
     }
 }
 
 namespace {
 template <typename T, int D> void launch(const QxaArgs &A, hipStream_t s) {
     const uint64_t rows = (uint64_t)A.a.batch * A.a.nodes * A.a.heads;
-    if (A.wide) hipLaunchKernelGGL((qxa_wide<T, D>), dim3(A.a.kv_heads * ((A.tiles + 3) / 4), A.splits, A.a.batch), dim3(256), 0, s, A);
-    else hipLaunchKernelGGL((qxa_tree<T, D>), dim3(A.a.kv_heads * A.tiles, A.splits, A.a.batch), dim3(256), 0, s, A);
+    if (A.wide) hipLaunchKernelGGL((qxa_wide<T, D>), dim3(A.a.kv_heads * ((A.tiles + 3) / 4), A.grid_splits, A.a.batch), dim3(256), 0, s, A);
+    else hipLaunchKernelGGL((qxa_tree<T, D>), dim3(A.a.kv_heads * A.tiles, A.grid_splits, A.a.batch), dim3(256), 0, s, A);
     if (A.splits > 1) hipLaunchKernelGGL((qxa_join<T, D>), dim3((unsigned)rows), dim3(256), 0, s, A);
     if (A.a.account) {
-        const uint32_t chunks = (uint32_t)std::min<uint64_t>(65535, ((uint64_t)A.a.max_len + A.a.nodes + 31) / 32);
-        hipLaunchKernelGGL((qxa_account<T, D>), dim3(chunks, A.a.batch), dim3(256), 0, s, A);
+        const uint64_t chunks = ((uint64_t)A.a.max_len + A.a.nodes + 31) / 32;
+        if (chunks * A.a.batch < 1024)
+            hipLaunchKernelGGL((qxa_account<T, D, 8>), dim3((unsigned)std::max<uint64_t>(1, chunks), A.a.batch), dim3(512), 0, s, A);
+        else
+            hipLaunchKernelGGL((qxa_account<T, D, 1>), dim3((unsigned)std::min<uint64_t>(65535, (chunks + 3) / 4), A.a.batch), dim3(256), 0, s, A);
     }
 }
 }  // namespace

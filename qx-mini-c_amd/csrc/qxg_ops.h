@@ -6,15 +6,18 @@
 
 // Tree attention.  A column is a (node, q head of the kv head) pair, node * group + head; a tile is
 // 32 columns.  With several splits of the positions, a split's unnormalised context goes to part
-// and its (reference, denominator) in base 2 to md, at [split][batch][node][head].
+// and its (reference, denominator) in base 2 to md, at [split of the batch][node][head].
 struct QxaArgs {
     qxg_tree_attention_args a;
-    uint32_t group, columns, tiles, splits, words;
+    uint32_t group, columns, tiles, words;
+    uint32_t splits, grid_splits;   // of the batch (of a sequence beyond 64 sequences); of a sequence at most
     uint32_t wide;     // tiles four at a time, chunks staged for all of them
     float scale2;      // scale * log2(e)
     float *part;
     float2 *md;
     float *lse;        // the caller's, or the workspace's for the account
+    uint4 *pack;       // with an account: q as matrix operands, [batch][kv head][tile][k-step][half][lane]
+    float *pack_sf;    // [batch][kv head][tile][column] what turns dot * kscale into base-2 scores
 };
 void qxa_launch(const QxaArgs &A, hipStream_t s);
 

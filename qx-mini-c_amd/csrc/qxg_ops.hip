@@ -66,10 +66,20 @@ template <size_t N> bool pointers_ok(const Arg (&args)[N], const Err &fail) {
 uint64_t up16(uint64_t v) { return (v + 15) & ~15ull; }
 
 // ---- tree attention
-// Splits of the positions: about 512 workgroups (two fit a CU) of at least four 32-position chunks.
-uint32_t tree_splits(const qxg_tree_attention_args &a, uint64_t wgs) {
-    const uint64_t most = std::max<uint64_t>(1, ((uint64_t)a.max_len + a.nodes) / 128);
-    return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(512 / wgs, most));
+// Splits of the positions over the batch: about 512 workgroups (two fit a CU) of at least two chunks of 64
+// positions each.
+void tree_splits(QxaArgs &A) {
+    const qxg_tree_attention_args &a = A.a;
+    const uint64_t wgs = (uint64_t)a.kv_heads * (A.wide ? (A.tiles + 3) / 4 : A.tiles);   // of one split
+    const uint64_t most = std::max<uint64_t>(1, ((uint64_t)a.max_len + a.nodes) / 128);   // of a sequence
+    if (a.batch > 64) {
+        A.splits = A.grid_splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(512 / (wgs * a.batch), most));
+        return;
+    }
+    A.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(512 / wgs, most * a.batch));
+    if (A.splits <= a.batch) A.splits = 1;   // (no more than one for each)
+    A.grid_splits = (uint32_t)std::min<uint64_t>(A.splits, most);
+    if (A.grid_splits == 1) A.splits = 1;
 }
 bool tree_plan(const qxg_tree_attention_args *p, QxaArgs &A, uint64_t &bytes, const Err &fail) {
     if (!p) return fail("invalid argument");
@@ -84,23 +94,28 @@ bool tree_plan(const qxg_tree_attention_args *p, QxaArgs &A, uint64_t &bytes, co
     if (a.q_batch * size % 16 || a.q_node * size % 16 || a.out_batch * size % 16 || a.out_node * size % 16)
         return fail("the strides of q and out must be multiples of 16 bytes");
     if (a.kv_batch % 16 || a.kv_row % 16) return fail("the strides of k and v must be multiples of 16 bytes");
+    if (a.kv_row >> 26) return fail("the row stride of k and v must be below 2^26 bytes");
     if (!std::isfinite(a.scale) || !(a.scale > 0.0f)) return fail("scale must be positive and finite");
     if (!std::isfinite(a.decay)) return fail("decay must be finite");
     A.group = a.heads / a.kv_heads;
     A.columns = a.nodes * A.group;
     A.tiles = (A.columns + 31) / 32;
     A.wide = A.tiles > 2;
-    A.splits = tree_splits(a, (uint64_t)a.kv_heads * a.batch * (A.wide ? (A.tiles + 3) / 4 : A.tiles));
+    tree_splits(A);
     A.words = (a.nodes + 31) / 32;
     A.scale2 = (float)((double)a.scale * 1.4426950408889634);
     const uint64_t rows = (uint64_t)a.batch * a.nodes * a.heads;
-    const uint64_t part = A.splits > 1 ? up16(A.splits * rows * a.dim * 4) : 0, md = A.splits > 1 ? up16(A.splits * rows * 8) : 0;
-    const uint64_t lse = a.account && !a.lse ? up16(rows * 4) : 0;
+    const uint64_t states = A.splits == 1 ? 0 : (a.batch > 64 ? (uint64_t)A.splits * a.batch : A.splits + a.batch) * a.nodes * a.heads;
+    const uint64_t part = up16(states * a.dim * 4), md = up16(states * 8);
+    const uint64_t lse = a.account && !a.lse ? up16(rows * 4) : 0, ptiles = a.account ? (uint64_t)a.batch * a.kv_heads * A.tiles : 0;
+    const uint64_t sf = ptiles * 128, pack = ptiles * (a.dim / 16) * (a.type == QXG_TYPE_F32 ? 2 : 1) * 1024;
     uint8_t *w = (uint8_t *)a.workspace;
     A.part = (float *)w;
     A.md = (float2 *)(w + part);
     A.lse = a.lse ? a.lse : a.account ? (float *)(w + part + md) : nullptr;
-    bytes = part + md + lse;
+    A.pack_sf = a.account ? (float *)(w + part + md + lse) : nullptr;
+    A.pack = a.account ? (uint4 *)(w + part + md + lse + sf) : nullptr;
+    bytes = part + md + lse + sf + pack;
     return true;
 }
 

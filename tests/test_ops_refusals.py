@@ -41,6 +41,9 @@ def tree(**kw):
     return a
 
 
+TREE_BYTES = qxg._tree_workspace((2, 3, 8, 128), (2, 50, 4, 128), None, True)
+
+
 @pytest.mark.parametrize("change,message", [
     ({}, "invalid context"),
     (dict(q=Fake((2, 3, 8, 128), "int32")), "dtype int32"),
@@ -64,8 +67,11 @@ def tree(**kw):
     (dict(lens=Fake((2,), "int8")), "lens has dtype"),
     (dict(lens=None), "lens is NULL"),
     (dict(out=Fake((2, 3, 8, 128), ptr=0)), "out is NULL"),
-    (dict(workspace=None, lse=None), "the workspace holds 0 bytes; this call needs 192"),
-    (dict(workspace=big(191), lse=None), "the workspace holds 191 bytes; this call needs 192"),
+    (dict(workspace=None, lse=None), f"the workspace holds 0 bytes; this call needs {TREE_BYTES}"),
+    (dict(workspace=big(TREE_BYTES - 1), lse=None), f"the workspace holds {TREE_BYTES - 1} bytes; this call needs {TREE_BYTES}"),
+    (dict(workspace=big(TREE_BYTES), lse=None), "invalid context"),
+    (dict(k=Fake((2, 50, 4, 128), "int8", strides=(1 << 34, 1 << 26, 128, 1)), v=Fake((2, 50, 4, 128), "int8", strides=(1 << 34, 1 << 26, 128, 1))),
+     "row stride of k and v must be below 2\\^26"),
     (dict(workspace=Fake((300,), "uint8", ptr=(1 << 20) + 8)), "workspace is not aligned to 16 bytes"),
     (dict(scale=float("nan")), "scale must be positive and finite"),
     (dict(scale=0.0), "scale must be positive and finite"),
@@ -78,7 +84,7 @@ def test_tree_attention(ctx, change, message):
 
 def test_tree_attention_small_calls_need_no_workspace(ctx):
     with pytest.raises(qxg.QxgError, match="invalid context"):
-        ctx.tree_attention(**tree(workspace=None))
+        ctx.tree_attention(**tree(workspace=None, account=None))
 
 
 @pytest.mark.parametrize("change,message", [
