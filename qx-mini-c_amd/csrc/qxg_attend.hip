@@ -49,36 +49,49 @@ DEV Seq sequence(const QxaArgs &A, uint32_t b) {
     s.len = min(A.a.lens[b], A.a.positions - s.count);
     return s;
 }
-// The splits of sequence b: their number and where they start among all sequences' (the states in part and md
+// The splits of a sequence: their number and where they start among all sequences' (the states in part and md
 // lie in that order).  About A.splits for the whole batch, shared out by the sequences' chunks of 32
 // positions, so that a split is about as long in each; beyond 64 sequences as many for each.
 struct Splits { uint32_t count, first; };
-DEV Splits splits_of(const QxaArgs &A, uint32_t b) {
-    Splits s;
-    if (A.a.batch > 64 || A.splits == 1) {
-        s.count = A.splits;
-        s.first = b * A.splits;
-        return s;
-    }
+DEV bool shared_out(const QxaArgs &A) { return A.a.batch <= 64 && A.splits > 1; }
+DEV Splits lane_splits(const QxaArgs &A) {   // of sequence `lane`
     const uint32_t lane = threadIdx.x & 63;
     uint32_t chunks = 0;
     if (lane < A.a.batch) {
         const Seq q = sequence(A, lane);
         chunks = max(1u, (q.len + q.count + 31) / 32);
     }
-    uint32_t all = chunks;
+    uint64_t all = chunks;
 #pragma unroll
-    for (int o = 32; o; o >>= 1) all += (uint32_t)__shfl_xor((int)all, o);
-    const uint32_t n = lane < A.a.batch ? min(min(chunks, A.grid_splits), max(1u, (uint32_t)((uint64_t)chunks * A.splits / all))) : 0u;
+    for (int o = 32; o; o >>= 1) all += (uint64_t)__shfl_xor((unsigned long long)all, o);
+    const uint32_t n = lane < A.a.batch ? min(chunks, max(1u, (uint32_t)((uint64_t)chunks * A.splits / all))) : 0u;
     uint32_t run = n;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
         const uint32_t x = (uint32_t)__shfl_up((int)run, o);
         run += lane >= (uint32_t)o ? x : 0u;
     }
-    s.count = (uint32_t)__builtin_amdgcn_readlane((int)n, (int)b);
-    s.first = (uint32_t)__builtin_amdgcn_readlane((int)(run - n), (int)b);
-    return s;
+    return {n, run - n};
+}
+DEV Splits splits_of(const QxaArgs &A, uint32_t b) {
+    if (!shared_out(A)) return {A.splits, b * A.splits};
+    const Splits s = lane_splits(A);
+    return {(uint32_t)__builtin_amdgcn_readlane((int)s.count, (int)b), (uint32_t)__builtin_amdgcn_readlane((int)s.first, (int)b)};
+}
+// The workgroup's sequence and split: of all sequences' splits in order, or by the grid.  count 0: none
+struct Job { uint32_t b, z; Splits s; };
+DEV Job job_of(const QxaArgs &A) {
+    Job j{blockIdx.z, blockIdx.y, {A.splits, blockIdx.z * A.splits}};
+    if (shared_out(A)) {
+        const Splits s = lane_splits(A);
+        const uint64_t mine = __ballot(s.count && s.first <= blockIdx.y);
+        j.b = 63u - (uint32_t)__builtin_clzll(mine);   // (the first sequence's start at 0)
+        j.s.count = (uint32_t)__builtin_amdgcn_readlane((int)s.count, (int)j.b);
+        j.s.first = (uint32_t)__builtin_amdgcn_readlane((int)s.first, (int)j.b);
+        j.z = blockIdx.y - j.s.first;
+        if (j.z >= j.s.count) j.s.count = 0;
+    }
+    return j;
 }
 // The positions from p0 on that the node sees, as bits: the cached ones, then the mask's nodes
 DEV uint32_t visible(const QxaArgs &A, const Seq &q, uint32_t b, uint32_t node, uint32_t p0) {
@@ -237,7 +250,8 @@ DEV void weigh(State<D> &S, f16x dot, float sf, const float *ks, const float *vs
 }
 // a column's result: out and lse, or with several splits its state
 template <typename T, int D>
-DEV void finish_column(const QxaArgs &A, const State<D> &S, float den, uint32_t b, uint32_t node, uint32_t head, Splits sp, int h) {
+DEV void finish_column(const QxaArgs &A, const State<D> &S, float den, const Job &job, uint32_t node, uint32_t head, int h) {
+    const uint32_t b = job.b;
     const uint64_t row = ((uint64_t)b * A.a.nodes + node) * A.a.heads + head;
     if (A.splits == 1) {
         const float inv = den == 0.0f ? 0.0f : 1.0f / den;
@@ -250,7 +264,7 @@ DEV void finish_column(const QxaArgs &A, const State<D> &S, float den, uint32_t 
                                                                  S.acc[d][4 * k + 2] * inv, S.acc[d][4 * k + 3] * inv));
         if (h == 0 && A.lse) A.lse[row] = den == 0.0f ? -INFINITY : (S.M + __log2f(den)) * 0.69314718055994531f;
     } else {
-        const uint64_t at = (uint64_t)(sp.first + blockIdx.y) * A.a.nodes * A.a.heads + node * A.a.heads + head;
+        const uint64_t at = (uint64_t)(job.s.first + job.z) * A.a.nodes * A.a.heads + node * A.a.heads + head;
 #pragma unroll
         for (int d = 0; d < D / 32; ++d)
 #pragma unroll
@@ -276,14 +290,14 @@ __global__ __launch_bounds__(256, 2) void qxa_tree(QxaArgs A) {
     __shared__ float s_m[2][32], s_den[2][32];
     __shared__ union { uint32_t vt[4][D * 9]; float acc[2][32][D + 1]; } u;
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), col = lane & 31, h = lane >> 5;
-    const uint32_t g = blockIdx.x / A.tiles, tile = blockIdx.x % A.tiles, b = blockIdx.z;
+    const Job job = job_of(A);
+    const uint32_t g = blockIdx.x / A.tiles, tile = blockIdx.x % A.tiles, b = job.b;
     const Seq q = sequence(A, b);
     const uint32_t c = tile * 32 + col, node = min(c / A.group, A.a.nodes - 1), head = g * A.group + c % A.group;
     const bool used = c < A.columns && node < q.count;
-    const Splits sp = splits_of(A, b);
-    if (tile * 32 / A.group >= q.count || blockIdx.y >= sp.count) return;   // the whole tile is behind count
+    if (job.s.count == 0 || tile * 32 / A.group >= q.count) return;   // the whole tile is behind count
     const uint32_t total = q.len + q.count, nchunk = (total + 31) / 32;
-    const uint32_t c_lo = (uint64_t)nchunk * blockIdx.y / sp.count, c_hi = (uint64_t)nchunk * (blockIdx.y + 1) / sp.count;
+    const uint32_t c_lo = (uint64_t)nchunk * job.z / job.s.count, c_hi = (uint64_t)nchunk * (job.z + 1) / job.s.count;
     struct { KRow<D> k; uint32_t v[4 * DT]; float ks, vs; } nx;
     auto load = [&](uint32_t ci) {   // (rows past the last read it again)
         const uint32_t pb = ci * 32, pk = min(pb + col, total - 1);
@@ -332,7 +346,7 @@ __global__ __launch_bounds__(256, 2) void qxa_tree(QxaArgs A) {
     }
     __syncthreads();
     const float sf = s_sf[col];
-    if (A.pack && blockIdx.y == 0) {   // the account's q
+    if (A.pack && job.z == 0) {   // the account's q
         const uint64_t at = ((uint64_t)b * A.a.kv_heads + g) * A.tiles + tile;
         for (int i = tid; i < KS * NP * 64; i += 256) A.pack[at * (KS * NP * 64) + i] = s_q[i];
         if (tid < 32) A.pack_sf[at * 32 + tid] = s_sf[tid];
@@ -409,50 +423,57 @@ __global__ __launch_bounds__(256, 2) void qxa_tree(QxaArgs A) {
         }
         __syncthreads();
     }
-    if (wave == 0 && used) finish_column<T, D>(A, S, den, b, node, head, sp, h);
+    if (wave == 0 && used) finish_column<T, D>(A, S, den, job, node, head, h);
 }
 
 // Many columns.  The 4 waves of a workgroup take a tile of 32 columns of one kv head each and go through the
-// same chunks of 4096 / D positions, whose codes the workgroup stages in LDS as fp16 (K by rows; V
+// same chunks of 64 positions (32 for f32 values of 128 dims, whose operands take the registers), whose codes the workgroup stages in LDS as fp16 (K by rows; V
 // transposed, a dim's 32 positions in the order of the second product's k): one conversion of a code
 // for 128 columns.  Two buffers, so one barrier a chunk; the next chunk's codes are on their way.
 // The softmax's vector work and the matrix products bound it, each about 1000 cycles a tile and chunk.
 template <typename T, int D>
 __global__ __launch_bounds__(256, 2) void qxa_wide(QxaArgs A) {
     constexpr bool SPLIT = two_halves_q<T>;
-    constexpr int KS = D / 16, DT = D / 32, SUB = 128 / D, CP = 32 * SUB;
+    constexpr int KS = D / 16, DT = D / 32, SUB = D == 64 || !SPLIT ? 2 : 1, CP = 32 * SUB, UNITS = CP * D / 4096;
     constexpr int KP = D + 8, VP = 40;   // fp16 from one row to the next: 16 rows' 16-byte pieces lie in 16 bank groups
     __shared__ __align__(16) _Float16 s_k[2][CP * KP], s_v[2][SUB * D * VP];
     __shared__ __align__(16) float s_ks[2][CP], s_vs[2][CP];
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), col = lane & 31, h = lane >> 5;
-    const uint32_t wgs = (A.tiles + 3) / 4, g = blockIdx.x / wgs, tile = blockIdx.x % wgs * 4 + wave, b = blockIdx.z;
+    const uint32_t wgs = (A.tiles + 3) / 4, g = blockIdx.x / wgs, tile = blockIdx.x % wgs * 4 + wave;
+    const Job job = job_of(A);
+    const uint32_t b = job.b;
     const Seq q = sequence(A, b);
-    const Splits sp = splits_of(A, b);
-    if (blockIdx.x % wgs * 128 / A.group >= q.count || blockIdx.y >= sp.count) return;   // all tiles are behind count
+    if (job.s.count == 0 || blockIdx.x % wgs * 128 / A.group >= q.count) return;   // all tiles are behind count
     const uint32_t c = tile * 32 + col, node = min(c / A.group, A.a.nodes - 1), head = g * A.group + c % A.group;
     const bool busy = tile < A.tiles && tile * 32 / A.group < q.count, used = c < A.columns && node < q.count;   // busy: of the wave
     const uint32_t total = q.len + q.count, nchunk = (total + CP - 1) / CP;
-    const uint32_t c_lo = (uint64_t)nchunk * blockIdx.y / sp.count, c_hi = (uint64_t)nchunk * (blockIdx.y + 1) / sp.count;
+    const uint32_t c_lo = (uint64_t)nchunk * job.z / job.s.count, c_hi = (uint64_t)nchunk * (job.z + 1) / job.s.count;
     // staging: K, a row's 16 bytes a thread; V, 4 positions x 4 dims.  Offsets inside a chunk fit 32 bits (the
     // row stride is below 2^26), the chunk's base is the same in all lanes.
     const uint32_t kpos = tid / (D / 16), kpiece = tid % (D / 16), dq = tid % (D / 4), pq = tid / (D / 4), row_bytes = (uint32_t)A.a.kv_row;
     const int8_t *kbase = A.a.k + b * A.a.kv_batch + g * D, *vbase = A.a.v + b * A.a.kv_batch + g * D;
     const float *ksb = A.a.kscale + b * A.a.scale_batch, *vsb = A.a.vscale + b * A.a.scale_batch;
-    const uint32_t koff = kpos * row_bytes + 16 * kpiece, voff = 4 * pq * row_bytes + 4 * dq;
-    nt4 nk;
-    uint32_t nv[4];
+    constexpr uint32_t KSTEP = 4096 / D, VSTEP = 4096 / D;   // positions of a round of the workgroup's units
+    nt4 nk[UNITS];
+    uint32_t nv[UNITS][4];
     float ns = 0.0f;
     auto load = [&](uint32_t ci) {
         const uint32_t pb = ci * CP, last = total - 1 - pb;   // (rows past the last read it again)
         const int8_t *kc = kbase + pb * A.a.kv_row, *vc = vbase + pb * A.a.kv_row;
-        if (pb + CP <= total) {
-            nk = *reinterpret_cast<const nt4 *>(kc + koff);
+        const bool whole = pb + CP <= total;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) nv[r] = *reinterpret_cast<const uint32_t *>(vc + r * A.a.kv_row + voff);
-        } else {
-            nk = *reinterpret_cast<const nt4 *>(kc + (min(kpos, last) * row_bytes + 16 * kpiece));
+        for (int u = 0; u < UNITS; ++u) {
+            const uint32_t kp = kpos + KSTEP * u, vp = 4 * pq + VSTEP * u;
+            if (whole) {
+                nk[u] = *reinterpret_cast<const nt4 *>(kc + KSTEP * u * A.a.kv_row + (kpos * row_bytes + 16 * kpiece));
 #pragma unroll
-            for (int r = 0; r < 4; ++r) nv[r] = *reinterpret_cast<const uint32_t *>(vc + (min(4 * pq + r, last) * row_bytes + 4 * dq));
+                for (int r = 0; r < 4; ++r)
+                    nv[u][r] = *reinterpret_cast<const uint32_t *>(vc + (VSTEP * u + r) * A.a.kv_row + (4 * pq * row_bytes + 4 * dq));
+            } else {
+                nk[u] = *reinterpret_cast<const nt4 *>(kc + (min(kp, last) * row_bytes + 16 * kpiece));
+#pragma unroll
+                for (int r = 0; r < 4; ++r) nv[u][r] = *reinterpret_cast<const uint32_t *>(vc + (min(vp + r, last) * row_bytes + 4 * dq));
+            }
         }
         if (tid < 2 * CP) ns = (tid < CP ? ksb : vsb)[pb + min((uint32_t)tid % CP, last)];
     };
@@ -484,7 +505,7 @@ __global__ __launch_bounds__(256, 2) void qxa_wide(QxaArgs A) {
             split8(v, sc, qh[s], lo);
             if constexpr (SPLIT) ql[s] = lo;
         }
-        if (A.pack && blockIdx.y == 0) {   // the account's q
+        if (A.pack && job.z == 0) {   // the account's q
             const uint64_t at = ((uint64_t)b * A.a.kv_heads + g) * A.tiles + tile;
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
@@ -500,42 +521,51 @@ __global__ __launch_bounds__(256, 2) void qxa_wide(QxaArgs A) {
 #pragma unroll 1
     for (uint32_t ci = c_lo; ci < c_hi; ++ci, buf ^= 1) {
         {
-            uint4 *to = reinterpret_cast<uint4 *>(&s_k[buf][kpos * KP + 16 * kpiece]);
-            to[0] = i8x8_to_f16(nk.x, nk.y);
-            to[1] = i8x8_to_f16(nk.z, nk.w);
-            const uint32_t a0 = perm(nv[1], nv[0], 0x05010400u), a1 = perm(nv[3], nv[2], 0x05010400u);
-            const uint32_t a2 = perm(nv[1], nv[0], 0x07030602u), a3 = perm(nv[3], nv[2], 0x07030602u);
-            const uint4 v01 = i8x8_to_f16(perm(a1, a0, 0x05040100u), perm(a1, a0, 0x07060302u));
-            const uint4 v23 = i8x8_to_f16(perm(a3, a2, 0x05040100u), perm(a3, a2, 0x07060302u));
-            // positions 4 w .. 4 w + 3 (w = pq % 8) are half w / 2 % 2 of the 16 bytes that lane half w % 2 reads in step
-            // w / 4; the place of the 16 bytes turns with dim / 16, so that the lanes' writes spread over the banks
-            const int w = pq & 7, slot = ((w >> 2) * 2 + (w & 1)) ^ ((dq >> 2) & 3);
-            uint2 *vd = reinterpret_cast<uint2 *>(&s_v[buf][((pq >> 3) * D + 4 * dq) * VP + 8 * slot + 4 * ((w >> 1) & 1)]);
-            vd[0] = make_uint2(v01.x, v01.y);
-            vd[VP / 4] = make_uint2(v01.z, v01.w);
-            vd[2 * (VP / 4)] = make_uint2(v23.x, v23.y);
-            vd[3 * (VP / 4)] = make_uint2(v23.z, v23.w);
+#pragma unroll
+            for (int u = 0; u < UNITS; ++u) {
+                uint4 *to = reinterpret_cast<uint4 *>(&s_k[buf][(kpos + KSTEP * u) * KP + 16 * kpiece]);
+                to[0] = i8x8_to_f16(nk[u].x, nk[u].y);
+                to[1] = i8x8_to_f16(nk[u].z, nk[u].w);
+                const uint32_t *w = nv[u];
+                const uint32_t a0 = perm(w[1], w[0], 0x05010400u), a1 = perm(w[3], w[2], 0x05010400u);
+                const uint32_t a2 = perm(w[1], w[0], 0x07030602u), a3 = perm(w[3], w[2], 0x07030602u);
+                const uint4 v01 = i8x8_to_f16(perm(a1, a0, 0x05040100u), perm(a1, a0, 0x07060302u));
+                const uint4 v23 = i8x8_to_f16(perm(a3, a2, 0x05040100u), perm(a3, a2, 0x07060302u));
+                // positions 4 w .. 4 w + 3 of 32 (w = pq % 8) are half w / 2 % 2 of the 16 bytes that lane half w % 2 reads
+                // in step w / 4; the place of the 16 bytes turns with dim / 16, so that the lanes' writes spread over
+                // the banks
+                const int p4 = pq + VSTEP / 4 * u, v4 = p4 & 7, slot = ((v4 >> 2) * 2 + (v4 & 1)) ^ ((dq >> 2) & 3);
+                uint2 *vd = reinterpret_cast<uint2 *>(&s_v[buf][((p4 >> 3) * D + 4 * dq) * VP + 8 * slot + 4 * ((v4 >> 1) & 1)]);
+                vd[0] = make_uint2(v01.x, v01.y);
+                vd[VP / 4] = make_uint2(v01.z, v01.w);
+                vd[2 * (VP / 4)] = make_uint2(v23.x, v23.y);
+                vd[3 * (VP / 4)] = make_uint2(v23.z, v23.w);
+            }
             if (tid < 2 * CP) (tid < CP ? s_ks : s_vs)[buf][tid % CP] = ns;
         }
         if (ci + 1 < c_hi) load(ci + 1);
         __syncthreads();
         if (!busy) continue;
+        f16x dot[SUB];
 #pragma unroll
         for (int sub = 0; sub < SUB; ++sub) {
-            const uint32_t pb = ci * CP + 32 * sub;
-            if (SUB > 1 && pb >= total) break;
-            f16x dot = zero16();
+            dot[sub] = zero16();
             const _Float16 *kr = &s_k[buf][(32 * sub + col) * KP + (D / 2) * h];
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
                 const uint4 kf = *reinterpret_cast<const uint4 *>(kr + 8 * s);
-                if constexpr (SPLIT) dot = mfma(kf, ql[s], dot);
-                dot = mfma(kf, qh[s], dot);
+                if constexpr (SPLIT) dot[sub] = mfma(kf, ql[s], dot[sub]);
+                dot[sub] = mfma(kf, qh[s], dot[sub]);
             }
+        }
+#pragma unroll
+        for (int sub = 0; sub < SUB; ++sub) {
+            const uint32_t pb = ci * CP + 32 * sub;
+            if (SUB > 1 && pb >= total) break;
             const bool edge = pb + 32 > q.len;   // the chunk holds nodes
             const uint32_t bits = edge ? visible(A, q, b, node, pb) : ~0u;
             uint4 phi[2], plo[2];
-            weigh<T, D>(S, dot, sf, &s_ks[buf][32 * sub], &s_vs[buf][32 * sub], edge, bits, h, phi, plo);
+            weigh<T, D>(S, dot[sub], sf, &s_ks[buf][32 * sub], &s_vs[buf][32 * sub], edge, bits, h, phi, plo);
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
                 const _Float16 *vr = &s_v[buf][(sub * D + 32 * d + col) * VP];
@@ -549,7 +579,7 @@ __global__ __launch_bounds__(256, 2) void qxa_wide(QxaArgs A) {
         }
     }
     const float den = S.den + __shfl_xor(S.den, 32);
-    if (busy && used) finish_column<T, D>(A, S, den, b, node, head, sp, h);
+    if (busy && used) finish_column<T, D>(A, S, den, job, node, head, h);
 }
 
 // The splits of a row joined: a workgroup a row, its 256 / (D / 4) strips of threads every so many splits, the
@@ -696,8 +726,10 @@ __global__ __launch_bounds__(SHARE == 1 ? 256 : 64 * SHARE, 1) void qxa_account(
 namespace {
 template <typename T, int D> void launch(const QxaArgs &A, hipStream_t s) {
     const uint64_t rows = (uint64_t)A.a.batch * A.a.nodes * A.a.heads;
-    if (A.wide) hipLaunchKernelGGL((qxa_wide<T, D>), dim3(A.a.kv_heads * ((A.tiles + 3) / 4), A.grid_splits, A.a.batch), dim3(256), 0, s, A);
-    else hipLaunchKernelGGL((qxa_tree<T, D>), dim3(A.a.kv_heads * A.tiles, A.grid_splits, A.a.batch), dim3(256), 0, s, A);
+    const bool shared = A.a.batch <= 64 && A.splits > 1;   // (a sequence's number of splits is rounded down, but at least one)
+    const dim3 grid(A.a.kv_heads * (A.wide ? (A.tiles + 3) / 4 : A.tiles), shared ? A.splits + A.a.batch : A.splits, shared ? 1 : A.a.batch);
+    if (A.wide) hipLaunchKernelGGL((qxa_wide<T, D>), grid, dim3(256), 0, s, A);
+    else hipLaunchKernelGGL((qxa_tree<T, D>), grid, dim3(256), 0, s, A);
     if (A.splits > 1) hipLaunchKernelGGL((qxa_join<T, D>), dim3((unsigned)rows), dim3(256), 0, s, A);
     if (A.a.account) {
         const uint64_t chunks = ((uint64_t)A.a.max_len + A.a.nodes + 31) / 32;

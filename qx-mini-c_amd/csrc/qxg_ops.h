@@ -10,7 +10,7 @@
 struct QxaArgs {
     qxg_tree_attention_args a;
     uint32_t group, columns, tiles, words;
-    uint32_t splits, grid_splits;   // of the batch (of a sequence beyond 64 sequences); of a sequence at most
+    uint32_t splits;   // of the batch; of a sequence beyond 64 sequences, and when it is 1
     uint32_t wide;     // tiles four at a time, chunks staged for all of them
     float scale2;      // scale * log2(e)
     float *part;

@@ -73,13 +73,11 @@ void tree_splits(QxaArgs &A) {
     const uint64_t wgs = (uint64_t)a.kv_heads * (A.wide ? (A.tiles + 3) / 4 : A.tiles);   // of one split
     const uint64_t most = std::max<uint64_t>(1, ((uint64_t)a.max_len + a.nodes) / 128);   // of a sequence
     if (a.batch > 64) {
-        A.splits = A.grid_splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(512 / (wgs * a.batch), most));
+        A.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(512 / (wgs * a.batch), most));
         return;
     }
     A.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(512 / wgs, most * a.batch));
     if (A.splits <= a.batch) A.splits = 1;   // (no more than one for each)
-    A.grid_splits = (uint32_t)std::min<uint64_t>(A.splits, most);
-    if (A.grid_splits == 1) A.splits = 1;
 }
 bool tree_plan(const qxg_tree_attention_args *p, QxaArgs &A, uint64_t &bytes, const Err &fail) {
     if (!p) return fail("invalid argument");
