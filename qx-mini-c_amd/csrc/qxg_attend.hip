@@ -51,30 +51,43 @@ DEV Seq sequence(const QxaArgs &A, uint32_t b) {
 }
 // The splits of a sequence: their number and where they start among all sequences' (the states in part and md
 // lie in that order).  About A.splits for the whole batch, shared out by the sequences' chunks of 32
-// positions, so that a split is about as long in each; beyond 64 sequences as many for each.
+// positions, so that a split is about as long in each; up to twice as many where nodes are not in use, so that
+// there are as many workgroups all the same; beyond 64 sequences as many for each.
 struct Splits { uint32_t count, first; };
 DEV bool shared_out(const QxaArgs &A) { return A.a.batch <= 64 && A.splits > 1; }
+// running sum over the wave's lanes
+DEV uint32_t wave_running(uint32_t v) {
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, true);   // row_shr:1, 2, 4, 8
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, true);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, true);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, true);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);   // row_bcast:15 into rows 1 and 3
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);   // row_bcast:31 into rows 2 and 3
+    return v;
+}
+DEV uint32_t chunks_of(const Seq &q) { return max(1u, (q.len + q.count + 31) / 32); }
 DEV Splits lane_splits(const QxaArgs &A) {   // of sequence `lane`
     const uint32_t lane = threadIdx.x & 63;
     uint32_t chunks = 0;
+    float all = 0.0f, busy = 0.0f;   // (shares need not be exact, only the same in every workgroup)
     if (lane < A.a.batch) {
         const Seq q = sequence(A, lane);
-        chunks = max(1u, (q.len + q.count + 31) / 32);
+        chunks = chunks_of(q);
+        all = (float)chunks;
+        busy = all * (float)((q.count * A.group + A.wg_columns - 1) / A.wg_columns);   // times workgroups with nodes in use
     }
-    uint64_t all = chunks;
 #pragma unroll
-    for (int o = 32; o; o >>= 1) all += (uint64_t)__shfl_xor((unsigned long long)all, o);
-    const uint32_t n = lane < A.a.batch ? min(chunks, max(1u, (uint32_t)((uint64_t)chunks * A.splits / all))) : 0u;
-    uint32_t run = n;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t x = (uint32_t)__shfl_up((int)run, o);
-        run += lane >= (uint32_t)o ? x : 0u;
+    for (int o = 32; o; o >>= 1) {
+        all += __shfl_xor(all, o);
+        busy += __shfl_xor(busy, o);
     }
-    return {n, run - n};
+    const float share = (float)chunks * (float)A.splits * fminf((float)A.wgs / busy, 2.0f / all);
+    const uint32_t n = lane < A.a.batch ? min(chunks, max(1u, (uint32_t)share)) : 0u;
+    return {n, wave_running(n) - n};
 }
 DEV Splits splits_of(const QxaArgs &A, uint32_t b) {
     if (!shared_out(A)) return {A.splits, b * A.splits};
+    if (A.a.batch == 1) return {min(chunks_of(sequence(A, 0)), A.splits), 0};
     const Splits s = lane_splits(A);
     return {(uint32_t)__builtin_amdgcn_readlane((int)s.count, (int)b), (uint32_t)__builtin_amdgcn_readlane((int)s.first, (int)b)};
 }
@@ -82,7 +95,10 @@ DEV Splits splits_of(const QxaArgs &A, uint32_t b) {
 struct Job { uint32_t b, z; Splits s; };
 DEV Job job_of(const QxaArgs &A) {
     Job j{blockIdx.z, blockIdx.y, {A.splits, blockIdx.z * A.splits}};
-    if (shared_out(A)) {
+    if (A.a.batch == 1 && A.splits > 1) {
+        j = {0, blockIdx.y, splits_of(A, 0)};
+        if (j.z >= j.s.count) j.s.count = 0;
+    } else if (shared_out(A)) {
         const Splits s = lane_splits(A);
         const uint64_t mine = __ballot(s.count && s.first <= blockIdx.y);
         j.b = 63u - (uint32_t)__builtin_clzll(mine);   // (the first sequence's start at 0)
@@ -113,8 +129,8 @@ DEV uint32_t visible(const QxaArgs &A, const Seq &q, uint32_t b, uint32_t node, 
     const uint32_t left = end > p0 ? end - p0 : 0u;
     return left < 32 ? bits & ((1u << left) - 1u) : bits;
 }
-// the mask's bit of register r in lane half h
-DEV bool seen(uint32_t bits, int r, int h) { return (bits >> (8 * (r >> 2) + 4 * h + (r & 3))) & 1; }
+// the mask's bit of register r, of bits >> 4 h in lane half h
+DEV bool seen(uint32_t w, int r) { return w & (1u << (8 * (r >> 2) + (r & 3))); }
 
 template <int D> struct KRow { uint4 k[D / 32]; };
 template <int D> DEV KRow<D> load_k(const QxaArgs &A, uint32_t b, uint32_t g, uint32_t pos, int h) {
@@ -153,6 +169,12 @@ DEV float max_of_halves(float v) {   // of lanes l and l ^ 32
     const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
 }
+DEV float max16(const float (&v)[16]) {   // (as a tree: a dependent instruction waits twice as long as another)
+    float m[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m[i] = fmaxf(fmaxf(v[4 * i], v[4 * i + 1]), fmaxf(v[4 * i + 2], v[4 * i + 3]));
+    return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+}
 template <typename T> constexpr bool two_halves_q = sizeof(T) == 4;
 template <typename T> constexpr bool two_halves_p = !__is_same(T, __bf16);
 
@@ -177,28 +199,18 @@ template <bool LO> DEV void split_pairs(const float *v, uint4 &hi, uint4 &lo) {
     if constexpr (LO) lo = make_uint4(b[0], b[1], b[2], b[3]);
 }
 
-// The chunk's scores (dots, not yet scaled) into weights: phi, plo the second product's operands.  ks, vs: the
-// scales of the chunk's 32 positions; bits: those that the column sees (edge: not all of them, for
-// some column; each of the two uses opens the word anew, or the tests of its bits move into every chunk).
-template <typename T, int D>
-DEV void weigh(State<D> &S, f16x dot, float sf, const float *ks, const float *vs, bool edge, uint32_t bits, int h, uint4 (&phi)[2],
-               uint4 (&plo)[2]) {
-    float s[16], cmax = -INFINITY, pmx = 0.0f;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        const f4x k4 = *reinterpret_cast<const f4x *>(ks + 8 * q + 4 * h);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) s[4 * q + r] = dot[4 * q + r] * k4[r];
-    }
+// A chunk's scores into weights, in steps.  bits: the chunk's positions that the column sees (edge: not all of them, for some column; each of the two uses opens the word anew, or the tests
+// of its bits move into every chunk).
+// Of the scores (still to be multiplied by sf): the mask, and the maximum, which moves M where it has grown by 8.
+template <int D>
+DEV void reference(State<D> &S, float sf, bool edge, uint32_t bits, int h, float (&s)[16]) {
     if (edge) {
-        uint32_t w = bits;
+        uint32_t w = bits >> (4 * h);
         asm volatile("" : "+v"(w));
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = seen(w, r, h) ? s[r] : -INFINITY;
+        for (int r = 0; r < 16; ++r) s[r] = seen(w, r) ? s[r] : -INFINITY;
     }
-#pragma unroll
-    for (int r = 0; r < 16; ++r) cmax = fmaxf(cmax, s[r]);
-    cmax = max_of_halves(cmax) * sf;   // (sf > 0, or NaN)
+    const float cmax = max_of_halves(max16(s)) * sf;   // (sf > 0, or NaN)
     if (__ballot(cmax > S.m + 8.0f) != 0) {   // (whole wave)
         const bool grow = cmax > S.m + 8.0f;
         const float mn = rintf(cmax);
@@ -208,37 +220,31 @@ DEV void weigh(State<D> &S, f16x dot, float sf, const float *ks, const float *vs
             S.m = mn;
         }
     }
-    const float M = S.M == -INFINITY ? 0.0f : S.M;
-    float p[16], den = 0.0f;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        const f4x v4 = *reinterpret_cast<const f4x *>(vs + 8 * q + 4 * h);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const float e = exp2_fast(fmaf(s[4 * q + r], sf, -M));
-            den += e;
-            p[4 * q + r] = e * v4[r];
-        }
-    }
+}
+// The weights as the second product's operands phi (and plo), M moved where they leave fp16's range
+template <typename T, int D>
+DEV void operands(State<D> &S, float den, float sf, bool edge, uint32_t bits, int h, float (&p)[16], uint4 (&phi)[2], uint4 (&plo)[2]) {
     if (edge) {   // (a masked position's scales do not count, whatever they are; fma(-inf, NaN) is NaN)
-        uint32_t w = bits;
+        uint32_t w = bits >> (4 * h);
         asm volatile("" : "+v"(w));
-        if (sf != sf && w == 0) den = 0.0f;
+        if (sf != sf && bits == 0) den = 0.0f;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) p[r] = seen(w, r, h) ? p[r] : 0.0f;
+        for (int r = 0; r < 16; ++r) p[r] = seen(w, r) ? p[r] : 0.0f;
     }
     S.den += den;
+    float a[16];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) pmx = fmaxf(pmx, fabsf(p[r]));
-    pmx = max_of_halves(pmx);
+    for (int r = 0; r < 16; ++r) a[r] = fabsf(p[r]);
+    const float pmx = max_of_halves(max16(a));
     if (__ballot(pmx > S.limit) != 0) {   // the first weights of a column, or one beyond fp16
+        const float M = S.M == -INFINITY ? 0.0f : S.M;
         const bool move = pmx > S.limit && pmx < INFINITY;
         // to [2^6, 2^7), but e itself (up to 2^8 times the shift) stays far inside f32
         int k = (int)(__float_as_uint(pow2_scale(pmx, 7)) >> 23) - 127;
-        k = move ? min(k, 96 - (int)(S.m - M)) : 0;
-        const float f = __uint_as_float((uint32_t)(127 + max(k, -126)) << 23);
+        k = move ? max(min(k, 96 - (int)(S.m - M)), -126) : 0;
+        const float f = __uint_as_float((uint32_t)(127 + k) << 23);
         if (move) {
-            S.M = M - (float)max(k, -126);
+            S.M = M - (float)k;
             S.limit = 32768.0f;
         }
         S.rescale(f);
@@ -248,7 +254,43 @@ DEV void weigh(State<D> &S, f16x dot, float sf, const float *ks, const float *vs
 #pragma unroll
     for (int i = 0; i < 2; ++i) split_pairs<two_halves_p<T>>(p + 8 * i, phi[i], plo[i]);
 }
-// a column's result: out and lse, or with several splits its state
+// all of a chunk at once
+template <typename T, int D>
+DEV void weigh(State<D> &S, const f16x &dot, float sf, const float *ks, const float *vs, bool edge, uint32_t bits, int h, uint4 (&phi)[2],
+               uint4 (&plo)[2]) {
+    float s[16], p[16], den[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const f4x k4 = *reinterpret_cast<const f4x *>(ks + 8 * j + 4 * h);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[4 * j + r] = dot[4 * j + r] * k4[r];
+    }
+    reference<D>(S, sf, edge, bits, h, s);
+    const float M = S.M == -INFINITY ? 0.0f : S.M;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const f4x v4 = *reinterpret_cast<const f4x *>(vs + 8 * j + 4 * h);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float e = exp2_fast(fmaf(s[4 * j + r], sf, -M));
+            den[r] += e;
+            p[4 * j + r] = e * v4[r];
+        }
+    }
+    operands<T, D>(S, (den[0] + den[1]) + (den[2] + den[3]), sf, edge, bits, h, p, phi, plo);
+}
+// column c of kv head g
+struct Column { uint32_t node, head; bool used; };
+DEV Column column(const QxaArgs &A, const Seq &q, uint32_t g, uint32_t c) {
+    const uint32_t node = min(c / A.group, A.a.nodes - 1);
+    return {node, g * A.group + c % A.group, c < A.columns && node < q.count};
+}
+// a column's sums: lse, or with several splits the state's part
+DEV void finish_sums(const QxaArgs &A, float M, float den, bool whole, uint64_t row, uint64_t state) {
+    if (!whole) A.md[state] = make_float2(M, den);
+    else if (A.lse) A.lse[row] = den == 0.0f ? -INFINITY : (M + __log2f(den)) * 0.69314718055994531f;
+}
+// a column's result: out, or with several splits its state
 template <typename T, int D>
 DEV void finish_column(const QxaArgs &A, const State<D> &S, float den, const Job &job, uint32_t node, uint32_t head, int h) {
     const uint32_t b = job.b;
@@ -262,7 +304,7 @@ DEV void finish_column(const QxaArgs &A, const State<D> &S, float den, const Job
             for (int k = 0; k < 4; ++k)
                 store4(out + 32 * d + 8 * k + 4 * h, make_float4(S.acc[d][4 * k] * inv, S.acc[d][4 * k + 1] * inv,
                                                                  S.acc[d][4 * k + 2] * inv, S.acc[d][4 * k + 3] * inv));
-        if (h == 0 && A.lse) A.lse[row] = den == 0.0f ? -INFINITY : (S.M + __log2f(den)) * 0.69314718055994531f;
+        if (h == 0) finish_sums(A, S.M, den, true, row, 0);
     } else {
         const uint64_t at = (uint64_t)(job.s.first + job.z) * A.a.nodes * A.a.heads + node * A.a.heads + head;
 #pragma unroll
@@ -271,7 +313,7 @@ DEV void finish_column(const QxaArgs &A, const State<D> &S, float den, const Job
             for (int k = 0; k < 4; ++k)
                 store4(A.part + at * D + 32 * d + 8 * k + 4 * h,
                        make_float4(S.acc[d][4 * k], S.acc[d][4 * k + 1], S.acc[d][4 * k + 2], S.acc[d][4 * k + 3]));
-        if (h == 0) A.md[at] = make_float2(S.M, den);
+        if (h == 0) finish_sums(A, S.M, den, false, row, at);
     }
 }
 }  // namespace
@@ -427,84 +469,135 @@ __global__ __launch_bounds__(256, 2) void qxa_tree(QxaArgs A) {
 }
 
 // Many columns.  The 4 waves of a workgroup take a tile of 32 columns of one kv head each and go through the
-// same chunks of 64 positions (32 for f32 values of 128 dims, whose operands take the registers), whose codes the workgroup stages in LDS as fp16 (K by rows; V
-// transposed, a dim's 32 positions in the order of the second product's k): one conversion of a code
-// for 128 columns.  Two buffers, so one barrier a chunk; the next chunk's codes are on their way.
-// The softmax's vector work and the matrix products bound it, each about 1000 cycles a tile and chunk.
+// same chunks of 32 positions, whose codes the workgroup stages in LDS as fp16 (K by rows; V transposed, a
+// dim's 32 positions in the order of the second product's k): one conversion of a code for 128 columns.  Two
+// buffers, so one barrier a chunk; the next chunk's codes are on their way.
+// Instruction issue bounds it: 2 x 48 nodes of 32 heads over 65500 positions (f16, weights as hi + lo, so 24
+// matrix instructions a chunk) take 162 us, 620 TFLOP/s of matrix work; the matrix pipe is busy a third of the
+// cycles, the vector pipe under half, LDS two fifths, and a wave's softmax does not fit behind the other wave's
+// products.  The same with chunks of 64 positions, with the next chunk's scores computed ahead, with three waves
+// a SIMD (10 registers spilled): 157 .. 164 us.  One tree of 16 nodes is a chain of latencies: 15.5 us of which
+// 3 are q's way in, 4 the two chunks and 2 the states' way out.
 template <typename T, int D>
 __global__ __launch_bounds__(256, 2) void qxa_wide(QxaArgs A) {
-    constexpr bool SPLIT = two_halves_q<T>;
-    constexpr int KS = D / 16, DT = D / 32, SUB = D == 64 || !SPLIT ? 2 : 1, CP = 32 * SUB, UNITS = CP * D / 4096;
+    constexpr bool SPLIT = two_halves_q<T>, LO = two_halves_p<T>;
+    constexpr int KS = D / 16, DT = D / 32;
     constexpr int KP = D + 8, VP = 40;   // fp16 from one row to the next: 16 rows' 16-byte pieces lie in 16 bank groups
-    __shared__ __align__(16) _Float16 s_k[2][CP * KP], s_v[2][SUB * D * VP];
-    __shared__ __align__(16) float s_ks[2][CP], s_vs[2][CP];
+    __shared__ __align__(16) union { struct { _Float16 k[2][32 * KP], v[2][D * VP]; } codes; _Float16 q[4][32 * KP]; float out[4][32 * 36]; } u;
+    __shared__ __align__(16) float s_ks[2][32], s_vs[2][32];
+    __shared__ float s_sf[4][32];
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), col = lane & 31, h = lane >> 5;
     const uint32_t wgs = (A.tiles + 3) / 4, g = blockIdx.x / wgs, tile = blockIdx.x % wgs * 4 + wave;
     const Job job = job_of(A);
     const uint32_t b = job.b;
     const Seq q = sequence(A, b);
     if (job.s.count == 0 || blockIdx.x % wgs * 128 / A.group >= q.count) return;   // all tiles are behind count
-    const uint32_t c = tile * 32 + col, node = min(c / A.group, A.a.nodes - 1), head = g * A.group + c % A.group;
-    const bool busy = tile < A.tiles && tile * 32 / A.group < q.count, used = c < A.columns && node < q.count;   // busy: of the wave
-    const uint32_t total = q.len + q.count, nchunk = (total + CP - 1) / CP;
+    const Column mine = column(A, q, g, tile * 32 + col);
+    const uint32_t node = mine.node, head = mine.head;
+    const bool busy = tile < A.tiles && tile * 32 / A.group < q.count, used = mine.used;   // busy: of the wave
+    const uint32_t total = q.len + q.count, nchunk = (total + 31) / 32;
     const uint32_t c_lo = (uint64_t)nchunk * job.z / job.s.count, c_hi = (uint64_t)nchunk * (job.z + 1) / job.s.count;
     // staging: K, a row's 16 bytes a thread; V, 4 positions x 4 dims.  Offsets inside a chunk fit 32 bits (the
     // row stride is below 2^26), the chunk's base is the same in all lanes.
-    const uint32_t kpos = tid / (D / 16), kpiece = tid % (D / 16), dq = tid % (D / 4), pq = tid / (D / 4), row_bytes = (uint32_t)A.a.kv_row;
+    const bool stager = D == 128 || tid < 128;
+    const uint32_t kpos = tid / (D / 16) % 32, kpiece = tid % (D / 16), dq = tid % (D / 4), pq = tid / (D / 4) % 8, row_bytes = (uint32_t)A.a.kv_row;
     const int8_t *kbase = A.a.k + b * A.a.kv_batch + g * D, *vbase = A.a.v + b * A.a.kv_batch + g * D;
-    const float *ksb = A.a.kscale + b * A.a.scale_batch, *vsb = A.a.vscale + b * A.a.scale_batch;
-    constexpr uint32_t KSTEP = 4096 / D, VSTEP = 4096 / D;   // positions of a round of the workgroup's units
-    nt4 nk[UNITS];
-    uint32_t nv[UNITS][4];
-    float ns = 0.0f;
-    auto load = [&](uint32_t ci) {
-        const uint32_t pb = ci * CP, last = total - 1 - pb;   // (rows past the last read it again)
+    const float *sbase = (tid < 32 ? A.a.kscale : A.a.vscale) + b * A.a.scale_batch;
+    struct Codes { nt4 k; uint32_t v[4]; float s; };   // a thread's part of a chunk
+    Codes in{};
+    auto load = [&](uint32_t ci, Codes &in) {
+        const uint32_t pb = ci * 32, last = total - 1 - pb;   // (rows past the last read it again)
         const int8_t *kc = kbase + pb * A.a.kv_row, *vc = vbase + pb * A.a.kv_row;
-        const bool whole = pb + CP <= total;
+        if (stager) {
+            if (pb + 32 <= total) {
+                in.k = *reinterpret_cast<const nt4 *>(kc + (kpos * row_bytes + 16 * kpiece));
 #pragma unroll
-        for (int u = 0; u < UNITS; ++u) {
-            const uint32_t kp = kpos + KSTEP * u, vp = 4 * pq + VSTEP * u;
-            if (whole) {
-                nk[u] = *reinterpret_cast<const nt4 *>(kc + KSTEP * u * A.a.kv_row + (kpos * row_bytes + 16 * kpiece));
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    nv[u][r] = *reinterpret_cast<const uint32_t *>(vc + (VSTEP * u + r) * A.a.kv_row + (4 * pq * row_bytes + 4 * dq));
+                for (int r = 0; r < 4; ++r) in.v[r] = *reinterpret_cast<const uint32_t *>(vc + r * A.a.kv_row + (4 * pq * row_bytes + 4 * dq));
             } else {
-                nk[u] = *reinterpret_cast<const nt4 *>(kc + (min(kp, last) * row_bytes + 16 * kpiece));
+                in.k = *reinterpret_cast<const nt4 *>(kc + (min(kpos, last) * row_bytes + 16 * kpiece));
 #pragma unroll
-                for (int r = 0; r < 4; ++r) nv[u][r] = *reinterpret_cast<const uint32_t *>(vc + (min(vp + r, last) * row_bytes + 4 * dq));
+                for (int r = 0; r < 4; ++r) in.v[r] = *reinterpret_cast<const uint32_t *>(vc + (min(4 * pq + r, last) * row_bytes + 4 * dq));
             }
         }
-        if (tid < 2 * CP) ns = (tid < CP ? ksb : vsb)[pb + min((uint32_t)tid % CP, last)];
+        if (tid < 64) in.s = sbase[pb + min((uint32_t)tid % 32, last)];
     };
-    if (c_lo < c_hi) load(c_lo);
+    // positions 4 w .. 4 w + 3 (w = pq) are half w / 2 % 2 of the 16 bytes that lane half w % 2 reads in step w / 4;
+    // the place of the 16 bytes turns with dim / 16, so that the lanes' writes spread over the banks
+    const int slot = ((pq >> 2) * 2 + (pq & 1)) ^ ((dq >> 2) & 3), vat = 4 * dq * VP + 8 * slot + 4 * ((pq >> 1) & 1);
+    auto stage_k = [&](uint32_t ci, const Codes &in) {
+        if (stager) {
+            uint4 *to = reinterpret_cast<uint4 *>(&u.codes.k[ci & 1][kpos * KP + 16 * kpiece]);
+            to[0] = i8x8_to_f16(in.k.x, in.k.y);
+            to[1] = i8x8_to_f16(in.k.z, in.k.w);
+        }
+        if (tid < 64) (tid < 32 ? s_ks : s_vs)[ci & 1][tid % 32] = in.s;
+    };
+    auto stage_v = [&](uint32_t ci, const Codes &in) {
+        if (stager) {
+            const uint32_t a0 = perm(in.v[1], in.v[0], 0x05010400u), a1 = perm(in.v[3], in.v[2], 0x05010400u);
+            const uint32_t a2 = perm(in.v[1], in.v[0], 0x07030602u), a3 = perm(in.v[3], in.v[2], 0x07030602u);
+            const uint4 v01 = i8x8_to_f16(perm(a1, a0, 0x05040100u), perm(a1, a0, 0x07060302u));
+            const uint4 v23 = i8x8_to_f16(perm(a3, a2, 0x05040100u), perm(a3, a2, 0x07060302u));
+            uint2 *vd = reinterpret_cast<uint2 *>(&u.codes.v[ci & 1][vat]);
+            vd[0] = make_uint2(v01.x, v01.y);
+            vd[VP / 4] = make_uint2(v01.z, v01.w);
+            vd[2 * (VP / 4)] = make_uint2(v23.x, v23.y);
+            vd[3 * (VP / 4)] = make_uint2(v23.z, v23.w);
+        }
+    };
+    if (c_lo < c_hi) load(c_lo, in);
     uint4 qh[KS], ql[SPLIT ? KS : 1];
     float sf = 0.0f;
-    if (busy) {   // q fragments: a lane holds its column's D / 2 dims of its half
-        const T *row = (const T *)A.a.q + b * A.a.q_batch + (used ? node : 0) * A.a.q_node + (used ? head : g * A.group) * D + (D / 2) * h;
-        float mx = 0.0f;
-        bool fin = true;
+    if (busy) {   // q fragments: 8 lanes read a column's row, the wave's part of LDS hands each lane its column's half
+        float v[4][D / 64][8];
+        const int seg = lane & 7;
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            float v[8];
-            load8(row + 8 * s, v);
+        for (int i = 0; i < 4; ++i) {
+            const Column to = column(A, q, g, tile * 32 + (lane >> 3) + 8 * i);
+            const T *row = (const T *)A.a.q + b * A.a.q_batch + (to.used ? to.node : 0) * A.a.q_node + (to.used ? to.head : g * A.group) * D + 8 * seg;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) { fin = fin && isfinite(v[j]); mx = fmaxf(mx, fabsf(v[j])); }
+            for (int j = 0; j < D / 64; ++j) load8(row + 64 * j, v[i][j]);
         }
-        mx = max_of_halves(fin ? mx : INFINITY);
-        const bool bad = !(mx < INFINITY);
-        const float sc = pow2_scale(bad ? 0.0f : mx, 14);
-        sf = bad ? NAN : A.scale2 / sc;
+        float sc[4];
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {   // (read again, from the caches: all of it at once would not fit the registers)
-            float v[8];
-            load8(row + 8 * s, v);
+        for (int i = 0; i < 4; ++i) {
+            uint32_t m = 0;   // the largest magnitude's bits; infinity and NaN are beyond all others
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = bad ? 0.0f : v[j];
-            uint4 lo;
-            split8(v, sc, qh[s], lo);
-            if constexpr (SPLIT) ql[s] = lo;
+            for (int j = 0; j < D / 64; ++j)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(v[i][j][e]) & 0x7fffffffu);
+            m = max(m, __float_as_uint(dppf<DPP_XOR1>(__uint_as_float(m))));
+            m = max(m, __float_as_uint(dppf<DPP_XOR2>(__uint_as_float(m))));
+            m = max(m, __float_as_uint(dppf<DPP_HALF_MIRROR>(__uint_as_float(m))));
+            const bool bad = m >= 0x7f800000u;   // makes its row NaN
+            sc[i] = pow2_scale(__uint_as_float(m), 14);
+            if (seg == 0) s_sf[wave][(lane >> 3) + 8 * i] = bad ? NAN : A.scale2 / sc[i];
         }
+#pragma unroll
+        for (int half = 0; half < (SPLIT ? 2 : 1); ++half) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < D / 64; ++j) {
+                    h8v x;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        if (half == 0) v[i][j][e] *= sc[i];
+                        x[e] = (_Float16)v[i][j][e];
+                        if (half == 0) v[i][j][e] -= (float)x[e];
+                    }
+                    *reinterpret_cast<h8v *>(&u.q[wave][((lane >> 3) + 8 * i) * KP + 8 * seg + 64 * j]) = x;
+                }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                const uint4 x = *reinterpret_cast<const uint4 *>(&u.q[wave][col * KP + (D / 2) * h + 8 * s]);
+                if (half == 0) qh[s] = x;
+                else ql[SPLIT ? s : 0] = x;
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
+        sf = s_sf[wave][col];
         if (A.pack && job.z == 0) {   // the account's q
             const uint64_t at = ((uint64_t)b * A.a.kv_heads + g) * A.tiles + tile;
 #pragma unroll
@@ -517,69 +610,68 @@ __global__ __launch_bounds__(256, 2) void qxa_wide(QxaArgs A) {
         }
     }
     State<D> S;
-    int buf = 0;
+    __syncthreads();
 #pragma unroll 1
-    for (uint32_t ci = c_lo; ci < c_hi; ++ci, buf ^= 1) {
-        {
-#pragma unroll
-            for (int u = 0; u < UNITS; ++u) {
-                uint4 *to = reinterpret_cast<uint4 *>(&s_k[buf][(kpos + KSTEP * u) * KP + 16 * kpiece]);
-                to[0] = i8x8_to_f16(nk[u].x, nk[u].y);
-                to[1] = i8x8_to_f16(nk[u].z, nk[u].w);
-                const uint32_t *w = nv[u];
-                const uint32_t a0 = perm(w[1], w[0], 0x05010400u), a1 = perm(w[3], w[2], 0x05010400u);
-                const uint32_t a2 = perm(w[1], w[0], 0x07030602u), a3 = perm(w[3], w[2], 0x07030602u);
-                const uint4 v01 = i8x8_to_f16(perm(a1, a0, 0x05040100u), perm(a1, a0, 0x07060302u));
-                const uint4 v23 = i8x8_to_f16(perm(a3, a2, 0x05040100u), perm(a3, a2, 0x07060302u));
-                // positions 4 w .. 4 w + 3 of 32 (w = pq % 8) are half w / 2 % 2 of the 16 bytes that lane half w % 2 reads
-                // in step w / 4; the place of the 16 bytes turns with dim / 16, so that the lanes' writes spread over
-                // the banks
-                const int p4 = pq + VSTEP / 4 * u, v4 = p4 & 7, slot = ((v4 >> 2) * 2 + (v4 & 1)) ^ ((dq >> 2) & 3);
-                uint2 *vd = reinterpret_cast<uint2 *>(&s_v[buf][((p4 >> 3) * D + 4 * dq) * VP + 8 * slot + 4 * ((v4 >> 1) & 1)]);
-                vd[0] = make_uint2(v01.x, v01.y);
-                vd[VP / 4] = make_uint2(v01.z, v01.w);
-                vd[2 * (VP / 4)] = make_uint2(v23.x, v23.y);
-                vd[3 * (VP / 4)] = make_uint2(v23.z, v23.w);
-            }
-            if (tid < 2 * CP) (tid < CP ? s_ks : s_vs)[buf][tid % CP] = ns;
-        }
-        if (ci + 1 < c_hi) load(ci + 1);
+    for (uint32_t ci = c_lo; ci < c_hi; ++ci) {
+        stage_k(ci, in);
+        stage_v(ci, in);
+        if (ci + 1 < c_hi) load(ci + 1, in);
         __syncthreads();
         if (!busy) continue;
-        f16x dot[SUB];
+        const uint32_t pb = ci * 32;
+        f16x dot = zero16();
+        const _Float16 *kr = &u.codes.k[ci & 1][col * KP + (D / 2) * h], *vr = &u.codes.v[ci & 1][col * VP];
 #pragma unroll
-        for (int sub = 0; sub < SUB; ++sub) {
-            dot[sub] = zero16();
-            const _Float16 *kr = &s_k[buf][(32 * sub + col) * KP + (D / 2) * h];
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                const uint4 kf = *reinterpret_cast<const uint4 *>(kr + 8 * s);
-                if constexpr (SPLIT) dot[sub] = mfma(kf, ql[s], dot[sub]);
-                dot[sub] = mfma(kf, qh[s], dot[sub]);
-            }
+        for (int s = 0; s < KS; ++s) {
+            const uint4 kf = *reinterpret_cast<const uint4 *>(kr + 8 * s);
+            if constexpr (SPLIT) dot = mfma(kf, ql[s], dot);
+            dot = mfma(kf, qh[s], dot);
         }
+        const bool edge = pb + 32 > q.len;   // the chunk holds nodes
+        const uint32_t bits = edge ? visible(A, q, b, node, pb) : ~0u;
+        uint4 phi[2], plo[2];
+        weigh<T, D>(S, dot, sf, s_ks[ci & 1], s_vs[ci & 1], edge, bits, h, phi, plo);
 #pragma unroll
-        for (int sub = 0; sub < SUB; ++sub) {
-            const uint32_t pb = ci * CP + 32 * sub;
-            if (SUB > 1 && pb >= total) break;
-            const bool edge = pb + 32 > q.len;   // the chunk holds nodes
-            const uint32_t bits = edge ? visible(A, q, b, node, pb) : ~0u;
-            uint4 phi[2], plo[2];
-            weigh<T, D>(S, dot[sub], sf, &s_ks[buf][32 * sub], &s_vs[buf][32 * sub], edge, bits, h, phi, plo);
+        for (int s = 0; s < 2; ++s) {
+            uint4 vf[DT];
 #pragma unroll
-            for (int d = 0; d < DT; ++d) {
-                const _Float16 *vr = &s_v[buf][(sub * D + 32 * d + col) * VP];
+            for (int d = 0; d < DT; ++d)
+                vf[d] = *reinterpret_cast<const uint4 *>(vr + 32 * d * VP + 8 * ((2 * s + h) ^ ((2 * d + (col >> 4)) & 3)));
+            if constexpr (LO) {
 #pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    const uint4 vf = *reinterpret_cast<const uint4 *>(vr + 8 * ((2 * s + h) ^ ((2 * d + (col >> 4)) & 3)));
-                    if constexpr (two_halves_p<T>) S.acc[d] = mfma(vf, plo[s], S.acc[d]);
-                    S.acc[d] = mfma(vf, phi[s], S.acc[d]);
-                }
+                for (int d = 0; d < DT; ++d) S.acc[d] = mfma(vf[d], plo[s], S.acc[d]);
             }
+#pragma unroll
+            for (int d = 0; d < DT; ++d) S.acc[d] = mfma(vf[d], phi[s], S.acc[d]);
         }
     }
     const float den = S.den + __shfl_xor(S.den, 32);
-    if (busy && used) finish_column<T, D>(A, S, den, job, node, head, h);
+    __syncthreads();
+    if (!busy) return;
+    // results: a tile of 32 dims after the other through the wave's part of LDS, so that 8 lanes write a column's line
+    const bool whole = A.splits == 1;
+    const float inv = !whole ? 1.0f : den == 0.0f ? 0.0f : 1.0f / den;
+    const uint64_t states = (uint64_t)(job.s.first + job.z) * A.a.nodes * A.a.heads;
+    float *o = u.out[wave];
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            *reinterpret_cast<f4x *>(o + col * 36 + 8 * k + 4 * h) = f4x{S.acc[d][4 * k] * inv, S.acc[d][4 * k + 1] * inv, S.acc[d][4 * k + 2] * inv,
+                                                                       S.acc[d][4 * k + 3] * inv};
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const Column to = column(A, q, g, tile * 32 + (lane >> 3) + 8 * i);
+            const float4 x = *reinterpret_cast<const float4 *>(o + ((lane >> 3) + 8 * i) * 36 + 4 * (lane & 7));
+            const uint32_t dim = 32 * d + 4 * (lane & 7);
+            if (!to.used) continue;
+            if (whole) store4((T *)A.a.out + b * A.a.out_batch + to.node * A.a.out_node + to.head * D + dim, x);
+            else store4(A.part + (states + to.node * A.a.heads + to.head) * D + dim, x);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+    if (used && h == 0) finish_sums(A, S.M, den, whole, ((uint64_t)b * A.a.nodes + node) * A.a.heads + head, states + node * A.a.heads + head);
 }
 
 // The splits of a row joined: a workgroup a row, its 256 / (D / 4) strips of threads every so many splits, the
@@ -682,11 +774,11 @@ __global__ __launch_bounds__(SHARE == 1 ? 256 : 64 * SHARE, 1) void qxa_account(
                 const bool none = l == -INFINITY;
                 const float f = none ? 0.0f : sf, l2 = none ? INFINITY : l * 1.4426950408889634f;
                 if (edge) {
-                    const uint32_t bits = visible(A, q, b, node, pb);
+                    const uint32_t bits = visible(A, q, b, node, pb) >> (4 * h);
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
                         const float e = exp2_fast(fmaf(dot[r] * ks[r], f, -l2));
-                        sum[r] += seen(bits, r, h) && !none ? e : 0.0f;
+                        sum[r] += seen(bits, r) && !none ? e : 0.0f;
                     }
                 } else {
 #pragma unroll
@@ -727,7 +819,7 @@ namespace {
 template <typename T, int D> void launch(const QxaArgs &A, hipStream_t s) {
     const uint64_t rows = (uint64_t)A.a.batch * A.a.nodes * A.a.heads;
     const bool shared = A.a.batch <= 64 && A.splits > 1;   // (a sequence's number of splits is rounded down, but at least one)
-    const dim3 grid(A.a.kv_heads * (A.wide ? (A.tiles + 3) / 4 : A.tiles), shared ? A.splits + A.a.batch : A.splits, shared ? 1 : A.a.batch);
+    const dim3 grid(A.a.kv_heads * A.wgs, shared && A.a.batch > 1 ? 2 * A.splits + A.a.batch : A.splits, shared ? 1 : A.a.batch);
     if (A.wide) hipLaunchKernelGGL((qxa_wide<T, D>), grid, dim3(256), 0, s, A);
     else hipLaunchKernelGGL((qxa_tree<T, D>), grid, dim3(256), 0, s, A);
     if (A.splits > 1) hipLaunchKernelGGL((qxa_join<T, D>), dim3((unsigned)rows), dim3(256), 0, s, A);

@@ -12,6 +12,7 @@ struct QxaArgs {
     uint32_t group, columns, tiles, words;
     uint32_t splits;   // of the batch; of a sequence beyond 64 sequences, and when it is 1
     uint32_t wide;     // tiles four at a time, chunks staged for all of them
+    uint32_t wgs, wg_columns;   // workgroups of a kv head and split, columns of one
     float scale2;      // scale * log2(e)
     float *part;
     float2 *md;

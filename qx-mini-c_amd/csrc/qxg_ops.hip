@@ -66,17 +66,21 @@ template <size_t N> bool pointers_ok(const Arg (&args)[N], const Err &fail) {
 uint64_t up16(uint64_t v) { return (v + 15) & ~15ull; }
 
 // ---- tree attention
-// Splits of the positions over the batch: about 512 workgroups (two fit a CU) of at least two chunks of 64
-// positions each.
+// Splits of the positions over the batch: about 480 workgroups (two fit a CU; with all 512 places taken some
+// workgroups of a launch waited for a second round: 217 us instead of 162 for 2 x 48 nodes of 32 heads over 65500
+// positions).  A split is at least two chunks of 32 positions in the wide kernel (16 nodes over 1500 positions:
+// 15.5 us; of four chunks 17.0; of one 15.8, but the join takes 5.0 instead of 4.0), else one for each wave.
 void tree_splits(QxaArgs &A) {
     const qxg_tree_attention_args &a = A.a;
-    const uint64_t wgs = (uint64_t)a.kv_heads * (A.wide ? (A.tiles + 3) / 4 : A.tiles);   // of one split
-    const uint64_t most = std::max<uint64_t>(1, ((uint64_t)a.max_len + a.nodes) / 128);   // of a sequence
+    A.wg_columns = A.wide ? 128 : 32;
+    A.wgs = (A.columns + A.wg_columns - 1) / A.wg_columns;
+    const uint64_t wgs = (uint64_t)a.kv_heads * A.wgs;   // of one split
+    const uint64_t most = std::max<uint64_t>(1, ((uint64_t)a.max_len + a.nodes) / (A.wide ? 64 : 128));   // of a sequence
     if (a.batch > 64) {
-        A.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(512 / (wgs * a.batch), most));
+        A.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(480 / (wgs * a.batch), most));
         return;
     }
-    A.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(512 / wgs, most * a.batch));
+    A.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(480 / wgs, most * a.batch));
     if (A.splits <= a.batch) A.splits = 1;   // (no more than one for each)
 }
 bool tree_plan(const qxg_tree_attention_args *p, QxaArgs &A, uint64_t &bytes, const Err &fail) {
@@ -103,7 +107,7 @@ bool tree_plan(const qxg_tree_attention_args *p, QxaArgs &A, uint64_t &bytes, co
     A.words = (a.nodes + 31) / 32;
     A.scale2 = (float)((double)a.scale * 1.4426950408889634);
     const uint64_t rows = (uint64_t)a.batch * a.nodes * a.heads;
-    const uint64_t states = A.splits == 1 ? 0 : (a.batch > 64 ? (uint64_t)A.splits * a.batch : A.splits + a.batch) * a.nodes * a.heads;
+    const uint64_t states = A.splits == 1 ? 0 : (a.batch > 64 ? (uint64_t)A.splits * a.batch : a.batch == 1 ? A.splits : 2ull * A.splits + a.batch) * a.nodes * a.heads;
     const uint64_t part = up16(states * a.dim * 4), md = up16(states * 8);
     const uint64_t lse = a.account && !a.lse ? up16(rows * 4) : 0, ptiles = a.account ? (uint64_t)a.batch * a.kv_heads * A.tiles : 0;
     const uint64_t sf = ptiles * 128, pack = ptiles * (a.dim / 16) * (a.type == QXG_TYPE_F32 ? 2 : 1) * 1024;
