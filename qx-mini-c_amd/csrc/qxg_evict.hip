@@ -2,8 +2,10 @@
 #include "qxg_dev.h"
 #include "qxg_ops.h"
 
+#include <type_traits>
+
 namespace {
-// Weights as unsigned numbers in their order, 1 or more; NaN as -inf, -0 as +0
+// Weights as unsigned numbers in their order, 0x007fffff (-inf) or more; NaN as -inf, -0 as +0
 DEV uint32_t weight_rank(float w) {
     const uint32_t u = __float_as_uint(fmaxf(w, -INFINITY) + 0.0f);   // (the larger of NaN and a number is the number)
     return u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
@@ -38,91 +40,119 @@ DEV uint32_t rank_at(const qxg_kv_select_args &A, float w, uint32_t p, uint32_t 
 }  // namespace
 
 namespace {
-// The smallest rank among the block's k[] (E a thread, 0: none) that `want` of them reach, found a bit at a time
-// from bit `top` down below the bits of `least`; `above`: how many are larger.  The count of ranks that
-// reach it is one ballot a wave and register.
+// The smallest rank among the block's k[] (E a thread, 0: none) that `want` of them reach, found two bits at a time
+// in the low `bits` ones (an even number) below the bits of `least`; `above`: how many are larger.  The count
+// of ranks that reach a number is one ballot a wave and register; lanes 16 t + w of every wave add up the waves'
+// counts of the step's number t.  The chain of barriers bounds it, so two bits a step (one bit a step: 1.3 us more for
+// 700 positions).
 template <int E>
-DEV uint32_t block_nth(const uint32_t (&k)[E], uint32_t want, uint32_t least, int top, uint32_t (&s_n)[2][16], uint32_t &above) {
+DEV uint32_t block_nth(const uint32_t (&k)[E], uint32_t want, uint32_t least, int bits, uint32_t (&s_n)[2][64], uint32_t &above) {
     const int lane = threadIdx.x & 63, wave = wave_id();
     above = 0;
 #pragma unroll 1
-    for (int b = top; b >= 0; --b) {
-        const uint32_t at = least | 1u << b;
-        uint32_t n = 0;
+    for (int b = bits - 2; b >= 0; b -= 2) {
+        uint32_t n[3] = {0, 0, 0};
 #pragma unroll
-        for (int i = 0; i < E; ++i) n += (uint32_t)__popcll(__ballot(k[i] >= at));
-        if (lane == 0) s_n[b & 1][wave] = n;
-        __syncthreads();   // (the other half is written next, so one barrier a bit is enough)
-        n = s_n[b & 1][lane & 15];
-        n += (uint32_t)dppi<DPP_XOR1>((int)n); n += (uint32_t)dppi<DPP_XOR2>((int)n);
-        n += (uint32_t)dppi<DPP_ROR4>((int)n); n += (uint32_t)dppi<DPP_ROR8>((int)n);
-        if (n >= want) least = at;
-        else above = n;
+        for (int i = 0; i < E; ++i)
+#pragma unroll
+            for (int t = 0; t < 3; ++t) n[t] += (uint32_t)__popcll(__ballot(k[i] >= (least | (uint32_t)(t + 1) << b)));
+        uint32_t (&to)[64] = s_n[(b >> 1) & 1];
+        if (lane < 3) to[16 * lane + wave] = lane == 0 ? n[0] : lane == 1 ? n[1] : n[2];
+        __syncthreads();   // (the other half is written next, so one barrier a step is enough)
+        uint32_t c = to[lane];   // (the last 16 are not used)
+        c += (uint32_t)dppi<DPP_XOR1>((int)c); c += (uint32_t)dppi<DPP_XOR2>((int)c);
+        c += (uint32_t)dppi<DPP_ROR4>((int)c); c += (uint32_t)dppi<DPP_ROR8>((int)c);
+        uint32_t digit = 0;
+#pragma unroll
+        for (int t = 0; t < 3; ++t) {   // fewer reach each next number
+            const uint32_t all = (uint32_t)__builtin_amdgcn_readlane((int)c, 16 * t);
+            if (all >= want) digit = t + 1;
+            else { above = all; break; }
+        }
+        least |= digit << b;
     }
     return least;
 }
-// Positions p0 + 64 E wave + 64 i + lane of a thread: a wave's 64 E are neighbours, read 64 at a time
-template <int E> DEV uint32_t place_of(uint32_t p0, int i) { return p0 + 64 * (E * wave_id() + i) + (threadIdx.x & 63); }
-// Lists the kept ones of the block's 1024 E positions from p0 on: ranks above `least`, and the lowest `need`
-// equal ones.  done: how many of either lie before p0.
-template <int E>
-DEV void list_kept(const uint32_t (&k)[E], uint32_t p0, uint32_t least, uint32_t need, uint2 &done, uint2 *s_w, uint32_t *keep) {
-    uint2 own = make_uint2(0, 0), all;
+// how many of a wave's ranks are above `least`, and how many are equal
+template <int E> DEV uint2 count_kept(const uint32_t (&k)[E], uint32_t least) {
+    uint2 n = make_uint2(0, 0);
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-        own.x += (uint32_t)__popcll(__ballot(k[i] > least));
-        own.y += (uint32_t)__popcll(__ballot(k[i] == least));
+        n.x += (uint32_t)__popcll(__ballot(k[i] > least));
+        n.y += (uint32_t)__popcll(__ballot(k[i] == least));
     }
-    uint2 at = waves_before(own, s_w, all);
-    at.x += done.x;
-    at.y += done.y;
+    return n;
+}
+// Lists the kept ones of a wave's 64 E positions from p0 on: ranks above `least`, and the lowest `need` equal ones.
+// at: how many of either lie before p0; moved on.
+template <int E>
+DEV void list_kept(const uint32_t (&k)[E], uint32_t p0, uint32_t least, uint32_t need, uint2 &at, uint32_t *keep) {
+    const uint32_t lane = threadIdx.x & 63;
 #pragma unroll
     for (int i = 0; i < E; ++i) {
         const uint64_t gt = __ballot(k[i] > least), eq = __ballot(k[i] == least);
         const uint32_t place = at.x + __builtin_amdgcn_mbcnt_hi((uint32_t)(gt >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)gt, 0));
         if (eq == 0 || at.y >= need) {   // (uniform)
-            if (k[i] > least) keep[place + min(at.y, need)] = place_of<E>(p0, i);
+            if (k[i] > least) keep[place + min(at.y, need)] = p0 + 64 * i + lane;
         } else {
             const uint32_t y = at.y + __builtin_amdgcn_mbcnt_hi((uint32_t)(eq >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)eq, 0));
-            if (k[i] > least || (k[i] == least && y < need)) keep[place + min(y, need)] = place_of<E>(p0, i);
+            if (k[i] > least || (k[i] == least && y < need)) keep[place + min(y, need)] = p0 + 64 * i + lane;
         }
         at.x += (uint32_t)__popcll(gt);
         at.y += (uint32_t)__popcll(eq);
     }
-    done.x += all.x;
-    done.y += all.y;
 }
+// weights of a wave's 64 E positions from p0 on, those before `end`
 template <int E>
-DEV void load_weights(const float *acc, uint32_t p0, uint32_t len, float (&w)[E]) {
-    if (p0 + 1024 * E <= len) {   // (uniform)
-        const float *p = acc + place_of<E>(p0, 0);
+DEV void load_weights(const float *acc, uint32_t p0, uint32_t end, float (&w)[E]) {
+    const uint32_t lane = threadIdx.x & 63;
+    if (p0 + 64 * E <= end) {   // (uniform)
+        const float *p = acc + p0 + lane;
 #pragma unroll
         for (int i = 0; i < E; ++i) w[i] = p[64 * i];
     } else {
 #pragma unroll
-        for (int i = 0; i < E; ++i) w[i] = place_of<E>(p0, i) < len ? acc[place_of<E>(p0, i)] : 0.0f;
+        for (int i = 0; i < E; ++i) w[i] = p0 + 64 * i + lane < end ? acc[p0 + 64 * i + lane] : 0.0f;
     }
 }
+// and their ranks, 0 from `end` on
 template <int E>
-DEV void ranks_of(const qxg_kv_select_args &A, const float (&w)[E], uint32_t p0, uint32_t len, uint32_t (&k)[E]) {
-    if (p0 >= A.sinks && p0 + 1024 * E <= len - A.recent) {   // (uniform; nothing kept in any case, nothing behind the end)
+DEV void ranks_of(const qxg_kv_select_args &A, const float (&w)[E], uint32_t p0, uint32_t end, uint32_t len, uint32_t (&k)[E]) {
+    const uint32_t lane = threadIdx.x & 63;
+    if (p0 >= A.sinks && p0 + 64 * E <= min(end, len - A.recent)) {   // (uniform; nothing kept in any case, nothing behind the end)
 #pragma unroll
         for (int i = 0; i < E; ++i) k[i] = weight_rank(w[i]);
     } else {
 #pragma unroll
-        for (int i = 0; i < E; ++i) k[i] = rank_at(A, w[i], place_of<E>(p0, i), len);
+        for (int i = 0; i < E; ++i) {
+            const uint32_t p = p0 + 64 * i + lane;
+            k[i] = p >= end ? 0u : rank_at(A, w[i], p, len);
+        }
+    }
+}
+// all batches of a wave's positions lo .. hi - 1, the next one's weights on their way: f(ranks, first position)
+template <int E, typename F>
+DEV void each_batch(const qxg_kv_select_args &A, const float *acc, uint32_t lo, uint32_t hi, uint32_t len, F f) {
+    uint32_t k[E];
+    float next[E];
+    load_weights<E>(acc, lo, hi, next);
+#pragma unroll 1
+    for (uint32_t p0 = lo; p0 < hi; p0 += 64 * E) {
+        ranks_of<E>(A, next, p0, hi, len, k);
+        load_weights<E>(acc, p0 + 64 * E, hi, next);
+        f(k, p0);
     }
 }
 }  // namespace
 
 // Up to 1024 E positions, a workgroup a group: a thread holds E positions' ranks in registers.  The
-// counts of its 32 steps bound it.  (Byte-wise histograms in LDS, their bins searched by one thread: 26 us
+// counts of its 16 steps bound it.  (Byte-wise histograms in LDS, their bins searched by one thread: 26 us
 // for 700 positions.)
 template <int E>
 __global__ __launch_bounds__(1024) void qxe_select(qxg_kv_select_args A) {
-    __shared__ uint32_t s_n[2][16];
+    __shared__ uint32_t s_n[2][64];
     __shared__ uint2 s_w[16];
-    const uint32_t g = blockIdx.x;
+    const uint32_t g = blockIdx.x, p0 = 64 * E * wave_id();
     const Group G = group_of(A, g);
     uint32_t *keep = A.keep + g * A.keep_group;
     if (threadIdx.x == 0) A.kept[g] = G.kept;
@@ -132,23 +162,24 @@ __global__ __launch_bounds__(1024) void qxe_select(qxg_kv_select_args A) {
     }
     uint32_t k[E], above;
     float w[E];
-    load_weights<E>(A.account + g * A.account_group, 0, G.len, w);
-    ranks_of<E>(A, w, 0, G.len, k);
-    const uint32_t least = block_nth<E>(k, A.budget, 0, 31, s_n, above);
-    uint2 done = make_uint2(0, 0);
-    list_kept<E>(k, 0, least, A.budget - above, done, s_w, keep);
+    load_weights<E>(A.account + g * A.account_group, p0, G.len, w);
+    ranks_of<E>(A, w, p0, G.len, G.len, k);
+    const uint32_t least = block_nth<E>(k, A.budget, 0, 32, s_n, above);
+    uint2 all, at = waves_before(count_kept<E>(k, least), s_w, all);
+    list_kept<E>(k, p0, least, A.budget - above, at, keep);
 }
 
-// More positions than registers hold: a histogram of the ranks' top 11 bits (each bin 16 times, by lane, as
-// equal bins of a wave's lanes would be added one after the other), then the ranks of the bin that holds
-// the smallest kept one go to LDS, where its other bits are found as above; a bin of more than ROOM ranks
-// is halved further by another histogram.  The account is read three times, from the caches after the
-// first: one workgroup's loads bound it.
+// More positions than registers hold, a sixteenth of them a wave.  A histogram of the ranks' top 12 bits (each
+// bin 8 times, by lane, as equal bins of a wave's lanes would be added one after the other), then the ranks of
+// the bin that holds the smallest kept one go to LDS, where its other bits are found as above; a bin of more
+// than ROOM ranks is halved further by another histogram.  The account is read three times, from the caches
+// after the first, and the waves meet only between the readings: one workgroup's loads bound it.
 __global__ __launch_bounds__(1024) void qxe_select_long(qxg_kv_select_args A) {
-    constexpr int E = 16, BINS = 2048, COPIES = 16, ROOM = 16384;
-    __shared__ uint32_t s_hist[BINS * COPIES], s_n[2][16], s_digit, s_above, s_count;
+    constexpr int E = 8, BITS = 12, BINS = 1 << BITS, COPIES = 8, ROOM = 16384;
+    __shared__ uint32_t s_hist[BINS * COPIES], s_n[2][64], s_digit, s_above, s_count, s_gt[16], s_eq[16];
+    __shared__ uint8_t s_wave[ROOM];   // of a rank in LDS: the wave that holds its position
     __shared__ uint2 s_w[16];
-    const int tid = threadIdx.x, lane = tid & 63;
+    const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
     const uint32_t g = blockIdx.x;
     const Group G = group_of(A, g);
     uint32_t *keep = A.keep + g * A.keep_group;
@@ -158,46 +189,45 @@ __global__ __launch_bounds__(1024) void qxe_select_long(qxg_kv_select_args A) {
         for (uint32_t p = tid; p < G.len; p += 1024) keep[p] = p;
         return;
     }
+    const uint32_t part = (G.len + 1023) / 1024 * 64, lo = min(wave * part, G.len), hi = min(lo + part, G.len);
     uint32_t least = 0, above = 0;   // bits found, and ranks above them
     int shift = 32;                  // bits still to find
+    bool counted = false;            // s_gt and s_eq hold the waves' numbers of kept ranks
     while (shift > 0) {
-        const int bits = min(shift, 11);
+        const int bits = min(shift, BITS);
         for (int i = tid; i < BINS * COPIES / 4; i += 1024) reinterpret_cast<uint4 *>(s_hist)[i] = make_uint4(0, 0, 0, 0);
         __syncthreads();
-        uint32_t k[E];
-        float next[E];   // the next round's weights, on their way
-        load_weights<E>(acc, 0, G.len, next);
-        for (uint32_t p0 = 0; p0 < G.len; p0 += 1024 * E) {
-            ranks_of<E>(A, next, p0, G.len, k);
-            load_weights<E>(acc, p0 + 1024 * E, G.len, next);
+        each_batch<E>(A, acc, lo, hi, G.len, [&](const uint32_t (&k)[E], uint32_t) {
 #pragma unroll
-            for (int i = 0; i < E; ++i)   // (positions behind the end have rank 0, no other has)
+            for (int i = 0; i < E; ++i)   // (positions behind the end have rank 0, whose first 12 bits no other has)
                 if (k[i] && (shift == 32 || k[i] >> shift == least >> shift))
-                    atomicAdd(&s_hist[((k[i] >> (shift - bits)) & ((1u << bits) - 1u)) * COPIES + (lane & 15)], 1u);
-        }
+                    atomicAdd(&s_hist[((k[i] >> (shift - bits)) & ((1u << bits) - 1u)) * COPIES + (lane & (COPIES - 1))], 1u);
+        });
         __syncthreads();
-        // the bins from the top: thread t has bins 2047 - 2 t and 2046 - 2 t
-        uint32_t n[2] = {0, 0};
+        // the bins from the top, four a thread
+        uint32_t n[4] = {0, 0, 0, 0}, run = 0;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < 4; ++i) {
 #pragma unroll
-            for (int c = 0; c < COPIES; ++c) n[i] += s_hist[(BINS - 1 - 2 * tid - i) * COPIES + ((c + tid) & 15)];
+            for (int c = 0; c < COPIES; ++c) n[i] += s_hist[(BINS - 1 - 4 * tid - i) * COPIES + ((c + tid) & (COPIES - 1))];
+            run += n[i];
+        }
+        const uint32_t mine = run;
         uint2 all;
-        uint32_t run = n[0] + n[1];   // running count over the wave's lanes
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
+        for (int o = 1; o < 64; o <<= 1) {   // running count over the wave's lanes
             const uint32_t y = (uint32_t)__shfl_up((int)run, o);
             if (lane >= o) run += y;
         }
-        const uint32_t before = above + run - n[0] - n[1] + waves_before(make_uint2((uint32_t)__shfl((int)run, 63), 0), s_w, all).x;
+        uint32_t before = above + run - mine + waves_before(make_uint2((uint32_t)__shfl((int)run, 63), 0), s_w, all).x;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const uint32_t b = before + (i ? n[0] : 0u);
-            if (b < A.budget && b + n[i] >= A.budget) {
-                s_digit = BINS - 1 - 2 * tid - i;
-                s_above = b;
+        for (int i = 0; i < 4; ++i) {
+            if (before < A.budget && before + n[i] >= A.budget) {
+                s_digit = BINS - 1 - 4 * tid - i;
+                s_above = before;
                 s_count = n[i];
             }
+            before += n[i];
         }
         __syncthreads();
         shift -= bits;
@@ -208,40 +238,64 @@ __global__ __launch_bounds__(1024) void qxe_select_long(qxg_kv_select_args A) {
         if (shift && count <= ROOM) {
             if (tid == 0) s_count = 0;
             __syncthreads();
-            load_weights<E>(acc, 0, G.len, next);
-            for (uint32_t p0 = 0; p0 < G.len; p0 += 1024 * E) {
-                ranks_of<E>(A, next, p0, G.len, k);
-                load_weights<E>(acc, p0 + 1024 * E, G.len, next);
+            const uint32_t width = 1u << shift;   // of the bin, from `least` on
+            uint32_t larger = 0;
+            each_batch<E>(A, acc, lo, hi, G.len, [&](const uint32_t (&k)[E], uint32_t) {
+                uint32_t in = 0;
 #pragma unroll
                 for (int i = 0; i < E; ++i) {
-                    const bool f = k[i] && k[i] >> shift == least >> shift;
-                    const uint64_t b = __ballot(f);
-                    if (!b) continue;
-                    uint32_t first = 0;
-                    if (lane == 0) first = atomicAdd(&s_count, (uint32_t)__popcll(b));
-                    first = (uint32_t)__builtin_amdgcn_readfirstlane((int)first);
-                    if (f) s_hist[first + (uint32_t)__popcll(b & ((1ull << lane) - 1ull))] = k[i];   // (< count, in any order)
+                    larger += (uint32_t)__popcll(__ballot(k[i] > least + (width - 1)));
+                    in += (uint32_t)__popcll(__ballot(k[i] - least < width));
                 }
-            }
-            __syncthreads();
-            uint32_t more;
+                if (!in) return;
+                uint32_t first = 0;
+                if (lane == 0) first = atomicAdd(&s_count, in);
+                first = (uint32_t)__builtin_amdgcn_readfirstlane((int)first);
 #pragma unroll
-            for (int i = 0; i < E; ++i) k[i] = (uint32_t)(1024 * i + tid) < count ? s_hist[1024 * i + tid] : 0u;
-            least = block_nth<E>(k, A.budget - above, least, shift - 1, s_n, more);
-            above += more;
+                for (int i = 0; i < E; ++i) {
+                    const bool f = k[i] - least < width;
+                    const uint64_t b = __ballot(f);
+                    if (f) {
+                        const uint32_t to = first + __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0));
+                        s_hist[to] = k[i];   // (< count, in any order)
+                        s_wave[to] = (uint8_t)wave;
+                    }
+                    first += (uint32_t)__popcll(b);
+                }
+            });
+            if (lane == 0) { s_gt[wave] = larger; s_eq[wave] = 0; }
+            __syncthreads();
+            const auto rest = [&](auto size) {   // the bin's other bits, and whose ranks they are
+                constexpr int N = decltype(size)::value;
+                uint32_t k[N], more;
+#pragma unroll
+                for (int i = 0; i < N; ++i) k[i] = (uint32_t)(1024 * i + tid) < count ? s_hist[1024 * i + tid] : 0u;
+                least = block_nth<N>(k, A.budget - above, least, shift, s_n, more);
+                above += more;
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                    if (k[i] >= least) atomicAdd(&(k[i] > least ? s_gt : s_eq)[s_wave[1024 * i + tid]], 1u);
+                __syncthreads();
+            };
+            if (count <= 4096) rest(std::integral_constant<int, 4>{});
+            else rest(std::integral_constant<int, 16>{});
             shift = 0;
+            counted = true;
         }
     }
-    uint2 done = make_uint2(0, 0);
-    uint32_t k[E];
-    float next[E];
-    load_weights<E>(acc, 0, G.len, next);
-    for (uint32_t p0 = 0; p0 < G.len; p0 += 1024 * E) {
-        ranks_of<E>(A, next, p0, G.len, k);
-        load_weights<E>(acc, p0 + 1024 * E, G.len, next);
-        list_kept<E>(k, p0, least, A.budget - above, done, s_w, keep);
-        __syncthreads();   // s_w is read
+    if (!counted) {
+        uint2 own = make_uint2(0, 0);
+        each_batch<E>(A, acc, lo, hi, G.len, [&](const uint32_t (&k)[E], uint32_t) {
+            const uint2 n = count_kept<E>(k, least);
+            own.x += n.x;
+            own.y += n.y;
+        });
+        if (lane == 0) { s_gt[wave] = own.x; s_eq[wave] = own.y; }
+        __syncthreads();
     }
+    uint2 at = make_uint2(0, 0);
+    for (int w = 0; w < wave; ++w) { at.x += s_gt[w]; at.y += s_eq[w]; }
+    each_batch<E>(A, acc, lo, hi, G.len, [&](const uint32_t (&k)[E], uint32_t p0) { list_kept<E>(k, p0, least, A.budget - above, at, keep); });
 }
 
 // Rows moved in place.  Tiles of R rows (32 KB of K, or one row) are claimed in order: a workgroup reads its tile's
