@@ -20,11 +20,10 @@ DEV float key_value(uint64_t k) {
     const uint32_t u = (uint32_t)(k >> 32);
     return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
 }
-// A bound that exactly n of the wave's 64 keys reach (unlike ones but for 0), found a bit at a time until it
-// is one; 0 when fewer than n are not 0.  The token bits are searched only where several keys share the
-// n-th's rank.
-DEV uint64_t wave_nth(uint64_t k, uint32_t n) {
-    const uint32_t hi = (uint32_t)(k >> 32), lo = (uint32_t)k;
+// A bound that exactly n of the wave's 64 keys reach (hi: their ranks, lo(): their other bits, unlike but where the
+// rank is 0), found a bit at a time until it is one; 0 when fewer than n are not 0.  The low bits are asked for
+// only where several keys share the n-th's rank.
+template <typename F> DEV uint64_t wave_nth(uint32_t hi, uint32_t n, F lo) {
     uint32_t th = 0, tl = 0;
     for (int b = 31; b >= 0; --b) {
         const uint32_t c = (uint32_t)__popcll(__ballot(hi >= (th | 1u << b)));
@@ -32,10 +31,10 @@ DEV uint64_t wave_nth(uint64_t k, uint32_t n) {
         if (c == n) return (uint64_t)th << 32;
     }
     if (th == 0) return 0;
-    const uint32_t above = (uint32_t)__popcll(__ballot(hi > th));
+    const uint32_t above = (uint32_t)__popcll(__ballot(hi > th)), low = lo();
     const bool at = hi == th;
     for (int b = 31; b >= 0; --b)
-        if (above + (uint32_t)__popcll(__ballot(at && lo >= (tl | 1u << b))) >= n) tl |= 1u << b;
+        if (above + (uint32_t)__popcll(__ballot(at && low >= (tl | 1u << b))) >= n) tl |= 1u << b;
     return (uint64_t)th << 32 | tl;
 }
 // (maximum, sum of exp(x - maximum)) of two sets; NaN in the sum stays
@@ -44,12 +43,41 @@ DEV float2 join(float2 a, float2 b) {
     return make_float2(m, a.y * (a.x == m ? 1.0f : __builtin_amdgcn_exp2f((a.x - m) * 1.4426950408889634f)) +
                               b.y * (b.x == m ? 1.0f : __builtin_amdgcn_exp2f((b.x - m) * 1.4426950408889634f)));
 }
-DEV float2 wave_join(float2 v) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v = join(v, make_float2(__shfl_xor(v.x, o), __shfl_xor(v.y, o)));
-    return v;
-}
 DEV float lse_of(float2 v) { return v.y != v.y ? NAN : fabsf(v.x) == INFINITY ? v.x : v.x + logf(v.y); }
+
+// Division by a number that many are divided by: its reciprocal, one correction of the quotient (exact
+// remainder, so an error of half a step and 2^-46 of it), and as it is where the quotient is 0, infinite or NaN.
+// Divisors whose reciprocal or remainders could leave the normal range are divided by as usual.
+struct Divisor {
+    float by, inverse;
+    bool usual;
+    DEV explicit Divisor(float d) : by(d), inverse(1.0f / d), usual(!(fabsf(d) >= 0x1p-64f && fabsf(d) <= 0x1p64f)) {}
+    DEV float quick(float y) const {
+        const float q = y * inverse;
+        return __builtin_amdgcn_classf(q, 0x198) ? fmaf(fmaf(-q, by, y), inverse, q) : q;   // normal and subnormal ones
+    }
+    DEV float operator()(float y) const { return usual ? y / by : quick(y); }   // (uniform)
+};
+// the larger ones of numbers and quiet NaN
+DEV float max_of(float a, float b, float c) {
+    float m;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(m) : "v"(a), "v"(b), "v"(c));
+    return m;
+}
+// the largest of the wave's values (numbers), and the sum of them
+DEV float wave_most(float v) {
+    v = fmaxf(v, dppf<DPP_XOR1>(v)); v = fmaxf(v, dppf<DPP_XOR2>(v)); v = fmaxf(v, dppf<DPP_ROR4>(v)); v = fmaxf(v, dppf<DPP_ROR8>(v));
+    return fmaxf(fmaxf(rdlanef(v, 0), rdlanef(v, 16)), fmaxf(rdlanef(v, 32), rdlanef(v, 48)));
+}
+DEV float wave_total(float v) {
+    v += dppf<DPP_XOR1>(v); v += dppf<DPP_XOR2>(v); v += dppf<DPP_ROR4>(v); v += dppf<DPP_ROR8>(v);
+    return (rdlanef(v, 0) + rdlanef(v, 16)) + (rdlanef(v, 32) + rdlanef(v, 48));
+}
+
+DEV float2 wave_join(float2 v) {
+    const float m = wave_most(v.x);
+    return make_float2(m, wave_total(v.y * (v.x == m ? 1.0f : __builtin_amdgcn_exp2f((v.x - m) * 1.4426950408889634f))));
+}
 
 // N values of 16 bytes
 template <typename T> struct Pack { T v[16 / sizeof(T)]; };
@@ -61,6 +89,10 @@ template <typename T> struct Pack { T v[16 / sizeof(T)]; };
 // tokens: a bound that n of a wave's 64 lanes' largest reach bounds the wave's n-th largest from below, and
 // so the slice's; at most n lanes of a wave reach the slice's, so at most PER n of its keys do, about n / 2 of most
 // rows.  Only of more than n are the n largest taken, by counting.
+// A workgroup's chain of latencies bounds it, not the bytes: 64 rows of 151936 f32 logits with 4000 tokens of
+// history each, best 32: 30 us (78 MB read and written, 15.5 us at the rate of a copy).  Of a workgroup's 12 us,
+// 5 are the first loads, 1 the history's counts, 3 the dense pass, 3 the best tokens; 6, 7 or 8 workgroups a CU
+// are alike.  One row: 6.7 us.
 template <typename T, int STEPS>
 __global__ __launch_bounds__(256) void qxs_slice(QxsArgs A) {
     constexpr int N = 16 / sizeof(T), PER = N * STEPS, EARLY = 16;
@@ -69,8 +101,8 @@ __global__ __launch_bounds__(256) void qxs_slice(QxsArgs A) {
         uint32_t token[SLICE];
         uint64_t keys[4][PER * QXG_MAX_TOPN];
     } u;
-    __shared__ uint32_t s_ids[QXS_BIASES];
-    __shared__ float s_sum[QXS_BIASES];
+    extern __shared__ uint32_t s_ids[];   // [biases], then their values
+    float *s_sum = reinterpret_cast<float *>(s_ids + A.a.biases);
     __shared__ uint64_t s_least[4];
     __shared__ uint32_t s_twice;
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
@@ -126,6 +158,7 @@ __global__ __launch_bounds__(256) void qxs_slice(QxsArgs A) {
     }
     if (!A.a.penalties) { rep = 1.0f; freq = pres = 0.0f; }
     if (!A.a.temperature) temp = 1.0f;
+    const Divisor by_rep(rep), by_temp(temp);
     entries = A.a.history_lens ? min(entries, slots) : slots;
     prompt = A.a.prompt_lens ? prompt : 0u;
     if (sparse) {
@@ -167,9 +200,7 @@ __global__ __launch_bounds__(256) void qxs_slice(QxsArgs A) {
         }
         __syncthreads();
     }
-    float m = -INFINITY;   // the thread's largest and its place (the first of equal ones is the lower token)
-    uint32_t at = 0;
-    bool nan = false;
+    float m = -INFINITY;   // the thread's largest
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
         const uint32_t t = (s * 256 + tid) * N;
@@ -184,20 +215,21 @@ __global__ __launch_bounds__(256) void qxs_slice(QxsArgs A) {
                 const uint32_t c = c4[k];
                 float y = x[s * N + j];
                 if (c) {
-                    if (c & SEEN) y = y > 0.0f ? y / rep : y * rep;
+                    if (c & SEEN) y = y > 0.0f ? by_rep(y) : y * rep;
                     if (c & COUNT) {
                         y -= freq * (float)(c & COUNT);
                         y -= pres;
                     }
                     if (c & HAS_BIAS) y += s_sum[(c >> BIAS_SHIFT) & (QXS_BIASES - 1)];
                 }
-                y /= temp;
-                if (!((open[s] >> j) & 1)) y = -INFINITY;
+                y = by_temp(y);
+                const uint32_t is = (uint32_t)__builtin_amdgcn_sbfe((int)open[s], j, 1);   // all bits of it
+                y = __uint_as_float((is & __float_as_uint(y)) | (~is & 0xff800000u));
                 x[s * N + j] = y;
                 p.v[j] = (T)y;
-                nan = nan || y != y;
-                if (y > m) { m = y; at = t + j; }
             }
+            // (the division has made every NaN a quiet one)
+            m = max_of(max_of(m, x[s * N + j4], x[s * N + j4 + 1]), x[s * N + j4 + 2], x[s * N + j4 + 3]);
         }
         if (wide_out && t + N <= here) *reinterpret_cast<nt4 *>(out + t) = __builtin_bit_cast(nt4, p);
         else
@@ -207,17 +239,29 @@ __global__ __launch_bounds__(256) void qxs_slice(QxsArgs A) {
     }
     const uint64_t list = (uint64_t)r * A.slices * 4 + blockIdx.x * 4 + wave;
     if (A.a.lse) {
+        const float most = wave_most(m);
         float sum = 0.0f;
-        if (m > -INFINITY) {
+        if (fabsf(most) < INFINITY) {
 #pragma unroll
-            for (int i = 0; i < PER; ++i) sum += x[i] == m ? 1.0f : __builtin_amdgcn_exp2f((x[i] - m) * 1.4426950408889634f);
+            for (int i = 0; i < PER; ++i) sum += __builtin_amdgcn_exp2f((x[i] - most) * 1.4426950408889634f);
+            sum = wave_total(sum);
+        } else {   // an infinite maximum is the result, but for NaN
+            bool nan = false;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) nan = nan || x[i] != x[i];
+            sum = __ballot(nan) ? NAN : most > 0.0f ? 1.0f : 0.0f;
         }
-        const float2 ms = wave_join(make_float2(m, nan ? NAN : sum));
+        const float2 ms = make_float2(most, sum);
         if (lane == 0) A.ms[list] = ms;
     }
     const uint32_t n = A.a.top_n;
     if (!n) return;
-    uint64_t least = wave_nth(key_of(rank_of(m), v0 + at), n);
+    uint64_t least = wave_nth(rank_of(m), n, [&] {   // (of equal ones the lower token counts more)
+        uint32_t at = 0;
+#pragma unroll
+        for (int i = PER - 1; i >= 0; --i) at = x[i] == m ? ((i / N) * 256 + tid) * N + i % N : at;
+        return ~(v0 + at);
+    });
     if (lane == 0) s_least[wave] = least;
     __syncthreads();   // (also: the tokens' words are read, their space takes the keys)
     least = umax64(umax64(s_least[0], s_least[1]), umax64(s_least[2], s_least[3]));
@@ -250,6 +294,7 @@ __global__ __launch_bounds__(256) void qxs_slice(QxsArgs A) {
 
 // The lists of a row joined: a workgroup a row.  The n-th largest of 64 strips' largest keys (strip: every
 // 64th key) bounds the n-th of all from below; the keys that reach it are ranked by counting.
+// (One row 4 .. 6 us, 64 rows of 38 slices 9.5 us: loads, one search, one count, each a latency.)
 template <typename T>
 __global__ __launch_bounds__(1024) void qxs_join(QxsArgs A) {
     constexpr uint32_t ROOM = 4096;
@@ -282,7 +327,7 @@ __global__ __launch_bounds__(1024) void qxs_join(QxsArgs A) {
     if (!n) return;
 #pragma unroll
     for (int w = 0; w < 16; ++w) best = umax64(best, s_best[w][lane]);
-    const uint64_t least = wave_nth(best, n);
+    const uint64_t least = wave_nth((uint32_t)(best >> 32), n, [&] { return (uint32_t)best; });
     auto offer = [&](uint64_t key) {
         if (key && key >= least) {
             const uint32_t at = atomicAdd(&s_have, 1u);
@@ -332,8 +377,8 @@ __global__ __launch_bounds__(1024) void qxs_join(QxsArgs A) {
 namespace {
 template <typename T> void launch(const QxsArgs &A, hipStream_t s) {
     constexpr int STEPS = QXS_SLICE * sizeof(T) / 4096;
-    if (A.small) hipLaunchKernelGGL((qxs_slice<T, 1>), dim3(A.slices, A.a.rows), dim3(256), 0, s, A);
-    else hipLaunchKernelGGL((qxs_slice<T, STEPS>), dim3(A.slices, A.a.rows), dim3(256), 0, s, A);
+    if (A.small) hipLaunchKernelGGL((qxs_slice<T, 1>), dim3(A.slices, A.a.rows), dim3(256), A.a.biases * 8, s, A);
+    else hipLaunchKernelGGL((qxs_slice<T, STEPS>), dim3(A.slices, A.a.rows), dim3(256), A.a.biases * 8, s, A);
     if (A.a.lse || A.a.top_n) hipLaunchKernelGGL(qxs_join<T>, dim3(A.a.rows), dim3(1024), 0, s, A);
 }
 }  // namespace
