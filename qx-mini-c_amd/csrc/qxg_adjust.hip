@@ -45,19 +45,6 @@ DEV float2 join(float2 a, float2 b) {
 }
 DEV float lse_of(float2 v) { return v.y != v.y ? NAN : fabsf(v.x) == INFINITY ? v.x : v.x + logf(v.y); }
 
-// Division by a number that many are divided by: its reciprocal, one correction of the quotient (exact
-// remainder, so an error of half a step and 2^-46 of it), and as it is where the quotient is 0, infinite or NaN.
-// Divisors whose reciprocal or remainders could leave the normal range are divided by as usual.
-struct Divisor {
-    float by, inverse;
-    bool usual;
-    DEV explicit Divisor(float d) : by(d), inverse(1.0f / d), usual(!(fabsf(d) >= 0x1p-64f && fabsf(d) <= 0x1p64f)) {}
-    DEV float quick(float y) const {
-        const float q = y * inverse;
-        return __builtin_amdgcn_classf(q, 0x198) ? fmaf(fmaf(-q, by, y), inverse, q) : q;   // normal and subnormal ones
-    }
-    DEV float operator()(float y) const { return usual ? y / by : quick(y); }   // (uniform)
-};
 // the larger ones of numbers and quiet NaN
 DEV float max_of(float a, float b, float c) {
     float m;
@@ -92,7 +79,7 @@ template <typename T> struct Pack { T v[16 / sizeof(T)]; };
 // A workgroup's chain of latencies bounds it, not the bytes: 64 rows of 151936 f32 logits with 4000 tokens of
 // history each, best 32: 30 us (78 MB read and written, 15.5 us at the rate of a copy).  Of a workgroup's 12 us,
 // 5 are the first loads, 1 the history's counts, 3 the dense pass, 3 the best tokens; 6, 7 or 8 workgroups a CU
-// are alike.  One row: 6.7 us.
+// are alike, and so are divisions and products with corrected reciprocals.  One row: 6.7 us.
 template <typename T, int STEPS>
 __global__ __launch_bounds__(256) void qxs_slice(QxsArgs A) {
     constexpr int N = 16 / sizeof(T), PER = N * STEPS, EARLY = 16;
@@ -158,7 +145,6 @@ __global__ __launch_bounds__(256) void qxs_slice(QxsArgs A) {
     }
     if (!A.a.penalties) { rep = 1.0f; freq = pres = 0.0f; }
     if (!A.a.temperature) temp = 1.0f;
-    const Divisor by_rep(rep), by_temp(temp);
     entries = A.a.history_lens ? min(entries, slots) : slots;
     prompt = A.a.prompt_lens ? prompt : 0u;
     if (sparse) {
@@ -215,14 +201,14 @@ __global__ __launch_bounds__(256) void qxs_slice(QxsArgs A) {
                 const uint32_t c = c4[k];
                 float y = x[s * N + j];
                 if (c) {
-                    if (c & SEEN) y = y > 0.0f ? by_rep(y) : y * rep;
+                    if (c & SEEN) y = y > 0.0f ? y / rep : y * rep;
                     if (c & COUNT) {
                         y -= freq * (float)(c & COUNT);
                         y -= pres;
                     }
                     if (c & HAS_BIAS) y += s_sum[(c >> BIAS_SHIFT) & (QXS_BIASES - 1)];
                 }
-                y = by_temp(y);
+                y /= temp;
                 const uint32_t is = (uint32_t)__builtin_amdgcn_sbfe((int)open[s], j, 1);   // all bits of it
                 y = __uint_as_float((is & __float_as_uint(y)) | (~is & 0xff800000u));
                 x[s * N + j] = y;
