@@ -198,10 +198,16 @@ __global__ __launch_bounds__(1024) void qxe_select_long(qxg_kv_select_args A) {
         for (int i = tid; i < BINS * COPIES / 4; i += 1024) reinterpret_cast<uint4 *>(s_hist)[i] = make_uint4(0, 0, 0, 0);
         __syncthreads();
         each_batch<E>(A, acc, lo, hi, G.len, [&](const uint32_t (&k)[E], uint32_t) {
+            // (positions behind the end have rank 0, whose first 12 bits no other has)
+            if (shift == 32) {   // no branch a rank
 #pragma unroll
-            for (int i = 0; i < E; ++i)   // (positions behind the end have rank 0, whose first 12 bits no other has)
-                if (k[i] && (shift == 32 || k[i] >> shift == least >> shift))
-                    atomicAdd(&s_hist[((k[i] >> (shift - bits)) & ((1u << bits) - 1u)) * COPIES + (lane & (COPIES - 1))], 1u);
+                for (int i = 0; i < E; ++i) atomicAdd(&s_hist[(k[i] >> (32 - BITS)) * COPIES + (lane & (COPIES - 1))], 1u);
+            } else {
+#pragma unroll
+                for (int i = 0; i < E; ++i)
+                    if (k[i] >> shift == least >> shift)
+                        atomicAdd(&s_hist[((k[i] >> (shift - bits)) & ((1u << bits) - 1u)) * COPIES + (lane & (COPIES - 1))], 1u);
+            }
         });
         __syncthreads();
         // the bins from the top, four a thread
@@ -255,6 +261,7 @@ __global__ __launch_bounds__(1024) void qxe_select_long(qxg_kv_select_args A) {
                 for (int i = 0; i < E; ++i) {
                     const bool f = k[i] - least < width;
                     const uint64_t b = __ballot(f);
+                    if (!b) continue;
                     if (f) {
                         const uint32_t to = first + __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0));
                         s_hist[to] = k[i];   // (< count, in any order)
