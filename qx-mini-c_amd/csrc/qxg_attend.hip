@@ -254,10 +254,10 @@ DEV void operands(State<D> &S, float den, float sf, bool edge, uint32_t bits, in
 #pragma unroll
     for (int i = 0; i < 2; ++i) split_pairs<two_halves_p<T>>(p + 8 * i, phi[i], plo[i]);
 }
-// all of a chunk at once
+// all of a chunk at once; its scores to keep, if there is one
 template <typename T, int D>
 DEV void weigh(State<D> &S, const f16x &dot, float sf, const float *ks, const float *vs, bool edge, uint32_t bits, int h, uint4 (&phi)[2],
-               uint4 (&plo)[2]) {
+               uint4 (&plo)[2], f4x *keep = nullptr) {
     float s[16], p[16], den[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -266,6 +266,10 @@ DEV void weigh(State<D> &S, const f16x &dot, float sf, const float *ks, const fl
         for (int r = 0; r < 4; ++r) s[4 * j + r] = dot[4 * j + r] * k4[r];
     }
     reference<D>(S, sf, edge, bits, h, s);
+    if (keep) {   // (a masked position stays -inf whatever sf is)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) keep[r / 4][r % 4] = s[r] == -INFINITY ? -INFINITY : s[r] * sf;
+    }
     const float M = S.M == -INFINITY ? 0.0f : S.M;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -320,9 +324,10 @@ DEV void finish_column(const QxaArgs &A, const State<D> &S, float den, const Job
 
 // Few columns (a tile or two a kv head).  A workgroup takes a tile of columns of one kv head and a run of
 // 32-position chunks; its 4 waves take every fourth chunk, each with a state of its own, merged at the end.  The
-// next chunk's rows are on their way while one is worked on.  The cache's bytes, or with few of them the
-// chain of latencies, bound it.
-template <typename T, int D>
+// next chunk's rows are on their way while one is worked on.  The cache's bytes bound it (single tokens over 4 x
+// 30000 positions of 8 kv heads: 46 us, 5.3 TB/s; 56 where scores are kept, KEEP), or with few of them the
+// chain of latencies: 8.8 us for a token over 24 positions.
+template <typename T, int D, bool KEEP>
 __global__ __launch_bounds__(256, 2) void qxa_tree(QxaArgs A) {
     constexpr bool SPLIT = two_halves_q<T>;
     constexpr int KS = D / 16, DT = D / 32, NP = SPLIT ? 2 : 1;
@@ -394,6 +399,13 @@ __global__ __launch_bounds__(256, 2) void qxa_tree(QxaArgs A) {
         if (tid < 32) A.pack_sf[at * 32 + tid] = s_sf[tid];
     }
     State<D> S;
+    f4x kept[KEEP ? 4 : 1];   // a chunk's scores, written before the loads that the next chunk issues (a wait for loads waits for older stores)
+    auto keep_scores = [&](uint32_t ci) {
+        float *to = A.scores + ((((uint64_t)b * A.a.kv_heads + g) * ((A.a.positions + 31) / 32) + ci) * A.columns + c) * 32 + 4 * h;
+        if (used)
+#pragma unroll
+            for (int j = 0; j < (KEEP ? 4 : 1); ++j) *reinterpret_cast<f4x *>(to + 8 * j) = kept[j];
+    };
     uint32_t *vt = u.vt[wave];
 #pragma unroll 1
     for (uint32_t ci = c_lo + wave; ci < c_hi; ci += 4) {
@@ -415,6 +427,7 @@ __global__ __launch_bounds__(256, 2) void qxa_tree(QxaArgs A) {
             vt[(4 * dq + 3) * 9 + pq] = perm(a3, a2, 0x07060302u);
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (KEEP && ci >= c_lo + 4) keep_scores(ci - 4);
         if (ci + 4 < c_hi) load(ci + 4);
         f16x dot = zero16();
 #pragma unroll
@@ -426,7 +439,7 @@ __global__ __launch_bounds__(256, 2) void qxa_tree(QxaArgs A) {
         const bool edge = pb + 32 > q.len;   // the chunk holds nodes
         const uint32_t bits = edge ? visible(A, q, b, node, pb) : ~0u;
         uint4 phi[2], plo[2];
-        weigh<T, D>(S, dot, sf, s_ks[wave], s_vs[wave], edge, bits, h, phi, plo);
+        weigh<T, D>(S, dot, sf, s_ks[wave], s_vs[wave], edge, bits, h, phi, plo, KEEP ? kept : nullptr);
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
             const uint32_t *row = vt + (32 * d + col) * 9;
@@ -438,6 +451,7 @@ __global__ __launch_bounds__(256, 2) void qxa_tree(QxaArgs A) {
             }
         }
     }
+    if (KEEP && c_lo + wave < c_hi) keep_scores(c_lo + wave + (c_hi - 1 - c_lo - wave) / 4 * 4);   // the last chunk's
     // merge the 4 waves: 2 + 3 into 0 + 1, then 1 into 0
     float den = S.den + __shfl_xor(S.den, 32);
     __syncthreads();
@@ -675,7 +689,9 @@ __global__ __launch_bounds__(256, 2) void qxa_wide(QxaArgs A) {
 }
 
 // The splits of a row joined: a workgroup a row, its 256 / (D / 4) strips of threads every so many splits, the
-// strips in order.  (A wave a row, a split's state after the other: 12 us for 32 splits of 128 rows.)
+// strips in order.  (A wave a row, a split's state after the other: 12 us for 32 splits of 128 rows.)  A
+// chain of loads bounds it: 4 us for 23 splits of 512 rows, 8.7 for 60 of 2048 (64 MB of states, 7.4 TB/s from the
+// caches).
 template <typename T, int D>
 __global__ __launch_bounds__(256) void qxa_join(QxaArgs A) {
     constexpr int W = D / 4, STRIPS = 256 / W;
@@ -717,12 +733,48 @@ __global__ __launch_bounds__(256) void qxa_join(QxaArgs A) {
     if (at == 0 && A.lse) A.lse[row] = den == 0.0f ? -INFINITY : (m + __log2f(den)) * 0.69314718055994531f;
 }
 
-// account[p] = decay * account[p] + sum over nodes and heads of 2^(s - lse), the scores computed again from the q
-// that the attention has left as matrix operands.  A wave keeps, per lane, its column's sums of the 16
+// account[p] = decay * account[p] + sum over nodes and heads of 2^(s - lse), of kept scores.  A wave takes 32
+// positions, 8 lanes of 4 positions a row and every eighth row; rows and strips are added up in a fixed order.
+__global__ __launch_bounds__(256) void qxa_account_kept(QxaArgs A) {
+    const uint32_t lane = threadIdx.x & 63, quad = lane & 7, b = blockIdx.y;
+    const Seq q = sequence(A, b);
+    const uint32_t total = q.len + q.count, nchunk = (total + 31) / 32, inuse = q.count * A.group, rows = A.a.kv_heads * inuse;
+    for (uint32_t ci = blockIdx.x * 4 + wave_id(); ci < nchunk; ci += gridDim.x * 4) {
+        f4x sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+        for (uint32_t r = lane >> 3; r < rows; r += 8) {
+            const uint32_t g = r / inuse, c = r % inuse, node = c / A.group, head = g * A.group + c % A.group;
+            const f4x s = *reinterpret_cast<const f4x *>(
+                A.scores + ((((uint64_t)b * A.a.kv_heads + g) * ((A.a.positions + 31) / 32) + ci) * A.columns + c) * 32 + 4 * quad);
+            const float l = A.lse[((uint64_t)b * A.a.nodes + node) * A.a.heads + head];
+            const float l2 = l == -INFINITY ? INFINITY : l * 1.4426950408889634f;   // (a row that sees nothing adds 0)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum[i] += exp2_fast(s[i] - l2);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {   // over the strips
+            float v = sum[i];
+            v += dppf<DPP_ROR8>(v);
+            const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+            v = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+            const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+            sum[i] = __uint_as_float(y[0]) + __uint_as_float(y[1]);
+        }
+        const uint32_t p = ci * 32 + 4 * quad;
+        if (lane >= 8) continue;
+        float *to = A.a.account + b * A.a.account_batch + p;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (p + i < total) to[i] = to[i] * A.a.decay + sum[i];
+    }
+}
+
+// The same, the scores computed again from the q that the attention has left as matrix operands.  A wave keeps, per lane, its column's sums of the 16
 // positions that its registers hold; columns and waves are added up in a fixed order, and no two
 // workgroups add to one position.  SHARE waves take the same 32 positions and every SHARE-th (kv head, tile): 8
 // where there are few positions, whose chain of pairs would be the time; else 1 and four chunks a
-// workgroup, which then read each q from the first-level cache.
+// workgroup, which then read each q from the first-level cache.  16 nodes of 32 heads over 1500 positions: 8.5 us,
+// the chain of 8 pairs; 128 columns a kv head over 8192 positions: the matrix instructions.
 template <typename T, int D, int SHARE>
 __global__ __launch_bounds__(SHARE == 1 ? 256 : 64 * SHARE, 1) void qxa_account(QxaArgs A) {
     constexpr bool SPLIT = two_halves_q<T>;
@@ -821,11 +873,14 @@ template <typename T, int D> void launch(const QxaArgs &A, hipStream_t s) {
     const bool shared = A.a.batch <= 64 && A.splits > 1;   // (a sequence's number of splits is rounded down, but at least one)
     const dim3 grid(A.a.kv_heads * A.wgs, shared && A.a.batch > 1 ? 2 * A.splits + A.a.batch : A.splits, shared ? 1 : A.a.batch);
     if (A.wide) hipLaunchKernelGGL((qxa_wide<T, D>), grid, dim3(256), 0, s, A);
-    else hipLaunchKernelGGL((qxa_tree<T, D>), grid, dim3(256), 0, s, A);
+    else if (A.scores) hipLaunchKernelGGL((qxa_tree<T, D, true>), grid, dim3(256), 0, s, A);
+    else hipLaunchKernelGGL((qxa_tree<T, D, false>), grid, dim3(256), 0, s, A);
     if (A.splits > 1) hipLaunchKernelGGL((qxa_join<T, D>), dim3((unsigned)rows), dim3(256), 0, s, A);
     if (A.a.account) {
         const uint64_t chunks = ((uint64_t)A.a.max_len + A.a.nodes + 31) / 32;
-        if (chunks * A.a.batch < 1024)
+        if (A.scores)
+            hipLaunchKernelGGL(qxa_account_kept, dim3((unsigned)std::min<uint64_t>(65535, std::max<uint64_t>(1, (chunks + 3) / 4)), A.a.batch), dim3(256), 0, s, A);
+        else if (chunks * A.a.batch < 1024)
             hipLaunchKernelGGL((qxa_account<T, D, 8>), dim3((unsigned)std::max<uint64_t>(1, chunks), A.a.batch), dim3(512), 0, s, A);
         else
             hipLaunchKernelGGL((qxa_account<T, D, 1>), dim3((unsigned)std::min<uint64_t>(65535, (chunks + 3) / 4), A.a.batch), dim3(256), 0, s, A);

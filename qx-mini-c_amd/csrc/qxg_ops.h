@@ -17,7 +17,8 @@ struct QxaArgs {
     float *part;
     float2 *md;
     float *lse;        // the caller's, or the workspace's for the account
-    uint4 *pack;       // with an account: q as matrix operands, [batch][kv head][tile][k-step][half][lane]
+    float *scores;     // with an account and few columns: base-2 scores, [batch][kv head][chunk of 32 positions][column][32]
+    uint4 *pack;       // with an account otherwise: q as matrix operands, [batch][kv head][tile][k-step][half][lane]
     float *pack_sf;    // [batch][kv head][tile][column] what turns dot * kscale into base-2 scores
 };
 void qxa_launch(const QxaArgs &A, hipStream_t s);
