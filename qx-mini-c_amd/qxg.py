@@ -167,7 +167,7 @@ def kvsnap_read(path, layers, ctx, seed):
 # ---- operators on device memory: device arrays and the argument structs of include/qxg.h
 #
 # A device array is a torch tensor on the GPU, or any object with its data_ptr(), shape, stride() (in
-# elements) and dtype.  torch brings a HIP runtime of its own: import it before this module, so that both
+# elements; both tuples) and dtype.  torch brings a HIP runtime of its own: import it before this module, so that both
 # use that one (memory of another runtime is refused).
 NO_TOKEN = 0xffffffff
 _TREE = struct.Struct("=12Q9Q8I2f")
@@ -177,14 +177,23 @@ _ADJUST = struct.Struct("=15Q4Q7I4x")
 _KINDS = {}   # dtype -> "f32", ...
 _NAMES = {"float32": "f32", "float16": "f16", "bfloat16": "bf16", "int32": "i32", "uint32": "i32", "int8": "i8", "uint8": "u8"}
 _VALUE_TYPES = {"f32": 0, "f16": 1, "bf16": 30}   # GGML's numbers
-_SIZES = {"f32": 4, "f16": 2, "bf16": 2}
 
 
-def _kind(t):
-    k = _KINDS.get(t.dtype)
+def _kind(dtype):
+    k = _KINDS.get(dtype)
     if k is None:
-        k = _KINDS[t.dtype] = _NAMES.get(str(t.dtype).rpartition(".")[2], str(t.dtype))
+        k = _KINDS[dtype] = _NAMES.get(str(dtype).rpartition(".")[2], str(dtype))
     return k
+
+
+def _ptr(t):
+    return 0 if t is None else t.data_ptr()
+
+
+def _layout(t):
+    """What the checks look at.  They are made once for the layouts of a call (the cached functions below): half
+    of a small call's time was theirs."""
+    return None if t is None else (t.dtype, t.shape, t.stride())
 
 
 @functools.lru_cache(maxsize=4096)
@@ -197,45 +206,116 @@ def _dense(shape):
     return tuple(reversed(out))
 
 
-def _arr(t, name, kind, shape, inner=None):
-    """Address of a device array of that kind and shape, its last `inner` dimensions (all of them if
-    None) contiguous; 0 for None."""
-    if t is None:
-        return 0
-    if _kind(t) != kind:
-        raise ValueError(f"{name} has dtype {t.dtype}, not {kind}")
-    if t.shape != shape:
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, not {shape}")
-    strides, dense = t.stride(), _dense(shape)
-    if strides != dense:
+def _fits(layout, name, kind, shape, inner=None):
+    """Refuses an array that is not of that kind and shape, its last `inner` dimensions (all of them if None)
+    contiguous; None is no array."""
+    if layout is None:
+        return
+    dtype, got, strides = layout
+    if _kind(dtype) != kind:
+        raise ValueError(f"{name} has dtype {dtype}, not {kind}")
+    if tuple(got) != tuple(shape):
+        raise ValueError(f"{name} has shape {tuple(got)}, not {tuple(shape)}")
+    dense = _dense(tuple(shape))
+    if tuple(strides) != dense:
         last = len(shape) - (len(shape) if inner is None else inner)
         if any(d != 1 and s != e for d, s, e in zip(shape[last:], strides[last:], dense[last:])):
             raise ValueError(f"{name} is not contiguous in its last {len(shape) - last} dimensions")
-    return t.data_ptr()
 
 
-def _sized(t, name):
-    """(address, bytes) of a workspace: a contiguous uint8 array."""
-    if t is None:
-        return 0, 0
-    return _arr(t, name, "u8", t.shape), t.shape[0]
+def _bytes(layout, name):
+    """Of a workspace: a contiguous uint8 array."""
+    if layout is None:
+        return 0
+    _fits(layout, name, "u8", layout[1])
+    return layout[1][0]
 
 
-def _tree_pack(ptrs, strides, kind, q_shape, k_shape, max_len, scale, decay, account_stride=0):
-    if len(q_shape) != 4 or len(k_shape) != 4:
+def _alike(a, b, what):
+    if a != b:
+        raise ValueError(f"{what} have different strides")
+
+
+def _outer(layout):
+    return layout[2][0] if layout is not None else 0
+
+
+def _value_type(layout, name):
+    kind = _kind(layout[0])
+    if kind not in _VALUE_TYPES:
+        raise ValueError(f"{name} has dtype {layout[0]}, not f32, f16 or bf16")
+    return kind
+
+
+@functools.lru_cache(maxsize=1024)
+def _tree_layout(q, k, v, kscale, vscale, lens, counts, mask, out, lse, account, workspace):
+    """The struct's fields from workspace_bytes to positions, of layouts."""
+    kind, qs, ks = _value_type(q, "q"), q[1], k[1]
+    if len(qs) != 4 or len(ks) != 4 or ks[0] != qs[0] or ks[3] != qs[3]:
         raise ValueError("q has the dimensions [batch, nodes, heads, dim], k and v [batch, positions, kv_heads, dim]")
-    batch, nodes, heads, dim = q_shape
-    positions, kv_heads = k_shape[1:3]
-    if max_len is None:
-        max_len = positions
-    if scale is None:
-        scale = dim ** -0.5
-    return _TREE.pack(*ptrs, *strides, account_stride, _VALUE_TYPES[kind], batch, nodes, heads, kv_heads, dim, positions, max_len, scale, decay)
+    batch, nodes, heads, dim = qs
+    _alike(tuple(k[2]), tuple(v[2]), "k and v")
+    _alike(_outer(kscale), _outer(vscale), "kscale and vscale")
+    for layout, name, of, shape, inner in (
+            (q, "q", kind, qs, 2), (k, "k", "i8", ks, 2), (v, "v", "i8", ks, 2), (kscale, "kscale", "f32", ks[:2], 1),
+            (vscale, "vscale", "f32", ks[:2], 1), (lens, "lens", "i32", (batch,), None), (counts, "counts", "i32", (batch,), None),
+            (mask, "mask", "i32", (batch, nodes, (nodes + 31) // 32), None), (out, "out", kind, qs, 2),
+            (lse, "lse", "f32", (batch, nodes, heads), None), (account, "account", "f32", ks[:2], 1)):
+        _fits(layout, name, of, shape, inner)
+    return (_bytes(workspace, "workspace"), q[2][0], q[2][1], out[2][0], out[2][1], k[2][0], k[2][1], _outer(kscale), _outer(account),
+            _VALUE_TYPES[kind], batch, nodes, heads, ks[2], dim, ks[1])
+
+
+@functools.lru_cache(maxsize=1024)
+def _select_layout(account, lens, keep, kept):
+    groups, positions = account[1]
+    for layout, name, of, shape, inner in ((account, "account", "f32", account[1], 1), (lens, "lens", "i32", (groups,), None),
+                                           (keep, "keep", "i32", (groups, keep[1][1]), 1), (kept, "kept", "i32", (groups,), None)):
+        _fits(layout, name, of, shape, inner)
+    return _outer(account), _outer(keep), groups, positions, keep[1][1]
+
+
+@functools.lru_cache(maxsize=1024)
+def _compact_layout(k, v, kscale, vscale, keep, kept, account, account_out, workspace):
+    groups, positions, row = k[1]
+    gp = (groups, positions)
+    _alike(tuple(k[2]), tuple(v[2]), "k and v")
+    _alike(_outer(kscale), _outer(vscale), "kscale and vscale")
+    for layout, name, of, shape, inner in (
+            (k, "k", "i8", (*gp, row), 1), (v, "v", "i8", (*gp, row), 1), (kscale, "kscale", "f32", gp, 1), (vscale, "vscale", "f32", gp, 1),
+            (keep, "keep", "i32", (groups, keep[1][1]), 1), (kept, "kept", "i32", (groups,), 0), (account, "account", "f32", gp, 1),
+            (account_out, "account_out", "f32", gp, 1)):
+        _fits(layout, name, of, shape, inner)
+    return ((_bytes(workspace, "workspace"), k[2][0], k[2][1], _outer(kscale), _outer(keep), _outer(kept), _outer(account), _outer(account_out),
+             groups, positions, keep[1][1]), row)
+
+
+@functools.lru_cache(maxsize=1024)
+def _adjust_layout(logits, out, history, history_lens, prompt_lens, penalties, temperature, bias_ids, bias_values, mask, mask_rows,
+                   top_ids, top_logits, lse, workspace):
+    kind, shape = _value_type(logits, "logits"), logits[1]
+    rows, vocab = shape
+    slots, biases, masks, top_n = (0 if x is None else x[1][i] for x, i in ((history, 1), (bias_ids, 1), (mask, 0), (top_ids, 1)))
+    for layout, name, of, want, inner in (
+            (logits, "logits", kind, shape, 1), (out, "out", kind, shape, 1), (history, "history", "i32", (rows, slots), 1),
+            (history_lens, "history_lens", "i32", (rows,), None), (prompt_lens, "prompt_lens", "i32", (rows,), None),
+            (penalties, "penalties", "f32", (rows, 3), None), (temperature, "temperature", "f32", (rows,), None),
+            (bias_ids, "bias_ids", "i32", (rows, biases), None), (bias_values, "bias_values", "f32", (rows, biases), None),
+            (mask, "mask", "i32", (masks, (vocab + 31) // 32), None), (mask_rows, "mask_rows", "i32", (rows,), None),
+            (top_ids, "top_ids", "i32", (rows, top_n), None), (top_logits, "top_logits", "f32", (rows, top_n), None),
+            (lse, "lse", "f32", (rows,), None)):
+        _fits(layout, name, of, want, inner)
+    return (_bytes(workspace, "workspace"), _outer(logits), _outer(out), _outer(history) if slots else 0, _VALUE_TYPES[kind], rows, vocab,
+            slots, biases, masks, top_n)
 
 
 @functools.lru_cache(maxsize=256)
 def _tree_workspace(q_shape, k_shape, max_len, account):
-    return _g.qxg_tree_attention_workspace(_tree_pack([0] * 10 + [16 * account] + [0], [0] * 8, "f32", q_shape, k_shape, max_len, 1.0, 1.0))
+    if len(q_shape) != 4 or len(k_shape) != 4:
+        raise ValueError("q has the dimensions [batch, nodes, heads, dim], k and v [batch, positions, kv_heads, dim]")
+    (batch, nodes, heads, dim), (positions, kv_heads) = q_shape, k_shape[1:3]
+    return _g.qxg_tree_attention_workspace(_TREE.pack(*[0] * 10, 16 * account, 0, *[0] * 9, 0, batch, nodes, heads, kv_heads, dim, positions,
+                                                      positions if max_len is None else max_len, 1.0, 1.0))
 
 
 @functools.lru_cache(maxsize=256)
@@ -526,36 +606,18 @@ class Context:
         kv_heads, dim] int8 with scales [batch, positions] f32; lens, counts [batch] int32; mask [batch,
         nodes, words] int32 bits (None: node i sees nodes 0 .. i); lse [batch, nodes, heads] f32; account
         [batch, positions] f32.  scale: 1 / sqrt(dim) unless given."""
-        kind, qs, ks = _kind(q), tuple(q.shape), tuple(k.shape)
-        if kind not in _VALUE_TYPES:
-            raise ValueError(f"q has dtype {q.dtype}, not f32, f16 or bf16")
-        if len(qs) != 4 or len(ks) != 4 or ks[0] != qs[0] or ks[3] != qs[3]:
-            raise ValueError("q has the dimensions [batch, nodes, heads, dim], k and v [batch, positions, kv_heads, dim]")
-        batch, nodes, heads, _ = qs
-        bp, q_st, o_st, k_st = ks[:2], q.stride(), out.stride(), k.stride()
-        if tuple(v.stride()) != tuple(k_st):
-            raise ValueError("k and v have different strides")
-        ws, wn = _sized(workspace, "workspace")
-        sc_st = kscale.stride()[0]
-        if vscale.stride()[0] != sc_st:
-            raise ValueError("kscale and vscale have different strides")
-        args = _tree_pack(
-            (_arr(q, "q", kind, qs, 2), _arr(k, "k", "i8", ks, 2), _arr(v, "v", "i8", ks, 2), _arr(kscale, "kscale", "f32", bp, 1),
-             _arr(vscale, "vscale", "f32", bp, 1), _arr(lens, "lens", "i32", (batch,)), _arr(counts, "counts", "i32", (batch,)),
-             _arr(mask, "mask", "i32", (batch, nodes, (nodes + 31) // 32)), _arr(out, "out", kind, qs, 2),
-             _arr(lse, "lse", "f32", (batch, nodes, heads)), _arr(account, "account", "f32", bp, 1), ws),
-            (wn, q_st[0], q_st[1], o_st[0], o_st[1], k_st[0], k_st[1], sc_st),
-            kind, qs, ks, max_len, scale, decay, account.stride()[0] if account is not None else 0)
+        fixed = _tree_layout(_layout(q), _layout(k), _layout(v), _layout(kscale), _layout(vscale), _layout(lens), _layout(counts),
+                             _layout(mask), _layout(out), _layout(lse), _layout(account), _layout(workspace))
+        args = _TREE.pack(_ptr(q), _ptr(k), _ptr(v), _ptr(kscale), _ptr(vscale), _ptr(lens), _ptr(counts), _ptr(mask), _ptr(out),
+                          _ptr(lse), _ptr(account), _ptr(workspace), *fixed, fixed[-1] if max_len is None else max_len,
+                          fixed[-2] ** -0.5 if scale is None else scale, decay)
         self._check(_g.qxg_tree_attention(self._c, args, stream, wait, self._err, 1024))
 
     def kv_select(self, account, lens, keep, kept, sinks=0, recent=0, max_len=None, stream=0, wait=True):
         """qxg_kv_select: account [groups, positions] f32, lens [groups] int32; writes keep [groups, budget]
         and kept [groups] int32."""
-        groups, positions = account.shape
-        args = _SELECT.pack(_arr(account, "account", "f32", (groups, positions), 1), _arr(lens, "lens", "i32", (groups,)),
-                            _arr(keep, "keep", "i32", (groups, keep.shape[1]), 1), _arr(kept, "kept", "i32", (groups,)),
-                            account.stride()[0], keep.stride()[0], groups, positions, keep.shape[1], sinks, recent,
-                            positions if max_len is None else max_len)
+        fixed = _select_layout(_layout(account), _layout(lens), _layout(keep), _layout(kept))
+        args = _SELECT.pack(_ptr(account), _ptr(lens), _ptr(keep), _ptr(kept), *fixed, sinks, recent, fixed[3] if max_len is None else max_len)
         self._check(_g.qxg_kv_select(self._c, args, stream, wait, self._err, 1024))
 
     def kv_compact_workspace(self, k_shape, keep_shape):
@@ -565,19 +627,10 @@ class Context:
     def kv_compact(self, k, v, kscale, vscale, keep, kept, account=None, account_out=None, first=0, workspace=None, stream=0, wait=True):
         """qxg_kv_compact: k, v [groups, positions, row bytes] int8, kscale, vscale and the accounts [groups,
         positions] f32, keep [groups, slots] and kept [groups] int32 (stride 0 over groups: one list for all)."""
-        groups, positions, row = k.shape
-        gp, st = (groups, positions), k.stride()
-        if tuple(v.stride()) != tuple(st):
-            raise ValueError("k and v have different strides")
-        if vscale.stride()[0] != kscale.stride()[0]:
-            raise ValueError("kscale and vscale have different strides")
-        ws, wn = _sized(workspace, "workspace")
-        args = _COMPACT.pack(_arr(k, "k", "i8", (*gp, row), 1), _arr(v, "v", "i8", (*gp, row), 1), _arr(kscale, "kscale", "f32", gp, 1),
-                             _arr(vscale, "vscale", "f32", gp, 1), _arr(keep, "keep", "i32", (groups, keep.shape[1]), 1),
-                             _arr(kept, "kept", "i32", (groups,), 0), _arr(account, "account", "f32", gp, 1),
-                             _arr(account_out, "account_out", "f32", gp, 1), ws, wn, st[0], st[1], kscale.stride()[0], keep.stride()[0],
-                             kept.stride()[0], account.stride()[0] if account is not None else 0,
-                             account_out.stride()[0] if account_out is not None else 0, groups, positions, keep.shape[1], first, row)
+        fixed, row = _compact_layout(_layout(k), _layout(v), _layout(kscale), _layout(vscale), _layout(keep), _layout(kept), _layout(account),
+                                     _layout(account_out), _layout(workspace))
+        args = _COMPACT.pack(_ptr(k), _ptr(v), _ptr(kscale), _ptr(vscale), _ptr(keep), _ptr(kept), _ptr(account), _ptr(account_out),
+                             _ptr(workspace), *fixed, first, row)
         self._check(_g.qxg_kv_compact(self._c, args, stream, wait, self._err, 1024))
 
     def adjust_logits_workspace(self, shape, top_n=0):
@@ -591,24 +644,9 @@ class Context:
         history_lens, prompt_lens [rows] int32; penalties [rows, 3] (repetition, frequency, presence) and
         temperature [rows] f32; bias_ids int32, bias_values f32 [rows, biases]; mask [masks, words] int32
         bits with mask_rows [rows] int32; top_ids int32, top_logits f32 [rows, top_n]; lse [rows] f32."""
-        kind = _kind(logits)
-        if kind not in _VALUE_TYPES:
-            raise ValueError(f"logits has dtype {logits.dtype}, not f32, f16 or bf16")
-        shape = rows, vocab = tuple(logits.shape)
-        slots = history.shape[1] if history is not None else 0
-        biases = bias_ids.shape[1] if bias_ids is not None else 0
-        masks = mask.shape[0] if mask is not None else 0
-        top_n = top_ids.shape[1] if top_ids is not None else 0
-        ws, wn = _sized(workspace, "workspace")
-        args = _ADJUST.pack(
-            _arr(logits, "logits", kind, shape, 1), _arr(out, "out", kind, shape, 1), _arr(history, "history", "i32", (rows, slots), 1),
-            _arr(history_lens, "history_lens", "i32", (rows,)), _arr(prompt_lens, "prompt_lens", "i32", (rows,)),
-            _arr(penalties, "penalties", "f32", (rows, 3)), _arr(temperature, "temperature", "f32", (rows,)),
-            _arr(bias_ids, "bias_ids", "i32", (rows, biases)), _arr(bias_values, "bias_values", "f32", (rows, biases)),
-            _arr(mask, "mask", "i32", (masks, (vocab + 31) // 32)), _arr(mask_rows, "mask_rows", "i32", (rows,)),
-            _arr(top_ids, "top_ids", "i32", (rows, top_n)), _arr(top_logits, "top_logits", "f32", (rows, top_n)),
-            _arr(lse, "lse", "f32", (rows,)), ws, wn, logits.stride()[0], out.stride()[0], history.stride()[0] if slots else 0,
-            _VALUE_TYPES[kind], rows, vocab, slots, biases, masks, top_n)
+        arrays = (logits, out, history, history_lens, prompt_lens, penalties, temperature, bias_ids, bias_values, mask, mask_rows, top_ids,
+                  top_logits, lse, workspace)
+        args = _ADJUST.pack(*map(_ptr, arrays), *_adjust_layout(*map(_layout, arrays)))
         self._check(_g.qxg_adjust_logits(self._c, args, stream, wait, self._err, 1024))
 
     def time_kernel(self, which, layer=0, iters=20):
