@@ -326,7 +326,7 @@ DEV void finish_column(const QxaArgs &A, const State<D> &S, float den, const Job
 // 32-position chunks; its 4 waves take every fourth chunk, each with a state of its own, merged at the end.  The
 // next chunk's rows are on their way while one is worked on.  The cache's bytes bound it (single tokens over 4 x
 // 30000 positions of 8 kv heads: 46 us, 5.3 TB/s; 56 where scores are kept, KEEP), or with few of them the
-// chain of latencies: 8.8 us for a token over 24 positions.
+// chain of latencies: 8.2 us for a token over 37 positions.
 template <typename T, int D, bool KEEP>
 __global__ __launch_bounds__(256, 2) void qxa_tree(QxaArgs A) {
     constexpr bool SPLIT = two_halves_q<T>;
@@ -337,17 +337,10 @@ __global__ __launch_bounds__(256, 2) void qxa_tree(QxaArgs A) {
     __shared__ float s_m[2][32], s_den[2][32];
     __shared__ union { uint32_t vt[4][D * 9]; float acc[2][32][D + 1]; } u;
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), col = lane & 31, h = lane >> 5;
-    const Job job = job_of(A);
-    const uint32_t g = blockIdx.x / A.tiles, tile = blockIdx.x % A.tiles, b = job.b;
-    const Seq q = sequence(A, b);
-    const uint32_t c = tile * 32 + col, node = min(c / A.group, A.a.nodes - 1), head = g * A.group + c % A.group;
-    const bool used = c < A.columns && node < q.count;
-    if (job.s.count == 0 || tile * 32 / A.group >= q.count) return;   // the whole tile is behind count
-    const uint32_t total = q.len + q.count, nchunk = (total + 31) / 32;
-    const uint32_t c_lo = (uint64_t)nchunk * job.z / job.s.count, c_hi = (uint64_t)nchunk * (job.z + 1) / job.s.count;
+    const uint32_t g = blockIdx.x / A.tiles, tile = blockIdx.x % A.tiles;
     struct { KRow<D> k; uint32_t v[4 * DT]; float ks, vs; } nx;
-    auto load = [&](uint32_t ci) {   // (rows past the last read it again)
-        const uint32_t pb = ci * 32, pk = min(pb + col, total - 1);
+    auto load = [&](uint32_t b, uint32_t ci) {   // (rows past the array's last read it again; those behind the nodes are masked)
+        const uint32_t pb = ci * 32, last = A.a.positions - 1, pk = min(pb + col, last);
         nx.k = load_k<D>(A, b, g, pk, h);
         nx.ks = A.a.kscale[b * A.a.scale_batch + pk];
         nx.vs = A.a.vscale[b * A.a.scale_batch + pk];
@@ -356,25 +349,41 @@ __global__ __launch_bounds__(256, 2) void qxa_tree(QxaArgs A) {
             const int bq = lane + 64 * i, dq = bq % (D / 4), pq = bq / (D / 4);
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-                nx.v[4 * i + r] = *reinterpret_cast<const uint32_t *>(A.a.v + b * A.a.kv_batch + min(pb + 4 * pq + r, total - 1) * A.a.kv_row +
-                                                                      g * D + 4 * dq);
+                nx.v[4 * i + r] = *reinterpret_cast<const uint32_t *>(A.a.v + b * A.a.kv_batch + min(pb + 4 * pq + r, last) * A.a.kv_row + g * D + 4 * dq);
         }
     };
-    if (c_lo + wave < c_hi) load(c_lo + wave);
-    {   // q fragments: a thread takes D / 8 dims of a column
-        const int qc = tid >> 3, seg = tid & 7;
-        const uint32_t cc = tile * 32 + qc, n = cc / A.group;
-        const bool ok = cc < A.columns && n < q.count;
-        const T *row = (const T *)A.a.q + b * A.a.q_batch + (uint64_t)(ok ? n : 0) * A.a.q_node +
-                       (g * A.group + (ok ? cc % A.group : 0)) * D + seg * (D / 8);
-        float v[D / 64][8], mx = 0.0f;
+    const int qc = tid >> 3, seg = tid & 7;   // q: a thread takes D / 8 dims of a column
+    const uint32_t qcc = tile * 32 + qc;
+    float qv[D / 64][8];
+    auto load_q = [&](uint32_t b) {
+        const T *row = (const T *)A.a.q + b * A.a.q_batch + (uint64_t)(qcc < A.columns ? qcc / A.group : 0) * A.a.q_node +
+                       (g * A.group + (qcc < A.columns ? qcc % A.group : 0)) * D + seg * (D / 8);
+#pragma unroll
+        for (int i = 0; i < D / 64; ++i) load8(row + 8 * i, qv[i]);
+    };
+    // Where the sequence needs no lengths to be known, q (and the first chunk, if the split starts at 0) need not wait
+    // for them (0.6 us of a small call).
+    const bool known = !shared_out(A) || A.a.batch == 1;
+    if (known) load_q(blockIdx.z);
+    if (A.splits == 1) load(blockIdx.z, wave);
+    const Job job = job_of(A);
+    const uint32_t b = job.b;
+    const Seq q = sequence(A, b);
+    const uint32_t c = tile * 32 + col, node = min(c / A.group, A.a.nodes - 1), head = g * A.group + c % A.group;
+    const bool used = c < A.columns && node < q.count;
+    if (job.s.count == 0 || tile * 32 / A.group >= q.count) return;   // the whole tile is behind count
+    const uint32_t total = q.len + q.count, nchunk = (total + 31) / 32;
+    const uint32_t c_lo = (uint64_t)nchunk * job.z / job.s.count, c_hi = (uint64_t)nchunk * (job.z + 1) / job.s.count;
+    if (A.splits > 1 && c_lo + wave < c_hi) load(b, c_lo + wave);
+    if (!known) load_q(b);
+    {
+        const bool ok = qcc < A.columns && qcc / A.group < q.count;
+        float mx = 0.0f;
         bool fin = true;
 #pragma unroll
-        for (int i = 0; i < D / 64; ++i) {
-            load8(row + 8 * i, v[i]);
+        for (int i = 0; i < D / 64; ++i)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) { fin = fin && isfinite(v[i][j]); mx = fmaxf(mx, fabsf(v[i][j])); }
-        }
+            for (int j = 0; j < 8; ++j) { fin = fin && isfinite(qv[i][j]); mx = fmaxf(mx, fabsf(qv[i][j])); }
         mx = fin ? mx : INFINITY;
         mx = fmaxf(mx, dppf<DPP_XOR1>(mx)); mx = fmaxf(mx, dppf<DPP_XOR2>(mx)); mx = fmaxf(mx, dppf<DPP_HALF_MIRROR>(mx));
         const bool bad = !(mx < INFINITY);   // a q that is not finite makes its row NaN
@@ -382,9 +391,9 @@ __global__ __launch_bounds__(256, 2) void qxa_tree(QxaArgs A) {
 #pragma unroll
         for (int i = 0; i < D / 64; ++i) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] = bad || !ok ? 0.0f : v[i][j];
+            for (int j = 0; j < 8; ++j) qv[i][j] = bad || !ok ? 0.0f : qv[i][j];
             uint4 hi, lo;
-            split8(v[i], sc, hi, lo);
+            split8(qv[i], sc, hi, lo);
             const int at = seg * (D / 64) + i, s = at % KS, l = qc + 32 * (at / KS);
             s_q[(s * NP) * 64 + l] = hi;
             if (SPLIT) s_q[(s * NP + 1) * 64 + l] = lo;
@@ -428,7 +437,7 @@ __global__ __launch_bounds__(256, 2) void qxa_tree(QxaArgs A) {
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         if (KEEP && ci >= c_lo + 4) keep_scores(ci - 4);
-        if (ci + 4 < c_hi) load(ci + 4);
+        if (ci + 4 < c_hi) load(b, ci + 4);
         f16x dot = zero16();
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
@@ -457,6 +466,7 @@ __global__ __launch_bounds__(256, 2) void qxa_tree(QxaArgs A) {
     __syncthreads();
 #pragma unroll 1
     for (int nw = 2; nw; nw >>= 1) {
+        if (c_hi - c_lo <= (uint32_t)nw) continue;   // (uniform) the others had no chunk
         if (wave >= nw && wave < 2 * nw) {
             const int slot = wave - nw;
 #pragma unroll
@@ -690,8 +700,7 @@ __global__ __launch_bounds__(256, 2) void qxa_wide(QxaArgs A) {
 
 // The splits of a row joined: a workgroup a row, its 256 / (D / 4) strips of threads every so many splits, the
 // strips in order.  (A wave a row, a split's state after the other: 12 us for 32 splits of 128 rows.)  A
-// chain of loads bounds it: 4 us for 23 splits of 512 rows, 8.7 for 60 of 2048 (64 MB of states, 7.4 TB/s from the
-// caches).
+// chain of loads bounds it: 4 us for 23 splits of 512 rows, 8.7 for 30 of 2048 (32 MB of states).
 template <typename T, int D>
 __global__ __launch_bounds__(256) void qxa_join(QxaArgs A) {
     constexpr int W = D / 4, STRIPS = 256 / W;
