@@ -345,9 +345,9 @@ int qxg_q8k_quantize(qxg_ctx *ctx, const float *x, uint32_t n, void *blocks_out,
  * count are left as they were.  With account, each position's weight is added to it:
  *     account[p] = decay * account[p] + sum over nodes and heads of softmax(s)[p]
  * for p < lens[b] + count, in a fixed order (equal calls give equal bits).
- * An F32 q is multiplied as two halves of 11 bits each, and its weights too (errors as of f32
- * products); for F16 and BF16 the weights are rounded to 11 bits.  nodes = 1 without a mask is
- * ordinary decoding. */
+ * An F32 q is multiplied as two halves of 11 bits each (F16 and BF16: as it is), the weights of F32 and F16
+ * too (errors as of f32 products); for BF16 they are rounded to 11 bits.  nodes = 1 without a mask is
+ * ordinary decoding.  Rows of out that overlap, and accounts that do, are refused. */
 typedef struct qxg_tree_attention_args {
     const void *q;            /* [batch][nodes][heads][dim] of `type`, 16-byte aligned */
     const int8_t *k, *v;      /* [batch][positions][kv_heads][dim], 16-byte aligned */
@@ -378,7 +378,8 @@ uint64_t qxg_tree_attention_workspace(const qxg_tree_attention_args *args);
 /* Which positions of each group (a layer, a sequence) to keep within `budget`: the first `sinks`,
  * the last `recent`, and of those between the ones with the largest account (the lower position
  * where equal; NaN as -inf).  keep[g][0 .. kept[g]) receives them in ascending order, kept[g] =
- * min(lens[g], budget); the rest of keep is left as it was. */
+ * min(lens[g], budget); the rest of keep is left as it was.  The account may be one for all groups
+ * (account_group 0), the lists of keep may not overlap. */
 typedef struct qxg_kv_select_args {
     const float *account;     /* [groups][positions] */
     const uint32_t *lens;     /* [groups] */

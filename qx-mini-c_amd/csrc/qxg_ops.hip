@@ -97,6 +97,9 @@ bool tree_plan(const qxg_tree_attention_args *p, QxaArgs &A, uint64_t &bytes, co
         return fail("the strides of q and out must be multiples of 16 bytes");
     if (a.kv_batch % 16 || a.kv_row % 16) return fail("the strides of k and v must be multiples of 16 bytes");
     if (a.kv_row >> 26) return fail("the row stride of k and v must be below 2^26 bytes");
+    if ((a.batch > 1 && a.out_batch < (uint64_t)a.heads * a.dim) || (a.nodes > 1 && a.out_node < (uint64_t)a.heads * a.dim)) return fail("rows of out overlap");
+    if (a.out && a.out == a.q) return fail("out must be another array than q");
+    if (a.account && a.batch > 1 && a.account_batch < a.positions) return fail("the accounts overlap");
     if (!std::isfinite(a.scale) || !(a.scale > 0.0f)) return fail("scale must be positive and finite");
     if (!std::isfinite(a.decay)) return fail("decay must be finite");
     A.group = a.heads / a.kv_heads;
@@ -135,6 +138,7 @@ bool select_ok(const qxg_kv_select_args *p, const Err &fail) {
     if (!p->positions || p->positions > 0x7fffffffu || p->max_len > 0x7fffffffu) return fail("positions and max_len must be below 2^31");
     if (!p->budget) return fail("budget must be positive");
     if ((uint64_t)p->sinks + p->recent > p->budget) return fail("sinks + recent exceed the budget");
+    if (p->groups > 1 && p->keep_group < p->budget) return fail("the lists of keep overlap");
     return true;
 }
 bool compact_plan(const qxg_kv_compact_args *p, QxeCompact &C, uint64_t &bytes, const Err &fail) {
@@ -145,7 +149,9 @@ bool compact_plan(const qxg_kv_compact_args *p, QxeCompact &C, uint64_t &bytes, 
     if (p->first >= p->positions) return fail("first is outside the cache");
     if (!p->row_bytes || p->row_bytes % 16 || p->row_bytes > 4096) return fail("row_bytes must be a multiple of 16 up to 4096");
     if (p->kv_group % 16 || p->kv_row % 16) return fail("the strides of k and v must be multiples of 16 bytes");
-    if (p->kv_row < p->row_bytes) return fail("the rows of k and v overlap");
+    if (p->kv_row < p->row_bytes || (p->groups > 1 && p->kv_group < p->row_bytes)) return fail("the rows of k and v overlap");
+    if (p->groups > 1 && p->scale_group < p->positions) return fail("the scales of groups overlap");
+    if (p->groups > 1 && p->account_out && p->account_out_group < p->positions) return fail("the accounts of groups overlap");
     if (!p->account != !p->account_out) return fail("account and account_out go together");
     if (p->account && p->account == p->account_out) return fail("account_out must be another array than account");
     C.a = *p;

@@ -314,13 +314,15 @@ def _tree_workspace(q_shape, k_shape, max_len, account):
     if len(q_shape) != 4 or len(k_shape) != 4:
         raise ValueError("q has the dimensions [batch, nodes, heads, dim], k and v [batch, positions, kv_heads, dim]")
     (batch, nodes, heads, dim), (positions, kv_heads) = q_shape, k_shape[1:3]
-    return _g.qxg_tree_attention_workspace(_TREE.pack(*[0] * 10, 16 * account, 0, *[0] * 9, 0, batch, nodes, heads, kv_heads, dim, positions,
-                                                      positions if max_len is None else max_len, 1.0, 1.0))
+    return _g.qxg_tree_attention_workspace(_TREE.pack(
+        *[0] * 10, 16 * account, 0, 0, 0, 0, nodes * heads * dim, heads * dim, 0, 0, 0, positions, 0, batch, nodes, heads, kv_heads, dim, positions,
+        positions if max_len is None else max_len, 1.0, 1.0))
 
 
 @functools.lru_cache(maxsize=256)
 def _compact_workspace(k_shape, keep_shape):
-    return _g.qxg_kv_compact_workspace(_COMPACT.pack(*[0] * 9, *[0, 0, k_shape[2]], *[0] * 5, k_shape[0], k_shape[1], keep_shape[1], 0, k_shape[2]))
+    groups, positions, row = k_shape
+    return _g.qxg_kv_compact_workspace(_COMPACT.pack(*[0] * 10, positions * row, row, positions, *[0] * 4, groups, positions, keep_shape[1], 0, row))
 
 
 @functools.lru_cache(maxsize=256)

@@ -247,3 +247,16 @@ def test_captured_and_replayed(ctx, hip):
         hip.hipStreamSynchronize(ctypes.c_void_p(s))
         now.check(out, ids, vals, lse)
         now.check(*now.run(ctx, hip))       # the eager call, between the replays
+
+
+def test_best_of_many_equal_slices(ctx, hip):
+    """More keys than the join has room for reach its bound: 40 large logits in each 1024 tokens, alike everywhere."""
+    rng = np.random.default_rng(5)
+    V, n = 600_000, 32
+    x = (rng.standard_normal((1, V)) - 20).astype(f32)
+    for j in range(40):
+        x[0, j::1024] = j + 1
+    ids, vals, out = hip.put(np.zeros((1, n), np.int32)), hip.put(np.zeros((1, n), f32)), hip.put(np.zeros_like(x))
+    ctx.adjust_logits(hip.put(x), out, top_ids=ids, top_logits=vals, workspace=hip.workspace(ctx.adjust_logits_workspace(x.shape, n)))
+    assert np.array_equal(out.get(), x)
+    assert np.array_equal(ids.get()[0], 39 + 1024 * np.arange(n)) and (vals.get() == 40).all()

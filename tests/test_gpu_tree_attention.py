@@ -5,8 +5,8 @@ whole (16 bits), and up to 24 accumulations round by 2^-24 of sums no larger tha
 sum |q| |code|: at most S * (2^-22 + 24 * 2^-24) < S * 2^-19 off.  Scaling and the exponent add 4 roundings
 of the score's own size, |s| * 2^-22.  Errors of the scores by d move a softmax average of values no
 larger than vmax by at most 2 d vmax; the second product, the joins and the division add less than
-2^-18 vmax (f32), and for F16 and BF16 values the weights' rounding to 11 bits half a step each, 2^-11
-vmax in all; the result's own rounding is half a step of its type.
+2^-18 vmax (f32), and for BF16 values the weights' rounding to 11 bits half a step each, 2^-11 vmax in
+all (allowed to F16 too); the result's own rounding is half a step of its type.
 """
 import numpy as np
 import pytest

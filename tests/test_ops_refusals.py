@@ -35,7 +35,7 @@ def big(n=1 << 30):
 
 def tree(**kw):
     a = dict(q=Fake((2, 3, 8, 128)), k=Fake((2, 50, 4, 128), "int8"), v=Fake((2, 50, 4, 128), "int8"), kscale=Fake((2, 50)), vscale=Fake((2, 50)),
-             lens=Fake((2,), "int32"), out=Fake((2, 3, 8, 128)), mask=Fake((2, 3, 1), "int32"), counts=Fake((2,), "int32"), lse=Fake((2, 3, 8)),
+             lens=Fake((2,), "int32"), out=Fake((2, 3, 8, 128), ptr=1 << 21), mask=Fake((2, 3, 1), "int32"), counts=Fake((2,), "int32"), lse=Fake((2, 3, 8)),
              account=Fake((2, 50)), workspace=big())
     a.update(kw)
     return a
@@ -73,6 +73,11 @@ TREE_BYTES = qxg._tree_workspace((2, 3, 8, 128), (2, 50, 4, 128), None, True)
     (dict(k=Fake((2, 50, 4, 128), "int8", strides=(1 << 34, 1 << 26, 128, 1)), v=Fake((2, 50, 4, 128), "int8", strides=(1 << 34, 1 << 26, 128, 1))),
      "row stride of k and v must be below 2\\^26"),
     (dict(workspace=Fake((300,), "uint8", ptr=(1 << 20) + 8)), "workspace is not aligned to 16 bytes"),
+    (dict(out=Fake((2, 3, 8, 128), strides=(0, 1024, 128, 1))), "rows of out overlap"),
+    (dict(out=Fake((2, 3, 8, 128), strides=(3 * 1024, 512, 128, 1))), "rows of out overlap"),
+    (dict(out=Fake((2, 3, 8, 128), strides=(1024, 2048, 128, 1), ptr=1 << 21)), "invalid context"),
+    (dict(out=Fake((2, 3, 8, 128))), "out must be another array than q"),
+    (dict(account=Fake((2, 50), strides=(0, 1))), "accounts overlap"),
     (dict(scale=float("nan")), "scale must be positive and finite"),
     (dict(scale=0.0), "scale must be positive and finite"),
     (dict(decay=float("inf")), "decay must be finite"),
@@ -97,6 +102,8 @@ def test_tree_attention_small_calls_need_no_workspace(ctx):
     (dict(account=Fake((3, 0))), "positions and max_len must be below"),
     (dict(account=Fake((3, 40), ptr=(1 << 20) + 2)), "account is not aligned"),
     (dict(kept=Fake((3,), "int32", ptr=0)), "kept is NULL"),
+    (dict(keep=Fake((3, 10), "int32", strides=(0, 1))), "lists of keep overlap"),
+    (dict(account=Fake((3, 40), strides=(0, 1))), "invalid context"),      # (one account for all groups)
 ])
 def test_kv_select(ctx, change, message):
     a = dict(account=Fake((3, 40)), lens=Fake((3,), "int32"), keep=Fake((3, 10), "int32"), kept=Fake((3,), "int32"))
@@ -117,6 +124,11 @@ def test_kv_select(ctx, change, message):
     (dict(account_out=Fake((3, 40), ptr=1 << 20)), "another array"),
     (dict(keep=Fake((3, 0), "int32")), "slots must be positive"),
     (dict(kscale=Fake((3, 41), strides=(40, 1))), "kscale has shape"),
+    (dict(k=Fake((3, 40, 64), "int8", strides=(0, 64, 1)), v=Fake((3, 40, 64), "int8", strides=(0, 64, 1))), "rows of k and v overlap"),
+    (dict(k=Fake((3, 40, 64), "int8", strides=(64, 192, 1)), v=Fake((3, 40, 64), "int8", strides=(64, 192, 1))), "invalid context"),
+    (dict(kscale=Fake((3, 40), strides=(0, 1)), vscale=Fake((3, 40), strides=(0, 1))), "scales of groups overlap"),
+    (dict(account_out=Fake((3, 40), strides=(0, 1), ptr=1 << 21)), "accounts of groups overlap"),
+    (dict(keep=Fake((3, 10), "int32", strides=(0, 1)), kept=Fake((3,), "int32", strides=(0,))), "invalid context"),      # (one list for all)
 ])
 def test_kv_compact(ctx, change, message):
     a = dict(k=Fake((3, 40, 64), "int8"), v=Fake((3, 40, 64), "int8"), kscale=Fake((3, 40)), vscale=Fake((3, 40)), keep=Fake((3, 10), "int32"),
