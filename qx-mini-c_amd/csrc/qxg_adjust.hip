@@ -333,12 +333,14 @@ __global__ __launch_bounds__(1024) void qxs_join(QxsArgs A) {
         if (A.a.top_logits) A.a.top_logits[(uint64_t)r * n + at] = x;
     };
     if (have <= ROOM) {
-        for (uint32_t i = tid; i < have; i += 1024) {
+        for (uint32_t i = tid >> 3; i < have; i += 128) {   // 8 threads a key
             const uint64_t k = s_key[i];
             uint32_t above = 0;
 #pragma unroll 4
-            for (uint32_t j = 0; j < have; ++j) above += s_key[j] > k;
-            if (above < n) put(above, k);
+            for (uint32_t j = tid & 7; j < have; j += 8) above += s_key[j] > k;
+            above += (uint32_t)dppi<DPP_XOR1>((int)above); above += (uint32_t)dppi<DPP_XOR2>((int)above);
+            above += (uint32_t)dppi<DPP_HALF_MIRROR>((int)above);
+            if ((tid & 7) == 0 && above < n) put(above, k);
         }
         if (tid >= have && tid < n) put(tid, 0);
         return;
