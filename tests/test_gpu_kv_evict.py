@@ -78,6 +78,16 @@ def test_select_long(ctx, hip, length, budget, max_len):
         assert np.array_equal(keep.get()[g], want)
 
 
+@pytest.mark.parametrize("name", sorted(ACCOUNTS))
+@pytest.mark.parametrize("budget", [17, 9000, 19000])
+def test_select_long_values(ctx, hip, name, budget):
+    """Equal ones beyond what one histogram can part, infinities, numbers next to each other."""
+    account = ACCOUNTS[name](np.random.default_rng(budget), 20000).astype(np.float32)[None]
+    keep, kept = hip.put(np.zeros((1, budget), np.int32)), hip.put(np.zeros(1, np.int32))
+    ctx.kv_select(hip.put(account), hip.put(np.array([20000], np.int32)), keep, kept, sinks=3, recent=5)
+    assert np.array_equal(keep.get()[0], chosen(account[0], 20000, budget, 3, 5))
+
+
 def test_select_lens_past_the_array_are_clamped(ctx, hip):
     account = np.arange(50, dtype=np.float32)[None]
     keep, kept = hip.put(np.zeros((1, 10), np.int32)), hip.put(np.zeros(1, np.int32))

@@ -170,6 +170,12 @@ CASES = {
     "splits_ragged": dict(batch=3, nodes=4, heads=8, kv_heads=4, dim=64, lens=(2500, 1, 600), counts=(4, 4, 2)),
     "many_columns": dict(nodes=64, heads=32, kv_heads=4, lens=(777,)),
     "many_columns_ragged": dict(batch=2, nodes=37, heads=16, kv_heads=2, dim=64, lens=(410, 95), counts=(37, 20)),
+    "many_sequences": dict(batch=33, nodes=2, heads=8, kv_heads=2, dim=64, lens=tuple(range(0, 990, 30)), counts=(2, 1, 0) * 11),
+    "sequences_beyond_64": dict(batch=70, nodes=1, heads=4, kv_heads=1, lens=tuple(range(0, 910, 13))),
+    "many_columns_beyond_64": dict(batch=66, nodes=20, heads=8, kv_heads=1, dim=64, lens=tuple(range(200, 464, 4)), counts=(20, 3, 0) * 22),
+    "scores_kept_of_8_columns": dict(batch=3, nodes=2, heads=8, kv_heads=2, lens=(700, 31, 0), counts=(1, 2, 2)),
+    "long_account": dict(nodes=9, heads=2, kv_heads=1, dim=64, lens=(33000,)),
+    "long_account_of_two_sequences": dict(batch=2, nodes=5, heads=4, kv_heads=1, lens=(16500, 17000), counts=(5, 2)),
     "sharp": dict(nodes=7, heads=8, kv_heads=2, lens=(300,), qscale=60.0),
     "flat": dict(nodes=7, heads=8, kv_heads=2, lens=(300,), qscale=1e-30),
 }
