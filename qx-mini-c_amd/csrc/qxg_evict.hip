@@ -151,7 +151,7 @@ DEV void each_batch(const qxg_kv_select_args &A, const float *acc, uint32_t lo, 
 }  // namespace
 
 // Up to 1024 E positions, a workgroup a group: a thread holds E positions' ranks in registers.  The
-// counts of its 16 steps bound it.  (Byte-wise histograms in LDS, their bins searched by one thread: 26 us
+// counts of its steps bound it: 16 at most, 0.3 us each.  (Byte-wise histograms in LDS, their bins searched by one thread: 26 us
 // for 700 positions.)
 template <int E>
 __global__ __launch_bounds__(1024) void qxe_select(qxg_kv_select_args A) {
@@ -178,7 +178,10 @@ __global__ __launch_bounds__(1024) void qxe_select(qxg_kv_select_args A) {
 // bin 8 times, by lane, as equal bins of a wave's lanes would be added one after the other), then the ranks of
 // the bin that holds the smallest kept one go to LDS, where its other bits are found as above; a bin of more
 // than ROOM ranks is halved further by another histogram.  The account is read three times, from the caches
-// after the first, and the waves meet only between the readings: one workgroup's loads bound it.
+// after the first, and the waves meet only between the readings.  The loads that one CU has on their way bound it:
+// 131000 positions 62 us, 14 .. 17 a reading (35 GB/s; alike with twice as many registers loaded ahead, and with
+// fewer instructions a rank), 3 the bins, 4 the last bits.  Shorter accounts in one workgroup's registers: 4096
+// positions 12.5 us, 700 6.5.
 __global__ __launch_bounds__(1024) void qxe_select_long(qxg_kv_select_args A) {
     constexpr int E = 8, BITS = 12, BINS = 1 << BITS, COPIES = 8, ROOM = 16384;
     __shared__ uint32_t s_hist[BINS * COPIES], s_n[2][64], s_digit, s_above, s_count, s_gt[16], s_eq[16];
@@ -314,7 +317,8 @@ __global__ __launch_bounds__(1024) void qxe_select_long(qxg_kv_select_args A) {
 // sources, says so, waits until the earlier tiles of its group whose sources lie where it is about to
 // write have been read, and writes.  A claimed tile reads without waiting, and waits only for tiles
 // claimed before it, so every wait ends (a bound on the polls ends it also where two calls share a workspace,
-// which is not allowed).  Each row is read and written once.  (Strips of columns, each walked in order by
+// which is not allowed).  Each row is read and written once: 48 groups of 2048 rows of
+// 512 bytes 43 .. 48 us (200 MB), 3 of 32768 rows picked from four times as many 60 (scattered rows).  (Strips of columns, each walked in order by
 // one workgroup, left most of the GPU idle: 989 us for 3 groups of 32768 rows.)  state: the ticket, then
 // a word a tile.
 extern "C" __global__ __launch_bounds__(256) void qxe_clear(uint32_t *state, uint32_t n) {
