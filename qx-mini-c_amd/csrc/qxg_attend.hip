@@ -65,6 +65,10 @@ DEV uint32_t wave_running(uint32_t v) {
     v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);   // row_bcast:31 into rows 2 and 3
     return v;
 }
+DEV float wave_sum(float v) {   // of all lanes, in a fixed order
+    v += dppf<DPP_XOR1>(v); v += dppf<DPP_XOR2>(v); v += dppf<DPP_ROR4>(v); v += dppf<DPP_ROR8>(v);
+    return (rdlanef(v, 0) + rdlanef(v, 16)) + (rdlanef(v, 32) + rdlanef(v, 48));
+}
 DEV uint32_t chunks_of(const Seq &q) { return max(1u, (q.len + q.count + 31) / 32); }
 DEV Splits lane_splits(const QxaArgs &A) {   // of sequence `lane`
     const uint32_t lane = threadIdx.x & 63;
@@ -76,11 +80,8 @@ DEV Splits lane_splits(const QxaArgs &A) {   // of sequence `lane`
         all = (float)chunks;
         busy = all * (float)((q.count * A.group + A.wg_columns - 1) / A.wg_columns);   // times workgroups with nodes in use
     }
-#pragma unroll
-    for (int o = 32; o; o >>= 1) {
-        all += __shfl_xor(all, o);
-        busy += __shfl_xor(busy, o);
-    }
+    all = wave_sum(all);
+    busy = wave_sum(busy);
     const float share = (float)chunks * (float)A.splits * fminf((float)A.wgs / busy, 2.0f / all);
     const uint32_t n = lane < A.a.batch ? min(chunks, max(1u, (uint32_t)share)) : 0u;
     return {n, wave_running(n) - n};
@@ -322,11 +323,12 @@ DEV void finish_column(const QxaArgs &A, const State<D> &S, float den, const Job
 }
 }  // namespace
 
-// Few columns (a tile or two a kv head).  A workgroup takes a tile of columns of one kv head and a run of
+// Few columns, or little work.  A workgroup takes a tile of columns of one kv head and a run of
 // 32-position chunks; its 4 waves take every fourth chunk, each with a state of its own, merged at the end.  The
 // next chunk's rows are on their way while one is worked on.  The cache's bytes bound it (single tokens over 4 x
 // 30000 positions of 8 kv heads: 46 us, 5.3 TB/s; 56 where scores are kept, KEEP), or with few of them the
-// chain of latencies: 8.2 us for a token over 37 positions.
+// chain of latencies: 8.2 us for a token over 37 positions, 13.4 for 16 nodes of 32 heads over 1500 (splits of a chunk
+// a wave), 26 for 64 nodes over 4032, where issue counts as well.
 template <typename T, int D, bool KEEP>
 __global__ __launch_bounds__(256, 2) void qxa_tree(QxaArgs A) {
     constexpr bool SPLIT = two_halves_q<T>;
@@ -492,7 +494,7 @@ __global__ __launch_bounds__(256, 2) void qxa_tree(QxaArgs A) {
     if (wave == 0 && used) finish_column<T, D>(A, S, den, job, node, head, h);
 }
 
-// Many columns.  The 4 waves of a workgroup take a tile of 32 columns of one kv head each and go through the
+// Many columns and much work.  The 4 waves of a workgroup take a tile of 32 columns of one kv head each and go through the
 // same chunks of 32 positions, whose codes the workgroup stages in LDS as fp16 (K by rows; V transposed, a
 // dim's 32 positions in the order of the second product's k): one conversion of a code for 128 columns.  Two
 // buffers, so one barrier a chunk; the next chunk's codes are on their way.
@@ -500,8 +502,7 @@ __global__ __launch_bounds__(256, 2) void qxa_tree(QxaArgs A) {
 // matrix instructions a chunk) take 162 us, 620 TFLOP/s of matrix work; the matrix pipe is busy a third of the
 // cycles, the vector pipe under half, LDS two fifths, and a wave's softmax does not fit behind the other wave's
 // products.  The same with chunks of 64 positions, with the next chunk's scores computed ahead, with three waves
-// a SIMD (10 registers spilled): 157 .. 164 us.  One tree of 16 nodes is a chain of latencies: 15.5 us of which
-// 3 are q's way in, 4 the two chunks and 2 the states' way out.
+// a SIMD (10 registers spilled): 157 .. 164 us.
 template <typename T, int D>
 __global__ __launch_bounds__(256, 2) void qxa_wide(QxaArgs A) {
     constexpr bool SPLIT = two_halves_q<T>, LO = two_halves_p<T>;
@@ -700,7 +701,7 @@ __global__ __launch_bounds__(256, 2) void qxa_wide(QxaArgs A) {
 
 // The splits of a row joined: a workgroup a row, its 256 / (D / 4) strips of threads every so many splits, the
 // strips in order.  (A wave a row, a split's state after the other: 12 us for 32 splits of 128 rows.)  A
-// chain of loads bounds it: 4 us for 23 splits of 512 rows, 8.7 for 30 of 2048 (32 MB of states).
+// chain of loads bounds it: 4 us for 11 splits of 512 rows, 10.3 for 2 x 1536 rows of 20 splits.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void qxa_join(QxaArgs A) {
     constexpr int W = D / 4, STRIPS = 256 / W;
@@ -782,8 +783,9 @@ __global__ __launch_bounds__(256) void qxa_account_kept(QxaArgs A) {
 // positions that its registers hold; columns and waves are added up in a fixed order, and no two
 // workgroups add to one position.  SHARE waves take the same 32 positions and every SHARE-th (kv head, tile): 8
 // where there are few positions, whose chain of pairs would be the time; else 1 and four chunks a
-// workgroup, which then read each q from the first-level cache.  16 nodes of 32 heads over 1500 positions: 8.5 us,
-// the chain of 8 pairs; 128 columns a kv head over 8192 positions: the matrix instructions.
+// workgroup, which then read each q from the first-level cache (calls of 16 nodes, BF16: over 16000 positions 40.5 us with
+// 8 and 45.4 with 1, over 30000 54.7 and 49.3).  16 nodes of 32 heads over 1500 positions: 9.5 us, a chain
+// of latencies (lengths, scales, K and q, two pairs a wave, the sums); of long ones the matrix instructions bound it.
 template <typename T, int D, int SHARE>
 __global__ __launch_bounds__(SHARE == 1 ? 256 : 64 * SHARE, 1) void qxa_account(QxaArgs A) {
     constexpr bool SPLIT = two_halves_q<T>;
@@ -889,7 +891,7 @@ template <typename T, int D> void launch(const QxaArgs &A, hipStream_t s) {
         const uint64_t chunks = ((uint64_t)A.a.max_len + A.a.nodes + 31) / 32;
         if (A.scores)
             hipLaunchKernelGGL(qxa_account_kept, dim3((unsigned)std::min<uint64_t>(65535, std::max<uint64_t>(1, (chunks + 3) / 4)), A.a.batch), dim3(256), 0, s, A);
-        else if (chunks * A.a.batch < 1024)
+        else if (chunks * A.a.batch < 768)
             hipLaunchKernelGGL((qxa_account<T, D, 8>), dim3((unsigned)std::max<uint64_t>(1, chunks), A.a.batch), dim3(512), 0, s, A);
         else
             hipLaunchKernelGGL((qxa_account<T, D, 1>), dim3((unsigned)std::min<uint64_t>(65535, (chunks + 3) / 4), A.a.batch), dim3(256), 0, s, A);

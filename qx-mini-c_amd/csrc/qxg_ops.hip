@@ -66,21 +66,37 @@ template <size_t N> bool pointers_ok(const Arg (&args)[N], const Err &fail) {
 uint64_t up16(uint64_t v) { return (v + 15) & ~15ull; }
 
 // ---- tree attention
-// Splits of the positions over the batch: about 480 workgroups (two fit a CU; with all 512 places taken some
-// workgroups of a launch waited for a second round: 217 us instead of 162 for 2 x 48 nodes of 32 heads over 65500
-// positions).  A split is at least two chunks of 32 positions in the wide kernel (16 nodes over 1500 positions:
-// 15.5 us; of four chunks 17.0; of one 15.8, but the join takes 5.0 instead of 4.0), else one for each wave.
+// Which kernel takes a tree, and the splits of its positions over the batch (F32, 32 heads of 128 dims, in us).
+//
+// The wide kernel's workgroups take four tiles at a time: a code is converted once for 128 columns, but a chunk's
+// latency is a workgroup's, where the other kernel's four waves have a chunk each.  It gains from about 12000 chunks
+// of all tiles on: 16 nodes, 4 kv heads, 12000 positions (6016 chunks) 32.1 against 26.1, 30000 (15008) 36.9 against 39.1; 64
+// nodes, 4000 positions (8128) 32.8 against 28.1, 12000 (24128) 47.6 against 52.9.
+//
+// Splits: a workgroup a CU where the work is small, else two (480 of the 512 places: with all taken some workgroups of a launch
+// waited for a second round, 217 instead of 162 for 2 x 48 nodes over 65500 positions): 16 nodes over 4000 positions
+// (2016 chunks) with 240 workgroups 17.6, with 480 20.7; 64 nodes over 4000 (8128) 33.0 and 28.4.  None where a wave has few
+// rounds of chunks anyway, as states and their join take 4, with a batch 5 to 10 (its shares are found in both
+// kernels): 8 x 16 nodes, 8 kv heads, 500 positions (4 rounds) 16.6 without, 24.6 with; 8 rounds 23.9 and 26.9, but with
+// a quarter of the workgroups 21.5 and 14.5; one tree of 64 nodes over 200 (3 rounds) 12.4 and 14.8, over 500 (5 rounds) 16.7 and 15.9.
 void tree_splits(QxaArgs &A) {
     const qxg_tree_attention_args &a = A.a;
+    const uint64_t chunks = ((uint64_t)a.max_len + a.nodes + 31) / 32;   // of a sequence
+    const uint64_t work = (uint64_t)a.batch * a.kv_heads * A.tiles * chunks;
+    A.wide = A.tiles > 2 && work > 12000;
     A.wg_columns = A.wide ? 128 : 32;
     A.wgs = (A.columns + A.wg_columns - 1) / A.wg_columns;
     const uint64_t wgs = (uint64_t)a.kv_heads * A.wgs;   // of one split
-    const uint64_t most = std::max<uint64_t>(1, ((uint64_t)a.max_len + a.nodes) / (A.wide ? 64 : 128));   // of a sequence
+    const uint64_t rounds = (chunks + 3) / 4;            // of a wave of the kernel of few columns, without splits
+    A.splits = 1;
+    if (!A.wide && rounds <= (a.batch == 1 ? 3u : wgs * a.batch < 96 ? 4u : 8u)) return;
+    const uint64_t target = !A.wide && work <= 3500 ? 240 : 480;
+    const uint64_t most = std::max<uint64_t>(1, ((uint64_t)a.max_len + a.nodes) / 128);   // of a sequence: a chunk a wave
     if (a.batch > 64) {
-        A.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(480 / (wgs * a.batch), most));
+        A.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(target / (wgs * a.batch), most));
         return;
     }
-    A.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(480 / wgs, most * a.batch));
+    A.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(target / wgs, most * a.batch));
     if (A.splits <= a.batch) A.splits = 1;   // (no more than one for each)
 }
 bool tree_plan(const qxg_tree_attention_args *p, QxaArgs &A, uint64_t &bytes, const Err &fail) {
@@ -105,7 +121,6 @@ bool tree_plan(const qxg_tree_attention_args *p, QxaArgs &A, uint64_t &bytes, co
     A.group = a.heads / a.kv_heads;
     A.columns = a.nodes * A.group;
     A.tiles = (A.columns + 31) / 32;
-    A.wide = A.tiles > 2;
     tree_splits(A);
     A.words = (a.nodes + 31) / 32;
     A.scale2 = (float)((double)a.scale * 1.4426950408889634);
@@ -113,9 +128,9 @@ bool tree_plan(const qxg_tree_attention_args *p, QxaArgs &A, uint64_t &bytes, co
     const uint64_t states = A.splits == 1 ? 0 : (a.batch > 64 ? (uint64_t)A.splits * a.batch : a.batch == 1 ? A.splits : 2ull * A.splits + a.batch) * a.nodes * a.heads;
     const uint64_t part = up16(states * a.dim * 4), md = up16(states * 8);
     // The account needs the scores again.  Of few columns they are kept (at most half as many bytes, written
-    // and read, as the K codes have): single tokens over 4 x 30000 positions, 8 kv heads of 4 columns, take 69 us
-    // with 56 for the attention and 5.5 for the account, instead of 90 with 46 and 26.  Of more they are
-    // computed again from q, which the attention leaves as matrix operands.
+    // and read, as the K codes have): single tokens over 4 x 30000 positions, 8 kv heads of 4 columns, take 65 us
+    // instead of 85, of 8 columns 77, of 16 96 instead of 86.  Of more they are computed again from q, which the
+    // attention leaves as matrix operands.
     const bool kept = a.account && A.columns * 16 <= a.dim;
     const uint64_t scores = kept ? (uint64_t)a.batch * a.kv_heads * (((uint64_t)a.positions + 31) / 32) * A.columns * 128 : 0;
     const uint64_t lse = a.account && !a.lse ? up16(rows * 4) : 0, ptiles = a.account && !kept ? (uint64_t)a.batch * a.kv_heads * A.tiles : 0;
@@ -183,7 +198,8 @@ bool adjust_plan(const qxg_adjust_logits_args *p, QxsArgs &A, uint64_t &bytes, c
     if (!a.mask != !a.masks || (!a.mask && a.mask_rows)) return fail("mask, masks and mask_rows go together");
     if (a.mask && !a.mask_rows && a.masks < a.rows) return fail("fewer masks than rows without mask_rows");
     if (!a.top_n != !a.top_ids || (!a.top_n && a.top_logits)) return fail("top_n, top_ids and top_logits go together");
-    // few rows: small slices, so that the launch is not a few workgroups' chain of latencies
+    // Few rows: small slices, so that the launch is not a few workgroups' chain of latencies (151936 F32 logits, best 8: one
+    // row 10.3 us, 11.8 with large ones; 6 rows 12.1 and 12.6; 12 rows 15.4 and 13.8).
     const uint32_t tokens = 4096 / type_size(a.type);   // of a small slice
     A.small = (uint64_t)a.rows * ((a.vocab + QXS_SLICE - 1) / QXS_SLICE) < 256;
     A.slices = (a.vocab + (A.small ? tokens : QXS_SLICE) - 1) / (A.small ? tokens : QXS_SLICE);

@@ -176,6 +176,7 @@ CASES = {
     "scores_kept_of_8_columns": dict(batch=3, nodes=2, heads=8, kv_heads=2, lens=(700, 31, 0), counts=(1, 2, 2)),
     "long_account": dict(nodes=9, heads=2, kv_heads=1, dim=64, lens=(33000,)),
     "long_account_of_two_sequences": dict(batch=2, nodes=5, heads=4, kv_heads=1, lens=(16500, 17000), counts=(5, 2)),
+    "empty_rows_of_many_columns": dict(batch=2, nodes=12, lens=(0, 3), sees=np.zeros((2, 12, 12), bool)),
     "sharp": dict(nodes=7, heads=8, kv_heads=2, lens=(300,), qscale=60.0),
     "flat": dict(nodes=7, heads=8, kv_heads=2, lens=(300,), qscale=1e-30),
 }
@@ -189,6 +190,19 @@ def test_formula(ctx, hip, name, kind):
         spec["qscale"] = 1e-3   # (1e-30 is 0 in F16)
     case = Case(kind=kind, **spec)
     _, out, lse, acc = run(ctx, hip, case)
+    check(case, out, lse, acc)
+
+
+# Cases of more than two tiles of columns, as a launch for many positions takes them (four tiles a workgroup)
+LONG = 1 << 20
+MANY_COLUMNS = sorted(n for n, c in CASES.items() if c.get("nodes", 1) * c.get("heads", 32) // c.get("kv_heads", 4) > 64)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("name", MANY_COLUMNS)
+def test_formula_many_columns(ctx, hip, name, kind):
+    case = Case(kind=kind, **CASES[name])
+    _, out, lse, acc = run(ctx, hip, case, max_len=LONG)
     check(case, out, lse, acc)
 
 
@@ -214,22 +228,24 @@ def test_without_account_and_lse(ctx, hip):
 
 
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
-def test_equal_calls_give_equal_bits(ctx, hip, kind):
+@pytest.mark.parametrize("max_len", [None, LONG])
+def test_equal_calls_give_equal_bits(ctx, hip, kind, max_len):
     case = Case(kind=kind, batch=2, nodes=20, heads=16, kv_heads=2, lens=(1500, 333))
     got = []
     for _ in range(3):
-        _, out, lse, acc = run(ctx, hip, case)
+        _, out, lse, acc = run(ctx, hip, case, max_len=max_len)
         got.append((out.get().tobytes(), lse.get().tobytes(), acc.get().tobytes()))
     assert got[0] == got[1] == got[2]
 
 
-def test_not_finite_q_stays_in_its_row(ctx, hip):
-    case = Case(nodes=4, heads=8, kv_heads=2, lens=(100,), sees="chain")
+@pytest.mark.parametrize("nodes,max_len", [(4, None), (24, LONG)])
+def test_not_finite_q_stays_in_its_row(ctx, hip, nodes, max_len):
+    case = Case(nodes=nodes, heads=8, kv_heads=2, lens=(100,), sees="chain")
     case.q[0, 1, 3, 5] = np.nan
     case.q[0, 2, 6, 0] = np.inf
-    _, out, lse, _ = run(ctx, hip, case, account=False)
+    _, out, lse, _ = run(ctx, hip, case, account=False, max_len=max_len)
     got, g_lse = out.get(), lse.get()
-    bad = np.zeros((4, 8), bool)
+    bad = np.zeros((nodes, 8), bool)
     bad[1, 3] = bad[2, 6] = True
     assert np.isnan(got[0][bad]).all() and np.isnan(g_lse[0][bad]).all()
     case.q[0, 1, 3], case.q[0, 2, 6] = 1, 1
@@ -237,13 +253,14 @@ def test_not_finite_q_stays_in_its_row(ctx, hip):
     assert (np.abs(got - w) <= t)[0][~bad].all() and (np.abs(g_lse - l) <= tl)[0][~bad].all()
 
 
-def test_masked_nodes_with_bad_scales(ctx, hip):
+@pytest.mark.parametrize("nodes,max_len", [(6, None), (30, LONG)])
+def test_masked_nodes_with_bad_scales(ctx, hip, nodes, max_len):
     """A node whose scales are not finite reaches only the nodes that see it."""
-    case = Case(nodes=6, heads=8, kv_heads=2, lens=(45,), sees=np.eye(6, dtype=bool)[None])
+    case = Case(nodes=nodes, heads=8, kv_heads=2, lens=(45,), sees=np.eye(nodes, dtype=bool)[None])
     w, l, _, t, tl, _ = case.expect()
     case.ks[0, 45 + 2], case.vs[0, 45 + 4] = np.inf, np.nan
-    _, out, lse, _ = run(ctx, hip, case, account=False)
-    ok = [0, 1, 3, 5]
+    _, out, lse, _ = run(ctx, hip, case, account=False, max_len=max_len)
+    ok = [i for i in range(nodes) if i not in (2, 4)]
     assert (np.abs(out.get() - w) <= t)[0, ok].all() and (np.abs(lse.get() - l) <= tl)[0, ok].all()
     assert np.isnan(out.get()[0, 4]).all()
 
@@ -259,9 +276,10 @@ def test_lens_past_the_cache_are_clamped(ctx, hip):
 
 
 @pytest.mark.parametrize("kind", ["f32", "f16"])
-def test_strides(ctx, hip, kind):
+@pytest.mark.parametrize("nodes,max_len", [(3, None), (40, LONG)])
+def test_strides(ctx, hip, kind, nodes, max_len):
     """q and out inside wider rows, one layer of a [layers][positions] cache, accounts with a stride."""
-    case = Case(kind=kind, batch=2, nodes=3, heads=8, kv_heads=2, dim=64, lens=(70, 41))
+    case = Case(kind=kind, batch=2, nodes=nodes, heads=8, kv_heads=2, dim=64, lens=(70, 41))
     B, n, H, D = case.q.shape
     P, Hk = case.positions, case.kv_heads
     wide = np.zeros((B, n, 3, H * D), case.q.dtype)
@@ -282,9 +300,9 @@ def test_strides(ctx, hip, kind):
     acc_all[:, :P] = case.account
     acc_dev = hip.put(acc_all)
     lse = hip.put(np.zeros((B, n, H), np.float32))
-    ws = hip.workspace(ctx.tree_attention_workspace(case.q.shape, case.k.shape, account=True))
+    ws = hip.workspace(ctx.tree_attention_workspace(case.q.shape, case.k.shape, max_len=max_len, account=True))
     ctx.tree_attention(q, k, v, ks, vs, hip.put(case.lens), out, mask=hip.put(bits(case.sees)), lse=lse,
-                       account=acc_dev.view(0, (B, P), (P + 11, 1)), decay=case.decay, workspace=ws)
+                       account=acc_dev.view(0, (B, P), (P + 11, 1)), decay=case.decay, max_len=max_len, workspace=ws)
     w_out, w_lse, w_acc, t_out, t_lse, t_acc = case.expect()
     got = o_all.get()
     assert not got[:, :, 0].any() and not got[:, :, 2].any()
@@ -294,10 +312,11 @@ def test_strides(ctx, hip, kind):
     assert (np.abs(g[:, :P] - w_acc) <= t_acc).all() and not g[:, P:].any()
 
 
-def test_cache_past_4_gib(ctx, hip):
+@pytest.mark.parametrize("nodes,max_len", [(2, None), (40, LONG)])
+def test_cache_past_4_gib(ctx, hip, nodes, max_len):
     """Rows 64 KiB apart: the last ones lie more than 2^32 bytes behind the first."""
     import ctypes
-    case = Case(kind="f16", nodes=2, heads=2, kv_heads=1, dim=64, lens=(66000,), spare=0)
+    case = Case(kind="f16", nodes=nodes, heads=2, kv_heads=1, dim=64, lens=(66000,), spare=0)
     P, pitch = case.positions, 1 << 16
     views = []
     for a in (case.k, case.v):
@@ -310,27 +329,28 @@ def test_cache_past_4_gib(ctx, hip):
         view.ptr = ptr
         views.append(view)
     acc = hip.put(case.account)
-    out, lse = hip.put(np.zeros_like(case.q), case.qtype), hip.put(np.zeros((1, 2, 2), np.float32))
-    ws = hip.workspace(ctx.tree_attention_workspace(case.q.shape, case.k.shape, account=True))
+    out, lse = hip.put(np.zeros_like(case.q), case.qtype), hip.put(np.zeros((1, nodes, 2), np.float32))
+    ws = hip.workspace(ctx.tree_attention_workspace(case.q.shape, case.k.shape, max_len=max_len, account=True))
     ctx.tree_attention(hip.put(case.q, case.qtype), *views, hip.put(case.ks), hip.put(case.vs), hip.put(case.lens), out,
-                       mask=hip.put(bits(case.sees)), lse=lse, account=acc, decay=case.decay, workspace=ws)
+                       mask=hip.put(bits(case.sees)), lse=lse, account=acc, decay=case.decay, max_len=max_len, workspace=ws)
     check(case, out, lse, acc)
 
 
-def test_captured_and_replayed(ctx, hip):
+@pytest.mark.parametrize("nodes,max_len", [(8, None), (24, LONG)])
+def test_captured_and_replayed(ctx, hip, nodes, max_len):
     """One graph, replayed with other lengths, masks and cache contents, other work between."""
     import ctypes
-    case = Case(batch=2, nodes=8, heads=8, kv_heads=2, lens=(900, 200))
+    case = Case(batch=2, nodes=nodes, heads=8, kv_heads=2, lens=(900, 200))
     s = hip.stream()
     B, n, H, D = case.q.shape
     q, k, v, ks, vs = hip.put(case.q, case.qtype), hip.put(case.k), hip.put(case.v), hip.put(case.ks), hip.put(case.vs)
     out, lse, acc = hip.put(np.zeros_like(case.q)), hip.put(np.zeros((B, n, H), np.float32)), hip.put(case.account)
     mask, lens = hip.put(bits(case.sees)), hip.put(case.lens)
-    ws = hip.workspace(ctx.tree_attention_workspace(case.q.shape, case.k.shape, account=True))
+    ws = hip.workspace(ctx.tree_attention_workspace(case.q.shape, case.k.shape, max_len=max_len, account=True))
     graph = hip.capture(s, lambda: ctx.tree_attention(q, k, v, ks, vs, lens, out, mask=mask, lse=lse, account=acc, decay=case.decay,
-                                                      workspace=ws, stream=s, wait=False))
+                                                      max_len=max_len, workspace=ws, stream=s, wait=False))
     for step, ln in enumerate([(900, 200), (17, 900), (0, 3), (640, 641)]):
-        now = Case(batch=2, nodes=8, heads=8, kv_heads=2, lens=(900, 200), seed=step)
+        now = Case(batch=2, nodes=nodes, heads=8, kv_heads=2, lens=(900, 200), seed=step)
         now.ks, now.vs = np.nan_to_num(now.ks, nan=0.03), np.nan_to_num(now.vs, posinf=0.03)
         now.lens = np.array(ln, np.int32)
         for d, a in ((q, now.q), (k, now.k), (v, now.v), (ks, now.ks), (vs, now.vs), (acc, now.account), (mask, bits(now.sees)), (lens, now.lens)):
@@ -338,7 +358,7 @@ def test_captured_and_replayed(ctx, hip):
         hip.hipGraphLaunch(graph, ctypes.c_void_p(s))
         hip.hipStreamSynchronize(ctypes.c_void_p(s))
         check(now, out, lse, acc)
-        _, o2, l2, a2 = run(ctx, hip, now)      # the eager call, between the replays
+        _, o2, l2, a2 = run(ctx, hip, now, max_len=max_len)      # the eager call, between the replays
         assert np.array_equal(o2.get(), out.get()) and np.array_equal(a2.get(), acc.get())
 
 
