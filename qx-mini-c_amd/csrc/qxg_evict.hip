@@ -148,16 +148,28 @@ DEV void each_batch(const qxg_kv_select_args &A, const float *acc, uint32_t lo, 
         f(k, p0);
     }
 }
+// A group of at most 1024 E positions, more than the budget: a thread holds E positions' ranks in registers.
+template <int E>
+DEV void select_held(const qxg_kv_select_args &A, const float *acc, const Group &G, uint32_t *keep, uint32_t (&s_n)[2][64], uint2 *s_w) {
+    const uint32_t p0 = 64 * E * wave_id();
+    uint32_t k[E], above;
+    float w[E];
+    load_weights<E>(acc, p0, G.len, w);
+    ranks_of<E>(A, w, p0, G.len, G.len, k);
+    const uint32_t least = block_nth<E>(k, A.budget, 0, 32, s_n, above);
+    uint2 all, at = waves_before(count_kept<E>(k, least), s_w, all);
+    list_kept<E>(k, p0, least, A.budget - above, at, keep);
+}
 }  // namespace
 
-// Up to 1024 E positions, a workgroup a group: a thread holds E positions' ranks in registers.  The
+// Up to 1024 E positions, a workgroup a group, in registers.  The
 // counts of its steps bound it: 16 at most, 0.3 us each.  (Byte-wise histograms in LDS, their bins searched by one thread: 26 us
 // for 700 positions.)
 template <int E>
 __global__ __launch_bounds__(1024) void qxe_select(qxg_kv_select_args A) {
     __shared__ uint32_t s_n[2][64];
     __shared__ uint2 s_w[16];
-    const uint32_t g = blockIdx.x, p0 = 64 * E * wave_id();
+    const uint32_t g = blockIdx.x;
     const Group G = group_of(A, g);
     uint32_t *keep = A.keep + g * A.keep_group;
     if (threadIdx.x == 0) A.kept[g] = G.kept;
@@ -165,16 +177,11 @@ __global__ __launch_bounds__(1024) void qxe_select(qxg_kv_select_args A) {
         for (uint32_t p = threadIdx.x; p < G.len; p += 1024) keep[p] = p;
         return;
     }
-    uint32_t k[E], above;
-    float w[E];
-    load_weights<E>(A.account + g * A.account_group, p0, G.len, w);
-    ranks_of<E>(A, w, p0, G.len, G.len, k);
-    const uint32_t least = block_nth<E>(k, A.budget, 0, 32, s_n, above);
-    uint2 all, at = waves_before(count_kept<E>(k, least), s_w, all);
-    list_kept<E>(k, p0, least, A.budget - above, at, keep);
+    select_held<E>(A, A.account + g * A.account_group, G, keep, s_n, s_w);
 }
 
-// More positions than registers hold, a sixteenth of them a wave.  A histogram of the ranks' top 12 bits (each
+// Caches of more positions; groups of up to 4096 go as above (700 of 131072: 8.2 us, as below 12.4; 4000: 9.3 and 13.9; with
+// 16 ranks a thread 5000: 26.0 and 17.2).  A sixteenth of them a wave.  A histogram of the ranks' top 12 bits (each
 // bin 8 times, by lane, as equal bins of a wave's lanes would be added one after the other), then the ranks of
 // the bin that holds the smallest kept one go to LDS, where its other bits are found as above; a bin of more
 // than ROOM ranks is halved further by another histogram.  The account is read three times, from the caches
@@ -197,6 +204,7 @@ __global__ __launch_bounds__(1024) void qxe_select_long(qxg_kv_select_args A) {
         for (uint32_t p = tid; p < G.len; p += 1024) keep[p] = p;
         return;
     }
+    if (G.len <= 4096) return select_held<4>(A, acc, G, keep, s_n, s_w);
     const uint32_t part = (G.len + 1023) / 1024 * 64, lo = min(wave * part, G.len), hi = min(lo + part, G.len);
     uint32_t least = 0, above = 0;   // bits found, and ranks above them
     int shift = 32;                  // bits still to find
@@ -412,7 +420,6 @@ extern "C" __global__ __launch_bounds__(256) void qxe_compact(QxeCompact C) {
 void qxe_launch_select(const qxg_kv_select_args &a, hipStream_t s) {
     if (a.positions <= 1024) hipLaunchKernelGGL(qxe_select<1>, dim3(a.groups), dim3(1024), 0, s, a);
     else if (a.positions <= 4096) hipLaunchKernelGGL(qxe_select<4>, dim3(a.groups), dim3(1024), 0, s, a);
-    else if (a.positions <= 16384) hipLaunchKernelGGL(qxe_select<16>, dim3(a.groups), dim3(1024), 0, s, a);
     else hipLaunchKernelGGL(qxe_select_long, dim3(a.groups), dim3(1024), 0, s, a);
 }
 void qxe_launch_compact(const QxeCompact &C, hipStream_t s) {

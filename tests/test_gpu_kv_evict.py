@@ -88,6 +88,19 @@ def test_select_long_values(ctx, hip, name, budget):
     assert np.array_equal(keep.get()[0], chosen(account[0], 20000, budget, 3, 5))
 
 
+@pytest.mark.parametrize("budget", [10, 600, 5000])
+def test_select_short_lengths_of_a_long_array(ctx, hip, budget):
+    rng = np.random.default_rng(budget)
+    lens = np.array([0, 9, 11, 700, 4095, 4096, 4097, 17000, 20000], np.int32)
+    account = np.exp(rng.standard_normal((len(lens), 20000))).astype(np.float32)
+    keep, kept = hip.put(np.full((len(lens), budget), -7, np.int32)), hip.put(np.zeros(len(lens), np.int32))
+    ctx.kv_select(hip.put(account), hip.put(lens), keep, kept, sinks=2, recent=7)
+    got, n = keep.get(), kept.get()
+    for g, length in enumerate(lens):
+        want = chosen(account[g], length, budget, 2, 7)
+        assert n[g] == len(want) and np.array_equal(got[g, :n[g]], want) and (got[g, n[g]:] == -7).all(), length
+
+
 def test_select_lens_past_the_array_are_clamped(ctx, hip):
     account = np.arange(50, dtype=np.float32)[None]
     keep, kept = hip.put(np.zeros((1, 10), np.int32)), hip.put(np.zeros(1, np.int32))
