@@ -200,8 +200,9 @@ template <bool LO> DEV void split_pairs(const float *v, uint4 &hi, uint4 &lo) {
     if constexpr (LO) lo = make_uint4(b[0], b[1], b[2], b[3]);
 }
 
-// A chunk's scores into weights, in steps.  bits: the chunk's positions that the column sees (edge: not all of them, for some column; each of the two uses opens the word anew, or the tests
-// of its bits move into every chunk).
+// A chunk's scores into weights, in steps.  bits: the chunk's positions that the column sees (edge: not all of them,
+// for some column; each of the two uses opens the word anew, or the tests of its bits move into every chunk).
+//
 // Of the scores (still to be multiplied by sf): the mask, and the maximum, which moves M where it has grown by 8.
 template <int D>
 DEV void reference(State<D> &S, float sf, bool edge, uint32_t bits, int h, float (&s)[16]) {
