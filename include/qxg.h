@@ -345,9 +345,8 @@ int qxg_q8k_quantize(qxg_ctx *ctx, const float *x, uint32_t n, void *blocks_out,
  * count are left as they were.  With account, each position's weight is added to it:
  *     account[p] = decay * account[p] + sum over nodes and heads of softmax(s)[p]
  * for p < lens[b] + count, in a fixed order (equal calls give equal bits).
- * An F32 q is multiplied as two halves of 11 bits each (F16 and BF16: as it is), the weights of F32 and F16
- * too (errors as of f32 products); for BF16 they are rounded to 11 bits.  nodes = 1 without a mask is
- * ordinary decoding.  Rows of out that overlap, and accounts that do, are refused. */
+ * An F32 q is multiplied as two halves of 11 bits each (F16 and BF16: as it is), the weights too (errors as of
+ * f32 products).  nodes = 1 without a mask is ordinary decoding.  Rows of out that overlap, and accounts that do, are refused. */
 typedef struct qxg_tree_attention_args {
     const void *q;            /* [batch][nodes][heads][dim] of `type`, 16-byte aligned */
     const int8_t *k, *v;      /* [batch][positions][kv_heads][dim], 16-byte aligned */

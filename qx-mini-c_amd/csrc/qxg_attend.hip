@@ -5,8 +5,9 @@
 // 22 bits), so the matrix cores' f32 sums are those of f32 products.  The softmax runs in base 2 in
 // one pass: a column keeps a reference M, the sum of e = 2^(s - M) and the context, the sum of e vs[pos] v.
 // M follows the running maximum to within 2^8 and is shifted by a power of two that keeps e vs, which enters
-// the second product as fp16 (hi + lo for f32 and f16 values, whose own rounding is not coarser than
-// that of 11 bits), in fp16's range; it cancels in the end.
+// the second product as fp16 hi + lo, in fp16's range; it cancels in the end.  (hi alone, 11 bits, put even BF16
+// results off by up to 2^-10 of their terms' size, which shows where terms cancel; lo costs 4 x 1 nodes over 30000 positions
+// 1 us of 58, 8 x 13 over 2900 nothing that shows.)
 //
 // Tiles.  v_mfma_f32_32x32x16_f16, rows positions, columns (node, q head of the kv head).  Lane half h
 // of A and B holds dims (D / 2) h + 8 s + j of k-step s, so a lane's K codes are D / 2 consecutive
@@ -177,12 +178,11 @@ DEV float max16(const float (&v)[16]) {   // (as a tree: a dependent instruction
     return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
 }
 template <typename T> constexpr bool two_halves_q = sizeof(T) == 4;
-template <typename T> constexpr bool two_halves_p = !__is_same(T, __bf16);
 
 // v = hi + lo (+ 2^-22 of it), a conversion for two values and one mixed-precision fma a remainder (its factor is
 // hidden, or it becomes a conversion back and a subtraction)
 typedef float f2v __attribute__((ext_vector_type(2)));
-template <bool LO> DEV void split_pairs(const float *v, uint4 &hi, uint4 &lo) {
+DEV void split_pairs(const float *v, uint4 &hi, uint4 &lo) {
     float minus = -1.0f;
     asm("" : "+s"(minus));
     uint32_t a[4], b[4];
@@ -191,13 +191,11 @@ template <bool LO> DEV void split_pairs(const float *v, uint4 &hi, uint4 &lo) {
         const f2v x = {v[2 * i], v[2 * i + 1]};
         const h2v h = __builtin_convertvector(x, h2v);
         a[i] = __builtin_bit_cast(uint32_t, h);
-        if constexpr (LO) {
-            const h2v l = {(_Float16)fmaf((float)h[0], minus, x[0]), (_Float16)fmaf((float)h[1], minus, x[1])};
-            b[i] = __builtin_bit_cast(uint32_t, l);
-        }
+        const h2v l = {(_Float16)fmaf((float)h[0], minus, x[0]), (_Float16)fmaf((float)h[1], minus, x[1])};
+        b[i] = __builtin_bit_cast(uint32_t, l);
     }
     hi = make_uint4(a[0], a[1], a[2], a[3]);
-    if constexpr (LO) lo = make_uint4(b[0], b[1], b[2], b[3]);
+    lo = make_uint4(b[0], b[1], b[2], b[3]);
 }
 
 // A chunk's scores into weights, in steps.  bits: the chunk's positions that the column sees (edge: not all of them,
@@ -223,8 +221,8 @@ DEV void reference(State<D> &S, float sf, bool edge, uint32_t bits, int h, float
         }
     }
 }
-// The weights as the second product's operands phi (and plo), M moved where they leave fp16's range
-template <typename T, int D>
+// The weights as the second product's operands phi and plo, M moved where they leave fp16's range
+template <int D>
 DEV void operands(State<D> &S, float den, float sf, bool edge, uint32_t bits, int h, float (&p)[16], uint4 (&phi)[2], uint4 (&plo)[2]) {
     if (edge) {   // (a masked position's scales do not count, whatever they are; fma(-inf, NaN) is NaN)
         uint32_t w = bits >> (4 * h);
@@ -254,10 +252,10 @@ DEV void operands(State<D> &S, float den, float sf, bool edge, uint32_t bits, in
         for (int r = 0; r < 16; ++r) p[r] *= f;
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i) split_pairs<two_halves_p<T>>(p + 8 * i, phi[i], plo[i]);
+    for (int i = 0; i < 2; ++i) split_pairs(p + 8 * i, phi[i], plo[i]);
 }
 // all of a chunk at once; its scores to keep, if there is one
-template <typename T, int D>
+template <int D>
 DEV void weigh(State<D> &S, const f16x &dot, float sf, const float *ks, const float *vs, bool edge, uint32_t bits, int h, uint4 (&phi)[2],
                uint4 (&plo)[2], f4x *keep = nullptr) {
     float s[16], p[16], den[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -283,7 +281,7 @@ DEV void weigh(State<D> &S, const f16x &dot, float sf, const float *ks, const fl
             p[4 * j + r] = e * v4[r];
         }
     }
-    operands<T, D>(S, (den[0] + den[1]) + (den[2] + den[3]), sf, edge, bits, h, p, phi, plo);
+    operands<D>(S, (den[0] + den[1]) + (den[2] + den[3]), sf, edge, bits, h, p, phi, plo);
 }
 // column c of kv head g
 struct Column { uint32_t node, head; bool used; };
@@ -451,14 +449,14 @@ __global__ __launch_bounds__(256, 2) void qxa_tree(QxaArgs A) {
         const bool edge = pb + 32 > q.len;   // the chunk holds nodes
         const uint32_t bits = edge ? visible(A, q, b, node, pb) : ~0u;
         uint4 phi[2], plo[2];
-        weigh<T, D>(S, dot, sf, s_ks[wave], s_vs[wave], edge, bits, h, phi, plo, KEEP ? kept : nullptr);
+        weigh<D>(S, dot, sf, s_ks[wave], s_vs[wave], edge, bits, h, phi, plo, KEEP ? kept : nullptr);
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
             const uint32_t *row = vt + (32 * d + col) * 9;
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
                 const uint4 vf = i8x8_to_f16(row[4 * s + h], row[4 * s + 2 + h]);
-                if constexpr (two_halves_p<T>) S.acc[d] = mfma(vf, plo[s], S.acc[d]);
+                S.acc[d] = mfma(vf, plo[s], S.acc[d]);
                 S.acc[d] = mfma(vf, phi[s], S.acc[d]);
             }
         }
@@ -506,7 +504,7 @@ __global__ __launch_bounds__(256, 2) void qxa_tree(QxaArgs A) {
 // a SIMD (10 registers spilled): 157 .. 164 us.
 template <typename T, int D>
 __global__ __launch_bounds__(256, 2) void qxa_wide(QxaArgs A) {
-    constexpr bool SPLIT = two_halves_q<T>, LO = two_halves_p<T>;
+    constexpr bool SPLIT = two_halves_q<T>;
     constexpr int KS = D / 16, DT = D / 32;
     constexpr int KP = D + 8, VP = 40;   // fp16 from one row to the next: 16 rows' 16-byte pieces lie in 16 bank groups
     __shared__ __align__(16) union { struct { _Float16 k[2][32 * KP], v[2][D * VP]; } codes; _Float16 q[4][32 * KP]; float out[4][32 * 36]; } u;
@@ -656,17 +654,15 @@ __global__ __launch_bounds__(256, 2) void qxa_wide(QxaArgs A) {
         const bool edge = pb + 32 > q.len;   // the chunk holds nodes
         const uint32_t bits = edge ? visible(A, q, b, node, pb) : ~0u;
         uint4 phi[2], plo[2];
-        weigh<T, D>(S, dot, sf, s_ks[ci & 1], s_vs[ci & 1], edge, bits, h, phi, plo);
+        weigh<D>(S, dot, sf, s_ks[ci & 1], s_vs[ci & 1], edge, bits, h, phi, plo);
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             uint4 vf[DT];
 #pragma unroll
             for (int d = 0; d < DT; ++d)
                 vf[d] = *reinterpret_cast<const uint4 *>(vr + 32 * d * VP + 8 * ((2 * s + h) ^ ((2 * d + (col >> 4)) & 3)));
-            if constexpr (LO) {
 #pragma unroll
-                for (int d = 0; d < DT; ++d) S.acc[d] = mfma(vf[d], plo[s], S.acc[d]);
-            }
+            for (int d = 0; d < DT; ++d) S.acc[d] = mfma(vf[d], plo[s], S.acc[d]);
 #pragma unroll
             for (int d = 0; d < DT; ++d) S.acc[d] = mfma(vf[d], phi[s], S.acc[d]);
         }

@@ -1,0 +1,71 @@
+"""Tree attention's numerics where products or scales are far apart, against its formula in 64 bits.
+
+Tolerances.  A score is off by at most d = 2^-19 of the sum of its products' magnitudes plus 2^-22 of its own size
+(f32 sums of products with at least 22 bits; scaling and exponent).  The result is an average with weights p of
+code * vscale: errors of the scores move it by at most 2 d of its size = 127 sum p vscale.  The weights enter the second
+product with 22 bits, or within 2^-31 of the largest p vscale where they are far smaller (of n positions: n 2^-31 of the
+size); with the f32 sums, joins and the division less than 2^-18 of the size for up to 4096 positions.  Then the
+result's own rounding, half a step of its type.
+"""
+import numpy as np
+import pytest
+
+from devmem import HALF_STEP, decode
+from test_gpu_tree_attention import LONG, Case, ctx, hip, run  # noqa: F401  (fixtures among them)
+
+pytestmark = pytest.mark.gpu
+
+
+def formula(case):
+    """out, lse, the account's new weights in 64 bits; a result's size; how far scores may be off by their sums and by themselves."""
+    q = decode(case.q, case.kind)
+    B, n, H, D = q.shape
+    out, size, lse = np.zeros(q.shape), np.zeros((B, n, H, 1)), np.full((B, n, H), -np.inf)
+    sums, scores = np.zeros((B, n, H, 1)), np.zeros((B, n, H, 1))
+    weight = np.zeros((B, case.positions))
+    for b in range(B):
+        L, c = int(case.lens[b]), int(case.counts[b])
+        T = L + c
+        vis = np.concatenate([np.ones((c, L), bool), case.sees[b, :c, :c]], 1)
+        some = vis.any(1)
+        ks, vs = case.ks[b, :T, None].astype(np.float64), case.vs[b, :T, None].astype(np.float64)
+        for h in range(H if T and c else 0):
+            g = h // (H // case.kv_heads)
+            k = case.k[b, :T, g] * ks
+            s = np.where(vis, q[b, :c, h] @ k.T * case.scale, -np.inf)
+            big = np.where(vis, np.abs(q[b, :c, h]) @ np.abs(k.T) * case.scale, 0)
+            top = np.where(some, s.max(1, initial=-np.inf), 0)
+            e = np.exp(s - top[:, None])
+            den = e.sum(1, keepdims=True)
+            p = e / np.where(den > 0, den, 1)
+            out[b, :c, h], size[b, :c, h] = p @ (case.v[b, :T, g] * vs), 127 * (p @ vs)
+            lse[b, :c, h] = np.where(some, top + np.log(np.where(den > 0, den, 1))[:, 0], -np.inf)
+            sums[b, :c, h, 0], scores[b, :c, h, 0] = big.max(1) * 2.0 ** -19, np.abs(np.where(vis, s, 0)).max(1) * 2.0 ** -22
+            weight[b, :T] += p.sum(0)
+    return out, lse, weight, size, sums, scores
+
+
+def check(case, out, lse, one_product=False, equal_scores=False):
+    """one_product: a score has one product, whose sum does not round.  equal_scores: the scores that count are equal, so
+    their errors cancel in the weights."""
+    w_out, w_lse, _, size, sums, scores = formula(case)
+    off = scores if one_product else sums + scores
+    got = decode(out.get(), case.kind)
+    err = np.abs(got - w_out)
+    tol = size * ((0 if equal_scores else 2 * off) + 2.0 ** -18) + np.abs(w_out) * HALF_STEP[case.kind]
+    l_tol = off[..., 0] + 2.0 ** -18 + np.abs(np.where(np.isneginf(w_lse), 0, w_lse)) * 2.0 ** -22
+    for b in range(case.batch):
+        c = int(case.counts[b])
+        assert (err[b, :c] <= tol[b, :c]).all(), (b, (err[b, :c] / np.maximum(size[b, :c], 1e-300)).max(), np.argwhere(~(err[b, :c] <= tol[b, :c]))[:4])
+        g, w = lse.get()[b, :c], w_lse[b, :c]
+        some = ~np.isneginf(w)
+        assert np.array_equal(np.isneginf(g), ~some) and (np.abs(g[some] - w[some]) <= l_tol[b, :c][some]).all()
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("nodes,max_len", [(1, None), (6, None), (24, LONG)])
+def test_weights_keep_their_bits(ctx, hip, kind, nodes, max_len):  # noqa: F811
+    """Small scores over a few positions: a weight rounded to 11 bits would show in the small results."""
+    case = Case(kind=kind, batch=2, nodes=nodes, heads=16, kv_heads=2, lens=(9, 3), qscale=2.0 ** -6)
+    _, out, lse, _ = run(ctx, hip, case, max_len=max_len)
+    check(case, out, lse)
