@@ -153,7 +153,10 @@ namespace {
 // sum.  m (the maximum, rounded, as of the last time that it grew by 8) and M are whole numbers, so that
 // moving M and scaling what has been summed by the power of two that belongs to it agree exactly.
 template <int D> struct State {
-    float m = -INFINITY, M = -INFINITY, den = 0.0f, limit = 0.0f;   // limit: the largest e vs before M has to move
+    // most: the largest |e vs| so far.  limit: what it may reach before M has to move; 0 where m has grown, so that the next
+    // weights place it anew (else values far smaller than those before them, which outweigh them, lost bits:
+    // V scales smaller by 10^6, scores higher by 2^80: 8e-5 off, by 10^9: 8e-2).
+    float m = -INFINITY, M = -INFINITY, den = 0.0f, most = 0.0f, limit = 0.0f;
     f16x acc[D / 32];
     DEV State() {
 #pragma unroll
@@ -214,10 +217,13 @@ DEV void reference(State<D> &S, float sf, bool edge, uint32_t bits, int h, float
     if (__ballot(cmax > S.m + 8.0f) != 0) {   // (whole wave)
         const bool grow = cmax > S.m + 8.0f;
         const float mn = rintf(cmax);
-        S.rescale(!grow || S.m == -INFINITY ? 1.0f : exp2_fast(S.m - mn));
+        const float f = !grow || S.m == -INFINITY ? 1.0f : exp2_fast(S.m - mn);
+        S.rescale(f);
+        S.most *= f;
         if (grow) {
             S.M = S.m == -INFINITY ? mn : mn - (S.m - S.M);
             S.m = mn;
+            S.limit = 0.0f;
         }
     }
 }
@@ -236,16 +242,19 @@ DEV void operands(State<D> &S, float den, float sf, bool edge, uint32_t bits, in
 #pragma unroll
     for (int r = 0; r < 16; ++r) a[r] = fabsf(p[r]);
     const float pmx = max_of_halves(max16(a));
-    if (__ballot(pmx > S.limit) != 0) {   // the first weights of a column, or one beyond fp16
+    S.most = fmaxf(S.most, pmx);
+    if (__ballot(pmx > S.limit) != 0) {   // the first weights after m has grown, or one beyond fp16
         const float M = S.M == -INFINITY ? 0.0f : S.M;
         const bool move = pmx > S.limit && pmx < INFINITY;
-        // to [2^6, 2^7), but e itself (up to 2^8 times the shift) stays far inside f32
-        int k = (int)(__float_as_uint(pow2_scale(pmx, 7)) >> 23) - 127;
+        // the largest so far to [2^6, 2^7), but e itself (up to 2^8 times the shift) stays far inside f32; a
+        // larger one, where that has kept it from there, moves M again
+        int k = (int)(__float_as_uint(pow2_scale(S.most, 7)) >> 23) - 127;
         k = move ? max(min(k, 96 - (int)(S.m - M)), -126) : 0;
         const float f = __uint_as_float((uint32_t)(127 + k) << 23);
+        S.most *= f;
         if (move) {
             S.M = M - (float)k;
-            S.limit = 32768.0f;
+            S.limit = S.most < 64.0f ? S.most : 32768.0f;
         }
         S.rescale(f);
 #pragma unroll

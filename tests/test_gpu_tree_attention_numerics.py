@@ -10,7 +10,7 @@ result's own rounding, half a step of its type.
 import numpy as np
 import pytest
 
-from devmem import HALF_STEP, decode
+from devmem import HALF_STEP, decode, encode
 from test_gpu_tree_attention import LONG, Case, ctx, hip, run  # noqa: F401  (fixtures among them)
 
 pytestmark = pytest.mark.gpu
@@ -68,4 +68,61 @@ def test_weights_keep_their_bits(ctx, hip, kind, nodes, max_len):  # noqa: F811
     """Small scores over a few positions: a weight rounded to 11 bits would show in the small results."""
     case = Case(kind=kind, batch=2, nodes=nodes, heads=16, kv_heads=2, lens=(9, 3), qscale=2.0 ** -6)
     _, out, lse, _ = run(ctx, hip, case, max_len=max_len)
+    check(case, out, lse)
+
+
+def taken_over(kind, ratio, nodes, positions=640, early=256, code=0, batch=1, kv_heads=2, dim=128, seed=0):
+    """The first `early` positions have V scales `ratio` times the last ones' and scores 0.  The others' scores are all 170,
+    or higher by 10.2 bits for every 5 of `code` with each 128 positions, the scales shrinking with them.  q has one value
+    that is not 0, so a score is one product, and equal scores come out equal."""
+    case = Case(kind=kind, batch=batch, nodes=nodes, heads=16, kv_heads=kv_heads, dim=dim, lens=(positions - nodes,) * batch,
+                sees=np.ones((batch, nodes, nodes), bool), spare=0, seed=seed)
+    q = np.zeros(case.q.shape)
+    q[..., 3] = 16
+    case.q = encode(q, kind)[0]
+    case.ks[:] = 1.0
+    at = np.arange(positions)
+    codes = np.where(at >= early, (at - early) // 128 + 1, 0) * code if code else np.where(at >= early, 120, 0)
+    case.k[..., 3] = codes[None, :, None]
+    fall = float(ratio) ** (1 - codes / codes.max())
+    case.vs = (case.vs * fall).astype(np.float32)
+    return case
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("ratio", [1e-9, 1e4, 1e6, 1e9, 1e25])
+@pytest.mark.parametrize("nodes,max_len", [(1, 0), (6, 0), (24, LONG)])
+def test_small_values_that_take_over(ctx, hip, kind, ratio, nodes, max_len):  # noqa: F811
+    """Positions whose V scales are far smaller (or larger) than those before them, and which outweigh them by 2^245."""
+    case = taken_over(kind, ratio, nodes)
+    _, out, lse, _ = run(ctx, hip, case, max_len=max_len, account=False)
+    check(case, out, lse, one_product=True, equal_scores=True)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("code,ratio", [(5, 1e6), (12, 1e12), (5, 1e20), (5, 1e30)])
+def test_small_values_that_take_over_in_steps(ctx, hip, kind, code, ratio):  # noqa: F811
+    """The maximum grows again and again while the values shrink; with 1e30, what comes first still counts most."""
+    case = taken_over(kind, ratio, 3, positions=1024, early=128, code=code)
+    _, out, lse, _ = run(ctx, hip, case, max_len=0, account=False)
+    check(case, out, lse, one_product=True)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("ratio", [1e-9, 1e6, 1e25])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_small_values_that_take_over_in_many_columns(ctx, hip, kind, ratio, dim):  # noqa: F811
+    """As many sequences and columns as take no splits: workgroups of four tiles, each over all chunks."""
+    case = taken_over(kind, ratio, 20, batch=66, kv_heads=4, dim=dim)
+    _, out, lse, _ = run(ctx, hip, case, account=False)
+    check(case, out, lse, one_product=True, equal_scores=True)
+
+
+@pytest.mark.parametrize("first,then", [(2.0 ** -130, 2.0 ** -20), (2.0 ** -112, 1.0)])
+def test_smallest_values_first(ctx, hip, first, then):  # noqa: F811
+    """V scales too small for the weights to be brought where they should do not keep those behind them from there."""
+    case = Case(nodes=2, heads=16, kv_heads=2, lens=(638,), qscale=2.0 ** -6, spare=0)
+    case.vs *= np.float32(then)
+    case.vs[:, :256] = first
+    _, out, lse, _ = run(ctx, hip, case, max_len=0, account=False)
     check(case, out, lse)
