@@ -765,7 +765,7 @@ __global__ __launch_bounds__(256) void qxa_account_kept(QxaArgs A) {
             const float l = A.lse[((uint64_t)b * A.a.nodes + node) * A.a.heads + head];
             const float l2 = l == -INFINITY ? INFINITY : l * 1.4426950408889634f;   // (a row that sees nothing adds 0)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sum[i] += exp2_fast(s[i] - l2);
+            for (int i = 0; i < 4; ++i) sum[i] += s[i] == -INFINITY ? 0.0f : exp2_fast(s[i] - l2);   // (not seen: 0, of a NaN row as well)
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {   // over the strips

@@ -126,3 +126,24 @@ def test_smallest_values_first(ctx, hip, first, then):  # noqa: F811
     case.vs[:, :256] = first
     _, out, lse, _ = run(ctx, hip, case, max_len=0, account=False)
     check(case, out, lse)
+
+
+@pytest.mark.parametrize("heads,nodes,dim", [(2, 3, 128), (8, 3, 128), (2, 2, 64), (16, 3, 64)])
+def test_not_finite_rows_in_the_account(ctx, hip, heads, nodes, dim):  # noqa: F811
+    """A row whose q is not finite makes the weights of the positions that it sees NaN, and of no others, whether its
+    scores are kept (few columns) or computed again."""
+    case = Case(nodes=nodes, heads=heads, kv_heads=1, dim=dim, lens=(40,), sees=np.eye(nodes, dtype=bool)[None])
+    case.q[0, 1, 1, 5] = np.nan
+    _, _, _, acc = run(ctx, hip, case)
+    got = acc.get()[0]
+    nan = np.zeros(case.positions, bool)
+    nan[:40] = nan[41] = True      # the cached positions and itself
+    assert np.array_equal(np.isnan(got), nan)
+    case.q[0, 1, 1, 5] = 0
+    case.sees[0, 1] = False        # the others' weights, as if it saw nothing of the nodes
+    _, _, weight, _, sums, scores = formula(case)
+    for p in (40, 42)[:nodes - 1]:
+        want = case.account[0, p] * case.decay + weight[0, p]
+        off = (sums + scores).max()
+        assert abs(got[p] - want) <= weight[0, p] * (2 * off + 2.0 ** -17) + want * 2.0 ** -22
+    assert np.array_equal(got[40 + nodes:], case.account[0, 40 + nodes:])
