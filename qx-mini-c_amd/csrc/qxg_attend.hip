@@ -134,6 +134,12 @@ DEV uint32_t visible(const QxaArgs &A, const Seq &q, uint32_t b, uint32_t node, 
 // the mask's bit of register r, of bits >> 4 h in lane half h
 DEV bool seen(uint32_t w, int r) { return w & (1u << (8 * (r >> 2) + (r & 3))); }
 
+// What turns dot * kscale into base-2 scores, of a q scaled by sc.  Not 0, with which -inf in a masked place would become
+// NaN (so small a factor, of dots below 2^28, leaves all scores as good as 0 anyway).
+DEV float score_factor(const QxaArgs &A, float sc, bool bad) {   // bad: a q that is not finite, which makes its row NaN
+    return bad ? NAN : fmaxf(A.scale2 / sc, 0x1p-126f);
+}
+
 template <int D> struct KRow { uint4 k[D / 32]; };
 template <int D> DEV KRow<D> load_k(const QxaArgs &A, uint32_t b, uint32_t g, uint32_t pos, int h) {
     KRow<D> x;
@@ -396,7 +402,7 @@ __global__ __launch_bounds__(256, 2) void qxa_tree(QxaArgs A) {
             for (int j = 0; j < 8; ++j) { fin = fin && isfinite(qv[i][j]); mx = fmaxf(mx, fabsf(qv[i][j])); }
         mx = fin ? mx : INFINITY;
         mx = fmaxf(mx, dppf<DPP_XOR1>(mx)); mx = fmaxf(mx, dppf<DPP_XOR2>(mx)); mx = fmaxf(mx, dppf<DPP_HALF_MIRROR>(mx));
-        const bool bad = !(mx < INFINITY);   // a q that is not finite makes its row NaN
+        const bool bad = !(mx < INFINITY);
         const float sc = pow2_scale(bad ? 0.0f : mx, 14);
 #pragma unroll
         for (int i = 0; i < D / 64; ++i) {
@@ -408,7 +414,7 @@ __global__ __launch_bounds__(256, 2) void qxa_tree(QxaArgs A) {
             s_q[(s * NP) * 64 + l] = hi;
             if (SPLIT) s_q[(s * NP + 1) * 64 + l] = lo;
         }
-        if (seg == 0) s_sf[qc] = bad ? NAN : A.scale2 / sc;
+        if (seg == 0) s_sf[qc] = score_factor(A, sc, bad);
     }
     __syncthreads();
     const float sf = s_sf[col];
@@ -602,9 +608,9 @@ __global__ __launch_bounds__(256, 2) void qxa_wide(QxaArgs A) {
             m = max(m, __float_as_uint(dppf<DPP_XOR1>(__uint_as_float(m))));
             m = max(m, __float_as_uint(dppf<DPP_XOR2>(__uint_as_float(m))));
             m = max(m, __float_as_uint(dppf<DPP_HALF_MIRROR>(__uint_as_float(m))));
-            const bool bad = m >= 0x7f800000u;   // makes its row NaN
+            const bool bad = m >= 0x7f800000u;
             sc[i] = pow2_scale(__uint_as_float(m), 14);
-            if (seg == 0) s_sf[wave][(lane >> 3) + 8 * i] = bad ? NAN : A.scale2 / sc[i];
+            if (seg == 0) s_sf[wave][(lane >> 3) + 8 * i] = score_factor(A, sc[i], bad);
         }
 #pragma unroll
         for (int half = 0; half < (SPLIT ? 2 : 1); ++half) {

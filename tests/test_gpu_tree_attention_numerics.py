@@ -11,7 +11,7 @@ import numpy as np
 import pytest
 
 from devmem import HALF_STEP, decode, encode
-from test_gpu_tree_attention import LONG, Case, ctx, hip, run  # noqa: F401  (fixtures among them)
+from test_gpu_tree_attention import LONG, Case, bits, ctx, hip, run  # noqa: F401  (fixtures among them)
 
 pytestmark = pytest.mark.gpu
 
@@ -147,3 +147,17 @@ def test_not_finite_rows_in_the_account(ctx, hip, heads, nodes, dim):  # noqa: F
         off = (sums + scores).max()
         assert abs(got[p] - want) <= weight[0, p] * (2 * off + 2.0 ** -17) + want * 2.0 ** -22
     assert np.array_equal(got[40 + nodes:], case.account[0, 40 + nodes:])
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("nodes,max_len", [(3, None), (24, LONG)])
+@pytest.mark.parametrize("qscale,scale", [(2.0 ** -110, 1e-30), (2.0 ** -124, 1e-8), (2.0 ** -124, 1e-45), (1e37, 1e-38)])
+def test_scales_at_the_ends(ctx, hip, kind, nodes, max_len, qscale, scale):  # noqa: F811
+    """Tiny q and scales: all scores are as good as 0, and masked positions still count nothing."""
+    case = Case(kind=kind, nodes=nodes, heads=8, kv_heads=2, lens=(37,), qscale=qscale)
+    case.scale = float(np.float32(scale))
+    q, k, v, ks, vs = hip.put(case.q, case.qtype), hip.put(case.k), hip.put(case.v), hip.put(case.ks), hip.put(case.vs)
+    out, lse = hip.put(np.zeros_like(case.q), case.qtype), hip.put(np.zeros(case.q.shape[:3], np.float32))
+    ws = hip.workspace(ctx.tree_attention_workspace(case.q.shape, case.k.shape, max_len=max_len))
+    ctx.tree_attention(q, k, v, ks, vs, hip.put(case.lens), out, mask=hip.put(bits(case.sees)), lse=lse, max_len=max_len, scale=scale, workspace=ws)
+    check(case, out, lse)
