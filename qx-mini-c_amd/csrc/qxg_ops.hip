@@ -124,6 +124,7 @@ bool tree_plan(const qxg_tree_attention_args *p, QxaArgs &A, uint64_t &bytes, co
     tree_splits(A);
     A.words = (a.nodes + 31) / 32;
     A.scale2 = (float)((double)a.scale * 1.4426950408889634);
+    if (!std::isfinite(A.scale2)) return fail("scale * log2(e) must be finite");
     const uint64_t rows = (uint64_t)a.batch * a.nodes * a.heads;
     const uint64_t states = A.splits == 1 ? 0 : (a.batch > 64 ? (uint64_t)A.splits * a.batch : a.batch == 1 ? A.splits : 2ull * A.splits + a.batch) * a.nodes * a.heads;
     const uint64_t part = up16(states * a.dim * 4), md = up16(states * 8);
