@@ -63,6 +63,22 @@ template <size_t N> bool pointers_ok(const Arg (&args)[N], const Err &fail) {
     }
     return true;
 }
+// Whether rows of `row` elements at i a + j b, i < na, j < nb, overlap.  (Most layouts are nested: the rows of one
+// index lie in a run of their own.)
+bool rows_overlap(uint64_t a, uint64_t na, uint64_t b, uint64_t nb, uint64_t row) {
+    using wide = unsigned __int128;
+    if (na < nb) { std::swap(a, b); std::swap(na, nb); }
+    if (na == 1) return false;
+    if (a < row) return true;
+    if (nb == 1) return false;
+    if (b < row) return true;
+    if (a >= (wide)(nb - 1) * b + row || b >= (wide)(na - 1) * a + row) return false;
+    for (uint64_t j = 1; j < nb; ++j) {   // the two rows (i, 0) next to (0, j)
+        const wide at = (wide)j * b, i = at / a;
+        if ((i && i < na && at - i * a < row) || (i + 1 < na && (i + 1) * a - at < row)) return true;
+    }
+    return false;
+}
 uint64_t up16(uint64_t v) { return (v + 15) & ~15ull; }
 
 // ---- tree attention
@@ -113,7 +129,7 @@ bool tree_plan(const qxg_tree_attention_args *p, QxaArgs &A, uint64_t &bytes, co
         return fail("the strides of q and out must be multiples of 16 bytes");
     if (a.kv_batch % 16 || a.kv_row % 16) return fail("the strides of k and v must be multiples of 16 bytes");
     if (a.kv_row >> 26) return fail("the row stride of k and v must be below 2^26 bytes");
-    if ((a.batch > 1 && a.out_batch < (uint64_t)a.heads * a.dim) || (a.nodes > 1 && a.out_node < (uint64_t)a.heads * a.dim)) return fail("rows of out overlap");
+    if (rows_overlap(a.out_batch, a.batch, a.out_node, a.nodes, (uint64_t)a.heads * a.dim)) return fail("rows of out overlap");
     if (a.out && a.out == a.q) return fail("out must be another array than q");
     if (a.account && a.batch > 1 && a.account_batch < a.positions) return fail("the accounts overlap");
     if (!std::isfinite(a.scale) || !(a.scale > 0.0f)) return fail("scale must be positive and finite");
@@ -165,7 +181,7 @@ bool compact_plan(const qxg_kv_compact_args *p, QxeCompact &C, uint64_t &bytes, 
     if (p->first >= p->positions) return fail("first is outside the cache");
     if (!p->row_bytes || p->row_bytes % 16 || p->row_bytes > 4096) return fail("row_bytes must be a multiple of 16 up to 4096");
     if (p->kv_group % 16 || p->kv_row % 16) return fail("the strides of k and v must be multiples of 16 bytes");
-    if (p->kv_row < p->row_bytes || (p->groups > 1 && p->kv_group < p->row_bytes)) return fail("the rows of k and v overlap");
+    if (rows_overlap(p->kv_row, p->positions, p->kv_group, p->groups, p->row_bytes)) return fail("the rows of k and v overlap");
     if (p->groups > 1 && p->scale_group < p->positions) return fail("the scales of groups overlap");
     if (p->groups > 1 && p->account_out && p->account_out_group < p->positions) return fail("the accounts of groups overlap");
     if (!p->account != !p->account_out) return fail("account and account_out go together");
