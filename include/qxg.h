@@ -383,7 +383,7 @@ typedef struct qxg_kv_select_args {
     const float *account;     /* [groups][positions] */
     const uint32_t *lens;     /* [groups] */
     uint32_t *keep;           /* [groups][budget] */
-    uint32_t *kept;           /* [groups] */
+    uint32_t *kept;           /* [groups]; may be lens itself, which then holds the new lengths */
     uint64_t account_group, keep_group;   /* strides in elements */
     uint32_t groups, positions, budget, sinks, recent;   /* sinks + recent <= budget */
     uint32_t max_len;         /* as in qxg_tree_attention */

@@ -33,6 +33,11 @@ DEV Group group_of(const qxg_kv_select_args &A, uint32_t g) {
     x.kept = min(x.len, A.budget);
     return x;
 }
+// A group that is kept whole.  (kept may be lens: a wave that reads its length only after this finds the same.)
+DEV void keep_all(const qxg_kv_select_args &A, uint32_t g, const Group &G, uint32_t *keep) {
+    if (threadIdx.x == 0) A.kept[g] = G.kept;
+    for (uint32_t p = threadIdx.x; p < G.len; p += 1024) keep[p] = p;
+}
 // rank of position p: the largest number for those kept in any case, 0 behind the end
 DEV uint32_t rank_at(const qxg_kv_select_args &A, float w, uint32_t p, uint32_t len) {
     return p >= len ? 0u : p < A.sinks || p >= len - A.recent ? ~0u : weight_rank(w);
@@ -172,12 +177,9 @@ __global__ __launch_bounds__(1024) void qxe_select(qxg_kv_select_args A) {
     const uint32_t g = blockIdx.x;
     const Group G = group_of(A, g);
     uint32_t *keep = A.keep + g * A.keep_group;
-    if (threadIdx.x == 0) A.kept[g] = G.kept;
-    if (G.len <= A.budget) {
-        for (uint32_t p = threadIdx.x; p < G.len; p += 1024) keep[p] = p;
-        return;
-    }
+    if (G.len <= A.budget) return keep_all(A, g, G, keep);
     select_held<E>(A, A.account + g * A.account_group, G, keep, s_n, s_w);
+    if (threadIdx.x == 0) A.kept[g] = G.kept;   // (kept may be lens: behind the barriers, so that every wave has its length)
 }
 
 // Caches of more positions; groups of up to 4096 go as above (700 of 131072: 8.2 us, as below 12.4; 4000: 9.3 and 13.9; with
@@ -199,12 +201,12 @@ __global__ __launch_bounds__(1024) void qxe_select_long(qxg_kv_select_args A) {
     const Group G = group_of(A, g);
     uint32_t *keep = A.keep + g * A.keep_group;
     const float *acc = A.account + g * A.account_group;
-    if (tid == 0) A.kept[g] = G.kept;
-    if (G.len <= A.budget) {
-        for (uint32_t p = tid; p < G.len; p += 1024) keep[p] = p;
+    if (G.len <= A.budget) return keep_all(A, g, G, keep);
+    if (G.len <= 4096) {
+        select_held<4>(A, acc, G, keep, s_n, s_w);
+        if (tid == 0) A.kept[g] = G.kept;
         return;
     }
-    if (G.len <= 4096) return select_held<4>(A, acc, G, keep, s_n, s_w);
     const uint32_t part = (G.len + 1023) / 1024 * 64, lo = min(wave * part, G.len), hi = min(lo + part, G.len);
     uint32_t least = 0, above = 0;   // bits found, and ranks above them
     int shift = 32;                  // bits still to find
@@ -319,6 +321,7 @@ __global__ __launch_bounds__(1024) void qxe_select_long(qxg_kv_select_args A) {
     uint2 at = make_uint2(0, 0);
     for (int w = 0; w < wave; ++w) { at.x += s_gt[w]; at.y += s_eq[w]; }
     each_batch<E>(A, acc, lo, hi, G.len, [&](const uint32_t (&k)[E], uint32_t p0) { list_kept<E>(k, p0, least, A.budget - above, at, keep); });
+    if (tid == 0) A.kept[g] = G.kept;   // (as above)
 }
 
 // Rows moved in place.  Tiles of R rows (32 KB of K, or one row) are claimed in order: a workgroup reads its tile's

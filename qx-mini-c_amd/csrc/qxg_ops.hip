@@ -171,6 +171,8 @@ bool select_ok(const qxg_kv_select_args *p, const Err &fail) {
     if (!p->budget) return fail("budget must be positive");
     if ((uint64_t)p->sinks + p->recent > p->budget) return fail("sinks + recent exceed the budget");
     if (p->groups > 1 && p->keep_group < p->budget) return fail("the lists of keep overlap");
+    const uintptr_t lens = (uintptr_t)p->lens, kept = (uintptr_t)p->kept, bytes = (uintptr_t)p->groups * 4;
+    if (kept != lens && kept < lens + bytes && lens < kept + bytes) return fail("kept overlaps lens (it may be lens itself)");
     return true;
 }
 bool compact_plan(const qxg_kv_compact_args *p, QxeCompact &C, uint64_t &bytes, const Err &fail) {

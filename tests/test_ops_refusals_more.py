@@ -40,3 +40,11 @@ def test_rows_of_a_cache_that_overlap(ctx, group, row):  # noqa: F811
     a = dict(k=k, v=k, kscale=Fake((3, 40)), vscale=Fake((3, 40)), keep=Fake((3, 10), "int32"), kept=Fake((3,), "int32"), workspace=big())
     with pytest.raises(qxg.QxgError, match="rows of k and v overlap" if overlaps((group, row), (3, 40), 64) else "invalid context"):
         ctx.kv_compact(**a)
+
+
+@pytest.mark.parametrize("offset,message", [(0, "invalid context"), (4, "kept overlaps lens"), (-8, "kept overlaps lens"), (12, "invalid context"),
+                                            (-12, "invalid context")])
+def test_kept_that_overlaps_lens(ctx, offset, message):  # noqa: F811
+    a = dict(account=Fake((3, 40)), lens=Fake((3,), "int32"), keep=Fake((3, 10), "int32", ptr=1 << 21), kept=Fake((3,), "int32", ptr=(1 << 20) + offset))
+    with pytest.raises(qxg.QxgError, match=message):
+        ctx.kv_select(**a)
