@@ -363,16 +363,16 @@ __global__ __launch_bounds__(1024) void qxs_join(QxsArgs A) {
 }
 
 namespace {
-template <typename T> void launch(const QxsArgs &A, hipStream_t s) {
+template <typename T> hipError_t launch(const QxsArgs &A, hipStream_t s) {
     constexpr int STEPS = QXS_SLICE * sizeof(T) / 4096;
-    if (A.small) hipLaunchKernelGGL((qxs_slice<T, 1>), dim3(A.slices, A.a.rows), dim3(256), A.a.biases * 8, s, A);
-    else hipLaunchKernelGGL((qxs_slice<T, STEPS>), dim3(A.slices, A.a.rows), dim3(256), A.a.biases * 8, s, A);
-    if (A.a.lse || A.a.top_n) hipLaunchKernelGGL(qxs_join<T>, dim3(A.a.rows), dim3(1024), 0, s, A);
+    auto *kernel = A.small ? qxs_slice<T, 1> : qxs_slice<T, STEPS>;
+    const hipError_t e = qxg_launch(kernel, dim3(A.slices, A.a.rows), dim3(256), A.a.biases * 8, s, A);
+    return e != hipSuccess || !(A.a.lse || A.a.top_n) ? e : qxg_launch(qxs_join<T>, dim3(A.a.rows), dim3(1024), 0, s, A);
 }
 }  // namespace
 
-void qxs_launch(const QxsArgs &A, hipStream_t s) {
-    if (A.a.type == QXG_TYPE_F32) launch<float>(A, s);
-    else if (A.a.type == QXG_TYPE_F16) launch<_Float16>(A, s);
-    else launch<__bf16>(A, s);
+hipError_t qxs_launch(const QxsArgs &A, hipStream_t s) {
+    if (A.a.type == QXG_TYPE_F32) return launch<float>(A, s);
+    if (A.a.type == QXG_TYPE_F16) return launch<_Float16>(A, s);
+    return launch<__bf16>(A, s);
 }

@@ -891,28 +891,24 @@ __global__ __launch_bounds__(SHARE == 1 ? 256 : 64 * SHARE, 1) void qxa_account(
 }
 
 namespace {
-template <typename T, int D> void launch(const QxaArgs &A, hipStream_t s) {
+template <typename T, int D> hipError_t launch(const QxaArgs &A, hipStream_t s) {
     const uint64_t rows = (uint64_t)A.a.batch * A.a.nodes * A.a.heads;
     const bool shared = A.a.batch <= 64 && A.splits > 1;   // (a sequence's number of splits is rounded down, but at least one)
     const dim3 grid(A.a.kv_heads * A.wgs, shared && A.a.batch > 1 ? 2 * A.splits + A.a.batch : A.splits, shared ? 1 : A.a.batch);
-    if (A.wide) hipLaunchKernelGGL((qxa_wide<T, D>), grid, dim3(256), 0, s, A);
-    else if (A.scores) hipLaunchKernelGGL((qxa_tree<T, D, true>), grid, dim3(256), 0, s, A);
-    else hipLaunchKernelGGL((qxa_tree<T, D, false>), grid, dim3(256), 0, s, A);
-    if (A.splits > 1) hipLaunchKernelGGL((qxa_join<T, D>), dim3((unsigned)rows), dim3(256), 0, s, A);
-    if (A.a.account) {
-        const uint64_t chunks = ((uint64_t)A.a.max_len + A.a.nodes + 31) / 32;
-        if (A.scores)
-            hipLaunchKernelGGL(qxa_account_kept, dim3((unsigned)std::min<uint64_t>(65535, std::max<uint64_t>(1, (chunks + 3) / 4)), A.a.batch), dim3(256), 0, s, A);
-        else if (chunks * A.a.batch < 768)
-            hipLaunchKernelGGL((qxa_account<T, D, 8>), dim3((unsigned)std::max<uint64_t>(1, chunks), A.a.batch), dim3(512), 0, s, A);
-        else
-            hipLaunchKernelGGL((qxa_account<T, D, 1>), dim3((unsigned)std::min<uint64_t>(65535, (chunks + 3) / 4), A.a.batch), dim3(256), 0, s, A);
-    }
+    auto *kernel = A.wide ? qxa_wide<T, D> : A.scores ? qxa_tree<T, D, true> : qxa_tree<T, D, false>;
+    hipError_t e = qxg_launch(kernel, grid, dim3(256), 0, s, A);
+    if (e == hipSuccess && A.splits > 1) e = qxg_launch(qxa_join<T, D>, dim3((unsigned)rows), dim3(256), 0, s, A);
+    if (e != hipSuccess || !A.a.account) return e;
+    const uint64_t chunks = ((uint64_t)A.a.max_len + A.a.nodes + 31) / 32;
+    const auto in_fours = [&] { return dim3((unsigned)std::min<uint64_t>(65535, (chunks + 3) / 4), A.a.batch); };
+    if (A.scores) return qxg_launch(qxa_account_kept, in_fours(), dim3(256), 0, s, A);
+    if (chunks * A.a.batch < 768) return qxg_launch(qxa_account<T, D, 8>, dim3((unsigned)chunks, A.a.batch), dim3(512), 0, s, A);
+    return qxg_launch(qxa_account<T, D, 1>, in_fours(), dim3(256), 0, s, A);
 }
 }  // namespace
 
-void qxa_launch(const QxaArgs &A, hipStream_t s) {
-    if (A.a.type == QXG_TYPE_F32) A.a.dim == 64 ? launch<float, 64>(A, s) : launch<float, 128>(A, s);
-    else if (A.a.type == QXG_TYPE_F16) A.a.dim == 64 ? launch<_Float16, 64>(A, s) : launch<_Float16, 128>(A, s);
-    else A.a.dim == 64 ? launch<__bf16, 64>(A, s) : launch<__bf16, 128>(A, s);
+hipError_t qxa_launch(const QxaArgs &A, hipStream_t s) {
+    if (A.a.type == QXG_TYPE_F32) return A.a.dim == 64 ? launch<float, 64>(A, s) : launch<float, 128>(A, s);
+    if (A.a.type == QXG_TYPE_F16) return A.a.dim == 64 ? launch<_Float16, 64>(A, s) : launch<_Float16, 128>(A, s);
+    return A.a.dim == 64 ? launch<__bf16, 64>(A, s) : launch<__bf16, 128>(A, s);
 }

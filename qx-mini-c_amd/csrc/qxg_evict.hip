@@ -420,13 +420,12 @@ extern "C" __global__ __launch_bounds__(256) void qxe_compact(QxeCompact C) {
     }
 }
 
-void qxe_launch_select(const qxg_kv_select_args &a, hipStream_t s) {
-    if (a.positions <= 1024) hipLaunchKernelGGL(qxe_select<1>, dim3(a.groups), dim3(1024), 0, s, a);
-    else if (a.positions <= 4096) hipLaunchKernelGGL(qxe_select<4>, dim3(a.groups), dim3(1024), 0, s, a);
-    else hipLaunchKernelGGL(qxe_select_long, dim3(a.groups), dim3(1024), 0, s, a);
+hipError_t qxe_launch_select(const qxg_kv_select_args &a, hipStream_t s) {
+    auto *kernel = a.positions <= 1024 ? qxe_select<1> : a.positions <= 4096 ? qxe_select<4> : qxe_select_long;
+    return qxg_launch(kernel, dim3(a.groups), dim3(1024), 0, s, a);
 }
-void qxe_launch_compact(const QxeCompact &C, hipStream_t s) {
+hipError_t qxe_launch_compact(const QxeCompact &C, hipStream_t s) {
     const uint32_t words = 1 + C.a.groups * C.tiles;
-    hipLaunchKernelGGL(qxe_clear, dim3(std::min<uint32_t>(64, (words + 255) / 256)), dim3(256), 0, s, C.state, words);
-    hipLaunchKernelGGL(qxe_compact, dim3(C.a.groups * C.tiles), dim3(256), 0, s, C);
+    const hipError_t e = qxg_launch(qxe_clear, dim3(std::min<uint32_t>(64, (words + 255) / 256)), dim3(256), 0, s, C.state, words);
+    return e != hipSuccess ? e : qxg_launch(qxe_compact, dim3(C.a.groups * C.tiles), dim3(256), 0, s, C);
 }

@@ -4,6 +4,14 @@
 #include "qxg.h"
 #include "qxg_internal.h"
 
+// A launch that returns its error: the last error of the runtime, which may be one that the caller has yet to ask for, is
+// not asked here.
+template <typename... P>
+hipError_t qxg_launch(void (*kernel)(P...), dim3 grid, dim3 block, uint32_t lds, hipStream_t s, P... args) {
+    void *at[] = {(void *)&args...};
+    return hipLaunchKernel((const void *)kernel, grid, block, at, lds, s);
+}
+
 // Tree attention.  A column is a (node, q head of the kv head) pair, node * group + head; a tile is
 // 32 columns.  With several splits of the positions, a split's unnormalised context goes to part
 // and its (reference, denominator) in base 2 to md, at [split of the batch][node][head].
@@ -21,7 +29,7 @@ struct QxaArgs {
     uint4 *pack;       // with an account otherwise: q as matrix operands, [batch][kv head][tile][k-step][half][lane]
     float *pack_sf;    // [batch][kv head][tile][column] what turns dot * kscale into base-2 scores
 };
-void qxa_launch(const QxaArgs &A, hipStream_t s);
+hipError_t qxa_launch(const QxaArgs &A, hipStream_t s);
 
 // Eviction.  A tile of the compaction is `rows` rows, QXE_UNITS 16-byte units of K (and of V) at most.
 constexpr uint32_t QXE_UNITS = 2048;
@@ -31,8 +39,8 @@ struct QxeCompact {
     uint32_t rows, tiles;      // of a tile; of a group
     uint32_t *state;           // 1 + groups * tiles words
 };
-void qxe_launch_select(const qxg_kv_select_args &a, hipStream_t s);
-void qxe_launch_compact(const QxeCompact &C, hipStream_t s);
+hipError_t qxe_launch_select(const qxg_kv_select_args &a, hipStream_t s);
+hipError_t qxe_launch_compact(const QxeCompact &C, hipStream_t s);
 
 // Logits.  Each of the 4 waves of a slice of a row leaves up to top_n keys, its largest among them, the
 // others 0, and (maximum, sum of exponentials) to the join.
@@ -44,7 +52,7 @@ struct QxsArgs {
     float2 *ms;        // [rows][slices * 4]
 };
 constexpr uint32_t QXS_SLICE = 4096, QXS_BIASES = 1024, QXS_HISTORY = (1u << 20) - 1;
-void qxs_launch(const QxsArgs &A, hipStream_t s);
+hipError_t qxs_launch(const QxsArgs &A, hipStream_t s);
 
 // the context's device (qxg_api.hip)
 __attribute__((visibility("hidden"))) int qxg_ctx_device(const qxg_ctx *c);

@@ -38,23 +38,31 @@ template <size_t N, typename F>
 bool on_device(const qxg_ctx *c, const Arg (&args)[N], hipStream_t s, int wait, const Err &fail, F go) {
     if (!c) return fail("invalid context");
     const int dev = qxg_ctx_device(c);
+    // An error of this call is reported by it and cleared, unless the caller had one pending before.
+    const bool pending = hipPeekAtLastError() != hipSuccess;
+    const auto clear = [&] { if (!pending) (void)hipGetLastError(); };
     for (const Arg &a : args) {
         if (!a.p) continue;
         hipPointerAttribute_t at{};
         if (hipPointerGetAttributes(&at, a.p) != hipSuccess) {
-            (void)hipGetLastError();
+            clear();
             return fail("%s is not device memory of this library's HIP runtime", a.name);
         }
         if (at.type != hipMemoryTypeDevice || at.device != dev) return fail("%s is not memory of the context's device %d", a.name, dev);
     }
     int before = dev;
-    if (hipGetDevice(&before) != hipSuccess || (before != dev && hipSetDevice(dev) != hipSuccess)) return fail("hipSetDevice failed");
-    (void)hipGetLastError();
-    go();
-    hipError_t e = hipGetLastError();
+    hipError_t e = hipGetDevice(&before);
+    if (e == hipSuccess && before != dev) e = hipSetDevice(dev);
+    if (e != hipSuccess) {
+        clear();
+        return fail("hipSetDevice failed");
+    }
+    e = go();
     if (e == hipSuccess && wait) e = hipStreamSynchronize(s);
     if (before != dev) (void)hipSetDevice(before);
-    return e == hipSuccess || fail("%s", hipGetErrorString(e));
+    if (e == hipSuccess) return true;
+    clear();
+    return fail("%s", hipGetErrorString(e));
 }
 template <size_t N> bool pointers_ok(const Arg (&args)[N], const Err &fail) {
     for (const Arg &a : args) {
@@ -246,7 +254,7 @@ int qxg_tree_attention(qxg_ctx *c, const qxg_tree_attention_args *p, void *strea
                         {p->out, "out", true, 16}, {p->lse, "lse", false, 4}, {p->account, "account", false, 4},
                         {p->workspace, "workspace", false, 16}};
     if (!pointers_ok(args, fail) || !workspace_ok(p->workspace, p->workspace_bytes, need, fail)) return 0;
-    return on_device(c, args, (hipStream_t)stream, wait, fail, [&] { qxa_launch(A, (hipStream_t)stream); });
+    return on_device(c, args, (hipStream_t)stream, wait, fail, [&] { return qxa_launch(A, (hipStream_t)stream); });
 }
 uint64_t qxg_tree_attention_workspace(const qxg_tree_attention_args *p) {
     QxaArgs A{};
@@ -259,7 +267,7 @@ int qxg_kv_select(qxg_ctx *c, const qxg_kv_select_args *p, void *stream, int wai
     if (!select_ok(p, fail)) return 0;
     const Arg args[] = {{p->account, "account", true, 4}, {p->lens, "lens", true, 4}, {p->keep, "keep", true, 4}, {p->kept, "kept", true, 4}};
     if (!pointers_ok(args, fail)) return 0;
-    return on_device(c, args, (hipStream_t)stream, wait, fail, [&] { qxe_launch_select(*p, (hipStream_t)stream); });
+    return on_device(c, args, (hipStream_t)stream, wait, fail, [&] { return qxe_launch_select(*p, (hipStream_t)stream); });
 }
 
 int qxg_kv_compact(qxg_ctx *c, const qxg_kv_compact_args *p, void *stream, int wait, char *err, uint64_t err_len) {
@@ -271,7 +279,7 @@ int qxg_kv_compact(qxg_ctx *c, const qxg_kv_compact_args *p, void *stream, int w
                         {p->keep, "keep", true, 4}, {p->kept, "kept", true, 4}, {p->account, "account", false, 4},
                         {p->account_out, "account_out", false, 4}, {p->workspace, "workspace", false, 16}};
     if (!pointers_ok(args, fail) || !workspace_ok(p->workspace, p->workspace_bytes, need, fail)) return 0;
-    return on_device(c, args, (hipStream_t)stream, wait, fail, [&] { qxe_launch_compact(C, (hipStream_t)stream); });
+    return on_device(c, args, (hipStream_t)stream, wait, fail, [&] { return qxe_launch_compact(C, (hipStream_t)stream); });
 }
 uint64_t qxg_kv_compact_workspace(const qxg_kv_compact_args *p) {
     QxeCompact C{};
@@ -292,7 +300,7 @@ int qxg_adjust_logits(qxg_ctx *c, const qxg_adjust_logits_args *p, void *stream,
                         {p->top_ids, "top_ids", false, 4}, {p->top_logits, "top_logits", false, 4}, {p->lse, "lse", false, 4},
                         {p->workspace, "workspace", false, 16}};
     if (!pointers_ok(args, fail) || !workspace_ok(p->workspace, p->workspace_bytes, need, fail)) return 0;
-    return on_device(c, args, (hipStream_t)stream, wait, fail, [&] { qxs_launch(A, (hipStream_t)stream); });
+    return on_device(c, args, (hipStream_t)stream, wait, fail, [&] { return qxs_launch(A, (hipStream_t)stream); });
 }
 uint64_t qxg_adjust_logits_workspace(const qxg_adjust_logits_args *p) {
     QxsArgs A{};

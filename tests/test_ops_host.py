@@ -1,0 +1,118 @@
+"""The host side of the operators on device memory on the CPU: ops_host.cpp compiled with a runtime of its own that writes
+down what is asked of it."""
+import ctypes
+import os
+import subprocess
+
+import pytest
+
+import qxg
+from test_ops_refusals import Fake, big, logits, tree
+
+INVALID_VALUE, CONFIGURATION, UNKNOWN = 1, 9, 999      # hipErrorInvalidValue, ...InvalidConfiguration, ...Unknown
+
+
+class Seen(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in ("last", "fail", "unknown", "device", "launches", "waits", "waits_that_fail")] + [
+        (n, ctypes.c_uint32) for n in ("wide", "splits", "tiles", "wgs", "kept", "packed")]
+
+
+@pytest.fixture(scope="module")
+def lib(root, tmp_path_factory):
+    out = tmp_path_factory.mktemp("ops_host") / "ops_host.so"
+    subprocess.run(["g++", "-std=c++17", "-D__HIP_PLATFORM_AMD__", "-shared", "-fPIC", "-Wl,-Bsymbolic", "-I/opt/rocm/include",
+                    "-I" + os.path.join(root, "include"), "-I" + os.path.join(root, "qx-mini-c_amd", "csrc"),
+                    os.path.join(root, "tests", "ops_host.cpp"), "-o", str(out)], check=True, capture_output=True)
+    lib = ctypes.CDLL(str(out))
+    for name in ("qxg_tree_attention", "qxg_kv_select", "qxg_kv_compact", "qxg_adjust_logits"):
+        getattr(lib, name).argtypes = getattr(qxg._g, name).argtypes
+    return lib
+
+
+@pytest.fixture()
+def host(lib, monkeypatch):
+    """(a context whose calls go to the library, what its runtime has seen)"""
+    monkeypatch.setattr(qxg, "_g", lib)
+    seen = Seen.in_dll(lib, "seen")
+    ctypes.memset(ctypes.addressof(seen), 0, ctypes.sizeof(seen))
+    c = qxg.Context.__new__(qxg.Context)
+    c._c, c._err = ctypes.c_void_p(1), ctypes.create_string_buffer(1024)
+    yield c, seen
+    c._c = None      # (nothing to close)
+
+
+def calls(c):
+    yield c.tree_attention, tree()
+    yield c.kv_select, dict(account=Fake((3, 40)), lens=Fake((3,), "int32"), keep=Fake((3, 10), "int32"), kept=Fake((3,), "int32"))
+    yield c.kv_compact, dict(k=Fake((3, 40, 64), "int8"), v=Fake((3, 40, 64), "int8"), kscale=Fake((3, 40)), vscale=Fake((3, 40)),
+                             keep=Fake((3, 10), "int32"), kept=Fake((3,), "int32"), workspace=big())
+    yield c.adjust_logits, logits()
+
+
+def test_calls(host):
+    c, seen = host
+    for n, (call, args) in enumerate(calls(c), 1):
+        call(**args, wait=False)
+        assert (seen.launches, seen.waits, seen.last) == (n, 0, 0)
+    for call, args in calls(c):
+        call(**args)
+    assert seen.waits == 4
+
+
+def test_an_error_that_the_caller_has_yet_to_ask_for_stays(host):
+    c, seen = host
+    seen.last = UNKNOWN
+    for call, args in calls(c):
+        call(**args)
+        assert seen.last == UNKNOWN
+
+
+def test_a_failed_launch_is_reported_once(host):
+    """By the call, not by the caller's next question; but an error from before it leaves one."""
+    c, seen = host
+    seen.fail = CONFIGURATION
+    for call, args in calls(c):
+        with pytest.raises(qxg.QxgError, match="configuration"):
+            call(**args, wait=False)
+        assert seen.last == 0 and seen.waits == 0
+    seen.last = UNKNOWN
+    for call, args in calls(c):
+        with pytest.raises(qxg.QxgError, match="configuration"):
+            call(**args, wait=False)
+        assert seen.last != 0
+
+
+def test_a_wait_that_fails_is_reported(host):
+    c, seen = host
+    seen.waits_that_fail = UNKNOWN
+    for call, args in calls(c):
+        with pytest.raises(qxg.QxgError, match="unknown"):
+            call(**args)
+        assert seen.last == 0
+
+
+def test_memory_of_another_runtime_is_refused(host):
+    c, seen = host
+    seen.unknown = 1
+    for call, args in calls(c):
+        with pytest.raises(qxg.QxgError, match="is not device memory of this library's HIP runtime"):
+            call(**args)
+        assert seen.last == 0 and seen.launches == 0
+    seen.last = UNKNOWN
+    for call, args in calls(c):
+        with pytest.raises(qxg.QxgError, match="is not device memory"):
+            call(**args)
+        assert seen.last != 0
+
+
+def test_the_callers_device_is_current_again(host):
+    c, seen = host
+    seen.device = 3
+    for call, args in calls(c):
+        call(**args)
+        assert seen.device == 3
+    seen.fail = CONFIGURATION
+    for call, args in calls(c):
+        with pytest.raises(qxg.QxgError):
+            call(**args)
+        assert seen.device == 3
