@@ -58,7 +58,10 @@ bool on_device(const qxg_ctx *c, const Arg (&args)[N], hipStream_t s, int wait, 
         return fail("hipSetDevice failed");
     }
     e = go();
-    if (e == hipSuccess && wait) e = hipStreamSynchronize(s);
+    if (wait) {   // also for what a launch that failed has left before it
+        const hipError_t w = hipStreamSynchronize(s);
+        if (e == hipSuccess) e = w;
+    }
     if (before != dev) (void)hipSetDevice(before);
     if (e == hipSuccess) return true;
     clear();

@@ -82,6 +82,15 @@ def test_a_failed_launch_is_reported_once(host):
         assert seen.last != 0
 
 
+def test_a_failed_launch_waits_for_the_kernels_before_it(host):
+    c, seen = host
+    seen.fail = CONFIGURATION
+    for n, (call, args) in enumerate(calls(c), 1):
+        with pytest.raises(qxg.QxgError, match="configuration"):
+            call(**args)
+        assert seen.waits == n
+
+
 def test_a_wait_that_fails_is_reported(host):
     c, seen = host
     seen.waits_that_fail = UNKNOWN
