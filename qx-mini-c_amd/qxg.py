@@ -6,6 +6,7 @@ import ctypes
 import functools
 import os
 import struct
+import threading
 
 import numpy as np
 
@@ -177,6 +178,17 @@ _ADJUST = struct.Struct("=15Q4Q7I4x")
 _KINDS = {}   # dtype -> "f32", ...
 _NAMES = {"float32": "f32", "float16": "f16", "bfloat16": "bf16", "int32": "i32", "uint32": "i32", "int8": "i8", "uint8": "u8"}
 _VALUE_TYPES = {"f32": 0, "f16": 1, "bf16": 30}   # GGML's numbers
+_thread = threading.local()
+
+
+def _queue(call, ctx, args, stream, wait):
+    """One of the operators' calls, its message in a buffer of the thread's (several threads may share a context)."""
+    try:
+        err = _thread.err
+    except AttributeError:
+        err = _thread.err = ctypes.create_string_buffer(1024)
+    if not call(ctx, args, stream, wait, err, 1024):
+        raise QxgError(err.value.decode())
 
 
 def _kind(dtype):
@@ -613,14 +625,14 @@ class Context:
         args = _TREE.pack(_ptr(q), _ptr(k), _ptr(v), _ptr(kscale), _ptr(vscale), _ptr(lens), _ptr(counts), _ptr(mask), _ptr(out),
                           _ptr(lse), _ptr(account), _ptr(workspace), *fixed, fixed[-1] if max_len is None else max_len,
                           fixed[-2] ** -0.5 if scale is None else scale, decay)
-        self._check(_g.qxg_tree_attention(self._c, args, stream, wait, self._err, 1024))
+        _queue(_g.qxg_tree_attention, self._c, args, stream, wait)
 
     def kv_select(self, account, lens, keep, kept, sinks=0, recent=0, max_len=None, stream=0, wait=True):
         """qxg_kv_select: account [groups, positions] f32, lens [groups] int32; writes keep [groups, budget]
         and kept [groups] int32."""
         fixed = _select_layout(_layout(account), _layout(lens), _layout(keep), _layout(kept))
         args = _SELECT.pack(_ptr(account), _ptr(lens), _ptr(keep), _ptr(kept), *fixed, sinks, recent, fixed[3] if max_len is None else max_len)
-        self._check(_g.qxg_kv_select(self._c, args, stream, wait, self._err, 1024))
+        _queue(_g.qxg_kv_select, self._c, args, stream, wait)
 
     def kv_compact_workspace(self, k_shape, keep_shape):
         """Bytes of workspace that kv_compact with these shapes needs."""
@@ -633,7 +645,7 @@ class Context:
                                      _layout(account_out), _layout(workspace))
         args = _COMPACT.pack(_ptr(k), _ptr(v), _ptr(kscale), _ptr(vscale), _ptr(keep), _ptr(kept), _ptr(account), _ptr(account_out),
                              _ptr(workspace), *fixed, first, row)
-        self._check(_g.qxg_kv_compact(self._c, args, stream, wait, self._err, 1024))
+        _queue(_g.qxg_kv_compact, self._c, args, stream, wait)
 
     def adjust_logits_workspace(self, shape, top_n=0):
         """Bytes of workspace that adjust_logits on [rows, vocab] logits needs."""
@@ -649,7 +661,7 @@ class Context:
         arrays = (logits, out, history, history_lens, prompt_lens, penalties, temperature, bias_ids, bias_values, mask, mask_rows, top_ids,
                   top_logits, lse, workspace)
         args = _ADJUST.pack(*map(_ptr, arrays), *_adjust_layout(*map(_layout, arrays)))
-        self._check(_g.qxg_adjust_logits(self._c, args, stream, wait, self._err, 1024))
+        _queue(_g.qxg_adjust_logits, self._c, args, stream, wait)
 
     def time_kernel(self, which, layer=0, iters=20):
         ms = c_float()

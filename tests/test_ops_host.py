@@ -3,6 +3,7 @@ down what is asked of it."""
 import ctypes
 import os
 import subprocess
+import threading
 
 import pytest
 
@@ -125,3 +126,31 @@ def test_the_callers_device_is_current_again(host):
         with pytest.raises(qxg.QxgError):
             call(**args)
         assert seen.device == 3
+
+
+def test_threads_have_their_own_messages(monkeypatch):
+    """A call that fails while another thread's call on the same context fails, too, has its own message."""
+    c = qxg.Context.__new__(qxg.Context)
+    c._c, c._err = None, ctypes.create_string_buffer(1024)
+    args = dict(account=Fake((3, 40)), lens=Fake((3,), "int32"), keep=Fake((3, 10), "int32"), kept=Fake((3,), "int32"))
+    seen = []
+
+    def one():
+        with pytest.raises(qxg.QxgError) as e:
+            c.kv_select(**args)
+        seen.append(str(e.value))
+
+    class Calls:
+        left = ["the first's", "the second's"]
+
+        def qxg_kv_select(self, ctx, packed, stream, wait, err, n):
+            err.value = self.left.pop(0).encode()
+            if self.left:
+                other = threading.Thread(target=one)
+                other.start()
+                other.join()
+            return 0
+
+    monkeypatch.setattr(qxg, "_g", Calls())
+    one()
+    assert seen == ["the second's", "the first's"]
