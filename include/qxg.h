@@ -385,7 +385,7 @@ typedef struct qxg_kv_select_args {
     uint32_t *keep;           /* [groups][budget] */
     uint32_t *kept;           /* [groups]; may be lens itself, which then holds the new lengths */
     uint64_t account_group, keep_group;   /* strides in elements */
-    uint32_t groups, positions, budget, sinks, recent;   /* sinks + recent <= budget */
+    uint32_t groups, positions, budget, sinks, recent;   /* groups < 2^22, sinks + recent <= budget */
     uint32_t max_len;         /* as in qxg_tree_attention */
 } qxg_kv_select_args;
 int qxg_kv_select(qxg_ctx *ctx, const qxg_kv_select_args *args, void *stream, int wait, char *err, uint64_t err_len);
@@ -409,7 +409,7 @@ typedef struct qxg_kv_compact_args {
     uint64_t scale_group;             /* in floats */
     uint64_t keep_group, kept_group;  /* in elements; 0: one list for all groups */
     uint64_t account_group, account_out_group;
-    uint32_t groups, positions, slots, first, row_bytes;   /* row_bytes a multiple of 16, at most 4096 */
+    uint32_t groups, positions, slots, first, row_bytes;   /* groups <= 65535; row_bytes a multiple of 16, at most 4096 */
 } qxg_kv_compact_args;
 int qxg_kv_compact(qxg_ctx *ctx, const qxg_kv_compact_args *args, void *stream, int wait, char *err, uint64_t err_len);
 uint64_t qxg_kv_compact_workspace(const qxg_kv_compact_args *args);

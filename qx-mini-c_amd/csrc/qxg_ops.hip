@@ -177,7 +177,7 @@ bool tree_plan(const qxg_tree_attention_args *p, QxaArgs &A, uint64_t &bytes, co
 // ---- eviction
 bool select_ok(const qxg_kv_select_args *p, const Err &fail) {
     if (!p) return fail("invalid argument");
-    if (!p->groups) return fail("groups must be positive");
+    if (!p->groups || p->groups >= 1u << 22) return fail("groups must be between 1 and 2^22 - 1");   // (a launch has less than 2^32 threads)
     if (!p->positions || p->positions > 0x7fffffffu || p->max_len > 0x7fffffffu) return fail("positions and max_len must be below 2^31");
     if (!p->budget) return fail("budget must be positive");
     if ((uint64_t)p->sinks + p->recent > p->budget) return fail("sinks + recent exceed the budget");
@@ -204,7 +204,7 @@ bool compact_plan(const qxg_kv_compact_args *p, QxeCompact &C, uint64_t &bytes, 
     C.inverse = ((1u << 20) + C.units - 1) / C.units;
     C.rows = QXE_UNITS / C.units;
     C.tiles = (std::min(p->slots, p->positions - p->first) + C.rows - 1) / C.rows;
-    if ((uint64_t)p->groups * C.tiles >= 1u << 31) return fail("too many rows for one call");
+    if ((uint64_t)p->groups * C.tiles >= 1u << 24) return fail("too many rows for one call");   // (a launch has less than 2^32 threads)
     C.state = (uint32_t *)p->workspace;
     bytes = up16(4 + 4ull * p->groups * C.tiles);
     return true;

@@ -48,3 +48,22 @@ def test_kept_that_overlaps_lens(ctx, offset, message):  # noqa: F811
     a = dict(account=Fake((3, 40)), lens=Fake((3,), "int32"), keep=Fake((3, 10), "int32", ptr=1 << 21), kept=Fake((3,), "int32", ptr=(1 << 20) + offset))
     with pytest.raises(qxg.QxgError, match=message):
         ctx.kv_select(**a)
+
+
+@pytest.mark.parametrize("groups,message", [((1 << 22) - 1, "invalid context"), (1 << 22, "groups must be between"), (0xffffffff, "groups must be between")])
+def test_groups_beyond_a_launch(ctx, groups, message):  # noqa: F811
+    a = dict(account=Fake((groups, 40), strides=(0, 1)), lens=Fake((groups,), "int32"), keep=Fake((groups, 10), "int32", ptr=1 << 40),
+             kept=Fake((groups,), "int32", ptr=1 << 39))
+    with pytest.raises(qxg.QxgError, match=message):
+        ctx.kv_select(**a)
+
+
+@pytest.mark.parametrize("positions,message", [(8 * 256, "invalid context"), (8 * 257, "too many rows for one call"), (8 * 1024, "too many rows")])
+def test_rows_beyond_a_launch(ctx, positions, message):  # noqa: F811
+    """Tiles of 8 rows of 4096 bytes, 65535 groups."""
+    groups, row = 65535, 4096
+    k = Fake((groups, positions, row), "int8")
+    a = dict(k=k, v=k, kscale=Fake((groups, positions)), vscale=Fake((groups, positions)), keep=Fake((groups, positions), "int32", strides=(0, 1)),
+             kept=Fake((groups,), "int32", strides=(0,)), workspace=big())
+    with pytest.raises(qxg.QxgError, match=message):
+        ctx.kv_compact(**a)
