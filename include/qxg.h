@@ -344,7 +344,9 @@ int qxg_q8k_quantize(qxg_ctx *ctx, const float *x, uint32_t n, void *blocks_out,
  * (scales that are infinite or NaN among them) does not reach it.  Rows of nodes at and behind
  * count are left as they were.  With account, each position's weight is added to it:
  *     account[p] = decay * account[p] + sum over nodes and heads of softmax(s)[p]
- * for p < lens[b] + count, in a fixed order (equal calls give equal bits).
+ * for p < lens[b] + count, in a fixed order (equal calls give equal bits).  The nodes' positions are among them: their
+ * entries are the caller's to clear before a token takes the place of another, and to move with a path's rows that it keeps
+ * (qxg_kv_compact's account_out).
  * An F32 q is multiplied as two halves of 11 bits each (F16 and BF16: as it is), the weights too (errors as of
  * f32 products).  nodes = 1 without a mask is ordinary decoding.  Rows of out that overlap, and accounts that do, are refused. */
 typedef struct qxg_tree_attention_args {
@@ -395,7 +397,9 @@ int qxg_kv_select(qxg_ctx *ctx, const qxg_kv_select_args *args, void *stream, in
  * qxg_kv_select writes it, or as a program lists the accepted nodes of a tree behind its cached
  * positions (first = lens[b]); of a list that does not, the moved rows are undefined (never
  * anything else).  Rows at and behind first + kept[g] are left as they were.  account_out[first +
- * i] = account[keep[i]] in another array.  Entries outside the cache are skipped. */
+ * i] = account[keep[i]] in another array, whose other entries are left as they were.  Entries outside the cache are skipped.
+ * first is the same for all groups: sequences of unlike lengths take a call each.  (Calls that share a workspace at the
+ * same time, which is not allowed, end all the same; their moved rows are undefined.) */
 typedef struct qxg_kv_compact_args {
     int8_t *k, *v;            /* [groups][positions][row_bytes], 16-byte aligned */
     float *kscale, *vscale;   /* [groups][positions] */
