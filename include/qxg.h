@@ -388,7 +388,7 @@ typedef struct qxg_kv_select_args {
     uint32_t *kept;           /* [groups]; may be lens itself, which then holds the new lengths */
     uint64_t account_group, keep_group;   /* strides in elements */
     uint32_t groups, positions, budget, sinks, recent;   /* groups < 2^22, sinks + recent <= budget */
-    uint32_t max_len;         /* as in qxg_tree_attention */
+    uint32_t max_len;         /* below 2^31; not used: each group's own length, in device memory, decides */
 } qxg_kv_select_args;
 int qxg_kv_select(qxg_ctx *ctx, const qxg_kv_select_args *args, void *stream, int wait, char *err, uint64_t err_len);
 

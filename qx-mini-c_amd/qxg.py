@@ -629,7 +629,7 @@ class Context:
 
     def kv_select(self, account, lens, keep, kept, sinks=0, recent=0, max_len=None, stream=0, wait=True):
         """qxg_kv_select: account [groups, positions] f32, lens [groups] int32; writes keep [groups, budget]
-        and kept [groups] int32."""
+        and kept [groups] int32 (which may be lens).  max_len is not used."""
         fixed = _select_layout(_layout(account), _layout(lens), _layout(keep), _layout(kept))
         args = _SELECT.pack(_ptr(account), _ptr(lens), _ptr(keep), _ptr(kept), *fixed, sinks, recent, fixed[3] if max_len is None else max_len)
         _queue(_g.qxg_kv_select, self._c, args, stream, wait)
