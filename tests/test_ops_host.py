@@ -8,6 +8,7 @@ import threading
 import pytest
 
 import qxg
+from test_gpu_tree_attention_long import PLANS
 from test_ops_refusals import Fake, big, logits, tree
 
 INVALID_VALUE, CONFIGURATION, UNKNOWN = 1, 9, 999      # hipErrorInvalidValue, ...InvalidConfiguration, ...Unknown
@@ -154,3 +155,31 @@ def test_threads_have_their_own_messages(monkeypatch):
     monkeypatch.setattr(qxg, "_g", Calls())
     one()
     assert seen == ["the second's", "the first's"]
+
+
+def splits_of(seen, case):
+    """(chunks, splits) of every sequence, as the kernels share them out."""
+    group = case["heads"] // case["kv_heads"]
+    counts = case.get("counts") or (case["nodes"],) * len(case["lens"])
+    chunks = [max(1, -(-(n + c) // 32)) for n, c in zip(case["lens"], counts)]
+    if seen.splits == 1 or len(chunks) > 64:
+        return [(n, seen.splits) for n in chunks]
+    if len(chunks) == 1:
+        return [(chunks[0], min(chunks[0], seen.splits))]
+    busy = sum(n * -(-c * group // (128 if seen.wide else 32)) for n, c in zip(chunks, counts))
+    return [(n, min(n, max(1, int(n * seen.splits * min(seen.wgs / busy, 2 / sum(chunks)))))) for n in chunks]
+
+
+@pytest.mark.parametrize("name", sorted(PLANS))
+def test_plans(host, name):
+    """The cases of test_gpu_tree_attention_long.py reach the kernels and loops that they are meant for."""
+    c, seen = host
+    case, wide, splits, least = PLANS[name]
+    batch, nodes, dim, longest = case.get("batch", 1), case["nodes"], case.get("dim", 128), max(case["lens"])
+    positions = longest + nodes + 3
+    cache, scales, q = (batch, positions, case["kv_heads"], dim), Fake((batch, positions)), (batch, nodes, case["heads"], dim)
+    c.tree_attention(Fake(q), Fake(cache, "int8"), Fake(cache, "int8"), scales, scales, Fake((batch,), "int32"), Fake(q, ptr=1 << 40), max_len=longest,
+                     workspace=big())
+    assert bool(seen.wide) == wide
+    assert (seen.splits == 1) == (splits == 1)
+    assert max(n // s for n, s in splits_of(seen, case)) >= least
