@@ -348,7 +348,7 @@ int qxg_q8k_quantize(qxg_ctx *ctx, const float *x, uint32_t n, void *blocks_out,
  * entries are the caller's to clear before a token takes the place of another, and to move with a path's rows that it keeps
  * (qxg_kv_compact's account_out).
  * An F32 q is multiplied as two halves of 11 bits each (F16 and BF16: as it is), the weights too (errors as of
- * f32 products).  nodes = 1 without a mask is ordinary decoding.  Rows of out that overlap, and accounts that do, are refused. */
+ * f32 products, where vscale is 2^-99 or more).  nodes = 1 without a mask is ordinary decoding.  Rows of out that overlap, and accounts that do, are refused. */
 typedef struct qxg_tree_attention_args {
     const void *q;            /* [batch][nodes][heads][dim] of `type`, 16-byte aligned */
     const int8_t *k, *v;      /* [batch][positions][kv_heads][dim], 16-byte aligned */

@@ -155,14 +155,17 @@ template <int D> DEV uint4 k_step(const KRow<D> &x, int s) {
 }  // namespace
 
 namespace {
-// A column's softmax state.  Both halves of a wave hold their columns' m, M and limit; den is each lane's own
-// sum.  m (the maximum, rounded, as of the last time that it grew by 8) and M are whole numbers, so that
-// moving M and scaling what has been summed by the power of two that belongs to it agree exactly.
+// A column's softmax state.  Both halves of a wave hold their columns' m, c, M, most and limit; den is each lane's own
+// sum.  m (the maximum, rounded, as of the last time that it grew by 8) and c (M's shift) are whole numbers, M = m - c, so
+// that moving M and scaling what has been summed by the power of two that belongs to it agree exactly.  Where f32 has no room
+// for that (far: a column's m from 2^22 on), e is 2^((s - m) + c) instead of 2^(s - M), with s rounded as m is: with M alone, equal
+// scores weighed differently from 2^24 on.
 template <int D> struct State {
     // most: the largest |e vs| so far.  limit: what it may reach before M has to move; 0 where m has grown, so that the next
     // weights place it anew (else values far smaller than those before them, which outweigh them, lost bits:
     // V scales smaller by 10^6, scores higher by 2^80: 8e-5 off, by 10^9: 8e-2).
-    float m = -INFINITY, M = -INFINITY, den = 0.0f, most = 0.0f, limit = 0.0f;
+    float m = -INFINITY, M = -INFINITY, den = 0.0f, most = 0.0f, limit = 0.0f, c = 0.0f;
+    bool far = false;   // of the wave
     f16x acc[D / 32];
     DEV State() {
 #pragma unroll
@@ -174,6 +177,11 @@ template <int D> struct State {
         for (int d = 0; d < D / 32; ++d)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[d][r] *= f;
+    }
+    DEV void close() {   // before it is joined with others: M holds the shift or there is none
+        if (!far) return;
+        rescale(exp2_fast(-c));
+        M = m;
     }
 };
 DEV float max_of_halves(float v) {   // of lanes l and l ^ 32
@@ -227,10 +235,11 @@ DEV void reference(State<D> &S, float sf, bool edge, uint32_t bits, int h, float
         S.rescale(f);
         S.most *= f;
         if (grow) {
-            S.M = S.m == -INFINITY ? mn : mn - (S.m - S.M);
+            S.M = mn - S.c;
             S.m = mn;
             S.limit = 0.0f;
         }
+        S.far = S.far || __ballot(grow && fabsf(mn) >= 4194304.0f) != 0;
     }
 }
 // The weights as the second product's operands phi and plo, M moved where they leave fp16's range
@@ -250,16 +259,16 @@ DEV void operands(State<D> &S, float den, float sf, bool edge, uint32_t bits, in
     const float pmx = max_of_halves(max16(a));
     S.most = fmaxf(S.most, pmx);
     if (__ballot(pmx > S.limit) != 0) {   // the first weights after m has grown, or one beyond fp16
-        const float M = S.M == -INFINITY ? 0.0f : S.M;
         const bool move = pmx > S.limit && pmx < INFINITY;
         // the largest so far to [2^6, 2^7), but e itself (up to 2^8 times the shift) stays far inside f32; a
         // larger one, where that has kept it from there, moves M again
         int k = (int)(__float_as_uint(pow2_scale(S.most, 7)) >> 23) - 127;
-        k = move ? max(min(k, 96 - (int)(S.m - M)), -126) : 0;
+        k = move ? max(min(k, 96 - (int)S.c), -126) : 0;
         const float f = __uint_as_float((uint32_t)(127 + k) << 23);
         S.most *= f;
         if (move) {
-            S.M = M - (float)k;
+            S.c += (float)k;
+            S.M = S.m - S.c;
             S.limit = S.most < 64.0f ? S.most : 32768.0f;
         }
         S.rescale(f);
@@ -286,12 +295,20 @@ DEV void weigh(State<D> &S, const f16x &dot, float sf, const float *ks, const fl
         for (int r = 0; r < 16; ++r) keep[r / 4][r % 4] = s[r] == -INFINITY ? -INFINITY : s[r] * sf;
     }
     const float M = S.M == -INFINITY ? 0.0f : S.M;
+    if (!S.far) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) p[r] = fmaf(s[r], sf, -M);
+    } else {
+        const float m = S.m == -INFINITY ? 0.0f : S.m;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) p[r] = (s[r] * sf - m) + S.c;
+    }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const f4x v4 = *reinterpret_cast<const f4x *>(vs + 8 * j + 4 * h);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const float e = exp2_fast(fmaf(s[4 * j + r], sf, -M));
+            const float e = exp2_fast(p[4 * j + r]);
             den[r] += e;
             p[4 * j + r] = e * v4[r];
         }
@@ -477,6 +494,7 @@ __global__ __launch_bounds__(256, 2) void qxa_tree(QxaArgs A) {
         }
     }
     if (KEEP && c_lo + wave < c_hi) keep_scores(c_lo + wave + (c_hi - 1 - c_lo - wave) / 4 * 4);   // the last chunk's
+    S.close();
     // merge the 4 waves: 2 + 3 into 0 + 1, then 1 into 0
     float den = S.den + __shfl_xor(S.den, 32);
     __syncthreads();
@@ -682,6 +700,7 @@ __global__ __launch_bounds__(256, 2) void qxa_wide(QxaArgs A) {
             for (int d = 0; d < DT; ++d) S.acc[d] = mfma(vf[d], phi[s], S.acc[d]);
         }
     }
+    S.close();
     const float den = S.den + __shfl_xor(S.den, 32);
     __syncthreads();
     if (!busy) return;

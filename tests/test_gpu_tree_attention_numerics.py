@@ -161,3 +161,21 @@ def test_scales_at_the_ends(ctx, hip, kind, nodes, max_len, qscale, scale):  # n
     ws = hip.workspace(ctx.tree_attention_workspace(case.q.shape, case.k.shape, max_len=max_len))
     ctx.tree_attention(q, k, v, ks, vs, hip.put(case.lens), out, mask=hip.put(bits(case.sees)), lse=lse, max_len=max_len, scale=scale, workspace=ws)
     check(case, out, lse)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("ks", [20.0, 35.0, 70.0, 140.0, -140.0, 300.0, -500.0, 1100.0, 30000.0])
+@pytest.mark.parametrize("wide", [False, True])
+def test_equal_scores_beyond_whole_numbers(ctx, hip, kind, ks, wide):  # noqa: F811
+    """Scores whose size f32 holds in steps of 1 and more: equal ones weigh the same, wherever they stand and whatever
+    the V scales around them.  A third of the positions have the largest score, the others one lower by an eighth."""
+    case = taken_over(kind, 1.0, 20 if wide else 3, batch=66 if wide else 1, kv_heads=4 if wide else 2, dim=64)
+    q = np.zeros(case.q.shape)
+    q[..., 3] = 2.0 ** 15
+    case.q, case.ks[:] = encode(q, kind)[0], ks
+    rng = np.random.default_rng(7)
+    top = rng.random(case.positions) < np.where(np.arange(case.positions) < 200, 0.1, 0.5)
+    case.k[..., 3] = np.where(top, 112, 98)[None, :, None] * (1 if ks > 0 else -1)
+    case.vs = (case.vs * np.exp2(rng.integers(-3, 4, case.positions))).astype(np.float32)
+    _, out, lse, _ = run(ctx, hip, case, max_len=None if wide else 0, account=False)
+    check(case, out, lse, one_product=True, equal_scores=True)
