@@ -158,14 +158,15 @@ namespace {
 // A column's softmax state.  Both halves of a wave hold their columns' m, c, M, most and limit; den is each lane's own
 // sum.  m (the maximum, rounded, as of the last time that it grew by 8) and c (M's shift) are whole numbers, M = m - c, so
 // that moving M and scaling what has been summed by the power of two that belongs to it agree exactly.  Where f32 has no room
-// for that (far: a column's m from 2^22 on), e is 2^((s - m) + c) instead of 2^(s - M), with s rounded as m is: with M alone, equal
-// scores weighed differently from 2^24 on.
+// for that (m from FAR on), e is 2^((s - m) + c) instead of 2^(s - M), with s rounded as m is: with M alone, equal scores
+// weighed differently from 2^24 on.
+constexpr float FAR = 4194304.0f;
 template <int D> struct State {
     // most: the largest |e vs| so far.  limit: what it may reach before M has to move; 0 where m has grown, so that the next
     // weights place it anew (else values far smaller than those before them, which outweigh them, lost bits:
     // V scales smaller by 10^6, scores higher by 2^80: 8e-5 off, by 10^9: 8e-2).
     float m = -INFINITY, M = -INFINITY, den = 0.0f, most = 0.0f, limit = 0.0f, c = 0.0f;
-    bool far = false;   // of the wave
+    bool far = false;   // one of the wave's columns is
     f16x acc[D / 32];
     DEV State() {
 #pragma unroll
@@ -239,7 +240,7 @@ DEV void reference(State<D> &S, float sf, bool edge, uint32_t bits, int h, float
             S.m = mn;
             S.limit = 0.0f;
         }
-        S.far = S.far || __ballot(grow && fabsf(mn) >= 4194304.0f) != 0;
+        S.far = S.far || __ballot(grow && fabsf(mn) >= FAR) != 0;
     }
 }
 // The weights as the second product's operands phi and plo, M moved where they leave fp16's range
@@ -290,18 +291,18 @@ DEV void weigh(State<D> &S, const f16x &dot, float sf, const float *ks, const fl
         for (int r = 0; r < 4; ++r) s[4 * j + r] = dot[4 * j + r] * k4[r];
     }
     reference<D>(S, sf, edge, bits, h, s);
-    if (keep) {   // (a masked position stays -inf whatever sf is)
+    if (keep) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) keep[r / 4][r % 4] = s[r] == -INFINITY ? -INFINITY : s[r] * sf;
+        for (int r = 0; r < 16; ++r) keep[r / 4][r % 4] = s[r];
     }
     const float M = S.M == -INFINITY ? 0.0f : S.M;
     if (!S.far) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) p[r] = fmaf(s[r], sf, -M);
     } else {
-        const float m = S.m == -INFINITY ? 0.0f : S.m;
+        const bool far = S.m != -INFINITY && fabsf(S.m) >= FAR;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) p[r] = (s[r] * sf - m) + S.c;
+        for (int r = 0; r < 16; ++r) p[r] = far ? (s[r] * sf - S.m) + S.c : fmaf(s[r], sf, -M);
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -321,10 +322,16 @@ DEV Column column(const QxaArgs &A, const Seq &q, uint32_t g, uint32_t c) {
     const uint32_t node = min(c / A.group, A.a.nodes - 1);
     return {node, g * A.group + c % A.group, c < A.columns && node < q.count};
 }
-// a column's sums: lse, or with several splits the state's part
+// A row's sums: lse, and for the account what makes weights of scores, as they were summed (weights by lse, in f32, were 10^-4
+// off for scores around 1000).
+DEV void finish_row(const QxaArgs &A, float M, float den, uint64_t row) {
+    if (A.a.lse) A.a.lse[row] = den == 0.0f ? -INFINITY : (M + __log2f(den)) * 0.69314718055994531f;
+    if (A.norm) A.norm[row] = den == 0.0f ? make_float2(0.0f, 0.0f) : make_float2(M, 1.0f / den);
+}
+// a column's sums, or with several splits the state's part
 DEV void finish_sums(const QxaArgs &A, float M, float den, bool whole, uint64_t row, uint64_t state) {
     if (!whole) A.md[state] = make_float2(M, den);
-    else if (A.lse) A.lse[row] = den == 0.0f ? -INFINITY : (M + __log2f(den)) * 0.69314718055994531f;
+    else finish_row(A, M, den, row);
 }
 // a column's result: out, or with several splits its state
 template <typename T, int D>
@@ -435,9 +442,10 @@ __global__ __launch_bounds__(256, 2) void qxa_tree(QxaArgs A) {
     }
     __syncthreads();
     const float sf = s_sf[col];
-    if (A.pack && job.z == 0) {   // the account's q
+    if (A.pack_sf && job.z == 0) {   // the account's q
         const uint64_t at = ((uint64_t)b * A.a.kv_heads + g) * A.tiles + tile;
-        for (int i = tid; i < KS * NP * 64; i += 256) A.pack[at * (KS * NP * 64) + i] = s_q[i];
+        if (A.pack)
+            for (int i = tid; i < KS * NP * 64; i += 256) A.pack[at * (KS * NP * 64) + i] = s_q[i];
         if (tid < 32) A.pack_sf[at * 32 + tid] = s_sf[tid];
     }
     State<D> S;
@@ -771,10 +779,15 @@ __global__ __launch_bounds__(256) void qxa_join(QxaArgs A) {
     }
     const float inv = den == 0.0f ? 0.0f : 1.0f / den;
     store4((T *)A.a.out + b * A.a.out_batch + node * A.a.out_node + head * D + 4 * at, make_float4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv));
-    if (at == 0 && A.lse) A.lse[row] = den == 0.0f ? -INFINITY : (m + __log2f(den)) * 0.69314718055994531f;
+    if (at == 0) finish_row(A, m, den, row);
 }
 
-// account[p] = decay * account[p] + sum over nodes and heads of 2^(s - lse), of kept scores.  A wave takes 32
+namespace {
+// The exponent of a weight, of dot * kscale: as it was for the row's own sums
+DEV float weight_exponent(float s, float sf, float M, bool far) { return far ? s * sf - M : fmaf(s, sf, -M); }
+}  // namespace
+
+// account[p] = decay * account[p] + sum over nodes and heads of 2^(s - M) / denominator, of kept scores.  A wave takes 32
 // positions, 8 lanes of 4 positions a row and every eighth row; rows and strips are added up in a fixed order.
 __global__ __launch_bounds__(256) void qxa_account_kept(QxaArgs A) {
     const uint32_t lane = threadIdx.x & 63, quad = lane & 7, b = blockIdx.y;
@@ -787,10 +800,11 @@ __global__ __launch_bounds__(256) void qxa_account_kept(QxaArgs A) {
             const uint32_t g = r / inuse, c = r % inuse, node = c / A.group, head = g * A.group + c % A.group;
             const f4x s = *reinterpret_cast<const f4x *>(
                 A.scores + ((((uint64_t)b * A.a.kv_heads + g) * ((A.a.positions + 31) / 32) + ci) * A.columns + c) * 32 + 4 * quad);
-            const float l = A.lse[((uint64_t)b * A.a.nodes + node) * A.a.heads + head];
-            const float l2 = l == -INFINITY ? INFINITY : l * 1.4426950408889634f;   // (a row that sees nothing adds 0)
+            const float2 norm = A.norm[((uint64_t)b * A.a.nodes + node) * A.a.heads + head];
+            const float sf = A.pack_sf[((uint64_t)b * A.a.kv_heads + g) * 32 + c];   // (one tile of columns)
+            const bool far = fabsf(norm.x) >= FAR;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sum[i] += s[i] == -INFINITY ? 0.0f : exp2_fast(s[i] - l2);   // (not seen: 0, of a NaN row as well)
+            for (int i = 0; i < 4; ++i) sum[i] += s[i] == -INFINITY ? 0.0f : exp2_fast(weight_exponent(s[i], sf, norm.x, far)) * norm.y;   // (not seen: 0, of a NaN row as well)
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {   // over the strips
@@ -851,7 +865,7 @@ __global__ __launch_bounds__(SHARE == 1 ? 256 : 64 * SHARE, 1) void qxa_account(
 #pragma unroll
                 for (int s = 0; s < KS * NP; ++s) qf[s] = qp[64 * s];
                 const float sf = A.pack_sf[at * 32 + col];
-                const float l = used ? A.lse[((uint64_t)b * A.a.nodes + node) * A.a.heads + head] : -INFINITY;
+                const float2 norm = used ? A.norm[((uint64_t)b * A.a.nodes + node) * A.a.heads + head] : make_float2(0.0f, 0.0f);
                 if (g != held) {
                     const KRow<D> kr = load_k<D>(A, b, g, pk, h);
 #pragma unroll
@@ -864,19 +878,24 @@ __global__ __launch_bounds__(SHARE == 1 ? 256 : 64 * SHARE, 1) void qxa_account(
                     if constexpr (SPLIT) dot = mfma(kf[s], qf[s * NP + 1], dot);
                     dot = mfma(kf[s], qf[s * NP], dot);
                 }
-                // a column that is not used or sees nothing adds 0: its exponent becomes -inf
-                const bool none = l == -INFINITY;
-                const float f = none ? 0.0f : sf, l2 = none ? INFINITY : l * 1.4426950408889634f;
+                // (a column that is not used or sees nothing adds 1 x 0)
+                const float f = norm.y == 0.0f ? 0.0f : sf;
+                const bool far = fabsf(norm.x) >= FAR;
+                float e[16];
+                if (__ballot(far) == 0) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) e[r] = exp2_fast(weight_exponent(dot[r] * ks[r], f, norm.x, false));
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) e[r] = exp2_fast(weight_exponent(dot[r] * ks[r], f, norm.x, far));
+                }
                 if (edge) {
                     const uint32_t bits = visible(A, q, b, node, pb) >> (4 * h);
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const float e = exp2_fast(fmaf(dot[r] * ks[r], f, -l2));
-                        sum[r] += seen(bits, r) && !none ? e : 0.0f;
-                    }
+                    for (int r = 0; r < 16; ++r) sum[r] = seen(bits, r) && norm.y != 0.0f ? fmaf(e[r], norm.y, sum[r]) : sum[r];
                 } else {
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) sum[r] += exp2_fast(fmaf(dot[r] * ks[r], f, -l2));
+                    for (int r = 0; r < 16; ++r) sum[r] = fmaf(e[r], norm.y, sum[r]);
                 }
             }
 #pragma unroll

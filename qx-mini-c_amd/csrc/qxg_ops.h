@@ -24,10 +24,10 @@ struct QxaArgs {
     float scale2;      // scale * log2(e)
     float *part;
     float2 *md;
-    float *lse;        // the caller's, or the workspace's for the account
-    float *scores;     // with an account and few columns: base-2 scores, [batch][kv head][chunk of 32 positions][column][32]
+    float2 *norm;      // with an account: a row's (M, 1 / denominator), [batch][node][head]: its weights are 2^(s - M) of that
+    float *scores;     // with an account and few columns: dot * kscale, -inf where masked, [batch][kv head][chunk of 32 positions][column][32]
     uint4 *pack;       // with an account otherwise: q as matrix operands, [batch][kv head][tile][k-step][half][lane]
-    float *pack_sf;    // [batch][kv head][tile][column] what turns dot * kscale into base-2 scores
+    float *pack_sf;    // with an account: [batch][kv head][tile][column] what turns dot * kscale into base-2 scores
 };
 hipError_t qxa_launch(const QxaArgs &A, hipStream_t s);
 

@@ -161,16 +161,16 @@ bool tree_plan(const qxg_tree_attention_args *p, QxaArgs &A, uint64_t &bytes, co
     // attention leaves as matrix operands.
     const bool kept = a.account && A.columns * 16 <= a.dim;
     const uint64_t scores = kept ? (uint64_t)a.batch * a.kv_heads * (((uint64_t)a.positions + 31) / 32) * A.columns * 128 : 0;
-    const uint64_t lse = a.account && !a.lse ? up16(rows * 4) : 0, ptiles = a.account && !kept ? (uint64_t)a.batch * a.kv_heads * A.tiles : 0;
-    const uint64_t sf = ptiles * 128, pack = ptiles * (a.dim / 16) * (a.type == QXG_TYPE_F32 ? 2 : 1) * 1024;
+    const uint64_t norm = a.account ? up16(rows * 8) : 0, tiles = a.account ? (uint64_t)a.batch * a.kv_heads * A.tiles : 0;
+    const uint64_t sf = tiles * 128, pack = kept ? 0 : tiles * (a.dim / 16) * (a.type == QXG_TYPE_F32 ? 2 : 1) * 1024;
     uint8_t *w = (uint8_t *)a.workspace;
     A.part = (float *)w;
     A.md = (float2 *)(w + part);
-    A.lse = a.lse ? a.lse : a.account ? (float *)(w + part + md) : nullptr;
-    A.scores = kept ? (float *)(w + part + md + lse) : nullptr;
-    A.pack_sf = ptiles ? (float *)(w + part + md + lse) : nullptr;
-    A.pack = ptiles ? (uint4 *)(w + part + md + lse + sf) : nullptr;
-    bytes = part + md + lse + scores + sf + pack;
+    A.norm = a.account ? (float2 *)(w + part + md) : nullptr;
+    A.pack_sf = a.account ? (float *)(w + part + md + norm) : nullptr;
+    A.scores = kept ? (float *)(w + part + md + norm + sf) : nullptr;
+    A.pack = pack ? (uint4 *)(w + part + md + norm + sf) : nullptr;
+    bytes = part + md + norm + sf + scores + pack;
     return true;
 }
 

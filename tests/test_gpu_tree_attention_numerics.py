@@ -179,3 +179,22 @@ def test_equal_scores_beyond_whole_numbers(ctx, hip, kind, ks, wide):  # noqa: F
     case.vs = (case.vs * np.exp2(rng.integers(-3, 4, case.positions))).astype(np.float32)
     _, out, lse, _ = run(ctx, hip, case, max_len=None if wide else 0, account=False)
     check(case, out, lse, one_product=True, equal_scores=True)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("ks", [2.0 ** -9, 20.0, -140.0, 30000.0])
+@pytest.mark.parametrize("nodes,batch,kv_heads", [(1, 1, 8), (3, 1, 2), (20, 66, 4), (20, 20, 2)])
+def test_account_of_large_scores(ctx, hip, kind, ks, nodes, batch, kv_heads):  # noqa: F811
+    """Scores from 900 on: the weights of equal ones are equal, and a row's weights are 1 in all, however far f32's steps
+    at the score's size are apart.  (A weight below 2^-126, f32's smallest normal number, may come out 0: of 900 and 1 / 8
+    less it is 2^-160, which f32 does not have.)"""
+    case = taken_over(kind, 1.0, nodes, batch=batch, kv_heads=kv_heads, dim=64)
+    q = np.zeros(case.q.shape)
+    q[..., 3] = 2.0 ** 15
+    case.q, case.ks[:] = encode(q, kind)[0], ks
+    top = np.random.default_rng(7).random(case.positions) < 0.3
+    case.k[..., 3] = np.where(top, 112, 98)[None, :, None] * (1 if ks > 0 else -1)
+    case.account[:] = 0
+    _, _, _, acc = run(ctx, hip, case)
+    _, _, weight, _, _, _ = formula(case)
+    assert (weight > 0.01).any() and (np.abs(acc.get() - weight) <= weight * 2.0 ** -17 + 2.0 ** -126 * nodes * 16).all()      # (of 16 heads)
