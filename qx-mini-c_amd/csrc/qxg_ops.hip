@@ -136,10 +136,10 @@ bool tree_plan(const qxg_tree_attention_args *p, QxaArgs &A, uint64_t &bytes, co
     if (a.dim != 64 && a.dim != 128) return fail("dim must be 64 or 128");
     if (!a.kv_heads || !a.heads || a.heads % a.kv_heads || a.heads > 1024) return fail("heads must be a multiple of kv_heads, at most 1024");
     if (!a.positions || a.positions > 0x7fffffffu || a.max_len > 0x7fffffffu) return fail("positions and max_len must be below 2^31");
-    if (a.q_batch * size % 16 || a.q_node * size % 16 || a.out_batch * size % 16 || a.out_node * size % 16)
+    if ((a.batch > 1 && (a.q_batch * size % 16 || a.out_batch * size % 16)) || (a.nodes > 1 && (a.q_node * size % 16 || a.out_node * size % 16)))
         return fail("the strides of q and out must be multiples of 16 bytes");
-    if (a.kv_batch % 16 || a.kv_row % 16) return fail("the strides of k and v must be multiples of 16 bytes");
-    if (a.kv_row >> 26) return fail("the row stride of k and v must be below 2^26 bytes");
+    if ((a.batch > 1 && a.kv_batch % 16) || (a.positions > 1 && a.kv_row % 16)) return fail("the strides of k and v must be multiples of 16 bytes");
+    if (a.positions > 1 && a.kv_row >> 26) return fail("the row stride of k and v must be below 2^26 bytes");
     if (rows_overlap(a.out_batch, a.batch, a.out_node, a.nodes, (uint64_t)a.heads * a.dim)) return fail("rows of out overlap");
     if (a.out && a.out == a.q) return fail("out must be another array than q");
     if (a.account && a.batch > 1 && a.account_batch < a.positions) return fail("the accounts overlap");
@@ -193,7 +193,7 @@ bool compact_plan(const qxg_kv_compact_args *p, QxeCompact &C, uint64_t &bytes, 
     if (!p->slots) return fail("slots must be positive");
     if (p->first >= p->positions) return fail("first is outside the cache");
     if (!p->row_bytes || p->row_bytes % 16 || p->row_bytes > 4096) return fail("row_bytes must be a multiple of 16 up to 4096");
-    if (p->kv_group % 16 || p->kv_row % 16) return fail("the strides of k and v must be multiples of 16 bytes");
+    if ((p->groups > 1 && p->kv_group % 16) || (p->positions > 1 && p->kv_row % 16)) return fail("the strides of k and v must be multiples of 16 bytes");
     if (rows_overlap(p->kv_row, p->positions, p->kv_group, p->groups, p->row_bytes)) return fail("the rows of k and v overlap");
     if (p->groups > 1 && p->scale_group < p->positions) return fail("the scales of groups overlap");
     if (p->groups > 1 && p->account_out && p->account_out_group < p->positions) return fail("the accounts of groups overlap");

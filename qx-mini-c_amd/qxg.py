@@ -208,6 +208,18 @@ def _layout(t):
     return None if t is None else (t.dtype, t.shape, t.stride())
 
 
+def _plain(layout):
+    """The layout with the strides that a contiguous array has in dimensions of 1, where any stride will do."""
+    if layout is None or 1 not in layout[1]:
+        return layout
+    return (*layout[:2], tuple(e if n == 1 else s for n, s, e in zip(layout[1], layout[2], _dense(tuple(layout[1])))))
+
+
+def _of_layouts(f):
+    """f of a call's layouts, worked out once for each set of them."""
+    return functools.lru_cache(maxsize=1024)(lambda *layouts: f(*map(_plain, layouts)))
+
+
 @functools.lru_cache(maxsize=4096)
 def _dense(shape):
     """The strides of a contiguous array."""
@@ -259,7 +271,7 @@ def _value_type(layout, name):
     return kind
 
 
-@functools.lru_cache(maxsize=1024)
+@_of_layouts
 def _tree_layout(q, k, v, kscale, vscale, lens, counts, mask, out, lse, account, workspace):
     """The struct's fields from workspace_bytes to positions, of layouts."""
     kind, qs, ks = _value_type(q, "q"), q[1], k[1]
@@ -278,7 +290,7 @@ def _tree_layout(q, k, v, kscale, vscale, lens, counts, mask, out, lse, account,
             _VALUE_TYPES[kind], batch, nodes, heads, ks[2], dim, ks[1])
 
 
-@functools.lru_cache(maxsize=1024)
+@_of_layouts
 def _select_layout(account, lens, keep, kept):
     groups, positions = account[1]
     for layout, name, of, shape, inner in ((account, "account", "f32", account[1], 1), (lens, "lens", "i32", (groups,), None),
@@ -287,7 +299,7 @@ def _select_layout(account, lens, keep, kept):
     return _outer(account), _outer(keep), groups, positions, keep[1][1]
 
 
-@functools.lru_cache(maxsize=1024)
+@_of_layouts
 def _compact_layout(k, v, kscale, vscale, keep, kept, account, account_out, workspace):
     groups, positions, row = k[1]
     gp = (groups, positions)
@@ -302,7 +314,7 @@ def _compact_layout(k, v, kscale, vscale, keep, kept, account, account_out, work
              groups, positions, keep[1][1]), row)
 
 
-@functools.lru_cache(maxsize=1024)
+@_of_layouts
 def _adjust_layout(logits, out, history, history_lens, prompt_lens, penalties, temperature, bias_ids, bias_values, mask, mask_rows,
                    top_ids, top_logits, lse, workspace):
     kind, shape = _value_type(logits, "logits"), logits[1]

@@ -1,4 +1,6 @@
 """More of what the operators on device memory refuse, on the CPU (as test_ops_refusals.py)."""
+import ctypes
+
 import pytest
 
 import qxg
@@ -67,3 +69,50 @@ def test_rows_beyond_a_launch(ctx, positions, message):  # noqa: F811
              kept=Fake((groups,), "int32", strides=(0,)), workspace=big())
     with pytest.raises(qxg.QxgError, match=message):
         ctx.kv_compact(**a)
+
+
+@pytest.mark.parametrize("change", [
+    dict(q=Fake((1, 3, 8, 128), strides=(1, 1024, 128, 1))),                     # (of a permuted [nodes, heads, dim, 1])
+    dict(out=Fake((1, 3, 8, 128), strides=(0, 1024, 128, 1), ptr=1 << 21)),
+    dict(k=Fake((1, 50, 4, 128), "int8", strides=(5, 512, 128, 1))),
+    dict(kscale=Fake((1, 50), strides=(1, 1))),
+    dict(account=Fake((1, 50), strides=(0, 1))),
+])
+def test_any_stride_of_a_dimension_of_one(ctx, change):  # noqa: F811
+    a = tree(q=Fake((1, 3, 8, 128)), k=Fake((1, 50, 4, 128), "int8"), v=Fake((1, 50, 4, 128), "int8"), kscale=Fake((1, 50)), vscale=Fake((1, 50)),
+             lens=Fake((1,), "int32"), out=Fake((1, 3, 8, 128), ptr=1 << 21), mask=None, counts=None, lse=None, account=None)
+    a.update(change)
+    with pytest.raises(qxg.QxgError, match="invalid context"):
+        ctx.tree_attention(**a)
+
+
+def test_any_stride_of_one_node_or_position(ctx):  # noqa: F811
+    one = dict(q=Fake((2, 1, 8, 128), strides=(1024, 3, 128, 1)), k=Fake((2, 1, 4, 128), "int8", strides=(512, 7, 128, 1)),
+               v=Fake((2, 1, 4, 128), "int8", strides=(512, 1 << 40, 128, 1)), kscale=Fake((2, 1)), vscale=Fake((2, 1), strides=(1, 9)),
+               out=Fake((2, 1, 8, 128), strides=(1024, 0, 128, 1), ptr=1 << 21), lse=None, mask=None, account=None)
+    with pytest.raises(qxg.QxgError, match="invalid context"):
+        ctx.tree_attention(**tree(**one))
+
+
+@pytest.mark.parametrize("change", [
+    dict(k=Fake((1, 40, 64), "int8", strides=(1, 64, 1))), dict(kscale=Fake((1, 40), strides=(3, 1))), dict(keep=Fake((1, 10), "int32", strides=(0, 1))),
+    dict(k=Fake((1, 40, 64), "int8", strides=(7, 64, 1)), v=Fake((1, 40, 64), "int8", strides=(9, 64, 1))),
+    dict(account_out=Fake((1, 40), strides=(1, 1), ptr=1 << 22)),
+])
+def test_any_stride_of_one_group(ctx, change):  # noqa: F811
+    k = Fake((1, 40, 64), "int8")
+    a = dict(k=k, v=k, kscale=Fake((1, 40)), vscale=Fake((1, 40)), keep=Fake((1, 10), "int32"), kept=Fake((1,), "int32", strides=(5,)),
+             account=Fake((1, 40)), account_out=Fake((1, 40), ptr=1 << 22), workspace=big())
+    a.update(change)
+    with pytest.raises(qxg.QxgError, match="invalid context"):
+        ctx.kv_compact(**a)
+
+
+def test_strides_that_the_c_interface_does_not_use(ctx):  # noqa: F811
+    """The same at the C interface: strides over one sequence, node, position or group are not looked at."""
+    err = ctypes.create_string_buffer(256)
+    p = 1 << 20
+    packed = qxg._TREE.pack(p, p, p, p, p, p, 0, 0, 1 << 21, 0, 0, p, 1 << 30, 3, 5, 7, 9, 11, 13, 1, 1, 0, 1, 1, 8, 4, 128, 1, 1, 0.1, 1.0)
+    assert qxg._g.qxg_tree_attention(None, packed, None, 1, err, 256) == 0 and err.value == b"invalid context"
+    packed = qxg._COMPACT.pack(p, p, p, p, p, p, 0, 0, p, 1 << 30, 3, 5, 1, 1, 1, 1, 1, 1, 1, 1, 0, 64)
+    assert qxg._g.qxg_kv_compact(None, packed, None, 1, err, 256) == 0 and err.value == b"invalid context"
