@@ -363,10 +363,10 @@ DEV void finish_column(const QxaArgs &A, const State<D> &S, float den, const Job
 
 // Few columns, or little work.  A workgroup takes a tile of columns of one kv head and a run of
 // 32-position chunks; its 4 waves take every fourth chunk, each with a state of its own, merged at the end.  The
-// next chunk's rows are on their way while one is worked on.  The cache's bytes bound it (single tokens over 4 x
-// 30000 positions of 8 kv heads: 46 us, 5.3 TB/s; 56 where scores are kept, KEEP), or with few of them the
-// chain of latencies: 8.2 us for a token over 37 positions, 13.4 for 16 nodes of 32 heads over 1500 (splits of a chunk
-// a wave), 26 for 64 nodes over 4032, where issue counts as well.
+// next chunk's rows are on their way while one is worked on.  The cache's bytes bound it (single BF16 tokens over 4 x
+// 30000 positions of 8 kv heads, 247 MB: 62 us, 4.0 TB/s where a copy has 5.1; over 14000 to 30000 each, 176 MB, 50 us, 59
+// where scores are kept, KEEP), or with few of them the chain of latencies: 8.5 us for a token over 37 positions, 12.8 for 16
+// nodes of 32 heads over 1500 (splits of a chunk a wave), 27 for 64 nodes over 4032, where issue counts as well.
 template <typename T, int D, bool KEEP>
 __global__ __launch_bounds__(256, 2) void qxa_tree(QxaArgs A) {
     constexpr bool SPLIT = two_halves_q<T>;
@@ -539,10 +539,10 @@ __global__ __launch_bounds__(256, 2) void qxa_tree(QxaArgs A) {
 // dim's 32 positions in the order of the second product's k): one conversion of a code for 128 columns.  Two
 // buffers, so one barrier a chunk; the next chunk's codes are on their way.
 // Instruction issue bounds it: 2 x 48 nodes of 32 heads over 65500 positions (f16, weights as hi + lo, so 24
-// matrix instructions a chunk) take 162 us, 620 TFLOP/s of matrix work; the matrix pipe is busy a third of the
+// matrix instructions a chunk) take 167 us, 600 TFLOP/s of matrix work; the matrix pipe is busy a third of the
 // cycles, the vector pipe under half, LDS two fifths, and a wave's softmax does not fit behind the other wave's
 // products.  The same with chunks of 64 positions, with the next chunk's scores computed ahead, with three waves
-// a SIMD (10 registers spilled): 157 .. 164 us.
+// a SIMD (10 registers spilled): 157 .. 164 us, where this form had 162.
 template <typename T, int D>
 __global__ __launch_bounds__(256, 2) void qxa_wide(QxaArgs A) {
     constexpr bool SPLIT = two_halves_q<T>;
@@ -740,7 +740,7 @@ __global__ __launch_bounds__(256, 2) void qxa_wide(QxaArgs A) {
 
 // The splits of a row joined: a workgroup a row, its 256 / (D / 4) strips of threads every so many splits, the
 // strips in order.  (A wave a row, a split's state after the other: 12 us for 32 splits of 128 rows.)  A
-// chain of loads bounds it: 4 us for 11 splits of 512 rows, 10.3 for 2 x 1536 rows of 20 splits.
+// chain of loads bounds it: 4 us for 11 splits of 512 rows, 10.6 for 2 x 1536 rows of 20 splits.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void qxa_join(QxaArgs A) {
     constexpr int W = D / 4, STRIPS = 256 / W;
@@ -828,8 +828,8 @@ __global__ __launch_bounds__(256) void qxa_account_kept(QxaArgs A) {
 // positions that its registers hold; columns and waves are added up in a fixed order, and no two
 // workgroups add to one position.  SHARE waves take the same 32 positions and every SHARE-th (kv head, tile): 8
 // where there are few positions, whose chain of pairs would be the time; else 1 and four chunks a
-// workgroup, which then read each q from the first-level cache (calls of 16 nodes, BF16: over 16000 positions 40.5 us with
-// 8 and 45.4 with 1, over 30000 54.7 and 49.3).  16 nodes of 32 heads over 1500 positions: 9.5 us, a chain
+// workgroup, which then read each q from the first-level cache (calls of 16 nodes, BF16: over 16000 positions 42.1 us with
+// 8 and 46.7 with 1, over 30000 57.3 and 52.8).  16 nodes of 32 heads over 1500 positions: 9.5 us, a chain
 // of latencies (lengths, scales, K and q, two pairs a wave, the sums); of long ones the matrix instructions bound it.
 template <typename T, int D, int SHARE>
 __global__ __launch_bounds__(SHARE == 1 ? 256 : 64 * SHARE, 1) void qxa_account(QxaArgs A) {

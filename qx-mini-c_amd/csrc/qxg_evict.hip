@@ -329,7 +329,7 @@ __global__ __launch_bounds__(1024) void qxe_select_long(qxg_kv_select_args A) {
 // write have been read, and writes.  A claimed tile reads without waiting, and waits only for tiles
 // claimed before it, so every wait ends (a bound on the polls ends it also where two calls share a workspace,
 // which is not allowed).  Each row is read and written once: 48 groups of 2048 rows of
-// 512 bytes 43 .. 48 us (200 MB), 3 of 32768 rows picked from four times as many 60 (scattered rows).  (Strips of columns, each walked in order by
+// 512 bytes 43 .. 48 us (200 MB), 3 of 32768 rows picked from four times as many 60 .. 65 (scattered rows).  (Strips of columns, each walked in order by
 // one workgroup, left most of the GPU idle: 989 us for 3 groups of 32768 rows.)  state: the ticket, then
 // a word a tile.
 extern "C" __global__ __launch_bounds__(256) void qxe_clear(uint32_t *state, uint32_t n) {

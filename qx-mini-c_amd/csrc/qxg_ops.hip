@@ -93,19 +93,20 @@ bool rows_overlap(uint64_t a, uint64_t na, uint64_t b, uint64_t nb, uint64_t row
 uint64_t up16(uint64_t v) { return (v + 15) & ~15ull; }
 
 // ---- tree attention
-// Which kernel takes a tree, and the splits of its positions over the batch (F32, 32 heads of 128 dims, in us).
+// Which kernel takes a tree, and the splits of its positions over the batch (F32, 32 heads of 128 dims, in us; BF16 of 64
+// dims has the same borders to within 2 us, but for 8 x 16 nodes over 1000 positions: 22 in splits, 16 without).
 //
 // The wide kernel's workgroups take four tiles at a time: a code is converted once for 128 columns, but a chunk's
 // latency is a workgroup's, where the other kernel's four waves have a chunk each.  It gains from about 12000 chunks
-// of all tiles on: 16 nodes, 4 kv heads, 12000 positions (6016 chunks) 32.1 against 26.1, 30000 (15008) 36.9 against 39.1; 64
-// nodes, 4000 positions (8128) 32.8 against 28.1, 12000 (24128) 47.6 against 52.9.
+// of all tiles on: 16 nodes, 4 kv heads, 12000 positions (6016 chunks) 31.8 against 26.9, 30000 (15008) 38.4 against 40.4; 64
+// nodes, 4000 positions (8128) 33.8 against 28.6, 12000 (24128) 48.1 against 52.8.
 //
 // Splits: a workgroup a CU where the work is small, else two (480 of the 512 places: with all taken some workgroups of a launch
 // waited for a second round, 217 instead of 162 for 2 x 48 nodes over 65500 positions): 16 nodes over 4000 positions
-// (2016 chunks) with 240 workgroups 17.6, with 480 20.7; 64 nodes over 4000 (8128) 33.0 and 28.4.  None where a wave has few
+// (2016 chunks) with 240 workgroups 17.8, with 480 21.0; 64 nodes over 4000 (8128) 33.7 and 28.8.  None where a wave has few
 // rounds of chunks anyway, as states and their join take 4, with a batch 5 to 10 (its shares are found in both
-// kernels): 8 x 16 nodes, 8 kv heads, 500 positions (4 rounds) 16.6 without, 24.6 with; 8 rounds 23.9 and 26.9, but with
-// a quarter of the workgroups 21.5 and 14.5; one tree of 64 nodes over 200 (3 rounds) 12.4 and 14.8, over 500 (5 rounds) 16.7 and 15.9.
+// kernels): 8 x 16 nodes, 8 kv heads, 500 positions (4 rounds) 17.2 without, 25.9 with; 8 rounds 24.0 and 27.6, but of
+// 4 nodes (64 workgroups) 21.9 and 17.7; one tree of 64 nodes over 200 (3 rounds) 12.7 and 15.0, over 500 (5 rounds) 17.1 and 16.1.
 void tree_splits(QxaArgs &A) {
     const qxg_tree_attention_args &a = A.a;
     const uint64_t chunks = ((uint64_t)a.max_len + a.nodes + 31) / 32;   // of a sequence
@@ -156,8 +157,8 @@ bool tree_plan(const qxg_tree_attention_args *p, QxaArgs &A, uint64_t &bytes, co
     const uint64_t states = A.splits == 1 ? 0 : (a.batch > 64 ? (uint64_t)A.splits * a.batch : a.batch == 1 ? A.splits : 2ull * A.splits + a.batch) * a.nodes * a.heads;
     const uint64_t part = up16(states * a.dim * 4), md = up16(states * 8);
     // The account needs the scores again.  Of few columns they are kept (at most half as many bytes, written
-    // and read, as the K codes have): single tokens over 4 x 30000 positions, 8 kv heads of 4 columns, take 65 us
-    // instead of 85, of 8 columns 77, of 16 96 instead of 86.  Of more they are computed again from q, which the
+    // and read, as the K codes have): single tokens over 4 x 30000 positions, 8 kv heads of 4 columns, take 67 us
+    // instead of 90, of 8 columns 77, of 16 99 instead of 90.  Of more they are computed again from q, which the
     // attention leaves as matrix operands.
     const bool kept = a.account && A.columns * 16 <= a.dim;
     const uint64_t scores = kept ? (uint64_t)a.batch * a.kv_heads * (((uint64_t)a.positions + 31) / 32) * A.columns * 128 : 0;
