@@ -198,3 +198,17 @@ def test_account_of_large_scores(ctx, hip, kind, ks, nodes, batch, kv_heads):  #
     _, _, _, acc = run(ctx, hip, case)
     _, _, weight, _, _, _ = formula(case)
     assert (weight > 0.01).any() and (np.abs(acc.get() - weight) <= weight * 2.0 ** -17 + 2.0 ** -126 * nodes * 16).all()      # (of 16 heads)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("code", [5, 8, 11, 14, 17])
+@pytest.mark.parametrize("first", [True, False])
+@pytest.mark.parametrize("wide", [False, True])
+def test_many_small_weights(ctx, hip, kind, code, first, wide):  # noqa: F811
+    """One position outweighs each of the others by 2^(2.04 code) and has the value 0: what the others sum up to."""
+    case = taken_over(kind, 1.0, 20 if wide else 2, positions=640 if wide else 4096, batch=66 if wide else 1, kv_heads=4 if wide else 2)
+    case.k[..., 3], case.v[:], case.vs[:] = 0, 101, 1 / 64
+    at = 0 if first else case.positions - 1
+    case.k[:, at, :, 3], case.v[:, at] = code, 0
+    _, out, lse, _ = run(ctx, hip, case, max_len=None if wide else 0, account=False)
+    check(case, out, lse, one_product=True)
