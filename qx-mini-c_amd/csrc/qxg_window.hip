@@ -7,6 +7,9 @@
 // several bf16 numbers: 3 for f32 (24 bits), for 16-bit types q as it is (f16: 2) and the weights as 2 (17 bits: their error is
 // 2^-18, where the result's rounding is 2^-12 or 2^-9).  bf16 has f32's range, so weights far below their row's largest keep their bits,
 // of which many may outweigh it; in f16 they would need a window that moves.  (Pieces below 2^-126 may count as 0.)
+// The exponent s - M of a score in base 2 is one fma.  Where |M| is from FAR on, it is the product rounded as the maximum was, less
+// M: an fma's would hold what that rounding left, half a step of the score, from 2^28 on more than the 8 that M allows, and from 2^31 on
+// more than e has room for.
 // Scores of an f32 q over INT8 codes are products of whole numbers instead, exact but for q's rounding: a column's q times a power of two, at
 // most 0x7f7f7f, as three of 8 bits (a step is at most 2^-22 of the column's largest magnitude).  The codes are operands as they lie
 // and the products 12 for 24: 512 tokens of 32 / 4 heads of 128 within 1024 + 4 positions take 44.5 us, in bf16 49.  (Of 16-bit types,
@@ -83,6 +86,8 @@ DEV float code(uint32_t w, int i) { return (float)(int8_t)(w >> (8 * i)); }
 DEV uint4 codes8(uint32_t x, uint32_t y) {   // 8 INT8 codes
     return make_uint4(pack_bf16(code(x, 0), code(x, 1)), pack_bf16(code(x, 2), code(x, 3)), pack_bf16(code(y, 0), code(y, 1)), pack_bf16(code(y, 2), code(y, 3)));
 }
+
+constexpr float FAR = 4194304.0f;
 
 struct Seq { uint32_t len, count; };   // of sequence b, clamped to the arrays
 DEV Seq sequence(const QxwArgs &A, uint32_t b) {
@@ -273,6 +278,7 @@ __global__ __launch_bounds__(256, CT == 2 || (D == 128 && (sizeof(T) == 4 || (__
         }
     }
     float m[CT], den[CT];
+    bool far = false;   // one of the wave's references is
     f4x acc[CT][DT];
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
@@ -357,30 +363,43 @@ __global__ __launch_bounds__(256, CT == 2 || (D == 128 && (sizeof(T) == 4 || (__
 #pragma unroll
             for (int i = 1; i < 8; ++i) most[c] = fmaxf(most[c], s[c][i / 4][i % 4]);
             most[c] *= A.scale2;
-            over = over || most[c] > m[c] + 8.0f;
+            over = over || most[c] - m[c] > 8.0f;   // (of infinities of one sign: no)
         }
-        if (__ballot(over) != 0) {   // M moves, of the columns where it has to
+        if (__ballot(over) != 0 || far) {   // M moves, of the columns where it has to
+            far = false;
 #pragma unroll
             for (int c = 0; c < CT; ++c) {
                 float x = fmaxf(most[c], __shfl_xor(most[c], 16));
                 x = fmaxf(x, __shfl_xor(x, 32));
-                const bool grow = x > m[c] + 8.0f;
+                const bool grow = x - m[c] > 8.0f;
                 const float mn = grow ? rintf(x) : m[c], f = !grow || m[c] == -INFINITY ? 1.0f : exp2_fast(m[c] - mn);
                 m[c] = mn;
+                far = far || __ballot(fabsf(mn) >= FAR && mn > -INFINITY) != 0;
                 den[c] *= f;
 #pragma unroll
                 for (int d = 0; d < DT; ++d)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) acc[c][d][r] *= f;
             }
+            if (far) {   // the exponents at once
+#pragma unroll
+                for (int c = 0; c < CT; ++c)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float M = m[c] == -INFINITY ? 0.0f : m[c], t = s[c][i / 4][i % 4] * A.scale2, rounded = t - M;
+                        const float exact = fmaf(s[c][i / 4][i % 4], A.scale2, -M);
+                        s[c][i / 4][i % 4] = fabsf(M) >= FAR ? rounded : exact;
+                    }
+            }
         }
+        const float scale2 = far ? 1.0f : A.scale2;
         uint4 pf[CT][NP];
 #pragma unroll
         for (int c = 0; c < CT; ++c) {
-            const float M = m[c] == -INFINITY ? 0.0f : m[c];
+            const float M = m[c] == -INFINITY || far ? 0.0f : m[c];
             float e[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) e[i] = exp2_fast(fmaf(s[c][i / 4][i % 4], A.scale2, -M));
+            for (int i = 0; i < 8; ++i) e[i] = exp2_fast(fmaf(s[c][i / 4][i % 4], scale2, -M));
             den[c] += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
             if constexpr (BITS == 8) {
 #pragma unroll
@@ -570,6 +589,7 @@ __global__ __launch_bounds__(256, 2) void qxw_many(QxwArgs A) {
     for (int k = 0; k < KS; ++k) qf[k] = reinterpret_cast<const uint4 *>((const T *)a.q + b * a.q_batch + token * a.q_token + head * D + h * (D / 2))[k];
     // the reference, how far over it a score may be (-inf: nothing is seen yet), this lane's sum
     float M = 0.0f, limit = -INFINITY, den = 0.0f;
+    bool far = false;   // one of the wave's references is
     f16x acc[DT], s;
 #pragma unroll
     for (int d = 0; d < DT; ++d) acc[d] = zero16();
@@ -643,17 +663,33 @@ __global__ __launch_bounds__(256, 2) void qxw_many(QxwArgs A) {
         float most = e[0];
 #pragma unroll
         for (int r = 1; r < 16; ++r) most = fmaxf(most, e[r]);
-        if (__ballot(most > limit) != 0) {   // M moves, of the columns where it has to, and what was summed with it
-            most = max_of_halves(most);
-            const bool grow = most > limit;
-            const float mn = grow ? rintf(M + most) : M, f = !grow || limit < 0.0f ? 1.0f : exp2_fast(M - mn);
-            M = mn;
-            limit = grow ? 8.0f : limit;
+        if (__ballot(most > limit) != 0 || far) {   // M moves, of the columns where it has to, and what was summed with it
+            // (from the scores again: equal ones are to weigh the same in all chunks, however large)
+            float top = -INFINITY;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {   // (from the scores again: equal ones are to weigh the same in all chunks, however large)
+            for (int j = 0; j < 4; ++j) {
                 const f4x ks = scale_of(0, j);
 #pragma unroll
-                for (int r = 4 * j; r < 4 * j + 4; ++r) e[r] = e[r] == -INFINITY ? e[r] : exponent(r, ks);
+                for (int r = 4 * j; r < 4 * j + 4; ++r) {
+                    const float t = s[r] * ks[r % 4];
+                    top = fmaxf(top, e[r] == -INFINITY ? e[r] : t);
+                }
+            }
+            top = max_of_halves(top);
+            const bool grow = top - M > limit;
+            const float mn = grow ? rintf(top) : M, f = !grow || limit < 0.0f ? 1.0f : exp2_fast(M - mn);
+            M = mn;
+            limit = grow ? 8.0f : limit;
+            const bool away = fabsf(M) >= FAR;
+            far = __ballot(away) != 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const f4x ks = scale_of(0, j);
+#pragma unroll
+                for (int r = 4 * j; r < 4 * j + 4; ++r) {
+                    const float t = s[r] * ks[r % 4], rounded = t - M, exact = exponent(r, ks), x = away ? rounded : exact;
+                    e[r] = e[r] == -INFINITY ? e[r] : x;
+                }
             }
             den *= f;
 #pragma unroll

@@ -1,0 +1,89 @@
+"""cache_attention where scores are large or not finite, in its kernels of 16, 32 and 128 columns (test_cache_plans.py: that they are
+reached)."""
+import numpy as np
+import pytest
+
+from cacheref import U, Cache, clamped, rounding
+from devmem import decode
+from test_gpu_cache_attention import Case, ctx, hip  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+# name: (arguments, columns of a tile)
+KERNELS = {
+    "f32 of 8 bits": (dict(kind="f32", bits=8, batch=1, tokens=3, heads=4, kv_heads=2, dim=128, positions=110, lens=[107]), 16),
+    "f32 of 4 bits": (dict(kind="f32", bits=4, batch=1, tokens=3, heads=4, kv_heads=2, dim=64, positions=110, lens=[107]), 16),
+    "f16 of 8 bits": (dict(kind="f16", bits=8, batch=1, tokens=3, heads=4, kv_heads=2, dim=64, positions=110, lens=[107]), 16),
+    "bf16 of 4 bits": (dict(kind="bf16", bits=4, batch=1, tokens=3, heads=4, kv_heads=2, dim=128, positions=110, lens=[107]), 16),
+    "bf16, in splits": (dict(kind="bf16", bits=8, batch=1, tokens=1, heads=4, kv_heads=2, dim=64, positions=3000, lens=[2990]), 16),
+    "32, f32": (dict(kind="f32", bits=8, batch=1, tokens=300, heads=8, kv_heads=2, dim=64, positions=4305, lens=[4000]), 32),
+    "32, f16 of 4 bits": (dict(kind="f16", bits=4, batch=1, tokens=300, heads=8, kv_heads=2, dim=128, positions=4305, lens=[4000]), 32),
+    "128": (dict(kind="bf16", bits=8, batch=1, tokens=256, heads=512, kv_heads=1, dim=64, positions=1900, lens=[1640]), 128),
+    "128, in splits": (dict(kind="bf16", bits=8, batch=1, tokens=256, heads=32, kv_heads=4, dim=128, positions=26262, lens=[26001]), 128),
+}
+
+
+def far(c, sizes, heads):
+    """A row of q a size, in turn: size times values of 1 to 2, of both signs."""
+    rng = np.random.default_rng(1)
+    q = rng.choice([-1, 1], (1, c["tokens"], c["heads"], c["dim"])) * rng.uniform(1, 2, (1, c["tokens"], c["heads"], c["dim"]))
+    return q * np.resize(sizes, c["tokens"] * heads).reshape(1, c["tokens"], heads, 1)
+
+
+def check(c, heads=None):
+    """Scores that are equal or far apart: softmax in 64 bits weighs them as the formula does, whatever a dot product in f32 is off by.
+    Tolerances are those of cacheref's attention without that, lse's with it."""
+    out, lse = decode(c.out.get(), c.kind), c.lse.get()
+    lens, counts = clamped(c.lens, c.counts, c.q.shape[1], c.cache.k.shape[1])
+    n, count, dim, all_heads = lens[0] + counts[0], counts[0], c.q.shape[3], c.q.shape[2]
+    p, j = lens[0] + np.arange(count)[:, None], np.arange(n)[None]
+    for h in heads or range(all_heads):
+        g = h * c.cache.k.shape[2] // all_heads
+        k, v, q = c.cache.values(0, 0)[:n, g], c.cache.values(1, 0)[:n, g], decode(c.q[0, :count, h], c.kind)
+        # exact before they are multiplied by the position's scale, or equal ones would differ here
+        dot = q @ c.cache.k[0, :n, g].T.astype(np.float64) * c.cache.kscale[0, :n].astype(np.float64) if c.bits == 8 else q @ k.T
+        s = np.where(j <= p, c.scale * dot, -np.inf)
+        m = s.max(1, keepdims=True)
+        w = np.exp(s - m)
+        den = w.sum(1, keepdims=True)
+        want, wlse, sums = w / den @ v, (m + np.log(den))[:, 0], (p + 65) * U
+        tol = (2 * sums + 2.0 ** -21 + (U if c.kind == "f32" else 2.0 ** -18)) * (w / den @ np.abs(v)) + rounding(c.kind, want)
+        assert (np.abs(out[0, :count, h] - want) <= tol).all(), (h, (np.abs(out[0, :count, h] - want) / tol).max(1))
+        mag = (c.scale * (np.abs(q) @ np.abs(k).T)).max(1)
+        ltol = (dim + 16) * U * mag + sums[:, 0] + 2.0 ** -20 + 2 * U * np.abs(wlse)
+        assert (np.abs(lse[0, :count, h] - wlse) <= ltol).all(), (h, lse[0, :count, h], wlse)
+
+
+def some(c):
+    return sorted({0, 1, c["heads"] // 2, c["heads"] - 1})
+
+
+SIZES = [2.0 ** e for e in (0, 10, 17, 18, 19, 20, 21, 22, 23, 24, 26, 28, 30, 31, 32, 34, 37, 40, 60, 100)]
+
+
+@pytest.mark.parametrize("name", sorted(KERNELS))
+@pytest.mark.parametrize("by", ["q", "scale"])
+def test_equal_scores_of_any_size(ctx, hip, name, by):  # noqa: F811
+    """All keys alike: the result is the mean of the values, of scores from 1 to 2^100 and -2^100."""
+    c = KERNELS[name][0]
+    cache = Cache(np.random.default_rng(0), c["bits"], 1, c["positions"], c["kv_heads"], c["dim"])
+    cache.k[:], cache.kscale[:] = cache.k[0, 0], cache.kscale[0, 0]
+    if by == "q":
+        check(Case(hip, **c, q=far(c, SIZES if c["kind"] != "f16" else [1.0, 2.0 ** 13], c["heads"]), cache=cache).run(ctx), some(c))
+        return
+    for scale in (0.125, 2.0 ** 14, 2.0 ** 18 / 3, 2.0 ** 22 / 7, 2.0 ** 25 / 3, 2.0 ** 29 / 5, 2.0 ** 35, 2.0 ** 90 / 3):
+        check(Case(hip, **c, q=far(c, [1.0], c["heads"]), cache=cache, scale=float(np.float32(scale))).run(ctx), some(c))
+
+
+@pytest.mark.parametrize("name", sorted(KERNELS))
+@pytest.mark.parametrize("rising", [True, False])
+def test_scores_far_apart(ctx, hip, name, rising):  # noqa: F811
+    """Keys of four sizes, in runs of positions: the largest scores have all of the weight, be they the first or the last that a row sees."""
+    c = KERNELS[name][0]
+    cache = Cache(np.random.default_rng(0), c["bits"], 1, c["positions"], c["kv_heads"], c["dim"])
+    run = np.arange(c["positions"]) * 4 // c["positions"]
+    run = run if rising else 3 - run
+    cache.k[:], cache.kscale[:] = cache.k[0, 0], cache.kscale[0, 0]
+    cache.kscale[:] = (2.0 ** run / 64 if c["bits"] == 8 else 124 + run).reshape(1, -1, *[1] * (cache.kscale.ndim - 2))
+    sizes = [2.0 ** e for e in (20, 24, 28, 31, 32, 34, 40, 60, 100)] if c["kind"] != "f16" else [1.0, 2.0 ** 13]
+    check(Case(hip, **c, q=far(c, sizes, c["heads"]), cache=cache, scale=1.0 if c["kind"] != "f16" else 2.0 ** 20).run(ctx), some(c))
