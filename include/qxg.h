@@ -503,7 +503,8 @@ int qxg_kv_append(qxg_ctx *ctx, const qxg_kv_append_args *args, void *stream, in
  * tokens at and behind count are left as they were; out is not to overlap q.  tokens = 1 is single-token decoding.
  * Products are those of f32 numbers for an F32 q, but that with 8 bits q is rounded to 2^-22 of its row's largest magnitude; for F16 and
  * BF16 the softmax weights enter theirs with 17 bits, q as it is.  Sums are f32, rounded once; weights are up to 2^8 before they are
- * divided by their sum, so values from 2^118 on may overflow.  A row that sees a scale of 8 bits that is not finite is NaN. */
+ * divided by their sum, so values from 2^118 on may overflow.  A row that sees a scale of 8 bits that is not finite
+ * is NaN, and so is its lse, as are a row whose q is not finite and one whose largest score is beyond f32. */
 typedef struct qxg_cache_attention_args {
     const void *q;            /* [batch][tokens][heads][dim] of `type`, 16-byte aligned */
     const void *k, *v;        /* 16-byte aligned */

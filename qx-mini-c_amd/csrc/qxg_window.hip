@@ -140,8 +140,10 @@ DEV Place place_of(const QxwArgs &A) {
 DEV uint64_t state_at(const QxwArgs &A, uint32_t b, uint32_t split, uint32_t token, uint32_t head) {
     return (((uint64_t)b * A.splits + split) * A.a.tokens + token) * A.a.heads + head;
 }
+// A row sees its own position at least, so its denominator is 0 only where all of its scores are -inf (an infinite q, or dot products
+// beyond f32): 1 / 0 makes the context NaN, as the formula is there, and lse is NaN with it.
 DEV void finish_lse(const QxwArgs &A, float M, float den, uint32_t b, uint32_t token, uint32_t head) {
-    if (A.a.lse) A.a.lse[((uint64_t)b * A.a.tokens + token) * A.a.heads + head] = den == 0.0f ? -INFINITY : (M + __log2f(den)) * 0.69314718055994531f;
+    if (A.a.lse) A.a.lse[((uint64_t)b * A.a.tokens + token) * A.a.heads + head] = den == 0.0f ? NAN : (M + __log2f(den)) * 0.69314718055994531f;
 }
 }  // namespace
 
@@ -470,7 +472,7 @@ __global__ __launch_bounds__(256, CT == 2 || (D == 128 && (sizeof(T) == 4 || (__
             for (int i = 0; i < N; i += 4) store4(at + i, make_float4(sum[i], sum[i + 1], sum[i + 2], sum[i + 3]));
         };
         if (A.splits == 1) {
-            const float inv = all == 0.0f ? 0.0f : 1.0f / all;
+            const float inv = 1.0f / all;
 #pragma unroll
             for (int i = 0; i < N; ++i) sum[i] *= inv;
             put((T *)a.out + b * a.out_batch + to * a.out_token + h * D + d0);
@@ -736,7 +738,7 @@ __global__ __launch_bounds__(256, 2) void qxw_many(QxwArgs A) {
     // results: a tile of 32 dims after the other through the wave's part of LDS, so that 8 lanes write a column's line
     const bool whole = A.splits == 1;
     den += __shfl_xor(den, 32);
-    const float inv = !whole ? 1.0f : den == 0.0f ? 0.0f : 1.0f / den;
+    const float inv = whole ? 1.0f / den : 1.0f;
     float *o = u.out[wave];
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
@@ -815,7 +817,7 @@ __global__ __launch_bounds__(256) void qxw_join(QxwArgs A) {
             }
         }
     }
-    const float inv = den == 0.0f ? 0.0f : 1.0f / den;
+    const float inv = 1.0f / den;
     T *out = (T *)a.out + b * a.out_batch + token * a.out_token + head * D + lane * (D / 64);
 #pragma unroll
     for (int i = 0; i < D / 64; ++i) out[i] = (T)(sum[i] * inv);

@@ -87,3 +87,41 @@ def test_scores_far_apart(ctx, hip, name, rising):  # noqa: F811
     cache.kscale[:] = (2.0 ** run / 64 if c["bits"] == 8 else 124 + run).reshape(1, -1, *[1] * (cache.kscale.ndim - 2))
     sizes = [2.0 ** e for e in (20, 24, 28, 31, 32, 34, 40, 60, 100)] if c["kind"] != "f16" else [1.0, 2.0 ** 13]
     check(Case(hip, **c, q=far(c, sizes, c["heads"]), cache=cache, scale=1.0 if c["kind"] != "f16" else 2.0 ** 20).run(ctx), some(c))
+
+
+@pytest.mark.parametrize("name", sorted(KERNELS))
+@pytest.mark.parametrize("bad", [np.inf, -np.inf])
+def test_rows_whose_scores_are_all_minus_infinity(ctx, hip, name, bad):  # noqa: F811
+    """An infinite value of q over codes of one sign: all scores of the row are infinite, of one sign or the other, and it is NaN either way; the
+    rows beside it are as they were."""
+    c = KERNELS[name][0]
+    cache = Cache(np.random.default_rng(0), c["bits"], 1, c["positions"], c["kv_heads"], c["dim"])
+    cache.k[..., 3] = -5 if c["bits"] == 8 else cache.k[..., 3] | 0x88      # (of 4 bits the dims 6 and 7)
+    if c["bits"] == 4:
+        cache.k[..., 3] |= 0x11
+    q = np.random.default_rng(1).standard_normal((1, c["tokens"], c["heads"], c["dim"]))
+    clean = Case(hip, **c, q=q, cache=cache).run(ctx)
+    rows = [(0, 1), (c["tokens"] - 1, c["heads"] - 1), (c["tokens"] // 2, 0)]
+    for token, head in rows:
+        q[0, token, head, 3 if c["bits"] == 8 else 7] = bad
+    got = Case(hip, **c, q=q, cache=cache).run(ctx)
+    out, lse, want, wlse = decode(got.out.get(), c["kind"]), got.lse.get(), decode(clean.out.get(), c["kind"]), clean.lse.get()
+    for token, head in rows:
+        assert np.isnan(out[0, token, head]).all() and np.isnan(lse[0, token, head])
+        out[0, token, head], lse[0, token, head] = want[0, token, head], wlse[0, token, head]
+    assert (out == want).all() and (lse == wlse).all()
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("lens,window", [([0], None), ([40], 1)])
+def test_one_position_whose_score_is_minus_infinity(ctx, hip, kind, bits, lens, window):  # noqa: F811
+    """The first token of a prompt, and a token that sees itself alone."""
+    cache = Cache(np.random.default_rng(0), bits, 1, 50, 2, 64)
+    cache.k[:] = np.abs(cache.k) // 2 + 1 if bits == 8 else (cache.k & 0x77) | 0x11
+    q = np.random.default_rng(1).standard_normal((1, 1, 4, 64))
+    q[0, 0, 1, 9], q[0, 0, 2, 9] = -np.inf, np.inf
+    c = Case(hip, kind, bits, 1, 1, 4, 2, 64, 50, lens, window=window, q=q, cache=cache).run(ctx)
+    out, lse = decode(c.out.get(), kind)[0, 0], c.lse.get()[0, 0]
+    assert np.isnan(out[1:3]).all() and np.isnan(lse[1:3]).all()
+    assert np.isfinite(out[[0, 3]]).all() and np.isfinite(lse[[0, 3]]).all()
