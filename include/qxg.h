@@ -501,8 +501,7 @@ int qxg_kv_append(qxg_ctx *ctx, const qxg_kv_append_args *args, void *stream, in
  *     s[j] = scale * sum_d q[i][h][d] k[j][g][d],  out[i][h] = sum_j softmax(s)[j] v[j][g],  lse[i][h] = log sum_j exp(s[j])
  * with k and v the values that the cache stands for.  What stands in positions that a row does not see does not reach it; rows of
  * tokens at and behind count are left as they were; out is not to overlap q.  tokens = 1 is single-token decoding.
- * Products are those of f32 numbers for an F32 q, but that with 8 bits q is rounded to 2^-22 of its row's largest magnitude; for F16 and
- * BF16 the softmax weights enter theirs with 17 bits, q as it is.  Sums are f32, rounded once; weights are up to 2^8 before they are
+ * Products are those of f32 numbers for an F32 q; for F16 and BF16 the softmax weights enter theirs with 17 bits, q as it is.  Sums are f32, rounded once; weights are up to 2^8 before they are
  * divided by their sum, so values from 2^118 on may overflow.  A row that sees a scale of 8 bits that is not finite
  * is NaN, and so is its lse, as are a row whose q is not finite and one whose largest score is beyond f32. */
 typedef struct qxg_cache_attention_args {

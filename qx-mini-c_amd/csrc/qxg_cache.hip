@@ -78,8 +78,8 @@ bool append_plan(const qxg_kv_append_args *p, QxkArgs &A, const Err &fail) {
 // launch costs a program 3 to 5.
 //
 // With 32 columns a workgroup shares the codes' loads and conversion, and a round takes 1.4 times as long.  (f32 has registers for it with
-// 64 dims: 512 tokens of 32 / 8 heads over 8000 positions of 8 bits 152 us with 16 and 130 with 32, of 4 bits 135 and 118; with 128
-// dims it spills: of 32 / 4 heads 227 and 250, 204 and 201.)  us with 16 and 32, 32 / 4 heads of 128 in bf16: 512
+// 64 dims: 512 tokens of 32 / 8 heads over 8000 positions of 8 bits 147 us with 16 and 120 with 32, of 4 bits 125 and 105; with 128
+// dims it spills: of 32 / 4 heads 239 and 346, 191 and 189.)  us with 16 and 32, 32 / 4 heads of 128 in bf16: 512
 // tokens over 8000 positions of 8 bits 223, 159, of 4 bits 154, 124; 8 x 5 over 6000 of 8 bits 37, 28; 256 over 600 17.8, 16.0; 32
 // over 600 9.8, 11.5; one token each of 16 sequences of 32000 of 4 bits (4 columns) 141, 153.
 // With 128, whose waves share them in LDS, more work is needed to pay: of 8 bits and a BF16 q, 512 tokens over 8000 positions

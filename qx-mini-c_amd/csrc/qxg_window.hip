@@ -2,7 +2,7 @@
 //
 // Mathematics.  One pass with a base-2 softmax: a column keeps a reference M, a whole number that follows the running maximum to
 // within 2^8, the sum of e = 2^(s - M) and the context, the sum of e v; both are scaled by a power of two when M moves.
-// Products are on the matrix cores in bf16, with f32 sums.  Codes are exact there: INT8 ones as whole numbers, whose scales
+// All products are on the matrix cores in bf16, with f32 sums.  Codes are exact there: INT8 ones as whole numbers, whose scales
 // multiply the scores and the weights e; E2M1 ones with their power of two.  What is not, q and the weights, is taken as the sum of
 // several bf16 numbers: 3 for f32 (24 bits), for 16-bit types q as it is (f16: 2) and the weights as 2 (17 bits: their error is
 // 2^-18, where the result's rounding is 2^-12 or 2^-9).  bf16 has f32's range, so weights far below their row's largest keep their bits,
@@ -10,10 +10,8 @@
 // The exponent s - M of a score in base 2 is one fma.  Where |M| is from FAR on, it is the product rounded as the maximum was, less
 // M: an fma's would hold what that rounding left, half a step of the score, from 2^28 on more than the 8 that M allows, and from 2^31 on
 // more than e has room for.
-// Scores of an f32 q over INT8 codes are products of whole numbers instead, exact but for q's rounding: a column's q times a power of two, at
-// most 0x7f7f7f, as three of 8 bits (a step is at most 2^-22 of the column's largest magnitude).  The codes are operands as they lie
-// and the products 12 for 24: 512 tokens of 32 / 4 heads of 128 within 1024 + 4 positions take 44.5 us, in bf16 49.  (Of 16-bit types,
-// whose q is one or two bf16 numbers, nothing is saved: 34 us and 33 for a token of 16 sequences within 4096 + 16.)
+// (An f32 q over INT8 codes as a column's whole numbers, in products of 8 bits, is faster for a prompt, 44.5 us for 49 of 512 tokens of 32 / 4
+// heads of 128 within 1024 + 4 positions, but a large value of q costs the others their low bits, from 2^22 times as large all of them.)
 #include "qxg_cache.h"
 #include "qxg_values.h"
 
@@ -21,15 +19,11 @@ namespace {
 typedef __bf16 b2v __attribute__((ext_vector_type(2)));
 typedef __bf16 b8v __attribute__((ext_vector_type(8)));
 typedef float f2v __attribute__((ext_vector_type(2)));
-typedef int i4x __attribute__((ext_vector_type(4)));
 template <typename T> constexpr int Q_PIECES = sizeof(T) == 4 ? 3 : __is_same(T, _Float16) ? 2 : 1;
 template <typename T> constexpr int P_PIECES = sizeof(T) == 4 ? 3 : 2;
 
 DEV f4x mfma16(uint4 a, uint4 b, f4x c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8v, a), __builtin_bit_cast(b8v, b), c, 0, 0, 0);
-}
-DEV i4x mfma16_i8(uint4 a, uint4 b, i4x c) {
-    return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i4x, a), __builtin_bit_cast(i4x, b), c, 0, 0, 0);
 }
 DEV uint32_t pack_bf16(float lo, float hi) {   // to nearest
     const f2v x = {lo, hi};
@@ -53,16 +47,6 @@ template <int N> DEV void pieces8(float (&v)[8], uint4 (&p)[N]) {
         }
         p[n] = make_uint4(w[0], w[1], w[2], w[3]);
     }
-}
-// 4 whole numbers of at most 0x7f7f7f in magnitude as 2^16 p[0] + 2^8 p[1] + p[2], each of 8 bits with a sign: byte i of a word is that of number i
-DEV void pieces_i8(const int (&x)[4], uint32_t (&p)[3]) {
-    uint32_t v[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = (uint32_t)x[i] + 0x808080u;   // (a byte less 128 is the piece: carries go on as they should)
-    const uint32_t a = perm(v[1], v[0], 0x06020501u), b = perm(v[3], v[2], 0x06020501u);   // byte 1 of both, byte 2 of both
-    p[0] = perm(b, a, 0x07060302u) ^ 0x80808080u;
-    p[1] = perm(b, a, 0x05040100u) ^ 0x80808080u;
-    p[2] = perm(perm(v[3], v[2], 0x0c0c0400u), perm(v[1], v[0], 0x0c0c0400u), 0x05040100u) ^ 0x80808080u;
 }
 // 8 codes of 4 bits times a power of two, exact
 DEV uint4 e2m1x8(uint32_t w, float scale) {
@@ -153,7 +137,7 @@ DEV void finish_lse(const QxwArgs &A, float M, float den, uint32_t b, uint32_t t
 // What bounds it.  Long caches and few tokens: bytes; one token each of 16 sequences of 30000 positions, 32 / 8 heads of 128 in bf16 over 8 bits,
 // 983 MB in 206 us, 4.8 TB/s (4 bits, 32000 positions: 557 MB in 141 us).  Otherwise the issue of instructions, about one in 4.7 cycles:
 // a chunk of 16 columns of 128 dims is some 300 vector instructions, half of them the conversion of codes, and 28 to 48 matrix ones, which add up
-// as a SIMD's waves all do the same; 512 tokens of 32 / 4 heads in f32 within 1024 + 4 positions 44.5 us.  Tried without gain: 8 waves a
+// as a SIMD's waves all do the same; 512 tokens of 32 / 4 heads in f32 within 1024 + 4 positions 49 us.  Tried without gain: 8 waves a
 // workgroup (15.0 us and 14.3 for a token over 36 chunks), which share the SIMDs; contexts of 64 columns a wave, which spill.
 // A first form, which staged chunks in LDS for four waves of 16 columns each, took 42 us where this takes 36 (16 x 1 token within
 // 4096 + 16), and 165 where it takes 107 (16 x 1 token over 10000 to 32000
@@ -229,54 +213,16 @@ __global__ __launch_bounds__(256, CT == 2 || (D == 128 && (sizeof(T) == 4 || (__
     uint32_t ci = part.lo + wave;
     const bool busy = ci < part.hi;   // of the wave
     if (busy) load(list.at(ci) * 32);
-    constexpr bool WHOLE = BITS == 8 && sizeof(T) == 4;
-    constexpr int QS = WHOLE ? D / 64 : KS, QN = WHOLE ? 3 : NQ;   // steps and pieces of q
-    uint4 qf[CT][QS][QN];
-    int power[CT];    // of two, of q's whole numbers
-    float of_high[CT];   // 256, NaN where q is not finite
+    uint4 qf[CT][KS][NQ];
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
         const uint32_t column = tile * COLUMNS + 16 * c + u;
         const T *row = (const T *)a.q + b * a.q_batch + min(column / A.group, last) * a.q_token + (g * A.group + column % A.group) * D + w * (D / 4);
-        if constexpr (WHOLE) {
-            float v[D / 32][8], top = 0.0f;
 #pragma unroll
-            for (int s = 0; s < D / 32; ++s) {
-                load8(row + 8 * s, v[s]);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[s][i]));
-            }
-            top = fmaxf(top, __shfl_xor(top, 16));
-            top = fmaxf(top, __shfl_xor(top, 32));
-            // times 2^(22 - exponent), or half of that, so that the largest is at most 0x7f7f7f, which 3 pieces hold
-            power[c] = (int)max((__float_as_uint(top) + 0x10200u) >> 23, 1u) - 149;
-            bool finite = true;
-#pragma unroll
-            for (int s = 0; s < QS; ++s)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    int x[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float y = v[2 * s + j / 2][4 * (j % 2) + i];
-                        finite = finite && isfinite(y);
-                        x[i] = (int)rintf(ldexpf(y, -power[c]));
-                    }
-                    uint32_t p[3];
-                    pieces_i8(x, p);
-#pragma unroll
-                    for (int n = 0; n < 3; ++n) reinterpret_cast<uint32_t *>(&qf[c][s][n])[j] = p[n];
-                }
-            finite = __shfl_xor((int)finite, 16) != 0 && finite;
-            finite = __shfl_xor((int)finite, 32) != 0 && finite;
-            of_high[c] = finite ? 256.0f : NAN;
-        } else {
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                float v[8];
-                load8(row + 8 * s, v);
-                pieces8<NQ>(v, qf[c][s]);
-            }
+        for (int s = 0; s < KS; ++s) {
+            float v[8];
+            load8(row + 8 * s, v);
+            pieces8<NQ>(v, qf[c][s]);
         }
     }
     float m[CT], den[CT];
@@ -303,35 +249,19 @@ __global__ __launch_bounds__(256, CT == 2 || (D == 128 && (sizeof(T) == 4 || (__
         f4x s[CT][2];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            if constexpr (WHOLE) {
-                uint4 kf[QS];
 #pragma unroll
-                for (int k = 0; k < QS; ++k) kf[k] = make_uint4(in.k[t][4 * k], in.k[t][4 * k + 1], in.k[t][4 * k + 2], in.k[t][4 * k + 3]);
+            for (int c = 0; c < CT; ++c) s[c][t] = f4x{0.0f, 0.0f, 0.0f, 0.0f};
+            float scale = 1.0f;
+            if constexpr (BITS == 4) scale = s_scale[wave][0][w * D / 128][16 * t + u];
 #pragma unroll
-                for (int c = 0; c < CT; ++c) {
-                    i4x x[3] = {};
+            for (int k = 0; k < KS; ++k) {
+                uint4 kf;
+                if constexpr (BITS == 4) kf = e2m1x8(in.k[t][k], scale);
+                else kf = codes8(in.k[t][2 * k], in.k[t][2 * k + 1]);
 #pragma unroll
-                    for (int k = 0; k < QS; ++k)
+                for (int n = NQ - 1; n >= 0; --n)
 #pragma unroll
-                        for (int n = 0; n < 3; ++n) x[n] = mfma16_i8(kf[k], qf[c][k][n], x[n]);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) s[c][t][r] = ldexpf(fmaf((float)(x[0][r] * 256 + x[1][r]), of_high[c], (float)x[2][r]), power[c]);
-                }
-            } else {
-#pragma unroll
-                for (int c = 0; c < CT; ++c) s[c][t] = f4x{0.0f, 0.0f, 0.0f, 0.0f};
-                float scale = 1.0f;
-                if constexpr (BITS == 4) scale = s_scale[wave][0][w * D / 128][16 * t + u];
-#pragma unroll
-                for (int k = 0; k < KS; ++k) {
-                    uint4 kf;
-                    if constexpr (BITS == 4) kf = e2m1x8(in.k[t][k], scale);
-                    else kf = codes8(in.k[t][2 * k], in.k[t][2 * k + 1]);
-#pragma unroll
-                    for (int n = NQ - 1; n >= 0; --n)
-#pragma unroll
-                        for (int c = 0; c < CT; ++c) s[c][t] = mfma16(kf, qf[c][k][n], s[c][t]);
-                }
+                    for (int c = 0; c < CT; ++c) s[c][t] = mfma16(kf, qf[c][k][n], s[c][t]);
             }
         }
         float vs[8];

@@ -3,7 +3,7 @@ reached)."""
 import numpy as np
 import pytest
 
-from cacheref import U, Cache, clamped, rounding
+from cacheref import U, Cache, check_attention, clamped, rounding
 from devmem import decode
 from test_gpu_cache_attention import Case, ctx, hip  # noqa: F401
 
@@ -125,3 +125,27 @@ def test_one_position_whose_score_is_minus_infinity(ctx, hip, kind, bits, lens, 
     out, lse = decode(c.out.get(), kind)[0, 0], c.lse.get()[0, 0]
     assert np.isnan(out[1:3]).all() and np.isnan(lse[1:3]).all()
     assert np.isfinite(out[[0, 3]]).all() and np.isfinite(lse[[0, 3]]).all()
+
+
+@pytest.mark.parametrize("name", sorted(n for n in KERNELS if KERNELS[n][0]["kind"] == "f32"))
+@pytest.mark.parametrize("large", [2.0 ** 10, 2.0 ** 20, 2.0 ** 40])
+def test_one_large_channel_of_q_costs_the_others_no_bits(ctx, hip, name, large):  # noqa: F811
+    """Where K is 0 there: products are those of f32 numbers, each value of q with all of its bits."""
+    c = KERNELS[name][0]
+    cache = Cache(np.random.default_rng(0), c["bits"], 1, c["positions"], c["kv_heads"], c["dim"])
+    cache.k[..., 0] = 0 if c["bits"] == 8 else cache.k[..., 0] & 0xf0
+    q = np.random.default_rng(1).standard_normal((1, c["tokens"], c["heads"], c["dim"]))
+    q[..., 0] = large
+    got = Case(hip, **c, q=q, cache=cache).run(ctx)
+    if c["tokens"] == 3:
+        got.check()
+    else:      # (some rows: the bounds are computed row by row)
+        some_rows(got, [0, 77, 299])
+
+
+def some_rows(c, tokens):
+    """check_attention of these tokens of sequence 0, each as a sequence of its own."""
+    for i in tokens:
+        n = int(c.lens[0]) + i
+        check_attention(c.out.get()[:, i:i + 1], c.lse.get()[:, i:i + 1], c.q[:, i:i + 1], c.cache, np.array([n], np.uint32), np.array([1], np.uint32), 0, 0,
+                        c.scale, c.kind)
