@@ -456,9 +456,10 @@ uint64_t qxg_adjust_logits_workspace(const qxg_adjust_logits_args *args);
 /* ---- a cache of 8 or 4 bits: its rows from projections, and attention over it ----
  *
  * bits 8: the context's own format: k, v [batch][positions][kv_heads][dim] int8, kscale, vscale [batch][positions] f32.
- * bits 4: E2M1 values with an E8M0 scale for each 32 dims, as the OCP Microscaling formats define them: k, v
+ * bits 4: E2M1 values with an E8M0 scale for each 32 dims, as the OCP Microscaling formats define them but for the scales' ends: k, v
  * [batch][positions][kv_heads][dim / 2], dim 2 i in the low half of byte i; kscale, vscale [batch][positions][kv_heads][dim / 32]
- * bytes e, for 2^(e - 127).  (A byte below 2 counts as 2 and one above 252 as 252, NaN's 255 among them: qxg_kv_append writes none.) */
+ * bytes e, for 2^(e - 127), and 255 for NaN.  (The formats' 2^-127 and 2^-126, bytes 0 and 1, are read as 2^-125, and 2^126 and 2^127, bytes 253 and
+ * 254, as 2^125: products with them leave f32's normal numbers.  qxg_kv_append writes none of the five.) */
 
 /* The rows of new tokens on their way from a projection into attention and the cache.  Token i < counts[b] of sequence b
  * stands at position lens[b] + i.  Per head of q and k, in this order:
@@ -502,8 +503,8 @@ int qxg_kv_append(qxg_ctx *ctx, const qxg_kv_append_args *args, void *stream, in
  * with k and v the values that the cache stands for.  What stands in positions that a row does not see does not reach it; rows of
  * tokens at and behind count are left as they were; out is not to overlap q.  tokens = 1 is single-token decoding.
  * Products are those of f32 numbers for an F32 q; for F16 and BF16 the softmax weights enter theirs with 17 bits, q as it is.  Sums are f32, rounded once; weights are up to 2^8 before they are
- * divided by their sum, so values from 2^118 on may overflow.  A row that sees a scale of 8 bits that is not finite
- * is NaN, and so is its lse, as are a row whose q is not finite and one whose largest score is beyond f32. */
+ * divided by their sum, so values from 2^118 on may overflow.  A row that sees a scale that is not finite is NaN,
+ * and so is its lse, as are a row whose q is not finite and one whose largest score is beyond f32. */
 typedef struct qxg_cache_attention_args {
     const void *q;            /* [batch][tokens][heads][dim] of `type`, 16-byte aligned */
     const void *k, *v;        /* 16-byte aligned */

@@ -66,6 +66,13 @@ DEV float finite_scales(uint32_t bits) {
     const uint32_t lane = threadIdx.x & 63, either = (uint32_t)all | (uint32_t)(all >> 32);
     return either >> (lane & 31) & 1 ? (lane < 32 ? NAN : 0.0f) : x;
 }
+// Of 4 bits, likewise: the positions one of whose scale bytes (K's in lanes 0 .. 31, V's in 32 .. 63) is 255, NaN.  Its power of two counts as
+// another's, so that for a row that does not see the position its weight times the value is 0; the scores of one that does become NaN.
+DEV uint32_t nan_scales(uint32_t bytes) {
+    const uint32_t x = ~bytes;   // a byte of 0: only where one is does the difference borrow
+    const uint64_t all = __ballot(((x - 0x01010101u) & ~x & 0x80808080u) != 0);
+    return (uint32_t)all | (uint32_t)(all >> 32);
+}
 DEV float code(uint32_t w, int i) { return (float)(int8_t)(w >> (8 * i)); }
 DEV uint4 codes8(uint32_t x, uint32_t y) {   // 8 INT8 codes
     return make_uint4(pack_bf16(code(x, 0), code(x, 1)), pack_bf16(code(x, 2), code(x, 3)), pack_bf16(code(y, 0), code(y, 1)), pack_bf16(code(y, 2), code(y, 3)));
@@ -276,6 +283,15 @@ __global__ __launch_bounds__(256, CT == 2 || (D == 128 && (sizeof(T) == 4 || (__
                 for (int c = 0; c < CT; ++c)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) s[c][t][r] *= ks[r];
+            }
+        }
+        if constexpr (BITS == 4) {
+            const uint32_t bad = nan_scales(in.scale);
+            if (bad != 0) {
+#pragma unroll
+                for (int c = 0; c < CT; ++c)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) s[c][i / 4][i % 4] = bad >> (16 * (i / 4) + 4 * w + i % 4) & 1 ? NAN : s[c][i / 4][i % 4];
             }
         }
         if (!all_seen(A, pb, p0, p1)) {

@@ -149,3 +149,26 @@ def some_rows(c, tokens):
         n = int(c.lens[0]) + i
         check_attention(c.out.get()[:, i:i + 1], c.lse.get()[:, i:i + 1], c.q[:, i:i + 1], c.cache, np.array([n], np.uint32), np.array([1], np.uint32), 0, 0,
                         c.scale, c.kind)
+
+
+@pytest.mark.parametrize("name", sorted(n for n in KERNELS if KERNELS[n][0]["bits"] == 4))
+@pytest.mark.parametrize("side", [2, 3])
+@pytest.mark.parametrize("window", [None, 40])
+def test_scale_bytes_that_are_nan(ctx, hip, name, side, window):  # noqa: F811
+    """E8M0's 255 is NaN: the rows of its kv head that see the position are NaN, all others as they were."""
+    c = {**KERNELS[name][0], "window": window}
+    tokens, heads, kv_heads = c["tokens"], c["heads"], c["kv_heads"]
+    cache = Cache(np.random.default_rng(0), 4, 1, c["positions"], kv_heads, c["dim"])
+    q = np.random.default_rng(1).standard_normal((1, tokens, heads, c["dim"]))
+    clean = Case(hip, **c, q=q, cache=cache).run(ctx)
+    want, wlse = decode(clean.out.get(), c["kind"]), clean.lse.get()
+    for at, g, block in ((c["lens"][0] + tokens // 2, 0, 0), (c["lens"][0] - 45, kv_heads - 1, c["dim"] // 32 - 1), (c["lens"][0] + tokens - 1, 0, 1)):
+        saved, cache.arrays()[side][0, at, g, block] = cache.arrays()[side][0, at, g, block], 255
+        got = Case(hip, **c, q=q, cache=cache).run(ctx)
+        cache.arrays()[side][0, at, g, block] = saved
+        p, group = c["lens"][0] + np.arange(tokens), heads // kv_heads
+        sees = np.zeros((tokens, heads), bool)
+        sees[:, g * group:(g + 1) * group] = ((at <= p) & ((p - at < window) if window else True))[:, None]
+        out, lse = decode(got.out.get(), c["kind"])[0], got.lse.get()[0]
+        assert np.isnan(out[sees]).all() and np.isnan(lse[sees]).all()
+        assert (out[~sees] == want[0][~sees]).all() and (lse[~sees] == wlse[0][~sees]).all()
