@@ -473,7 +473,8 @@ uint64_t qxg_adjust_logits_workspace(const qxg_adjust_logits_args *args);
  *     bits 4: the least power of two, of 2^-125 to 2^125, of which a block's largest magnitude is not over 7 times; each value the
  *             nearest E2M1 value times it, of two equally near ones that of the even code, at most 6 times it
  * Rows of tokens at and behind counts, and all other positions, are left as they were.  q, k and v may be parts of one array's rows.
- * q_out may be q itself; otherwise outputs overlap nothing else.  at is clamped to the table's last row. */
+ * q_out may be q itself; otherwise outputs share memory with nothing else.  (Refused are q_out in q, and all outputs in each other and in k and v; rows
+ * that lie between another array's are told apart where both arrays' strides are the same.)  at is clamped to the table's last row. */
 typedef struct qxg_kv_append_args {
     const void *q;            /* [batch][tokens][heads][dim] of `type`, 16-byte aligned */
     const void *k, *v;        /* [batch][tokens][kv_heads][dim] of `type`, 16-byte aligned */
@@ -501,7 +502,8 @@ int qxg_kv_append(qxg_ctx *ctx, const qxg_kv_append_args *args, void *stream, in
  * with p - j < window or j < sinks (window 0: all of them).  As qxg_tree_attention otherwise:
  *     s[j] = scale * sum_d q[i][h][d] k[j][g][d],  out[i][h] = sum_j softmax(s)[j] v[j][g],  lse[i][h] = log sum_j exp(s[j])
  * with k and v the values that the cache stands for.  What stands in positions that a row does not see does not reach it; rows of
- * tokens at and behind count are left as they were; out is not to overlap q.  tokens = 1 is single-token decoding.
+ * tokens at and behind count are left as they were; out shares memory with nothing else, nor does lse (refused: in each other, in
+ * the cache, out in q).  tokens = 1 is single-token decoding.
  * Products are those of f32 numbers for an F32 q; for F16 and BF16 the softmax weights enter theirs with 17 bits, q as it is.  Sums are f32, rounded once; weights are up to 2^8 before they are
  * divided by their sum, so values from 2^118 on may overflow.  A row that sees a scale that is not finite is NaN,
  * and so is its lse, as are a row whose q is not finite and one whose largest score is beyond f32. */

@@ -26,6 +26,24 @@ template <typename A> bool rows_aligned(const A &a, uint64_t batch, uint64_t tok
     const uint32_t size = type_size(a.type);
     return (a.batch == 1 || batch * size % 16 == 0) && (a.tokens == 1 || token * size % 16 == 0);
 }
+// The rows of an array [batch][n][..] of `size` bytes an element and `row` elements a row
+template <typename A> Rows rows_of(const A &a, const void *p, const char *name, uint64_t batch, uint64_t next, uint64_t n, uint64_t row, uint64_t size) {
+    return {p, name, batch * size, a.batch, next * size, n, row * size};
+}
+template <typename A> Rows codes_of(const A &a, const void *p, const char *name) {
+    return rows_of(a, p, name, a.kv_batch, a.kv_row, a.positions, (uint64_t)a.kv_heads * a.dim * a.bits / 8, 1);
+}
+template <typename A> Rows scales_of(const A &a, const void *p, const char *name) {
+    return a.bits == 8 ? rows_of(a, p, name, a.scale_batch, 0, 1, a.positions, 4)
+                       : rows_of(a, p, name, a.scale_batch, a.scale_row, a.positions, (uint64_t)a.kv_heads * a.dim / 32, 1);
+}
+// Refuses what is written, the first `written` arrays, where it shares memory with another of them.
+template <size_t N> bool apart(const Rows (&rows)[N], size_t written, const Err &fail) {
+    for (size_t i = 0; i < written; ++i)
+        for (size_t j = i + 1; j < N; ++j)
+            if (rows[i].p && rows[j].p && rows_meet(rows[i], rows[j])) return fail("%s and %s share memory", rows[i].name, rows[j].name);
+    return true;
+}
 
 // ---- append
 bool append_plan(const qxg_kv_append_args *p, QxkArgs &A, const Err &fail) {
@@ -160,6 +178,14 @@ int qxg_kv_append(qxg_ctx *c, const qxg_kv_append_args *p, void *stream, int wai
                         {p->q_norm, "q_norm", false, 4}, {p->k_norm, "k_norm", false, 4}, {p->rope, "rope", false, 4},
                         {p->rope_at, "rope_at", false, 4}};
     if (!pointers_ok(args, fail)) return 0;
+    const uint32_t size = type_size(p->type);
+    const uint64_t q_row = (uint64_t)p->heads * p->dim, row = (uint64_t)p->kv_heads * p->dim;
+    const Rows q_out = rows_of(*p, p->q_out, "q_out", p->out_batch, p->out_token, p->tokens, q_row, size);
+    const Rows rows[] = {q_out, codes_of(*p, p->k_cache, "k_cache"), codes_of(*p, p->v_cache, "v_cache"), scales_of(*p, p->kscale, "kscale"),
+                         scales_of(*p, p->vscale, "vscale"), rows_of(*p, p->k, "k", p->k_batch, p->k_token, p->tokens, row, size),
+                         rows_of(*p, p->v, "v", p->v_batch, p->v_token, p->tokens, row, size)};
+    const Rows turned[] = {q_out, rows_of(*p, p->q == p->q_out ? nullptr : p->q, "q", p->q_batch, p->q_token, p->tokens, q_row, size)};
+    if (!apart(rows, 5, fail) || !apart(turned, 1, fail)) return 0;
     return on_device(c, args, (hipStream_t)stream, wait, fail, [&] { return qxk_launch_append(A, (hipStream_t)stream); });
 }
 
@@ -173,6 +199,13 @@ int qxg_cache_attention(qxg_ctx *c, const qxg_cache_attention_args *p, void *str
                         {p->vscale, "vscale", true, scale}, {p->lens, "lens", true, 4}, {p->counts, "counts", false, 4},
                         {p->out, "out", true, 16}, {p->lse, "lse", false, 4}, {p->workspace, "workspace", false, 16}};
     if (!pointers_ok(args, fail) || !workspace_ok(p->workspace, p->workspace_bytes, need, fail)) return 0;
+    const uint32_t size = type_size(p->type);
+    const uint64_t row = (uint64_t)p->heads * p->dim;
+    const Rows out = rows_of(*p, p->out, "out", p->out_batch, p->out_token, p->tokens, row, size);
+    const Rows rows[] = {out, {p->lse, "lse", 0, 1, 0, 1, (uint64_t)p->batch * p->tokens * p->heads * 4}, codes_of(*p, p->k, "k"), codes_of(*p, p->v, "v"),
+                         scales_of(*p, p->kscale, "kscale"), scales_of(*p, p->vscale, "vscale")};
+    const Rows answers[] = {out, rows_of(*p, p->q, "q", p->q_batch, p->q_token, p->tokens, row, size)};
+    if (!apart(rows, 2, fail) || !apart(answers, 1, fail)) return 0;
     return on_device(c, args, (hipStream_t)stream, wait, fail, [&] { return qxw_launch(A, (hipStream_t)stream); });
 }
 // (The plan goes by the value type as well; a program that asks before it has q's gets what all of them need.)

@@ -91,6 +91,31 @@ bool rows_overlap(uint64_t a, uint64_t na, uint64_t b, uint64_t nb, uint64_t row
     }
     return false;
 }
+// Rows of `row` bytes at p + i a + j b, i < na, j < nb
+struct Rows {
+    const void *p;
+    const char *name;
+    uint64_t a, na, b, nb, row;
+};
+// Whether rows of two arrays share memory.  Where the strides are the arrays' own, unlike ones, rows between each other's rows are not told
+// apart: then it is whether the arrays' ranges meet.
+bool rows_meet(const Rows &x, const Rows &y) {
+    using wide = __int128;
+    const auto size = [](const Rows &r) { return (wide)(r.na - 1) * r.a + (wide)(r.nb - 1) * r.b + r.row; };
+    const wide d = (wide)(uintptr_t)y.p - (wide)(uintptr_t)x.p;
+    if (d >= size(x) || -d >= size(y)) return false;
+    if ((x.na > 1 && y.na > 1 && x.a != y.a) || (x.nb > 1 && y.nb > 1 && x.b != y.b)) return true;
+    wide s = x.na > 1 ? x.a : y.a, t = x.nb > 1 ? x.b : y.b;
+    // the rows' distances are d + i s + j t; they meet where one is between -y.row and x.row
+    wide ilo = -(wide)(x.na - 1), ihi = y.na - 1, jlo = -(wide)(x.nb - 1), jhi = y.nb - 1;
+    if (ihi - ilo > jhi - jlo) { std::swap(s, t); std::swap(ilo, jlo); std::swap(ihi, jhi); }
+    const auto down = [](wide n, wide by) { return n / by - (n % by < 0); };
+    for (wide i = ilo; i <= ihi; ++i) {
+        const wide at = d + i * s, least = -(wide)y.row + 1 - at, most = (wide)x.row - 1 - at;   // of j t
+        if (t == 0 ? least <= 0 && 0 <= most : std::max(jlo, -down(-least, t)) <= std::min(jhi, down(most, t))) return true;
+    }
+    return false;
+}
 uint64_t up16(uint64_t v) { return (v + 15) & ~15ull; }
 bool workspace_ok(const void *p, uint64_t have, uint64_t need, const Err &fail) {
     return !need || (p && have >= need) || fail("the workspace holds %llu bytes; this call needs %llu", (unsigned long long)(p ? have : 0), (unsigned long long)need);
