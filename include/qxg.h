@@ -504,9 +504,11 @@ int qxg_kv_append(qxg_ctx *ctx, const qxg_kv_append_args *args, void *stream, in
  * with k and v the values that the cache stands for.  What stands in positions that a row does not see does not reach it; rows of
  * tokens at and behind count are left as they were; out shares memory with nothing else, nor does lse (refused: in each other, in
  * the cache, out in q).  tokens = 1 is single-token decoding.
- * Products are those of f32 numbers for an F32 q; for F16 and BF16 the softmax weights enter theirs with 17 bits, q as it is.  Sums are f32, rounded once; weights are up to 2^8 before they are
- * divided by their sum, so values from 2^118 on may overflow.  A row that sees a scale that is not finite is NaN,
- * and so is its lse, as are a row whose q is not finite and one whose largest score is beyond f32. */
+ * Products are those of f32 numbers for an F32 q; for F16 and BF16 q enters them as it is, and the softmax weights with 17 bits (off by 2^-18 of a
+ * term, where the result is rounded by 2^-12 or 2^-9).  Sums are f32, rounded once: a dot product, over 8 bits before it is multiplied by its
+ * position's scale, has to be within f32, as scale times a position's scale has; weights are up to 2^8 before they are divided by their sum, so
+ * values from 2^118 on may overflow.  A row that sees a scale that is not finite is NaN, and so is its lse, as are a row whose q is not finite
+ * and one whose largest score is beyond f32. */
 typedef struct qxg_cache_attention_args {
     const void *q;            /* [batch][tokens][heads][dim] of `type`, 16-byte aligned */
     const void *k, *v;        /* 16-byte aligned */

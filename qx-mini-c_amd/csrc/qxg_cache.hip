@@ -91,7 +91,8 @@ bool append_plan(const qxg_kv_append_args *p, QxkArgs &A, const Err &fail) {
 // Sequences of a batch are of unlike lengths, taken as 13/16 of the longest on average: with small splits (12, 6 or 3 rounds) the CUs are
 // done at about the same time, each with its share of the work, and workgroups start while others work.  16 sequences of 10000 to 32000
 // positions of 4 bits in 2, 24, 48 splits 128, 101, 100 us, all of 32000 in 2, 23, 42 145, 142, 149; 36 of 2700 to 8000 of 8 bits in 4, 12
-// splits 100, 87.
+// splits 100, 87.  (Within a window the lists of sequences longer than it are of one length, and nothing is less there: their calls, and batches of
+// equal lengths, may get more splits than they need.)
 // Short lists stay whole: a token of 32 / 4 heads in f32 over 1024 + 4 positions takes 15 us on the card and 10 with the join, whose
 // launch costs a program 3 to 5.
 //
@@ -101,7 +102,7 @@ bool append_plan(const qxg_kv_append_args *p, QxkArgs &A, const Err &fail) {
 // tokens over 8000 positions of 8 bits 223, 159, of 4 bits 154, 124; 8 x 5 over 6000 of 8 bits 37, 28; 256 over 600 17.8, 16.0; 32
 // over 600 9.8, 11.5; one token each of 16 sequences of 32000 of 4 bits (4 columns) 141, 153.
 // With 128, whose waves share them in LDS, more work is needed to pay: of 8 bits and a BF16 q, 512 tokens over 8000 positions
-// (work 256000) 157, 2 x 4096 within 2048 + 4 (1600000) 253 where 32 columns take 297.  Two of its workgroups go on a CU.
+// (work 256000) 136 where 32 columns take 141, 2 x 4096 within 2048 + 4 (1600000) 271 and 313.  Two of its workgroups go on a CU.
 void attention_splits(QxwArgs &A, uint64_t columns) {
     const qxg_cache_attention_args &a = A.a;
     // the chunks of a tile, at most

@@ -10,7 +10,7 @@
 // The exponent s - M of a score in base 2 is one fma.  Where |M| is from FAR on, it is the product rounded as the maximum was, less
 // M: an fma's would hold what that rounding left, half a step of the score, from 2^28 on more than the 8 that M allows, and from 2^31 on
 // more than e has room for.
-// (An f32 q over INT8 codes as a column's whole numbers, in products of 8 bits, is faster for a prompt, 44.5 us for 49 of 512 tokens of 32 / 4
+// (An f32 q over INT8 codes as a column's whole numbers, in products of 8 bits, is faster for a prompt, 40 us a call for 45 of 512 tokens of 32 / 4
 // heads of 128 within 1024 + 4 positions, but a large value of q costs the others their low bits, from 2^22 times as large all of them.)
 #include "qxg_cache.h"
 #include "qxg_values.h"
@@ -144,11 +144,12 @@ DEV void finish_lse(const QxwArgs &A, float M, float den, uint32_t b, uint32_t t
 // What bounds it.  Long caches and few tokens: bytes; one token each of 16 sequences of 30000 positions, 32 / 8 heads of 128 in bf16 over 8 bits,
 // 983 MB in 206 us, 4.8 TB/s (4 bits, 32000 positions: 557 MB in 141 us).  Otherwise the issue of instructions, about one in 4.7 cycles:
 // a chunk of 16 columns of 128 dims is some 300 vector instructions, half of them the conversion of codes, and 28 to 48 matrix ones, which add up
-// as a SIMD's waves all do the same; 512 tokens of 32 / 4 heads in f32 within 1024 + 4 positions 49 us.  Tried without gain: 8 waves a
+// as a SIMD's waves all do the same; 512 tokens of 32 / 4 heads in f32 within 1024 + 4 positions 45 us a call (queued one after the other; under a tracer, at
+// another clock, 48.5).  Tried without gain: 8 waves a
 // workgroup (15.0 us and 14.3 for a token over 36 chunks), which share the SIMDs; contexts of 64 columns a wave, which spill.
-// A first form, which staged chunks in LDS for four waves of 16 columns each, took 42 us where this takes 36 (16 x 1 token within
-// 4096 + 16), and 165 where it takes 107 (16 x 1 token over 10000 to 32000
-// positions of 4 bits).
+// 16 x 1 token within 4096 + 16 took 42 us a call in a first form, which staged chunks in LDS for four waves of 16 columns each, 39 without the
+// staging, and 33 to 36 with the present splits; 16 x 1 over 10000 to 32000 positions of 4 bits 165 in that form, and 130 without it and with the
+// order of the kv heads on the XCDs (163 without that order), 95 to 107 with the smaller splits of batches.
 //
 // Tiles.  v_mfma_f32_16x16x32_bf16: lane l holds 8 values of k of row (column) l % 16, those of group l / 16; result register r of
 // lane l is row 4 (l / 16) + r, column l % 16.  Scores have positions as rows, two tiles a chunk, and columns (token, head): a lane's
@@ -442,8 +443,8 @@ __global__ __launch_bounds__(256, CT == 2 || (D == 128 && (sizeof(T) == 4 || (__
 // A step works on three chunks at once, so that matrix and vector instructions do not wait for each other: the second product of
 // chunk i - 1, the weights of chunk i, the scores of chunk i + 1.
 //
-// What bounds it: 2 x 4096 tokens of 32 / 8 heads of 128 within 2048 + 4 positions take 253 to 280 us on the card (up to 370 on one that clocks
-// lower under the matrix cores' power) for products that a large matrix product's rate would do in 124 with one piece of the weights
+// What bounds it: 2 x 4096 tokens of 32 / 8 heads of 128 within 2048 + 4 positions take 258 to 350 us on the card, as it clocks
+// under the matrix cores' power, for products that a large matrix product's rate would do in 124 with one piece of the weights
 // for their two: 24 matrix instructions of a chunk (768 cycles of a SIMD) and some 250 vector ones.  The first form, without the three chunks at once,
 // took 560.  Other orders of the loop's parts, 8 waves a workgroup or raised priorities changed nothing.
 namespace {
